@@ -1,0 +1,559 @@
+// Distillation from a teacher's top logits, forward and backward, for gfx950. A row of V student logits z, up to K teacher
+// logits t_j at tokens k_j, a temperature tau, a weight w and, optionally, the row's label:
+//   p = softmax of t / tau over the row's live slots (k_j >= 0 and t_j > -inf), q = softmax(z / tau), P = softmax(z)
+//   row  = w tau^2 sum_j p_j (log p_j - log q_{k_j}) + (1 - w) (-log P_label)
+//   loss = the sum or mean of the rows that are not ignored (label == ignore_index), or every row (0 where ignored)
+//   dz_v = g w tau (q_v - sum_{j: k_j = v} p_j) + g (1 - w) (P_v - [v = label])
+// with g the upstream factor (over the number of rows for the mean). A row without a live slot has no first term.
+//
+// Forward: one pass over the row with the running maximum m and the sums of exp((z - m) / tau) and exp(z - m) (one sum where
+// the two are equal or only one is used); the read of z bounds it. Few rows are split over several workgroups, whose sums
+// are joined by a second launch. Backward: z once more, and dz; q and P come from m and the sums the forward kept. The
+// tokens that the teacher or the label names are written again after the row, in full fp32, by one thread each, so that
+// a token named twice is the sum of its slots in a fixed order.
+//
+// Exponents are taken of z - m (exact for bf16 inputs near m), never of z times a constant: rows of the type's lowest value
+// stay finite. The few operations on a row's sums are in fp64: log p - log q is a small difference of larger numbers.
+
+#include "dh_common.h"
+
+namespace {
+
+constexpr int kT = 256;                    // threads of a row (or of its part)
+constexpr int kW = kT / 64;
+constexpr int kMaxSlots = 256;
+constexpr int kSlotsPerLane = kMaxSlots / 64;
+constexpr int kMaxParts = 32;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr double kLn2 = 0.6931471805599453;
+
+__device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
+__device__ __forceinline__ float finite_ref(float m) { return m == -INFINITY ? 0.f : m; }
+
+template <typename T> constexpr int kE = 16 / (int)sizeof(T);
+
+// 16 bytes from any element address, as fp32
+template <typename T>
+__device__ __forceinline__ uint4 load16(const T* p) {
+  uint4 v;
+  __builtin_memcpy(&v, p, 16);
+  return v;
+}
+template <typename T> __device__ __forceinline__ void unpack(const uint4& v, float (&x)[kE<T>]) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int j = 0; j < kE<T>; ++j) {
+    if constexpr (sizeof(T) == 2)
+      x[j] = __uint_as_float((j & 1) ? (w[j >> 1] & 0xffff0000u) : (w[j >> 1] << 16));
+    else
+      x[j] = __uint_as_float(w[j]);
+  }
+}
+template <typename T> __device__ __forceinline__ uint4 pack(const float (&x)[kE<T>]) {
+  uint32_t w[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if constexpr (sizeof(T) == 2)
+      w[j] = (uint32_t)f32_to_bf16(x[2 * j]) | ((uint32_t)f32_to_bf16(x[2 * j + 1]) << 16);
+    else
+      w[j] = __float_as_uint(x[j]);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+__device__ __forceinline__ float wave_max(float v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
+  return v;
+}
+__device__ __forceinline__ double wave_sum64(double v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+  return v;
+}
+
+// what a row is computed from (by value to every kernel)
+struct Rows {
+  const void* logits;
+  int64_t sb, st;                          // strides of row (b, t), b = r / T
+  int64_t rows;
+  int T, V;
+  const void* t_logits;
+  const void* t_tokens;
+  const void* labels;                      // null: none
+  int64_t ignore;
+  int t_bf16, token_wide, label_wide, K;
+  float tau, weight;
+  int soft, hard;                          // which terms there are
+};
+
+template <typename T>
+__device__ __forceinline__ const T* row_of(const Rows& a, int64_t r) {
+  return reinterpret_cast<const T*>(a.logits) + (r / a.T) * a.sb + (r % a.T) * a.st;
+}
+__device__ __forceinline__ int64_t whole(const void* p, int wide, int64_t i) {
+  return wide ? reinterpret_cast<const int64_t*>(p)[i] : (int64_t) reinterpret_cast<const int32_t*>(p)[i];
+}
+__device__ __forceinline__ float teacher_logit(const Rows& a, int64_t i) {
+  return a.t_bf16 ? bf16_to_f32(reinterpret_cast<const bf16_t*>(a.t_logits)[i]) : reinterpret_cast<const float*>(a.t_logits)[i];
+}
+
+// kept of a row for the backward pass: the maximum, the reciprocals of the two sums, and what there is to differentiate
+struct Kept {
+  float m, inv_soft, inv_hard;
+  int terms;                               // bit 0: the row counts, bit 1: it has live slots
+};
+
+struct Sums {
+  float m, s0, s1;                         // s0: of exp((z - m) c0), s1: of exp((z - m) c1), c as in scales()
+};
+// c0: the soft term's (or, without one, the hard term's) scale of the exponent in base 2; c1: the hard term's
+__device__ __forceinline__ void scales(const Rows& a, float& c0, float& c1) {
+  c0 = a.soft ? kLog2e / a.tau : kLog2e;
+  c1 = kLog2e;
+}
+template <int NS>
+__device__ __forceinline__ Sums join(const Sums& a, const Sums& b, float c0, float c1) {
+  Sums r;
+  r.m = fmaxf(a.m, b.m);
+  const float ref = finite_ref(r.m);
+  r.s0 = a.s0 * exp2_hw((a.m - ref) * c0) + b.s0 * exp2_hw((b.m - ref) * c0);
+  r.s1 = NS == 2 ? a.s1 * exp2_hw((a.m - ref) * c1) + b.s1 * exp2_hw((b.m - ref) * c1) : 0.f;
+  return r;
+}
+template <int NS>
+__device__ __forceinline__ Sums wave_join(Sums v, float c0, float c1) {
+  const float m = wave_max(v.m), ref = finite_ref(m);
+  v.s0 = wave_sum(v.s0 * exp2_hw((v.m - ref) * c0));
+  v.s1 = NS == 2 ? wave_sum(v.s1 * exp2_hw((v.m - ref) * c1)) : 0.f;
+  v.m = m;
+  return v;
+}
+
+// The teacher's probabilities of a row, in one wave: slot lane + 64 i of p[i], its token (-1: empty) and (t_j - max) / tau.
+// Returns log of their sum, or sets live to false; bad: a token past the vocabulary.
+__device__ __forceinline__ double teacher_row(const Rows& a, int64_t r, int lane, float (&p)[kSlotsPerLane],
+                                              int (&token)[kSlotsPerLane], float (&t)[kSlotsPerLane], float& top, bool& live,
+                                              bool& bad) {
+  float most = -INFINITY;
+  bool some = false, over = false;
+#pragma unroll
+  for (int i = 0; i < kSlotsPerLane; ++i) {
+    const int j = i * 64 + lane;
+    token[i] = -1;
+    t[i] = -INFINITY;
+    if (j < a.K) {
+      const int64_t k = whole(a.t_tokens, a.token_wide, r * a.K + j);
+      const float x = teacher_logit(a, r * a.K + j);
+      if (k >= a.V) over = true;
+      if (k >= 0 && k < a.V && !(x == -INFINITY)) {
+        token[i] = (int)k;
+        t[i] = x;
+        some = true;
+      }
+    }
+    most = fmaxf(most, t[i]);
+  }
+  live = __ballot(some) != 0;
+  bad = __ballot(over) != 0;
+  most = wave_max(most);
+  top = finite_ref(most);
+  const float c = kLog2e / a.tau;
+  float s = 0.f;
+#pragma unroll
+  for (int i = 0; i < kSlotsPerLane; ++i) {
+    p[i] = token[i] >= 0 ? exp2_hw((t[i] - top) * c) : 0.f;
+    s += p[i];
+  }
+  s = wave_sum(s);
+#pragma unroll
+  for (int i = 0; i < kSlotsPerLane; ++i) p[i] = token[i] >= 0 ? p[i] / s : 0.f;
+  return live ? log((double)s) : 0.0;
+}
+
+// the row's loss and what the backward pass keeps, by one wave
+template <typename T>
+__device__ __forceinline__ void finish_row(const Rows& a, int64_t r, const Sums& v, int lane, float* losses, Kept* kept) {
+  const T* z = row_of<T>(a, r);
+  const int64_t label = a.labels ? whole(a.labels, a.label_wide, r) : 0;
+  const bool counts = !a.labels || label != a.ignore;
+  const double s1 = a.hard && a.soft && a.tau != 1.f ? v.s1 : v.s0;
+  double row = 0.0;
+  bool live = false, bad = false;
+  if (counts) {                            // uniform
+    if (a.soft) {
+      float p[kSlotsPerLane], t[kSlotsPerLane], top;
+      int token[kSlotsPerLane];
+      const double lt = teacher_row(a, r, lane, p, token, t, top, live, bad);
+      const double lz = log((double)v.s0);
+      double sum = 0.0;
+#pragma unroll
+      for (int i = 0; i < kSlotsPerLane; ++i)
+        if (token[i] >= 0 && !(p[i] == 0.f)) {
+          const double log_p = ((double)t[i] - (double)top) / (double)a.tau - lt;
+          const double log_q = ((double)Elem<T>::load(z + token[i]) - (double)v.m) / (double)a.tau - lz;
+          sum += (double)p[i] * (log_p - log_q);
+        }
+      row = (double)a.weight * (double)a.tau * (double)a.tau * wave_sum64(sum);
+    }
+    if (a.labels && (label < 0 || label >= a.V)) bad = true;
+    if (a.hard && !bad)
+      row += (1.0 - (double)a.weight) * (log(s1) - ((double)Elem<T>::load(z + label) - (double)v.m));
+    if (bad) row = __builtin_nan("");
+  }
+  if (lane == 0) {
+    losses[r] = (float)row;
+    const float nan = __builtin_nanf("");
+    kept[r] = Kept{v.m, bad ? nan : 1.f / v.s0, bad ? nan : (float)(1.0 / s1), (counts ? 1 : 0) | (live || bad ? 2 : 0)};
+  }
+}
+
+// ---- forward: a row, or one of its parts ----------------------------------------------------------------------------
+template <typename T, int NS>
+__global__ __launch_bounds__(kT) void forward_kernel(Rows a, int parts, Sums* part, float* losses, Kept* kept) {
+  constexpr int E = kE<T>, U = 4;
+  __shared__ Sums ws[kW];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int64_t r = blockIdx.x / parts;
+  const int which = (int)(blockIdx.x % parts);
+  const T* z = row_of<T>(a, r);
+  float c0, c1;
+  scales(a, c0, c1);
+  // 16-byte pieces from the boundary at or below the row (a piece that holds an element of the row is mapped whole); what
+  // the first and last hold of others counts as -inf
+  const int mis = (int)((reinterpret_cast<uintptr_t>(z) & 15u) / sizeof(T));
+  const uint4* base = reinterpret_cast<const uint4*>(z - mis);
+  const int pieces = (mis + a.V + E - 1) / E, per = (pieces + parts - 1) / parts;
+  const int p0 = min(which * per, pieces), p1 = min(p0 + per, pieces);
+  const uint32_t none = sizeof(T) == 2 ? 0xff80ff80u : 0xff800000u;
+  Sums v{-INFINITY, 0.f, 0.f};
+  for (int p = p0 + tid; p < p1; p += kT * U) {
+    uint4 q[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      q[u] = make_uint4(none, none, none, none);
+      if (p + u * kT < p1) q[u] = base[p + u * kT];
+    }
+    float x[U][E];
+    float most = v.m;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      unpack<T>(q[u], x[u]);
+      const int k = p + u * kT;
+      if (k == 0 || k == pieces - 1) {
+#pragma unroll
+        for (int j = 0; j < E; ++j)
+          if (k * E + j < mis || k * E + j >= mis + a.V) x[u][j] = -INFINITY;
+      }
+#pragma unroll
+      for (int j = 0; j < E; ++j) most = fmaxf(most, x[u][j]);
+    }
+    const float ref = finite_ref(most);
+    v.s0 *= exp2_hw((v.m - ref) * c0);
+    if (NS == 2) v.s1 *= exp2_hw((v.m - ref) * c1);
+    v.m = most;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int j = 0; j < E; ++j) {
+        const float d = x[u][j] - ref;
+        v.s0 += exp2_hw(d * c0);
+        if (NS == 2) v.s1 += exp2_hw(d * c1);
+      }
+  }
+  v = wave_join<NS>(v, c0, c1);
+  if (lane == 0) ws[wave] = v;
+  __syncthreads();
+  if (wave) return;
+  v = ws[0];
+#pragma unroll
+  for (int w = 1; w < kW; ++w) v = join<NS>(v, ws[w], c0, c1);
+  if (parts > 1) {
+    if (lane == 0) part[blockIdx.x] = v;
+  } else {
+    finish_row<T>(a, r, v, lane, losses, kept);
+  }
+}
+
+// the sum or mean of the rows in a fixed order, and its divisor, by one workgroup
+__device__ __forceinline__ void reduce_rows(const float* losses, const Kept* kept, int64_t rows, int mean, float* loss,
+                                            float* divisor, double* red, int* cnt) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, W = blockDim.x >> 6;
+  double s = 0.0;
+  int n = 0;
+  for (int64_t r = tid; r < rows; r += blockDim.x) {
+    s += losses[r];
+    n += kept[r].terms & 1;
+  }
+  s = wave_sum64(s);
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) n += __shfl_xor(n, o);
+  if (lane == 0) {
+    red[wave] = s;
+    cnt[wave] = n;
+  }
+  __syncthreads();
+  if (tid == 0) {
+    for (int w = 1; w < W; ++w) {
+      s += red[w];
+      n += cnt[w];
+    }
+    // (the mean of no rows is NaN)
+    *loss = (float)(mean ? s / (double)n : s);
+    *divisor = mean ? (float)n : 1.f;
+  }
+}
+
+constexpr int kRT = 1024;                  // threads of the reduction, and of the join that ends with it
+
+// rows split over workgroups: their sums joined, a wave a row; loss non-null: one workgroup, which reduces the rows too
+template <typename T, int NS>
+__global__ __launch_bounds__(kRT) void join_kernel(Rows a, int parts, const Sums* part, float* losses, Kept* kept, int mean,
+                                                   float* loss, float* divisor) {
+  __shared__ double red[kRT / 64];
+  __shared__ int cnt[kRT / 64];
+  const int lane = threadIdx.x & 63, W = blockDim.x >> 6;
+  float c0, c1;
+  scales(a, c0, c1);
+  for (int64_t r = (int64_t)blockIdx.x * W + (threadIdx.x >> 6); r < a.rows; r += (int64_t)gridDim.x * W) {
+    Sums v{-INFINITY, 0.f, 0.f};
+    if (lane < parts) v = part[r * parts + lane];
+    finish_row<T>(a, r, wave_join<NS>(v, c0, c1), lane, losses, kept);
+  }
+  if (!loss) return;
+  __syncthreads();
+  reduce_rows(losses, kept, a.rows, mean, loss, divisor, red, cnt);
+}
+
+__global__ __launch_bounds__(kRT) void reduce_kernel(const float* losses, const Kept* kept, int64_t rows, int mean,
+                                                     float* loss, float* divisor) {
+  __shared__ double red[kRT / 64];
+  __shared__ int cnt[kRT / 64];
+  reduce_rows(losses, kept, rows, mean, loss, divisor, red, cnt);
+}
+
+// ---- backward -------------------------------------------------------------------------------------------------------
+template <typename T, int NS>
+__global__ __launch_bounds__(kT) void backward_kernel(Rows a, int parts, const Kept* kept, const float* dloss,
+                                                      int64_t dloss_stride, const float* divisor, T* dz) {
+  constexpr int E = kE<T>, U = 2;
+  __shared__ float sp[kMaxSlots];
+  __shared__ int stok[kMaxSlots];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int64_t r = blockIdx.x / parts;
+  const int which = (int)(blockIdx.x % parts);
+  const T* z = row_of<T>(a, r);
+  T* out = dz + r * a.V;
+  // pieces by the output's 16-byte boundaries
+  const int mis = (int)((reinterpret_cast<uintptr_t>(out) & 15u) / sizeof(T));
+  const int pieces = (mis + a.V + E - 1) / E, per = (pieces + parts - 1) / parts;
+  const int p0 = min(which * per, pieces), p1 = min(p0 + per, pieces);
+  const Kept k = kept[r];
+  const bool counts = k.terms & 1, soft = counts && a.soft && (k.terms & 2), hard = counts && a.hard;
+  const float g = dloss[dloss_stride * r] / (divisor ? *divisor : 1.f);
+  const float gs = soft ? g * a.weight * a.tau : 0.f, gh = hard ? g * (1.f - a.weight) : 0.f;
+  float c0, c1;
+  scales(a, c0, c1);
+  // dz of a logit without the teacher's and the label's part: f0 exp((z - m) c0) + f1 exp((z - m) c1)
+  const float ref = finite_ref(k.m);
+  const float f0 = NS == 2 ? gs * k.inv_soft : (gs + gh) * k.inv_soft, f1 = gh * k.inv_hard;
+  const bool use0 = NS == 2 ? soft : soft || hard, use1 = NS == 2 && hard;
+  auto value = [&](float x) {
+    const float d = x - ref;
+    float y = 0.f;
+    if (use0) y = f0 * exp2_hw(d * c0);
+    if (use1) y += f1 * exp2_hw(d * c1);
+    return y;
+  };
+  if (soft && wave == 0) {
+    float p[kSlotsPerLane], t[kSlotsPerLane], top;
+    int token[kSlotsPerLane];
+    bool live, bad;
+    teacher_row(a, r, lane, p, token, t, top, live, bad);
+#pragma unroll
+    for (int i = 0; i < kSlotsPerLane; ++i) {
+      sp[i * 64 + lane] = p[i];
+      stok[i * 64 + lane] = token[i];
+    }
+  }
+  for (int p = p0 + tid; p < p1; p += kT * U) {
+    uint4 q[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = (p + u * kT) * E - mis;
+      if (p + u * kT < p1 && i >= 0 && i + E <= a.V) q[u] = load16(z + i);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = (p + u * kT) * E - mis;
+      if (p + u * kT >= p1) break;
+      if (i >= 0 && i + E <= a.V) {
+        float x[E];
+        unpack<T>(q[u], x);
+#pragma unroll
+        for (int j = 0; j < E; ++j) x[j] = value(x[j]);
+        *reinterpret_cast<uint4*>(out + i) = pack<T>(x);
+      } else {
+        for (int j = max(i, 0); j < min(i + E, a.V); ++j) Elem<T>::store(out + j, value(Elem<T>::load(z + j)));
+      }
+    }
+  }
+  if (!soft && !hard) return;              // uniform
+  __syncthreads();
+  // the named tokens of this part, the label behind the slots
+  const int64_t label = hard ? whole(a.labels, a.label_wide, r) : -1;
+  const int lo = max(p0 * E - mis, 0), hi = min(p1 * E - mis, a.V);
+  const int K = soft ? a.K : 0;
+  for (int j = tid; j <= K; j += kT) {
+    const int64_t v = j < K ? stok[j] : label;
+    if (v < lo || v >= hi) continue;
+    float p = 0.f;
+    for (int i = 0; i < K; ++i) p += stok[i] == v ? sp[i] : 0.f;
+    float y = value(Elem<T>::load(z + v)) - gs * p;
+    if (v == label) y -= gh;
+    Elem<T>::store(out + v, y);
+  }
+}
+
+// ---- sizes ----------------------------------------------------------------------------------------------------------
+// workgroups a row: enough for 1024 in all, each with at least two pieces a thread
+int parts_of(int64_t rows, int V, int dtype) {
+  const int64_t pieces = ((int64_t)V * (dtype == DH_BF16 ? 2 : 4) + 15) / 16;
+  int64_t p = 1024 / (rows > 0 ? rows : 1);
+  const int64_t most = pieces / (2 * kT);
+  if (p > most) p = most;
+  if (p > kMaxParts) p = kMaxParts;
+  return p < 1 ? 1 : (int)p;
+}
+
+int check(const char* who, int dtype, const Rows& a, int t_dtype, int token_bits, int label_bits) {
+  DH_REQUIRE(dtype == DH_F32 || dtype == DH_BF16, DH_ERR_UNSUPPORTED_DTYPE, "%s: dtype %d", who, dtype);
+  DH_REQUIRE(t_dtype == DH_F32 || t_dtype == DH_BF16, DH_ERR_UNSUPPORTED_DTYPE, "%s: teacher dtype %d", who, t_dtype);
+  DH_REQUIRE((token_bits == 32 || token_bits == 64) && (!a.labels || label_bits == 32 || label_bits == 64),
+             DH_ERR_UNSUPPORTED_DTYPE, "%s: tokens of %d bits, labels of %d", who, token_bits, label_bits);
+  DH_REQUIRE(a.rows >= 0 && a.rows < ((int64_t)1 << 22) && a.T >= 1 && a.V >= 1 && a.V <= (1 << 24), DH_ERR_UNSUPPORTED_SHAPE,
+             "%s: rows=%lld T=%d V=%d", who, (long long)a.rows, a.T, a.V);
+  DH_REQUIRE(a.K >= 1 && a.K <= kMaxSlots, DH_ERR_UNSUPPORTED_SHAPE, "%s: K=%d must be in [1, %d]", who, a.K, kMaxSlots);
+  DH_REQUIRE(a.tau > 0.f && a.tau < INFINITY && a.weight >= 0.f && a.weight <= 1.f, DH_ERR_INVALID_ARG,
+             "%s: temperature %g, weight %g", who, (double)a.tau, (double)a.weight);
+  DH_REQUIRE(a.rows == 0 || a.labels || a.weight == 1.f, DH_ERR_INVALID_ARG, "%s: weight %g without labels", who, (double)a.weight);
+  DH_REQUIRE(a.rows == 0 || (a.logits && a.t_logits && a.t_tokens), DH_ERR_INVALID_ARG, "%s: null pointer argument", who);
+  return 0;
+}
+
+Rows rows_of(const void* logits, int64_t sb, int64_t st, int64_t B, int T, int V, int t_dtype, const void* t_logits,
+             const void* t_tokens, int token_bits, int K, const void* labels, int label_bits, int64_t ignore, float tau,
+             float weight) {
+  Rows a;
+  a.logits = logits;
+  a.sb = sb;
+  a.st = st;
+  a.rows = B * T;
+  a.T = T;
+  a.V = V;
+  a.t_logits = t_logits;
+  a.t_tokens = t_tokens;
+  a.labels = labels;
+  a.ignore = ignore;
+  a.t_bf16 = t_dtype == DH_BF16;
+  a.token_wide = token_bits == 64;
+  a.label_wide = label_bits == 64;
+  a.K = K;
+  a.tau = tau;
+  a.weight = weight;
+  a.soft = weight > 0.f;
+  a.hard = labels != nullptr && weight < 1.f;
+  return a;
+}
+
+bool two_sums(const Rows& a) { return a.soft && a.hard && a.tau != 1.f; }
+
+template <typename T, int NS>
+int forward(const Rows& a, int parts, int reduction, float* losses, Kept* kept, float* loss, float* divisor, Sums* part,
+            hipStream_t s) {
+  forward_kernel<T, NS><<<dim3((unsigned)(a.rows * parts)), dim3(kT), 0, s>>>(a, parts, part, losses, kept);
+  if (int st = dh_check_launch("dh_distill_fwd")) return st;
+  const int mean = reduction == 1;
+  if (parts > 1) {
+    const bool ends = reduction != 0 && a.rows <= 64;          // one workgroup joins all rows and reduces them
+    if (ends)
+      join_kernel<T, NS><<<dim3(1), dim3(kRT), 0, s>>>(a, parts, part, losses, kept, mean, loss, divisor);
+    else
+      join_kernel<T, NS><<<dim3((unsigned)((a.rows + 3) / 4)), dim3(256), 0, s>>>(a, parts, part, losses, kept, mean, nullptr,
+                                                                                nullptr);
+    if (int st = dh_check_launch("dh_distill_fwd")) return st;
+    if (ends) return 0;
+  }
+  if (reduction == 0) return 0;
+  reduce_kernel<<<dim3(1), dim3(kRT), 0, s>>>(losses, kept, a.rows, mean, loss, divisor);
+  return dh_check_launch("dh_distill_fwd");
+}
+
+template <typename T, int NS>
+int backward(const Rows& a, int parts, const Kept* kept, const float* dloss, int64_t stride, const float* divisor, void* dz,
+             hipStream_t s) {
+  backward_kernel<T, NS><<<dim3((unsigned)(a.rows * parts)), dim3(kT), 0, s>>>(a, parts, kept, dloss, stride, divisor,
+                                                                             (T*)dz);
+  return dh_check_launch("dh_distill_bwd");
+}
+
+}  // namespace
+
+extern "C" int64_t dh_distill_workspace_bytes(int dtype, int64_t rows, int V) {
+  const int parts = parts_of(rows, V, dtype);
+  return parts > 1 ? rows * parts * (int64_t)sizeof(Sums) : 0;
+}
+
+extern "C" int dh_distill_fwd(int dtype, const void* logits, int64_t stride_b, int64_t stride_t, int64_t B, int T, int V,
+                              int teacher_dtype, const void* teacher_logits, const void* teacher_tokens, int token_bits, int K,
+                              const void* labels, int label_bits, int64_t ignore_index, float temperature, float weight,
+                              int reduction, float* row_loss, void* row_kept, float* loss, float* divisor, void* workspace,
+                              int64_t workspace_bytes, void* stream) {
+  const char* who = "dh_distill_fwd";
+  const Rows a = rows_of(logits, stride_b, stride_t, B, T, V, teacher_dtype, teacher_logits, teacher_tokens, token_bits, K,
+                         labels, label_bits, ignore_index, temperature, weight);
+  if (int st = check(who, dtype, a, teacher_dtype, token_bits, label_bits)) return st;
+  DH_REQUIRE(reduction >= 0 && reduction <= 2, DH_ERR_INVALID_ARG, "%s: reduction %d", who, reduction);
+  DH_REQUIRE(a.rows == 0 || (row_loss && row_kept && (uintptr_t)row_kept % 16 == 0), DH_ERR_INVALID_ARG,
+             "%s: null or unaligned pointer argument", who);
+  DH_REQUIRE(reduction == 0 || (loss && divisor), DH_ERR_INVALID_ARG, "%s: null pointer argument", who);
+  const int64_t need = dh_distill_workspace_bytes(dtype, a.rows, V);
+  DH_REQUIRE(workspace_bytes >= need && (need == 0 || workspace), DH_ERR_INVALID_ARG, "%s: workspace of %lld bytes, %lld needed",
+             who, (long long)workspace_bytes, (long long)need);
+  hipStream_t s = (hipStream_t)stream;
+  Kept* kept = (Kept*)row_kept;
+  if (a.rows == 0) {
+    if (reduction == 0) return 0;
+    reduce_kernel<<<dim3(1), dim3(kRT), 0, s>>>(row_loss, kept, 0, reduction == 1, loss, divisor);
+    return dh_check_launch(who);
+  }
+  const int parts = parts_of(a.rows, V, dtype);
+  Sums* part = (Sums*)workspace;
+  if (dtype == DH_BF16)
+    return two_sums(a) ? forward<bf16_t, 2>(a, parts, reduction, row_loss, kept, loss, divisor, part, s)
+                       : forward<bf16_t, 1>(a, parts, reduction, row_loss, kept, loss, divisor, part, s);
+  return two_sums(a) ? forward<float, 2>(a, parts, reduction, row_loss, kept, loss, divisor, part, s)
+                     : forward<float, 1>(a, parts, reduction, row_loss, kept, loss, divisor, part, s);
+}
+
+extern "C" int dh_distill_bwd(int dtype, const void* logits, int64_t stride_b, int64_t stride_t, int64_t B, int T, int V,
+                              int teacher_dtype, const void* teacher_logits, const void* teacher_tokens, int token_bits, int K,
+                              const void* labels, int label_bits, int64_t ignore_index, float temperature, float weight,
+                              const void* row_kept, const float* dloss, int64_t dloss_stride, const float* divisor, void* dlogits,
+                              void* stream) {
+  const char* who = "dh_distill_bwd";
+  const Rows a = rows_of(logits, stride_b, stride_t, B, T, V, teacher_dtype, teacher_logits, teacher_tokens, token_bits, K,
+                         labels, label_bits, ignore_index, temperature, weight);
+  if (int st = check(who, dtype, a, teacher_dtype, token_bits, label_bits)) return st;
+  if (a.rows == 0) return 0;
+  DH_REQUIRE(row_kept && (uintptr_t)row_kept % 16 == 0 && dloss && dlogits && dloss_stride >= 0, DH_ERR_INVALID_ARG,
+             "%s: null or unaligned pointer argument", who);
+  const int parts = parts_of(a.rows, V, dtype);
+  const Kept* kept = (const Kept*)row_kept;
+  hipStream_t s = (hipStream_t)stream;
+  if (dtype == DH_BF16)
+    return two_sums(a) ? backward<bf16_t, 2>(a, parts, kept, dloss, dloss_stride, divisor, dlogits, s)
+                       : backward<bf16_t, 1>(a, parts, kept, dloss, dloss_stride, divisor, dlogits, s);
+  return two_sums(a) ? backward<float, 2>(a, parts, kept, dloss, dloss_stride, divisor, dlogits, s)
+                     : backward<float, 1>(a, parts, kept, dloss, dloss_stride, divisor, dlogits, s);
+}

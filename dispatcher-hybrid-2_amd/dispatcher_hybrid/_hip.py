@@ -15,7 +15,7 @@ import os
 
 import torch
 
-ABI_VERSION = 20
+ABI_VERSION = 21
 _LIB_NAME = "libdh_mixer.so"
 
 DH_F32, DH_BF16 = 0, 1
@@ -108,6 +108,15 @@ def _load():
                                        + [vp, vp, vp, i64, vp, vp, i64, vp, i64, vp], i32),
         "dh_decode_persistent_phases": ([vp, i32], i32),
         "dh_silu_mul": ([i32, vp, vp, vp, i64, vp], i32),
+        "dh_embed_fwd": ([i32, vp, i64, i64, i32, vp, i32, i64, ctypes.c_float, i64, vp, i64, vp], i32),
+        "dh_embed_bwd_workspace_bytes": ([i64, i64, i32], i64),
+        "dh_embed_bwd": ([i32, vp, i64, vp, i32, i64, i64, i32, ctypes.c_float, i64, vp, vp, i64, vp], i32),
+        "dh_top_logits": ([i32, vp, i64, i64, i32, i32, vp, vp, vp], i32),
+        "dh_distill_workspace_bytes": ([i32, i64, i32], i64),
+        "dh_distill_fwd": ([i32, vp, i64, i64, i64, i32, i32, i32, vp, vp, i32, i32, vp, i32, i64, ctypes.c_float,
+                            ctypes.c_float, i32, vp, vp, vp, vp, vp, i64, vp], i32),
+        "dh_distill_bwd": ([i32, vp, i64, i64, i64, i32, i32, i32, vp, vp, i32, i32, vp, i32, i64, ctypes.c_float,
+                            ctypes.c_float, vp, vp, i64, vp, vp, vp], i32),
         "dh_add_rmsnorm": ([i32, vp, vp, vp, ctypes.c_float, vp, vp, i64, i32, vp], i32),
     }
     for name, (argtypes, restype) in sigs.items():

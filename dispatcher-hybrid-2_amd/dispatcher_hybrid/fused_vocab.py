@@ -1,0 +1,398 @@
+"""The vocabulary's ends of a training step on gfx950 kernels.
+
+    embed_tokens         rows of the embedding times a factor; its gradient groups the positions by token
+    top_logits           a teacher's k largest logits of every position and their tokens
+    distillation_loss    a student's loss on them (and on labels), one pass over the logits a direction
+
+Kernels: ``dh_embed_fwd`` / ``dh_embed_bwd``, ``dh_top_logits``, ``dh_distill_fwd`` / ``dh_distill_bwd``. The model runs them
+under ``model.enable_fused_vocab()``; ``distillation.py`` has the formulas as torch operations. fp32 and bf16; sums are fp32
+or wider, in an order that does not change from call to call.
+
+Each is one registered operation (``dispatcher::embed_tokens``, ...) for compilers and transforms, and in plain eager
+execution launched without one.
+
+Importing this module loads the kernel library and raises ImportError if it is missing.
+"""
+
+import contextlib
+from typing import List, Optional
+
+import torch
+import torch.nn as nn
+
+from . import _hip
+from . import distillation as plain
+from .fused_gates import _function_mode, _has_any_global_hook, plain_eager
+
+_PLAIN = (torch.Tensor, nn.Parameter)
+_INTS = (torch.int32, torch.int64)
+_REDUCTION = {"none": 0, "mean": 1, "sum": 2}
+
+
+def _on(t):
+    """The device of t as the current one (a launch goes to the current device)."""
+    return contextlib.nullcontext() if t.get_device() == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
+def _bits(t):
+    return 32 if t.dtype == torch.int32 else 64
+
+
+def _unit_rows(t):
+    """t with unit-stride rows (any other layout copied); broadcast rows stay."""
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+# ---------------------------------------------------------------------------------------------
+# embedding
+# ---------------------------------------------------------------------------------------------
+def _lookup(weight, tokens, scale, zero_token):
+    what = "embed_tokens"
+    _hip.same_gpu(what, weight, tokens)
+    V, d = weight.shape
+    code = _hip.dtype_code(weight.dtype)
+    w = weight if weight.stride(1) == 1 and weight.stride(0) >= d else weight.contiguous()
+    ids = tokens.contiguous()
+    out = torch.empty(*tokens.shape, d, device=w.device, dtype=w.dtype)
+    with _on(w):
+        st = _hip.lib.dh_embed_fwd(code, _hip.ptr(w), w.stride(0), V, d, _hip.ptr(ids), _bits(ids), ids.numel(), scale,
+                                   zero_token, _hip.ptr(out), d, _hip.stream_handle(w.device))
+    _hip.check(st, what)
+    return out
+
+
+def _lookup_grad(dy, tokens, rows, scale, skip_token):
+    what = "embed_tokens gradient"
+    _hip.same_gpu(what, dy, tokens)
+    d = dy.shape[-1]
+    code = _hip.dtype_code(dy.dtype)
+    dy2, ids = dy.reshape(-1, d), tokens.contiguous()
+    if not (dy2.stride(1) == 1 and dy2.stride(0) >= d):
+        dy2 = dy2.clone(memory_format=torch.contiguous_format)
+    out = torch.empty(rows, d, device=dy.device, dtype=dy.dtype)
+    nbytes = _hip.lib.dh_embed_bwd_workspace_bytes(ids.numel(), rows, d)
+    ws = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=dy.device)     # refused sizes: the call below says why
+    with _on(dy):
+        st = _hip.lib.dh_embed_bwd(code, _hip.ptr(dy2), dy2.stride(0), _hip.ptr(ids), _bits(ids), ids.numel(), rows, d,
+                                   scale, skip_token, _hip.ptr(out), _hip.ptr(ws), ws.numel(), _hip.stream_handle(dy.device))
+    _hip.check(st, what)
+    return out
+
+
+@torch.library.custom_op("dispatcher::embed_tokens", mutates_args=(), device_types="cuda")
+def _embed_op(weight: torch.Tensor, tokens: torch.Tensor, scale: float, zero_token: int, skip_token: int) -> torch.Tensor:
+    return _lookup(weight, tokens, scale, zero_token)
+
+
+@_embed_op.register_fake
+def _(weight, tokens, scale, zero_token, skip_token):
+    return weight.new_empty(*tokens.shape, weight.shape[1])
+
+
+@torch.library.custom_op("dispatcher::embed_tokens_grad", mutates_args=(), device_types="cuda")
+def _embed_grad_op(dy: torch.Tensor, tokens: torch.Tensor, rows: int, scale: float, skip_token: int) -> torch.Tensor:
+    return _lookup_grad(dy, tokens, rows, scale, skip_token)
+
+
+@_embed_grad_op.register_fake
+def _(dy, tokens, rows, scale, skip_token):
+    return dy.new_empty(rows, dy.shape[-1])
+
+
+def _embed_setup(ctx, inputs, output):
+    weight, tokens, scale, _, skip_token = inputs
+    ctx.save_for_backward(tokens)
+    ctx.args = (weight.shape[0], scale, skip_token)
+
+
+def _embed_backward(ctx, dy):
+    tokens, = ctx.saved_tensors
+    return torch.ops.dispatcher.embed_tokens_grad(dy, tokens, *ctx.args), None, None, None, None
+
+
+def _embed_grad_setup(ctx, inputs, output):
+    _, tokens, _, scale, skip_token = inputs
+    ctx.save_for_backward(tokens)
+    ctx.args = (scale, skip_token)
+
+
+def _embed_grad_backward(ctx, g):
+    # the gradient is linear in dy: its own gradient looks the rows of g up, zeros where positions were left out
+    tokens, = ctx.saved_tensors
+    scale, skip_token = ctx.args
+    return torch.ops.dispatcher.embed_tokens(g, tokens, scale, skip_token, skip_token), None, None, None, None
+
+
+torch.library.register_autograd("dispatcher::embed_tokens", _embed_backward, setup_context=_embed_setup)
+torch.library.register_autograd("dispatcher::embed_tokens_grad", _embed_grad_backward, setup_context=_embed_grad_setup)
+
+
+class _Embed(torch.autograd.Function):
+    """dispatcher::embed_tokens without the registered operation's per-call bookkeeping."""
+
+    @staticmethod
+    def forward(ctx, weight, tokens, scale, zero_token, skip_token):
+        _embed_setup(ctx, (weight, tokens, scale, zero_token, skip_token), None)
+        return _lookup(weight, tokens, scale, zero_token)
+
+    @staticmethod
+    def backward(ctx, dy):
+        tokens, = ctx.saved_tensors
+        return _EmbedGrad.apply(dy, tokens, *ctx.args), None, None, None, None
+
+
+class _EmbedGrad(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, dy, tokens, rows, scale, skip_token):
+        _embed_grad_setup(ctx, (dy, tokens, rows, scale, skip_token), None)
+        return _lookup_grad(dy, tokens, rows, scale, skip_token)
+
+    @staticmethod
+    def backward(ctx, g):
+        tokens, = ctx.saved_tensors
+        scale, skip_token = ctx.args
+        return _Embed.apply(g, tokens, scale, skip_token, skip_token), None, None, None, None
+
+
+def embed_tokens(tokens, weight, scale=1.0, padding_idx=None):
+    """weight[tokens] * scale, (*tokens.shape, d), differentiable in weight; rounded once.
+
+    tokens: int32 or int64 of any shape; weight (V, d) fp32 or bf16 of any width. A token outside [0, V) gives a row of NaN
+    (it is neither read nor reported) and no gradient. padding_idx: this token's row gets no gradient, as nn.Embedding's. The
+    gradient is dense: (V, d) in weight's dtype, every token's positions summed in fp32 in ascending order and rounded once,
+    the same bits on every call."""
+    if tokens.dtype not in _INTS:
+        raise TypeError(f"embed_tokens: tokens must be int32 or int64, got {tokens.dtype}")
+    if weight.dim() != 2 or weight.shape[0] < 1 or weight.shape[1] < 1:
+        raise ValueError(f"embed_tokens: weight (V, d) expected, got {tuple(weight.shape)}")
+    skip = -1
+    if padding_idx is not None:
+        V = weight.shape[0]
+        if not -V <= padding_idx < V:
+            raise ValueError(f"embed_tokens: padding_idx {padding_idx} outside a vocabulary of {V}")
+        skip = padding_idx % V
+    if type(weight) in _PLAIN and weight.is_cuda and plain_eager():
+        return _Embed.apply(weight, tokens, float(scale), -1, skip)
+    _hip.require_gpu(weight, "embed_tokens")
+    return torch.ops.dispatcher.embed_tokens(weight, tokens, float(scale), -1, skip)
+
+
+def embedding_fits(module):
+    """Whether embed_tokens is all that calling this module does: an nn.Embedding itself with a plain weight of the kernels'
+    dtypes on the GPU, no renormalisation, sparse or frequency-scaled gradient, hook or replaced forward."""
+    return (type(module) is nn.Embedding and type(module.weight) in _PLAIN and module.weight.is_cuda
+            and module.weight.dtype in (torch.float32, torch.bfloat16) and module.max_norm is None and not module.sparse
+            and not module.scale_grad_by_freq and "forward" not in module.__dict__
+            and not (module._forward_hooks or module._forward_pre_hooks or module._backward_hooks
+                     or module._backward_pre_hooks) and not _has_any_global_hook() and not _function_mode())
+
+
+# ---------------------------------------------------------------------------------------------
+# a teacher's targets
+# ---------------------------------------------------------------------------------------------
+def _top(logits, k):
+    what = "top_logits"
+    _hip.require_gpu(logits, what)
+    V = logits.shape[-1]
+    code = _hip.dtype_code(logits.dtype)
+    rows = _unit_rows(logits.reshape(-1, V))
+    values = torch.empty(*logits.shape[:-1], max(k, 0), device=logits.device, dtype=logits.dtype)
+    tokens = torch.empty(values.shape, device=logits.device, dtype=torch.int64)
+    with _on(logits):
+        st = _hip.lib.dh_top_logits(code, _hip.ptr(rows), rows.stride(0), rows.shape[0], V, k, _hip.ptr(values),
+                                    _hip.ptr(tokens), _hip.stream_handle(logits.device))
+    _hip.check(st, what)
+    return [values, tokens]
+
+
+@torch.library.custom_op("dispatcher::top_logits", mutates_args=(), device_types="cuda")
+def _top_op(logits: torch.Tensor, k: int) -> List[torch.Tensor]:
+    return _top(logits, k)
+
+
+@_top_op.register_fake
+def _(logits, k):
+    shape = (*logits.shape[:-1], k)
+    return [logits.new_empty(shape), logits.new_empty(shape, dtype=torch.int64)]
+
+
+def top_logits(logits, k):
+    """(values, tokens), each (..., k): the k largest of logits (..., V) and where they stand, falling; equal values (0.0 and
+    -0.0 are) by the lower token, NaN above every number. k up to 256. values keep the dtype; constants: no gradient flows to
+    `logits`."""
+    if logits.dim() < 1 or logits.shape[-1] < 1:
+        raise ValueError(f"top_logits: logits (..., vocabulary) expected, got {tuple(logits.shape)}")
+    if not 1 <= k <= min(plain.MAX_TARGETS, logits.shape[-1]):
+        raise ValueError(f"top_logits: k={k} must be in [1, min({plain.MAX_TARGETS}, vocabulary {logits.shape[-1]})]")
+    logits = logits.detach()
+    if type(logits) in _PLAIN and logits.is_cuda and plain_eager():
+        return tuple(_top(logits, k))
+    _hip.require_gpu(logits, "top_logits")
+    values, tokens = torch.ops.dispatcher.top_logits(logits, k)
+    return values, tokens
+
+
+# ---------------------------------------------------------------------------------------------
+# distillation loss
+# ---------------------------------------------------------------------------------------------
+def _rows_of(logits):
+    """(tensor, stride_b, stride_t, B, T): the rows of logits (..., V) by two strides."""
+    V = logits.shape[-1]
+    z = _unit_rows(logits)
+    if z.dim() > 3:
+        z = _unit_rows(z.reshape(-1, V))
+    B, T = (1, z.shape[0]) if z.dim() == 2 else tuple(z.shape[:2]) if z.dim() == 3 else (1, 1)
+    sb, st = (0, z.stride(0)) if z.dim() == 2 else tuple(z.stride()[:2]) if z.dim() == 3 else (0, 0)
+    return z, sb, st, B, T
+
+
+def _distill_args(logits, teacher_logits, teacher_tokens, labels, temperature, weight, ignore_index):
+    """The arguments both directions share, and the tensors they point to (held until the launch)."""
+    z, sb, st, B, T = _rows_of(logits)
+    tl, tt = teacher_logits.contiguous(), teacher_tokens.contiguous()
+    lb = None if labels is None else labels.contiguous()
+    p = _hip.ptr
+    return (_hip.dtype_code(z.dtype), p(z), sb, st, B, max(T, 1) if B * T else 1, z.shape[-1], _hip.dtype_code(tl.dtype), p(tl),
+            p(tt), _bits(tt), tl.shape[-1], p(lb), 64 if lb is None else _bits(lb), ignore_index, temperature,
+            weight), (z, tl, tt, lb)
+
+
+def _distill_fwd(logits, teacher_logits, teacher_tokens, labels, temperature, weight, ignore_index, reduction):
+    what = "distillation_loss"
+    _hip.same_gpu(what, logits, teacher_logits, teacher_tokens, labels)
+    dev, lead = logits.device, logits.shape[:-1]
+    n = lead.numel()
+    args, held = _distill_args(logits, teacher_logits, teacher_tokens, labels, temperature, weight, ignore_index)
+    if n == 0:
+        args = (*args[:4], 0, 1, *args[6:])
+    rows = torch.empty(lead, device=dev, dtype=torch.float32)
+    kept = torch.empty(n, 4, device=dev, dtype=torch.float32)
+    # (apart: the loss may be changed in place, and the backward pass reads the divisor)
+    loss, divisor = (torch.empty((), device=dev, dtype=torch.float32) if reduction else None for _ in range(2))
+    nbytes = _hip.lib.dh_distill_workspace_bytes(args[0], n, logits.shape[-1])
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    with _on(logits):
+        st = _hip.lib.dh_distill_fwd(*args, reduction, _hip.ptr(rows), _hip.ptr(kept), _hip.ptr(loss), _hip.ptr(divisor),
+                                     _hip.ptr(ws), nbytes, _hip.stream_handle(dev))
+    _hip.check(st, what)
+    return (rows, kept, None) if reduction == 0 else (loss, kept, divisor)
+
+
+def _distill_bwd(g, logits, teacher_logits, teacher_tokens, labels, kept, divisor, temperature, weight, ignore_index, reduction):
+    what = "distillation_loss gradient"
+    _hip.same_gpu(what, logits, g, teacher_logits, teacher_tokens, labels, kept, divisor)
+    dz = torch.empty(logits.shape, device=logits.device, dtype=logits.dtype)
+    if dz.numel() == 0:
+        return dz
+    args, held = _distill_args(logits, teacher_logits, teacher_tokens, labels, temperature, weight, ignore_index)
+    g = g.float().reshape(-1)
+    kept = kept.contiguous()                                                   # (a saved-tensor hook may change the layout)
+    with _on(logits):
+        st = _hip.lib.dh_distill_bwd(*args, _hip.ptr(kept), _hip.ptr(g), g.stride(0) if reduction == 0 else 0,
+                                     _hip.ptr(divisor), _hip.ptr(dz), _hip.stream_handle(logits.device))
+    _hip.check(st, what)
+    return dz
+
+
+@torch.library.custom_op("dispatcher::distillation_loss", mutates_args=(), device_types="cuda")
+def _distill_op(logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_tokens: torch.Tensor,
+                labels: Optional[torch.Tensor], temperature: float, weight: float, ignore_index: int,
+                reduction: int) -> List[torch.Tensor]:
+    loss, kept, divisor = _distill_fwd(logits, teacher_logits, teacher_tokens, labels, temperature, weight, ignore_index,
+                                       reduction)
+    return [loss, kept, loss.new_empty(0) if divisor is None else divisor]
+
+
+@_distill_op.register_fake
+def _(logits, teacher_logits, teacher_tokens, labels, temperature, weight, ignore_index, reduction):
+    f32 = torch.float32
+    lead = logits.shape[:-1]
+    n = 1
+    for s in lead:
+        n = n * s
+    return [logits.new_empty(lead if reduction == 0 else (), dtype=f32), logits.new_empty((n, 4), dtype=f32),
+            logits.new_empty((0,) if reduction == 0 else (), dtype=f32)]
+
+
+@torch.library.custom_op("dispatcher::distillation_loss_grad", mutates_args=(), device_types="cuda")
+def _distill_grad_op(g: torch.Tensor, logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_tokens: torch.Tensor,
+                     labels: Optional[torch.Tensor], kept: torch.Tensor, divisor: torch.Tensor, temperature: float,
+                     weight: float, ignore_index: int, reduction: int) -> torch.Tensor:
+    return _distill_bwd(g, logits, teacher_logits, teacher_tokens, labels, kept, divisor if reduction else None, temperature,
+                        weight, ignore_index, reduction)
+
+
+@_distill_grad_op.register_fake
+def _(g, logits, teacher_logits, teacher_tokens, labels, kept, divisor, temperature, weight, ignore_index, reduction):
+    return logits.new_empty(logits.shape)
+
+
+def _distill_setup(ctx, inputs, output):
+    logits, teacher_logits, teacher_tokens, labels, *args = inputs
+    _, kept, divisor = output
+    ctx.set_materialize_grads(False)
+    ctx.save_for_backward(logits, teacher_logits, teacher_tokens, labels, kept, divisor)
+    ctx.args = tuple(args)
+
+
+def _again(ctx, g):
+    """The gradient in the logits from the formula as torch operations, differentiable itself (create_graph)."""
+    logits, teacher_logits, teacher_tokens, labels, _, _ = ctx.saved_tensors
+    temperature, weight, ignore_index, reduction = ctx.args
+    z = logits.view_as(logits)
+    loss = plain.distillation_loss(z, teacher_logits, teacher_tokens, labels, temperature, weight, ignore_index,
+                                   plain.REDUCTIONS[reduction])
+    return torch.autograd.grad(loss, z, g, create_graph=True)[0]
+
+
+def _distill_backward(ctx, grads):
+    if grads[0] is None:
+        return (None,) * 8
+    if torch.is_grad_enabled():
+        return (_again(ctx, grads[0]), *(None,) * 7)
+    return (torch.ops.dispatcher.distillation_loss_grad(grads[0], *ctx.saved_tensors, *ctx.args), *(None,) * 7)
+
+
+torch.library.register_autograd("dispatcher::distillation_loss", _distill_backward, setup_context=_distill_setup)
+
+
+class _Distill(torch.autograd.Function):
+    """dispatcher::distillation_loss without the registered operation's per-call bookkeeping."""
+
+    @staticmethod
+    def forward(ctx, *inputs):
+        output = _distill_fwd(*inputs)
+        _distill_setup(ctx, inputs, output)
+        return output[0]
+
+    @staticmethod
+    def backward(ctx, g):
+        if g is None:
+            return (None,) * 8
+        if torch.is_grad_enabled():
+            return (_again(ctx, g), *(None,) * 7)
+        return (_distill_bwd(g, *ctx.saved_tensors, *ctx.args), *(None,) * 7)
+
+
+def distillation_loss(logits, teacher_logits, teacher_tokens, labels=None, temperature=1.0, weight=1.0, ignore_index=-100,
+                      reduction="mean"):
+    """Distillation from a teacher's top logits, differentiable in `logits`; a scalar, or (reduction="none") the positions'
+    losses, fp32.
+
+    logits (..., V) fp32 or bf16; teacher_logits, teacher_tokens (..., k) as top_logits gives them (fp32 or bf16, int32 or
+    int64; k up to 256), a slot with a token below 0 or a logit of -inf being empty; labels (...) int32 or int64, or None.
+    Per position, with p the softmax of the teacher's live logits over the temperature and q that of `logits`,
+
+        weight * temperature^2 * sum_j p_j (log p_j - log q_j)  +  (1 - weight) * cross-entropy of the label
+
+    without the first term where every slot is empty. weight < 1 needs labels. A position whose label is ignore_index counts
+    for nothing: no loss, a gradient of zeros, whatever its logits hold. reduction: "mean" over the other positions (NaN when
+    there is none, as the cross-entropy's mean), "sum" or "none". A teacher token past the vocabulary, or a label outside it,
+    makes its position's loss and gradient NaN. The teacher's logits are constants."""
+    plain.check_targets(logits, teacher_logits, teacher_tokens, labels, temperature, weight, reduction)
+    args = (logits, teacher_logits, teacher_tokens, labels, float(temperature), float(weight), int(ignore_index),
+            _REDUCTION[reduction])
+    if type(logits) in _PLAIN and logits.is_cuda and plain_eager():
+        return _Distill.apply(*args)
+    _hip.require_gpu(logits, "distillation_loss")
+    return torch.ops.dispatcher.distillation_loss(*args)[0]

@@ -28,6 +28,7 @@ from transformers import PreTrainedModel
 from transformers.generation import GenerationMixin
 from transformers.modeling_outputs import CausalLMOutput
 
+from . import distillation
 from .configuration_dispatcher import DispatcherConfig
 
 
@@ -480,7 +481,15 @@ class DispatcherHybridForCausalLM(DispatcherPreTrainedModel, GenerationMixin):
 
     def forward(self, input_ids=None, attention_mask=None, labels=None, inputs_embeds=None,
                 use_cache=None, output_attentions=None, output_hidden_states=None,
-                return_dict=None, **kwargs):
+                return_dict=None, teacher_logits=None, teacher_tokens=None, distill_temperature=1.0,
+                distill_weight=1.0, **kwargs):
+        """labels (B, T): the loss is the mean cross-entropy of the next tokens (-100: ignored).
+
+        teacher_logits, teacher_tokens (B, T, k), as teacher_targets gives them for the same tokens: the loss is the
+        mean over the positions of distill_weight times the distillation loss at distill_temperature plus
+        (1 - distill_weight) times the cross-entropy of the next token (distillation.py). With labels, positions
+        without a next token or whose next token is -100 count for nothing; without, every position counts and
+        distill_weight must be 1."""
         if input_ids is None:
             raise ValueError("DispatcherHybridForCausalLM requires input_ids "
                              "(the tree mask is built from token identities)")
@@ -488,9 +497,11 @@ class DispatcherHybridForCausalLM(DispatcherPreTrainedModel, GenerationMixin):
         length = input_ids.size(1)
         if length > self.config.max_len:
             raise ValueError(f"sequence length {length} exceeds max_len {self.config.max_len}")
+        if (teacher_logits is None) != (teacher_tokens is None):
+            raise ValueError("teacher_logits and teacher_tokens come together")
         mask = self._tree_mask(input_ids, length)
         hidden_states = () if output_hidden_states else None
-        x = self.embedding(input_ids)
+        x = self._embed(input_ids)
         if self._fused_norm_ok(x, output_hidden_states):
             x = self._blocks_fused_norms(x, mask)
         else:
@@ -506,12 +517,57 @@ class DispatcherHybridForCausalLM(DispatcherPreTrainedModel, GenerationMixin):
             hidden_states = hidden_states + (x,)
         logits = self.lm_head(x)
         loss = None
-        if labels is not None:
+        if teacher_logits is not None:
+            loss = self._distillation_loss(logits, teacher_logits, teacher_tokens, labels, distill_temperature,
+                                           distill_weight)
+        elif labels is not None:
             loss = F.cross_entropy(logits[:, :-1].reshape(-1, logits.size(-1)),
                                    labels[:, 1:].reshape(-1))
         if not return_dict:
             return (loss, logits) if loss is not None else (logits,)
         return CausalLMOutput(loss=loss, logits=logits, hidden_states=hidden_states)
+
+    def _embed(self, input_ids):
+        if getattr(self, "_fused_vocab", False):
+            from .fused_vocab import embed_tokens, embedding_fits
+            if embedding_fits(self.embedding):
+                return embed_tokens(input_ids, self.embedding.weight, padding_idx=self.embedding.padding_idx)
+        return self.embedding(input_ids)
+
+    def _distillation_loss(self, logits, teacher_logits, teacher_tokens, labels, temperature, weight):
+        # the logits stay whole and the labels move instead: a slice of the logits costs a copy of them, and another
+        # one of their gradient
+        if labels is not None:
+            labels = F.pad(labels[:, 1:], (0, 1), value=-100)
+        loss = distillation.distillation_loss
+        if getattr(self, "_fused_vocab", False):
+            if not logits.is_cuda:
+                raise RuntimeError("the fused loss is enabled but the logits are on the CPU; move the model to the GPU "
+                                   "or call enable_fused_vocab(False)")
+            from .fused_vocab import distillation_loss as loss
+        return loss(logits, teacher_logits, teacher_tokens, labels, temperature, weight)
+
+    @torch.no_grad()
+    def teacher_targets(self, input_ids, k):
+        """The targets this model sets a student: the k largest logits of every position and their tokens, (values,
+        tokens), each (B, T, k), falling; equal logits by the lower token."""
+        logits = self(input_ids).logits
+        if getattr(self, "_fused_vocab", False) and logits.is_cuda:
+            from .fused_vocab import top_logits
+            return top_logits(logits, k)
+        return distillation.top_logits(logits, k)
+
+    def enable_fused_vocab(self, enabled=True):
+        """Run the vocabulary's ends of training on the gfx950 kernels: the embedding rows and their gradient
+        (dh_embed_fwd / dh_embed_bwd, while nothing stands around the embedding), the distillation loss and its gradient
+        (dh_distill_fwd / dh_distill_bwd) and teacher_targets (dh_top_logits). Independent of enable_fused_gates.
+
+        Loads the kernel library now (raising ImportError if it is missing). fp32 and bf16 on the GPU; returns self.
+        """
+        if enabled:
+            from . import fused_vocab  # noqa: F401  (fail now, not mid-forward)
+        self._fused_vocab = bool(enabled)
+        return self
 
     def prepare_inputs_for_generation(self, input_ids, **kwargs):
         return {"input_ids": input_ids[:, -self.config.max_len:]}

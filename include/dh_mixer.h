@@ -29,7 +29,7 @@
 extern "C" {
 #endif
 
-#define DH_ABI_VERSION 20
+#define DH_ABI_VERSION 21
 
 enum dh_status {
   DH_OK = 0,
@@ -562,6 +562,69 @@ int dh_decode_persistent_phases(const int* kinds, int n_layers);
 /* status words of the last persistent steps on `scratch`: out2[0] non-zero after a timeout,
  * out2[1] the first failing phase + 1 (synchronises the stream) */
 int dh_decode_persistent_status(const void* scratch, uint32_t* out2, void* stream);
+
+/*
+ * Embedding rows: out[n] = scale * W[ids[n]], rounded once. The parallel forward's lookup (reference
+ * dispatcher_hybrid/modeling_dispatcher.py:340).
+ *   W (V, d) rows ldw apart; out (n, d) rows ldo apart; any d (rows that start on 16-byte boundaries with d * size a
+ *   multiple of 16 move in 16-byte pieces). ids: n integers of ids_bits (32 or 64) bits. An id outside [0, V) gives a row of
+ *   NaN and is not read; positions that hold zero_token (-1: none) give a row of zeros.
+ *   Limits of both: n < 2^24, V <= 2^24, d <= 2^20.
+ */
+int dh_embed_fwd(int dtype, const void* W, int64_t ldw, int64_t V, int d, const void* ids, int ids_bits, int64_t n,
+                 float scale, int64_t zero_token, void* out, int64_t ldo, void* stream);
+/*
+ * The lookup's gradient: dW[v] = scale * sum of dy[n] over the positions n with ids[n] = v, ascending, for every v (rows of
+ * zeros where there is none): fp32 sums in an order that depends on the ids alone, rounded once. Positions that hold
+ * skip_token (-1: none) or an id outside [0, V) are left out. dy (n, d) rows ldy apart; dW (V, d) contiguous.
+ *   workspace: dh_embed_bwd_workspace_bytes(n, V, d) bytes (-1: sizes outside the limits), 16-byte aligned; contents are
+ *   needed during the call only.
+ */
+int64_t dh_embed_bwd_workspace_bytes(int64_t n, int64_t V, int d);
+int dh_embed_bwd(int dtype, const void* dy, int64_t ldy, const void* ids, int ids_bits, int64_t n, int64_t V, int d,
+                 float scale, int64_t skip_token, void* dW, void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * The K largest logits of every row, falling, and their tokens; equal values (0.0 and -0.0 are) by the lower token, NaN above
+ * every number. logits (rows, V) of unit stride, rows row_stride apart (any alignment to elements); values (rows, K) of
+ * `dtype` and tokens (rows, K), contiguous. 1 <= K <= min(256, V), V <= 2^24, rows < 2^22. No counterpart in the reference.
+ */
+int dh_top_logits(int dtype, const void* logits, int64_t row_stride, int64_t rows, int V, int K, void* values,
+                  int64_t* tokens, void* stream);
+
+/*
+ * Distillation from a teacher's top logits; no counterpart in the reference. Row r = b * T + t of the student's logits z (V
+ * of unit stride at b * stride_b + t * stride_t), K teacher logits t_j at tokens k_j, temperature tau, weight w, label y:
+ *   p = softmax of t / tau over the live slots (k_j >= 0 and t_j > -inf), q = softmax(z / tau), P = softmax(z)
+ *   row_loss[r] = w tau^2 sum_j p_j (log p_j - log q_{k_j}) - (1 - w) log P_y
+ * A row without live slots has no first term; with labels, a row whose label is ignore_index has loss 0 and is not read; a
+ * teacher token past the vocabulary, or another label outside it, makes its row NaN. The sums over V are fp32, a row's few
+ * other operations fp64.
+ *   teacher_logits (B * T, K) of teacher_dtype; teacher_tokens (B * T, K) of token_bits (32 or 64) bits; labels (B * T) of
+ *   label_bits bits, null: none (weight must be 1). All contiguous.
+ *   reduction 0: rows only (loss, divisor unused); 1: loss = the mean over the rows that are not ignored (NaN if there is
+ *   none), divisor = their number; 2: loss = the sum, divisor = 1. row_loss (B * T) fp32; row_kept: 16 bytes a row, 16-byte
+ *   aligned, for the backward pass; loss, divisor: one fp32 each.
+ *   workspace: dh_distill_workspace_bytes(dtype, B * T, V) bytes (0 for many rows), needed during the call only.
+ *   1 <= K <= 256, V <= 2^24, B * T < 2^22, 0 < tau, 0 <= w <= 1.
+ */
+int64_t dh_distill_workspace_bytes(int dtype, int64_t rows, int V);
+int dh_distill_fwd(int dtype, const void* logits, int64_t stride_b, int64_t stride_t, int64_t B, int T, int V,
+                   int teacher_dtype, const void* teacher_logits, const void* teacher_tokens, int token_bits, int K,
+                   const void* labels, int label_bits, int64_t ignore_index, float temperature, float weight, int reduction,
+                   float* row_loss, void* row_kept, float* loss, float* divisor, void* workspace, int64_t workspace_bytes,
+                   void* stream);
+/*
+ * Its gradient in z: dlogits (B * T, V) contiguous, every element written,
+ *   dz_v = g (w tau (q_v - sum_{j: k_j = v} p_j) + (1 - w) (P_v - [v = y])),   zeros where the row is ignored,
+ * with g = dloss[r * dloss_stride] / *divisor (divisor null: 1). dloss fp32 on the device: stride 0 for one value. The other
+ * arguments are the forward call's; row_kept as it wrote it.
+ */
+int dh_distill_bwd(int dtype, const void* logits, int64_t stride_b, int64_t stride_t, int64_t B, int T, int V,
+                   int teacher_dtype, const void* teacher_logits, const void* teacher_tokens, int token_bits, int K,
+                   const void* labels, int label_bits, int64_t ignore_index, float temperature, float weight,
+                   const void* row_kept, const float* dloss, int64_t dloss_stride, const float* divisor, void* dlogits,
+                   void* stream);
 
 #ifdef __cplusplus
 }
