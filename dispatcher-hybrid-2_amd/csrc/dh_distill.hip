@@ -9,8 +9,8 @@
 // Forward: one pass over the row with the running maximum m and the sums of exp((z - m) / tau) and exp(z - m) (one sum where
 // the two are equal or only one is used); the read of z bounds it. Few rows are split over several workgroups, whose sums
 // are joined by a second launch. Backward: z once more, and dz; q and P come from m and the sums the forward kept. The
-// tokens that the teacher or the label names are written again after the row, in full fp32, by one thread each, so that
-// a token named twice is the sum of its slots in a fixed order.
+// tokens that the teacher or the label names are written again after the row, from fp32, by a wave that has them ready by then;
+// a token named twice gets the sum of its slots in their order.
 //
 // Exponents are taken of z - m (exact for bf16 inputs near m), never of z times a constant: rows of the type's lowest value
 // stay finite. The few operations on a row's sums are in fp64: log p - log q is a small difference of larger numbers.
@@ -19,7 +19,7 @@
 
 namespace {
 
-constexpr int kT = 256;                    // threads of a row (or of its part)
+constexpr int kT = 256;                    // threads that read a row (or its part); one more wave takes the named tokens
 constexpr int kW = kT / 64;
 constexpr int kMaxSlots = 256;
 constexpr int kSlotsPerLane = kMaxSlots / 64;
@@ -84,6 +84,7 @@ struct Rows {
   int64_t ignore;
   int t_bf16, token_wide, label_wide, K;
   float tau, weight;
+  double inv_tau;
   int soft, hard;                          // which terms there are
 };
 
@@ -104,6 +105,11 @@ struct Kept {
   int terms;                               // bit 0: the row counts, bit 1: it has live slots
 };
 
+// How the two sums of exponentials are had: one alone (only one term, or tau = 1), both, or, where tau is 2 or 4, the
+// second from powers of the first's terms: exp(z - m) = exp((z - m) / tau)^tau in one or two products in place of an exp,
+// which takes as long as four (forward of 4096 x 50257 bf16: ALUWAS us).
+enum Mode { kOne = 1, kTwo = 2, kSquare = 3, kFourth = 4 };
+
 struct Sums {
   float m, s0, s1;                         // s0: of exp((z - m) c0), s1: of exp((z - m) c1), c as in scales()
 };
@@ -112,26 +118,41 @@ __device__ __forceinline__ void scales(const Rows& a, float& c0, float& c1) {
   c0 = a.soft ? kLog2e / a.tau : kLog2e;
   c1 = kLog2e;
 }
-template <int NS>
+template <int M> __device__ __forceinline__ float second(float e, float d, float c1) {
+  if (M == kSquare) return e * e;
+  if (M == kFourth) {
+    const float f = e * e;
+    return f * f;
+  }
+  return exp2_hw(d * c1);
+}
+template <int M>
 __device__ __forceinline__ Sums join(const Sums& a, const Sums& b, float c0, float c1) {
   Sums r;
   r.m = fmaxf(a.m, b.m);
   const float ref = finite_ref(r.m);
   r.s0 = a.s0 * exp2_hw((a.m - ref) * c0) + b.s0 * exp2_hw((b.m - ref) * c0);
-  r.s1 = NS == 2 ? a.s1 * exp2_hw((a.m - ref) * c1) + b.s1 * exp2_hw((b.m - ref) * c1) : 0.f;
+  r.s1 = M != kOne ? a.s1 * exp2_hw((a.m - ref) * c1) + b.s1 * exp2_hw((b.m - ref) * c1) : 0.f;
   return r;
 }
-template <int NS>
+template <int M>
 __device__ __forceinline__ Sums wave_join(Sums v, float c0, float c1) {
   const float m = wave_max(v.m), ref = finite_ref(m);
   v.s0 = wave_sum(v.s0 * exp2_hw((v.m - ref) * c0));
-  v.s1 = NS == 2 ? wave_sum(v.s1 * exp2_hw((v.m - ref) * c1)) : 0.f;
+  v.s1 = M != kOne ? wave_sum(v.s1 * exp2_hw((v.m - ref) * c1)) : 0.f;
   v.m = m;
   return v;
 }
 
-// The teacher's probabilities of a row, in one wave: slot lane + 64 i of p[i], its token (-1: empty) and (t_j - max) / tau.
-// Returns log of their sum, or sets live to false; bad: a token past the vocabulary.
+// log of a sum: the exponent in fp64, the logarithm of the rest (at most ln 2 in size) in fp32
+__device__ __forceinline__ double log_sum(float s) {
+  int e;
+  const float f = frexpf(s, &e);
+  return isfinite(s) ? (double)e * kLn2 + (double)logf(f) : (double)s;         // (log 0 = -inf + 0)
+}
+
+// The teacher's probabilities of a row, by one wave: slot lane + 64 i in p[i], token[i] (-1: empty) and t[i]. Returns the log
+// of the sum of exp((t - top) / tau); live: there is a slot that is not empty; bad: a token past the vocabulary.
 __device__ __forceinline__ double teacher_row(const Rows& a, int64_t r, int lane, float (&p)[kSlotsPerLane],
                                               int (&token)[kSlotsPerLane], float (&t)[kSlotsPerLane], float& top, bool& live,
                                               bool& bad) {
@@ -168,111 +189,158 @@ __device__ __forceinline__ double teacher_row(const Rows& a, int64_t r, int lane
   s = wave_sum(s);
 #pragma unroll
   for (int i = 0; i < kSlotsPerLane; ++i) p[i] = token[i] >= 0 ? p[i] / s : 0.f;
-  return live ? log((double)s) : 0.0;
+  return live ? log_sum(s) : 0.0;
 }
 
-// the row's loss and what the backward pass keeps, by one wave
+// What a row's loss needs of the logits that are named, without the sums over the vocabulary: the wave beside those that read
+// the row has it by the time they end.
+struct Named {
+  double cross, mass;                      // sum_j p_j (log p_j - (z_{k_j} - ref) / tau), sum_j p_j
+  float ref;                               // the largest of those z: near the row's own maximum, or as far below it as all
+  float label;                             // the label's logit
+  int terms;                               // bit 0: the row counts, bit 1: it has live slots, bit 2: out of the vocabulary
+};
+
+__device__ __forceinline__ bool counted(const Rows& a, int64_t r) {
+  return !a.labels || whole(a.labels, a.label_wide, r) != a.ignore;
+}
+
 template <typename T>
-__device__ __forceinline__ void finish_row(const Rows& a, int64_t r, const Sums& v, int lane, float* losses, Kept* kept) {
+__device__ __forceinline__ Named named_of(const Rows& a, int64_t r, int lane) {
   const T* z = row_of<T>(a, r);
-  const int64_t label = a.labels ? whole(a.labels, a.label_wide, r) : 0;
-  const bool counts = !a.labels || label != a.ignore;
-  const double s1 = a.hard && a.soft && a.tau != 1.f ? v.s1 : v.s0;
-  double row = 0.0;
+  Named n{0.0, 0.0, 0.f, 0.f, 1};
   bool live = false, bad = false;
-  if (counts) {                            // uniform
-    if (a.soft) {
-      float p[kSlotsPerLane], t[kSlotsPerLane], top;
-      int token[kSlotsPerLane];
-      const double lt = teacher_row(a, r, lane, p, token, t, top, live, bad);
-      const double lz = log((double)v.s0);
-      double sum = 0.0;
+  if (a.labels) {
+    const int64_t label = whole(a.labels, a.label_wide, r);
+    bad = label < 0 || label >= a.V;
+    if (a.hard && !bad) n.label = Elem<T>::load(z + label);
+  }
+  if (a.soft) {
+    float p[kSlotsPerLane], t[kSlotsPerLane], top;
+    int token[kSlotsPerLane];
+    bool over;
+    const double lt = teacher_row(a, r, lane, p, token, t, top, live, over);
+    bad |= over;
+    float x[kSlotsPerLane], most = -INFINITY;
 #pragma unroll
-      for (int i = 0; i < kSlotsPerLane; ++i)
-        if (token[i] >= 0 && !(p[i] == 0.f)) {
-          const double log_p = ((double)t[i] - (double)top) / (double)a.tau - lt;
-          const double log_q = ((double)Elem<T>::load(z + token[i]) - (double)v.m) / (double)a.tau - lz;
-          sum += (double)p[i] * (log_p - log_q);
-        }
-      row = (double)a.weight * (double)a.tau * (double)a.tau * wave_sum64(sum);
+    for (int i = 0; i < kSlotsPerLane; ++i) {
+      if (p[i] == 0.f) token[i] = -1;      // (0 log 0 = 0)
+      x[i] = token[i] >= 0 ? Elem<T>::load(z + token[i]) : -INFINITY;
+      most = fmaxf(most, x[i]);
     }
-    if (a.labels && (label < 0 || label >= a.V)) bad = true;
-    if (a.hard && !bad)
-      row += (1.0 - (double)a.weight) * (log(s1) - ((double)Elem<T>::load(z + label) - (double)v.m));
-    if (bad) row = __builtin_nan("");
+    n.ref = finite_ref(wave_max(most));
+    double cross = 0.0, mass = 0.0;
+#pragma unroll
+    for (int i = 0; i < kSlotsPerLane; ++i)
+      if (token[i] >= 0) {
+        const double log_p = ((double)t[i] - (double)top) * a.inv_tau - lt;
+        cross += (double)p[i] * (log_p - ((double)x[i] - (double)n.ref) * a.inv_tau);
+        mass += (double)p[i];
+      }
+    n.cross = wave_sum64(cross);
+    n.mass = wave_sum64(mass);
   }
-  if (lane == 0) {
-    losses[r] = (float)row;
-    const float nan = __builtin_nanf("");
-    kept[r] = Kept{v.m, bad ? nan : 1.f / v.s0, bad ? nan : (float)(1.0 / s1), (counts ? 1 : 0) | (live || bad ? 2 : 0)};
-  }
+  n.terms |= (live ? 2 : 0) | (bad ? 4 : 0);
+  return n;
+}
+
+// the loss of a row that counts, and what the backward pass keeps of it, by one thread
+__device__ __forceinline__ void finish_row(const Rows& a, int64_t r, const Sums& v, const Named& n, float* losses, Kept* kept) {
+  const float s1 = a.hard && a.soft && a.tau != 1.f ? v.s1 : v.s0;
+  const bool live = n.terms & 2, bad = n.terms & 4;
+  double row = 0.0;
+  if (a.soft && live)
+    row = (double)a.weight * (double)a.tau * (double)a.tau *
+          (n.cross + n.mass * (((double)v.m - (double)n.ref) * a.inv_tau + log_sum(v.s0)));
+  if (a.hard) row += (1.0 - (double)a.weight) * (log_sum(s1) - ((double)n.label - (double)v.m));
+  const float nan = __builtin_nanf("");
+  losses[r] = bad ? nan : (float)row;
+  kept[r] = Kept{v.m, bad ? nan : 1.f / v.s0, bad ? nan : 1.f / s1, 1 | (live || bad ? 2 : 0)};
 }
 
 // ---- forward: a row, or one of its parts ----------------------------------------------------------------------------
-template <typename T, int NS>
-__global__ __launch_bounds__(kT) void forward_kernel(Rows a, int parts, Sums* part, float* losses, Kept* kept) {
+template <typename T, int M>
+__global__ __launch_bounds__(kT + 64) void forward_kernel(Rows a, int parts, Sums* part, Named* named, float* losses,
+                                                          Kept* kept) {
   constexpr int E = kE<T>, U = 4;
   __shared__ Sums ws[kW];
+  __shared__ Named wn;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t r = blockIdx.x / parts;
   const int which = (int)(blockIdx.x % parts);
-  const T* z = row_of<T>(a, r);
+  if (!counted(a, r)) {                    // uniform: the row is not read
+    if (tid == 0 && which == 0) {
+      losses[r] = 0.f;
+      kept[r] = Kept{0.f, 0.f, 0.f, 0};
+    }
+    return;
+  }
   float c0, c1;
   scales(a, c0, c1);
-  // 16-byte pieces from the boundary at or below the row (a piece that holds an element of the row is mapped whole); what
-  // the first and last hold of others counts as -inf
-  const int mis = (int)((reinterpret_cast<uintptr_t>(z) & 15u) / sizeof(T));
-  const uint4* base = reinterpret_cast<const uint4*>(z - mis);
-  const int pieces = (mis + a.V + E - 1) / E, per = (pieces + parts - 1) / parts;
-  const int p0 = min(which * per, pieces), p1 = min(p0 + per, pieces);
-  const uint32_t none = sizeof(T) == 2 ? 0xff80ff80u : 0xff800000u;
-  Sums v{-INFINITY, 0.f, 0.f};
-  for (int p = p0 + tid; p < p1; p += kT * U) {
-    uint4 q[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      q[u] = make_uint4(none, none, none, none);
-      if (p + u * kT < p1) q[u] = base[p + u * kT];
-    }
-    float x[U][E];
-    float most = v.m;
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      unpack<T>(q[u], x[u]);
-      const int k = p + u * kT;
-      if (k == 0 || k == pieces - 1) {
-#pragma unroll
-        for (int j = 0; j < E; ++j)
-          if (k * E + j < mis || k * E + j >= mis + a.V) x[u][j] = -INFINITY;
+  if (wave == kW) {
+    if (which == 0) {
+      const Named n = named_of<T>(a, r, lane);
+      if (lane == 0) {
+        wn = n;
+        if (parts > 1) named[r] = n;
       }
-#pragma unroll
-      for (int j = 0; j < E; ++j) most = fmaxf(most, x[u][j]);
     }
-    const float ref = finite_ref(most);
-    v.s0 *= exp2_hw((v.m - ref) * c0);
-    if (NS == 2) v.s1 *= exp2_hw((v.m - ref) * c1);
-    v.m = most;
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-#pragma unroll
-      for (int j = 0; j < E; ++j) {
-        const float d = x[u][j] - ref;
-        v.s0 += exp2_hw(d * c0);
-        if (NS == 2) v.s1 += exp2_hw(d * c1);
-      }
-  }
-  v = wave_join<NS>(v, c0, c1);
-  if (lane == 0) ws[wave] = v;
-  __syncthreads();
-  if (wave) return;
-  v = ws[0];
-#pragma unroll
-  for (int w = 1; w < kW; ++w) v = join<NS>(v, ws[w], c0, c1);
-  if (parts > 1) {
-    if (lane == 0) part[blockIdx.x] = v;
   } else {
-    finish_row<T>(a, r, v, lane, losses, kept);
+    const T* z = row_of<T>(a, r);
+    // 16-byte pieces from the boundary at or below the row (a piece that holds an element of the row is mapped whole);
+    // what the first and last hold of others counts as -inf
+    const int mis = (int)((reinterpret_cast<uintptr_t>(z) & 15u) / sizeof(T));
+    const uint4* base = reinterpret_cast<const uint4*>(z - mis);
+    const int pieces = (mis + a.V + E - 1) / E, per = (pieces + parts - 1) / parts;
+    const int p0 = min(which * per, pieces), p1 = min(p0 + per, pieces);
+    const uint32_t none = sizeof(T) == 2 ? 0xff80ff80u : 0xff800000u;
+    Sums v{-INFINITY, 0.f, 0.f};
+    for (int p = p0 + tid; p < p1; p += kT * U) {
+      uint4 q[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        q[u] = make_uint4(none, none, none, none);
+        if (p + u * kT < p1) q[u] = base[p + u * kT];
+      }
+      float x[U][E];
+      float most = v.m;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        unpack<T>(q[u], x[u]);
+        const int k = p + u * kT;
+        if (k == 0 || k == pieces - 1) {
+#pragma unroll
+          for (int j = 0; j < E; ++j)
+            if (k * E + j < mis || k * E + j >= mis + a.V) x[u][j] = -INFINITY;
+        }
+#pragma unroll
+        for (int j = 0; j < E; ++j) most = fmaxf(most, x[u][j]);
+      }
+      const float ref = finite_ref(most);
+      v.s0 *= exp2_hw((v.m - ref) * c0);
+      if (M != kOne) v.s1 *= exp2_hw((v.m - ref) * c1);
+      v.m = most;
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int j = 0; j < E; ++j) {
+          const float d = x[u][j] - ref, e = exp2_hw(d * c0);
+          v.s0 += e;
+          if (M != kOne) v.s1 += second<M>(e, d, c1);
+        }
+    }
+    v = wave_join<M>(v, c0, c1);
+    if (lane == 0) ws[wave] = v;
   }
+  __syncthreads();
+  if (tid) return;
+  Sums v = ws[0];
+#pragma unroll
+  for (int w = 1; w < kW; ++w) v = join<M>(v, ws[w], c0, c1);
+  if (parts > 1)
+    part[blockIdx.x] = v;
+  else
+    finish_row(a, r, v, wn, losses, kept);
 }
 
 // the sum or mean of the rows in a fixed order, and its divisor, by one workgroup
@@ -307,18 +375,20 @@ __device__ __forceinline__ void reduce_rows(const float* losses, const Kept* kep
 constexpr int kRT = 1024;                  // threads of the reduction, and of the join that ends with it
 
 // rows split over workgroups: their sums joined, a wave a row; loss non-null: one workgroup, which reduces the rows too
-template <typename T, int NS>
-__global__ __launch_bounds__(kRT) void join_kernel(Rows a, int parts, const Sums* part, float* losses, Kept* kept, int mean,
-                                                   float* loss, float* divisor) {
+template <int M>
+__global__ __launch_bounds__(kRT) void join_kernel(Rows a, int parts, const Sums* part, const Named* named, float* losses,
+                                                   Kept* kept, int mean, float* loss, float* divisor) {
   __shared__ double red[kRT / 64];
   __shared__ int cnt[kRT / 64];
   const int lane = threadIdx.x & 63, W = blockDim.x >> 6;
   float c0, c1;
   scales(a, c0, c1);
   for (int64_t r = (int64_t)blockIdx.x * W + (threadIdx.x >> 6); r < a.rows; r += (int64_t)gridDim.x * W) {
+    if (!counted(a, r)) continue;          // uniform; the first launch wrote it
     Sums v{-INFINITY, 0.f, 0.f};
     if (lane < parts) v = part[r * parts + lane];
-    finish_row<T>(a, r, wave_join<NS>(v, c0, c1), lane, losses, kept);
+    v = wave_join<M>(v, c0, c1);
+    if (lane == 0) finish_row(a, r, v, named[r], losses, kept);
   }
   if (!loss) return;
   __syncthreads();
@@ -333,14 +403,15 @@ __global__ __launch_bounds__(kRT) void reduce_kernel(const float* losses, const 
 }
 
 // ---- backward -------------------------------------------------------------------------------------------------------
-template <typename T, int NS>
-__global__ __launch_bounds__(kT) void backward_kernel(Rows a, int parts, const Kept* kept, const float* dloss,
-                                                      int64_t dloss_stride, const float* divisor, T* dz) {
+// Rows in descending order: the forward pass read the last rows last, and what the caches still hold of them is read first.
+template <typename T, int M>
+__global__ __launch_bounds__(kT + 64) void backward_kernel(Rows a, int parts, const Kept* kept, const float* dloss,
+                                                           int64_t dloss_stride, const float* divisor, T* dz) {
   constexpr int E = kE<T>, U = 2;
   __shared__ float sp[kMaxSlots];
   __shared__ int stok[kMaxSlots];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int64_t r = blockIdx.x / parts;
+  const int64_t r = a.rows - 1 - blockIdx.x / parts;
   const int which = (int)(blockIdx.x % parts);
   const T* z = row_of<T>(a, r);
   T* out = dz + r * a.V;
@@ -350,68 +421,97 @@ __global__ __launch_bounds__(kT) void backward_kernel(Rows a, int parts, const K
   const int p0 = min(which * per, pieces), p1 = min(p0 + per, pieces);
   const Kept k = kept[r];
   const bool counts = k.terms & 1, soft = counts && a.soft && (k.terms & 2), hard = counts && a.hard;
+  if (!soft && !hard) {                    // uniform: no gradient, whatever the row holds
+    for (int p = p0 + tid; p < p1; p += kT + 64) {
+      const int i = p * E - mis;
+      if (i >= 0 && i + E <= a.V)
+        *reinterpret_cast<uint4*>(out + i) = make_uint4(0u, 0u, 0u, 0u);
+      else
+        for (int j = max(i, 0); j < min(i + E, a.V); ++j) Elem<T>::store(out + j, 0.f);
+    }
+    return;
+  }
   const float g = dloss[dloss_stride * r] / (divisor ? *divisor : 1.f);
   const float gs = soft ? g * a.weight * a.tau : 0.f, gh = hard ? g * (1.f - a.weight) : 0.f;
   float c0, c1;
   scales(a, c0, c1);
   // dz of a logit without the teacher's and the label's part: f0 exp((z - m) c0) + f1 exp((z - m) c1)
   const float ref = finite_ref(k.m);
-  const float f0 = NS == 2 ? gs * k.inv_soft : (gs + gh) * k.inv_soft, f1 = gh * k.inv_hard;
-  const bool use0 = NS == 2 ? soft : soft || hard, use1 = NS == 2 && hard;
+  const float f0 = M != kOne ? gs * k.inv_soft : (gs + gh) * k.inv_soft, f1 = gh * k.inv_hard;
+  const bool use0 = M == kOne || soft;     // (a row without live slots has no soft term, and 0 * inf none either)
   auto value = [&](float x) {
-    const float d = x - ref;
-    float y = 0.f;
-    if (use0) y = f0 * exp2_hw(d * c0);
-    if (use1) y += f1 * exp2_hw(d * c1);
+    const float d = x - ref, e = exp2_hw(d * c0);
+    float y = use0 ? f0 * e : 0.f;
+    if (M != kOne) y += f1 * second<M>(e, d, c1);
     return y;
   };
-  if (soft && wave == 0) {
+  // the named tokens of this part, by the wave beside those that write it: slots lane + 64 i, the label behind them
+  const int K = soft ? a.K : 0;
+  float y[kSlotsPerLane + 1];
+  int64_t at[kSlotsPerLane + 1];
+  if (wave == kW) {
+    const int64_t label = hard ? whole(a.labels, a.label_wide, r) : -1;
+    const int lo = max(p0 * E - mis, 0), hi = min(p1 * E - mis, a.V);
     float p[kSlotsPerLane], t[kSlotsPerLane], top;
     int token[kSlotsPerLane];
-    bool live, bad;
-    teacher_row(a, r, lane, p, token, t, top, live, bad);
-#pragma unroll
-    for (int i = 0; i < kSlotsPerLane; ++i) {
-      sp[i * 64 + lane] = p[i];
-      stok[i * 64 + lane] = token[i];
-    }
-  }
-  for (int p = p0 + tid; p < p1; p += kT * U) {
-    uint4 q[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int i = (p + u * kT) * E - mis;
-      if (p + u * kT < p1 && i >= 0 && i + E <= a.V) q[u] = load16(z + i);
+    if (soft) {
+      bool live, bad;
+      teacher_row(a, r, lane, p, token, t, top, live, bad);
     }
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int i = (p + u * kT) * E - mis;
-      if (p + u * kT >= p1) break;
-      if (i >= 0 && i + E <= a.V) {
-        float x[E];
-        unpack<T>(q[u], x);
+    for (int i = 0; i <= kSlotsPerLane; ++i) {
+      at[i] = i == kSlotsPerLane ? (lane == 0 ? label : -1) : soft ? token[i] : -1;
+      if (at[i] < lo || at[i] >= hi) at[i] = -1;
+      y[i] = at[i] >= 0 ? Elem<T>::load(z + at[i]) : 0.f;
+      if (i < kSlotsPerLane && soft) {
+        sp[i * 64 + lane] = p[i];
+        stok[i * 64 + lane] = token[i];
+      }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    float sum[kSlotsPerLane + 1];
 #pragma unroll
-        for (int j = 0; j < E; ++j) x[j] = value(x[j]);
-        *reinterpret_cast<uint4*>(out + i) = pack<T>(x);
-      } else {
-        for (int j = max(i, 0); j < min(i + E, a.V); ++j) Elem<T>::store(out + j, value(Elem<T>::load(z + j)));
+    for (int i = 0; i <= kSlotsPerLane; ++i) sum[i] = 0.f;
+    for (int j = 0; j < K; ++j) {
+      const int v = stok[j];
+      const float q = sp[j];
+#pragma unroll
+      for (int i = 0; i <= kSlotsPerLane; ++i) sum[i] += at[i] == v ? q : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i <= kSlotsPerLane; ++i) {
+      y[i] = value(y[i]) - gs * sum[i];
+      if (at[i] == label) y[i] -= gh;
+    }
+  } else {
+    for (int p = p0 + tid; p < p1; p += kT * U) {
+      uint4 q[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int i = (p + u * kT) * E - mis;
+        if (p + u * kT < p1 && i >= 0 && i + E <= a.V) q[u] = load16(z + i);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int i = (p + u * kT) * E - mis;
+        if (p + u * kT >= p1) break;
+        if (i >= 0 && i + E <= a.V) {
+          float x[E];
+          unpack<T>(q[u], x);
+#pragma unroll
+          for (int j = 0; j < E; ++j) x[j] = value(x[j]);
+          *reinterpret_cast<uint4*>(out + i) = pack<T>(x);
+        } else {
+          for (int j = max(i, 0); j < min(i + E, a.V); ++j) Elem<T>::store(out + j, value(Elem<T>::load(z + j)));
+        }
       }
     }
   }
-  if (!soft && !hard) return;              // uniform
   __syncthreads();
-  // the named tokens of this part, the label behind the slots
-  const int64_t label = hard ? whole(a.labels, a.label_wide, r) : -1;
-  const int lo = max(p0 * E - mis, 0), hi = min(p1 * E - mis, a.V);
-  const int K = soft ? a.K : 0;
-  for (int j = tid; j <= K; j += kT) {
-    const int64_t v = j < K ? stok[j] : label;
-    if (v < lo || v >= hi) continue;
-    float p = 0.f;
-    for (int i = 0; i < K; ++i) p += stok[i] == v ? sp[i] : 0.f;
-    float y = value(Elem<T>::load(z + v)) - gs * p;
-    if (v == label) y -= gh;
-    Elem<T>::store(out + v, y);
+  if (wave == kW) {
+#pragma unroll
+    for (int i = 0; i <= kSlotsPerLane; ++i)
+      if (at[i] >= 0) Elem<T>::store(out + at[i], y[i]);
   }
 }
 
@@ -461,26 +561,32 @@ Rows rows_of(const void* logits, int64_t sb, int64_t st, int64_t B, int T, int V
   a.K = K;
   a.tau = tau;
   a.weight = weight;
+  a.inv_tau = 1.0 / (double)tau;
   a.soft = weight > 0.f;
   a.hard = labels != nullptr && weight < 1.f;
   return a;
 }
 
-bool two_sums(const Rows& a) { return a.soft && a.hard && a.tau != 1.f; }
+Mode mode_of(const Rows& a) {
+  if (!(a.soft && a.hard && a.tau != 1.f)) return kOne;
+  return a.tau == 2.f ? kSquare : a.tau == 4.f ? kFourth : kTwo;
+}
 
-template <typename T, int NS>
-int forward(const Rows& a, int parts, int reduction, float* losses, Kept* kept, float* loss, float* divisor, Sums* part,
+template <typename T, int M>
+int forward(const Rows& a, int parts, int reduction, float* losses, Kept* kept, float* loss, float* divisor, char* ws,
             hipStream_t s) {
-  forward_kernel<T, NS><<<dim3((unsigned)(a.rows * parts)), dim3(kT), 0, s>>>(a, parts, part, losses, kept);
+  Named* named = (Named*)ws;
+  Sums* part = (Sums*)(ws + a.rows * sizeof(Named));
+  forward_kernel<T, M><<<dim3((unsigned)(a.rows * parts)), dim3(kT + 64), 0, s>>>(a, parts, part, named, losses, kept);
   if (int st = dh_check_launch("dh_distill_fwd")) return st;
   const int mean = reduction == 1;
   if (parts > 1) {
     const bool ends = reduction != 0 && a.rows <= 64;          // one workgroup joins all rows and reduces them
     if (ends)
-      join_kernel<T, NS><<<dim3(1), dim3(kRT), 0, s>>>(a, parts, part, losses, kept, mean, loss, divisor);
+      join_kernel<M><<<dim3(1), dim3(kRT), 0, s>>>(a, parts, part, named, losses, kept, mean, loss, divisor);
     else
-      join_kernel<T, NS><<<dim3((unsigned)((a.rows + 3) / 4)), dim3(256), 0, s>>>(a, parts, part, losses, kept, mean, nullptr,
-                                                                                nullptr);
+      join_kernel<M><<<dim3((unsigned)((a.rows + 3) / 4)), dim3(256), 0, s>>>(a, parts, part, named, losses, kept, mean,
+                                                                             nullptr, nullptr);
     if (int st = dh_check_launch("dh_distill_fwd")) return st;
     if (ends) return 0;
   }
@@ -488,20 +594,38 @@ int forward(const Rows& a, int parts, int reduction, float* losses, Kept* kept, 
   reduce_kernel<<<dim3(1), dim3(kRT), 0, s>>>(losses, kept, a.rows, mean, loss, divisor);
   return dh_check_launch("dh_distill_fwd");
 }
+template <typename T, typename... A>
+int forward_mode(const Rows& a, A... rest) {
+  switch (mode_of(a)) {
+    case kOne: return forward<T, kOne>(a, rest...);
+    case kTwo: return forward<T, kTwo>(a, rest...);
+    case kSquare: return forward<T, kSquare>(a, rest...);
+    default: return forward<T, kFourth>(a, rest...);
+  }
+}
 
-template <typename T, int NS>
+template <typename T, int M>
 int backward(const Rows& a, int parts, const Kept* kept, const float* dloss, int64_t stride, const float* divisor, void* dz,
              hipStream_t s) {
-  backward_kernel<T, NS><<<dim3((unsigned)(a.rows * parts)), dim3(kT), 0, s>>>(a, parts, kept, dloss, stride, divisor,
-                                                                             (T*)dz);
+  backward_kernel<T, M><<<dim3((unsigned)(a.rows * parts)), dim3(kT + 64), 0, s>>>(a, parts, kept, dloss, stride, divisor,
+                                                                                  (T*)dz);
   return dh_check_launch("dh_distill_bwd");
+}
+template <typename T, typename... A>
+int backward_mode(const Rows& a, A... rest) {
+  switch (mode_of(a)) {
+    case kOne: return backward<T, kOne>(a, rest...);
+    case kTwo: return backward<T, kTwo>(a, rest...);
+    case kSquare: return backward<T, kSquare>(a, rest...);
+    default: return backward<T, kFourth>(a, rest...);
+  }
 }
 
 }  // namespace
 
 extern "C" int64_t dh_distill_workspace_bytes(int dtype, int64_t rows, int V) {
   const int parts = parts_of(rows, V, dtype);
-  return parts > 1 ? rows * parts * (int64_t)sizeof(Sums) : 0;
+  return parts > 1 ? rows * (int64_t)(sizeof(Named) + parts * sizeof(Sums)) : 0;
 }
 
 extern "C" int dh_distill_fwd(int dtype, const void* logits, int64_t stride_b, int64_t stride_t, int64_t B, int T, int V,
@@ -518,7 +642,7 @@ extern "C" int dh_distill_fwd(int dtype, const void* logits, int64_t stride_b, i
              "%s: null or unaligned pointer argument", who);
   DH_REQUIRE(reduction == 0 || (loss && divisor), DH_ERR_INVALID_ARG, "%s: null pointer argument", who);
   const int64_t need = dh_distill_workspace_bytes(dtype, a.rows, V);
-  DH_REQUIRE(workspace_bytes >= need && (need == 0 || workspace), DH_ERR_INVALID_ARG, "%s: workspace of %lld bytes, %lld needed",
+  DH_REQUIRE(workspace_bytes >= need && (need == 0 || (workspace && (uintptr_t)workspace % 8 == 0)), DH_ERR_INVALID_ARG, "%s: workspace of %lld bytes, %lld needed",
              who, (long long)workspace_bytes, (long long)need);
   hipStream_t s = (hipStream_t)stream;
   Kept* kept = (Kept*)row_kept;
@@ -528,12 +652,8 @@ extern "C" int dh_distill_fwd(int dtype, const void* logits, int64_t stride_b, i
     return dh_check_launch(who);
   }
   const int parts = parts_of(a.rows, V, dtype);
-  Sums* part = (Sums*)workspace;
-  if (dtype == DH_BF16)
-    return two_sums(a) ? forward<bf16_t, 2>(a, parts, reduction, row_loss, kept, loss, divisor, part, s)
-                       : forward<bf16_t, 1>(a, parts, reduction, row_loss, kept, loss, divisor, part, s);
-  return two_sums(a) ? forward<float, 2>(a, parts, reduction, row_loss, kept, loss, divisor, part, s)
-                     : forward<float, 1>(a, parts, reduction, row_loss, kept, loss, divisor, part, s);
+  return dtype == DH_BF16 ? forward_mode<bf16_t>(a, parts, reduction, row_loss, kept, loss, divisor, (char*)workspace, s)
+                          : forward_mode<float>(a, parts, reduction, row_loss, kept, loss, divisor, (char*)workspace, s);
 }
 
 extern "C" int dh_distill_bwd(int dtype, const void* logits, int64_t stride_b, int64_t stride_t, int64_t B, int T, int V,
@@ -551,9 +671,6 @@ extern "C" int dh_distill_bwd(int dtype, const void* logits, int64_t stride_b, i
   const int parts = parts_of(a.rows, V, dtype);
   const Kept* kept = (const Kept*)row_kept;
   hipStream_t s = (hipStream_t)stream;
-  if (dtype == DH_BF16)
-    return two_sums(a) ? backward<bf16_t, 2>(a, parts, kept, dloss, dloss_stride, divisor, dlogits, s)
-                       : backward<bf16_t, 1>(a, parts, kept, dloss, dloss_stride, divisor, dlogits, s);
-  return two_sums(a) ? backward<float, 2>(a, parts, kept, dloss, dloss_stride, divisor, dlogits, s)
-                     : backward<float, 1>(a, parts, kept, dloss, dloss_stride, divisor, dlogits, s);
+  return dtype == DH_BF16 ? backward_mode<bf16_t>(a, parts, kept, dloss, dloss_stride, divisor, dlogits, s)
+                          : backward_mode<float>(a, parts, kept, dloss, dloss_stride, divisor, dlogits, s);
 }

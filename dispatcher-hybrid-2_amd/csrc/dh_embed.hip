@@ -5,11 +5,10 @@
 //
 // The gradient groups the positions by token: sums in fp32 over a token's positions in ascending order, split at fixed
 // places, so the same call gives the same bits whatever the launch order. Three launches:
-//   place  every workgroup owns a range of token ids and reads ALL ids itself (8 n bytes from L2, cheaper than the launches
-//          of a sort that shares work between workgroups): it counts the ids below its range (its offset in the grouped
-//          order) and its own per (wave, token), scans, and writes its (token, position) pairs, positions ascending. The
-//          rows of its range that no position holds it fills with zeros: most of dW's bytes, written while other
-//          workgroups still count.
+//   place  every workgroup owns every 256th token id and reads ALL ids itself (8 n bytes from L2, cheaper than the launches
+//          of a sort that shares work between workgroups): it counts the ids of the owners before it (its offset in the
+//          grouped order) and its own per (wave, token), scans, and writes its (token, position) pairs, positions
+//          ascending. The rows of its ids that no position holds it fills with zeros: most of dW's bytes.
 //   sum    the grouped list in equal chunks, whatever the distribution of the tokens: a wave adds the dy rows of a chunk and
 //          writes a token's row when the token's positions all lie in the chunk; the sums of a first or last token that
 //          reaches into the neighbouring chunks go to the workspace.
@@ -99,14 +98,22 @@ struct Pair {
   int32_t token, pos;
 };
 
+// Which ids a workgroup of `place` owns: those equal to its number modulo 2^lg. Low ids are the frequent ones of a
+// vocabulary ordered by frequency, so neighbouring ids go to different workgroups (contiguous ranges: 130 us in place of 27
+// at 32768 tokens of text, two fifths of them in the first of 256 ranges). The grouped order is by (owner, id).
+struct Owners {
+  int lg, range;                           // 2^lg workgroups of `range` ids
+  __host__ __device__ int slot(int token) const { return (token & ((1 << lg) - 1)) * range + (token >> lg); }
+  __host__ __device__ int slots() const { return range << lg; }
+};
+
 template <typename T, int N>
-__global__ __launch_bounds__(kPT) void place_kernel(const void* ids, int wide, int n, int64_t V, int range, int64_t skip,
+__global__ __launch_bounds__(kPT) void place_kernel(const void* ids, int wide, int n, int64_t V, Owners own, int64_t skip,
                                                     int* starts, Pair* pairs, T* dW, int pieces) {
-  extern __shared__ int counts[];          // [wave][token of the range]
+  extern __shared__ int counts[];          // [wave][id owned]
   __shared__ int wsum[kPW], wbelow[kPW];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int64_t first = (int64_t)blockIdx.x * range;
-  const int own = (int)min((int64_t)range, V - first);
+  const int me = blockIdx.x, mask = (1 << own.lg) - 1, range = own.range;
   for (int i = tid; i < kPW * range; i += kPT) counts[i] = 0;
   __syncthreads();
 
@@ -114,19 +121,24 @@ __global__ __launch_bounds__(kPT) void place_kernel(const void* ids, int wide, i
   const int groups = (n + 63) / 64, per = (groups + kPW - 1) / kPW;
   const int g0 = min(wave * per, groups), g1 = min(g0 + per, groups);
   int* mine = counts + wave * range;
-  int below = 0;
-  for (int g = g0; g < g1; g += kBatch) {
-    int64_t id[kBatch];
+  auto load = [&](int g, int (&id)[kBatch]) {                  // -1: no gradient there
+    int64_t v[kBatch];
 #pragma unroll
     for (int k = 0; k < kBatch; ++k) {
       const int i = (g + k) * 64 + lane;
-      id[k] = g + k < g1 && i < n ? load_id(ids, wide, i) : -1;
+      v[k] = g + k < g1 && i < n ? load_id(ids, wide, i) : -1;
     }
 #pragma unroll
+    for (int k = 0; k < kBatch; ++k) id[k] = (uint64_t)v[k] < (uint64_t)V && v[k] != skip ? (int)v[k] : -1;
+  };
+  int below = 0;
+  for (int g = g0; g < g1; g += kBatch) {
+    int id[kBatch];
+    load(g, id);
+#pragma unroll
     for (int k = 0; k < kBatch; ++k) {
-      const bool live = id[k] >= 0 && id[k] < V && id[k] != skip;
-      below += live && id[k] < first;
-      if (live && id[k] >= first && id[k] < first + own) atomicAdd(&mine[(int)(id[k] - first)], 1);
+      below += id[k] >= 0 && (id[k] & mask) < me;
+      if (id[k] >= 0 && (id[k] & mask) == me) atomicAdd(&mine[id[k] >> own.lg], 1);
     }
   }
 #pragma unroll
@@ -134,9 +146,9 @@ __global__ __launch_bounds__(kPT) void place_kernel(const void* ids, int wide, i
   if (lane == 0) wbelow[wave] = below;
   __syncthreads();
 
-  // exclusive scan: over the tokens of the range (a thread each), then over a token's waves
+  // exclusive scan: over the ids owned (a thread each), then over an id's waves
   int total = 0;
-  if (tid < own)
+  if (tid < range)
     for (int w = 0; w < kPW; ++w) total += counts[w * range + tid];
   int incl = total;
 #pragma unroll
@@ -148,9 +160,9 @@ __global__ __launch_bounds__(kPT) void place_kernel(const void* ids, int wide, i
   __syncthreads();
   int at = incl - total;
   for (int w = 0; w < kPW; ++w) at += wbelow[w] + (w < wave ? wsum[w] : 0);
-  if (tid < own) {
-    starts[first + tid] = at;
-    if (first + tid == V - 1) starts[V] = at + total;
+  if (tid < range) {
+    starts[me * range + tid] = at;
+    if (me == mask && tid == range - 1) starts[own.slots()] = at + total;
     for (int w = 0; w < kPW; ++w) {
       const int c = counts[w * range + tid];
       counts[w * range + tid] = at;
@@ -161,26 +173,21 @@ __global__ __launch_bounds__(kPT) void place_kernel(const void* ids, int wide, i
 
   // the pairs, in order of the position within a token: of the lanes that hold one token the first draws their places
   for (int g = g0; g < g1; g += kBatch) {
-    int64_t id[kBatch];
+    int id[kBatch];
+    load(g, id);
 #pragma unroll
     for (int k = 0; k < kBatch; ++k) {
-      const int i = (g + k) * 64 + lane;
-      id[k] = g + k < g1 && i < n ? load_id(ids, wide, i) : -1;
-    }
-#pragma unroll
-    for (int k = 0; k < kBatch; ++k) {
-      const bool hit = id[k] >= first && id[k] < first + own && id[k] != skip;
-      const int t = hit ? (int)(id[k] - first) : -1;
+      const bool hit = id[k] >= 0 && (id[k] & mask) == me;
       uint64_t left = __ballot(hit);
       while (left) {                                           // uniform; a token leaves in each turn
         const int lead = __builtin_ctzll(left);
-        const int lt = __builtin_amdgcn_readlane(t, lead);
-        const uint64_t same = __ballot(hit && t == lt);
+        const int token = __builtin_amdgcn_readlane(id[k], lead);
+        const uint64_t same = __ballot(hit && id[k] == token);
         int base = 0;
-        if (lane == lead) base = atomicAdd(&mine[lt], __popcll(same));
+        if (lane == lead) base = atomicAdd(&mine[token >> own.lg], __popcll(same));
         base = __builtin_amdgcn_readlane(base, lead);
-        if (hit && t == lt)
-          pairs[base + __popcll(same & ((1ull << lane) - 1))] = Pair{(int32_t)id[k], (g + k) * 64 + lane};
+        if (hit && id[k] == token)
+          pairs[base + __popcll(same & ((1ull << lane) - 1))] = Pair{token, (g + k) * 64 + lane};
         left &= ~same;
       }
     }
@@ -188,7 +195,7 @@ __global__ __launch_bounds__(kPT) void place_kernel(const void* ids, int wide, i
 
   // rows that no position holds
   __syncthreads();
-  if (tid < own) counts[tid] = total;
+  if (tid < range) counts[tid] = total;
   __syncthreads();
   typedef typename Piece<T, N>::raw raw;
   raw zero;
@@ -198,16 +205,18 @@ __global__ __launch_bounds__(kPT) void place_kernel(const void* ids, int wide, i
     for (int j = 0; j < N; ++j) z[j] = 0.f;
     zero = Piece<T, N>::pack(z);
   }
-  for (int r = wave; r < own; r += kPW) {
-    if (counts[r]) continue;                                   // uniform in the wave
-    raw* row = reinterpret_cast<raw*>(dW) + (first + r) * pieces;
+  for (int r = wave; r < range; r += kPW) {
+    const int64_t token = ((int64_t)r << own.lg) + me;
+    if (counts[r] || token >= V) continue;                     // uniform in the wave
+    raw* row = reinterpret_cast<raw*>(dW) + token * pieces;
     for (int c = lane; c < pieces; c += 64) row[c] = zero;
   }
 }
 
 // ---- gradient: sum and join -----------------------------------------------------------------------------------------
 constexpr int kST = 256;                   // threads of `sum`: four waves, a chunk and 64 pieces of the row each
-constexpr int kRows = 8;                   // dy rows in flight
+constexpr int kRows = 32;                  // dy rows in flight a wave: a whole chunk of up to 32768 positions, so that the
+                                           // rows cost one round trip (8 in flight: 33 us in place of 2x at 32768 x 1024)
 
 // partial sums of chunk c: [2 c] of a first token that began in an earlier chunk, [2 c + 1] of a last token that began in
 // this chunk and goes on in the next; d floats each
@@ -217,97 +226,111 @@ __global__ __launch_bounds__(kST) void sum_kernel(const T* dy, int64_t ldy, cons
   typedef Piece<T, N> P;
   typedef typename P::raw raw;
   const int lane = threadIdx.x & 63;
-  const int64_t unit = (int64_t)blockIdx.x * (kST / 64) + (threadIdx.x >> 6);
-  const int64_t c = unit / slices;
-  const int piece = (int)(unit % slices) * 64 + lane;
+  const int unit = __builtin_amdgcn_readfirstlane(blockIdx.x * (kST / 64) + (threadIdx.x >> 6));
+  const int c = unit / slices;
+  const int piece = (unit % slices) * 64 + lane;
   const int m = load_uniform(count);
-  const int64_t b = c * chunk;
-  if (b >= m) return;
-  const int e = (int)min(b + chunk, (int64_t)m);
+  const int64_t b64 = (int64_t)c * chunk;
+  if (b64 >= m) return;
+  const int b = (int)b64, e = min(b + chunk, m);
+  const int col = min(piece, pieces - 1);                      // (lanes past the row read its last piece and write nothing)
   const bool in = piece < pieces;
   const int before = b > 0 ? pairs[b - 1].token : -1, after = e < m ? pairs[e].token : -1;
   float acc[N];
 #pragma unroll
   for (int j = 0; j < N; ++j) acc[j] = 0.f;
-  int token = pairs[b].token;
-  bool open = token == before;             // the token in hand began before this chunk
+  int token = -1;
+  bool open = false;                                           // the token in hand began before this chunk
   auto flush = [&](bool ends) {
-    if (in) {
-      if (!open && ends) {
-        float o[N];
+    if (!open && ends) {
+      float o[N];
 #pragma unroll
-        for (int j = 0; j < N; ++j) o[j] = acc[j] * scale;
-        reinterpret_cast<raw*>(dW)[(int64_t)token * pieces + piece] = P::pack(o);
-      } else {
-        float* p = part + (2 * c + (open ? 0 : 1)) * d + piece * N;
+      for (int j = 0; j < N; ++j) o[j] = acc[j] * scale;
+      if (in) reinterpret_cast<raw*>(dW)[(int64_t)token * pieces + piece] = P::pack(o);
+    } else if (in) {
+      float* p = part + (2 * (int64_t)c + (open ? 0 : 1)) * d + piece * N;
 #pragma unroll
-        for (int j = 0; j < N; ++j) p[j] = acc[j];
-      }
+      for (int j = 0; j < N; ++j) p[j] = acc[j];
     }
 #pragma unroll
     for (int j = 0; j < N; ++j) acc[j] = 0.f;
     open = false;
   };
-  for (int i = (int)b; i < e; i += kRows) {
-    Pair pr[kRows];
+  for (int i = b; i < e; i += kRows) {
+    const Pair pr = pairs[min(i + (lane & (kRows - 1)), e - 1)];
     raw v[kRows];
 #pragma unroll
-    for (int k = 0; k < kRows; ++k) {
-      pr[k] = pairs[min(i + k, e - 1)];
-      if (in) v[k] = reinterpret_cast<const raw*>(dy + (int64_t)pr[k].pos * ldy)[piece];
+    for (int k = 0; k < kRows; ++k)                            // (behind the chunk's end: its last row again)
+      v[k] = reinterpret_cast<const raw*>(dy + (int64_t)__builtin_amdgcn_readlane(pr.pos, k) * ldy)[col];
+    if (i == b) {
+      token = __builtin_amdgcn_readlane(pr.token, 0);
+      open = token == before;
     }
 #pragma unroll
     for (int k = 0; k < kRows; ++k) {
-      if (i + k < e) {
-        if (pr[k].token != token) {
+      if (i + k < e) {                                         // uniform
+        const int t = __builtin_amdgcn_readlane(pr.token, k);
+        if (t != token) {
           flush(true);
-          token = pr[k].token;
+          token = t;
         }
-        if (in) {
-          float x[N];
-          P::unpack(v[k], x);
+        float x[N];
+        P::unpack(v[k], x);
 #pragma unroll
-          for (int j = 0; j < N; ++j) acc[j] += x[j];
-        }
+        for (int j = 0; j < N; ++j) acc[j] += x[j];
       }
     }
   }
   flush(token != after);
 }
 
-constexpr int kJT = 256;                   // threads of `join`: four waves, each a quarter of a token's chunks, 64 columns
+constexpr int kJW = 8;                     // waves of `join`: each an eighth of a token's chunks, 64 lanes of M columns
 
-template <typename T>
-__global__ __launch_bounds__(kJT) void join_kernel(const Pair* pairs, const int* starts, int64_t V, int chunk, float scale,
-                                                   const float* part, T* dW, int d) {
-  __shared__ float quarter[kJT / 64][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int m = load_uniform(starts + V);
+template <typename T, int M>
+__global__ __launch_bounds__(kJW * 64) void join_kernel(const Pair* pairs, const int* starts, Owners own, int chunk,
+                                                        float scale, const float* part, T* dW, int d) {
+  __shared__ float eighth[kJW][64 * M];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int m = load_uniform(starts + own.slots());
   const int64_t c = blockIdx.x;
   const int64_t e = (c + 1) * chunk;
   if (e >= m) return;                                          // uniform: the last chunk, or none
   const int token = pairs[e - 1].token;
   if (pairs[e].token != token) return;
-  if (starts[token] < c * chunk) return;                       // began earlier: that chunk joins it
-  const int last = (starts[token + 1] - 1) / chunk;            // chunks c .. last hold the token
-  const int count = last - (int)c + 1, per = (count + 3) / 4;
+  const int slot = own.slot(token);
+  if (starts[slot] < c * chunk) return;                        // began earlier: that chunk joins it
+  const int last = (starts[slot + 1] - 1) / chunk;             // chunks c .. last hold the token
+  const int count = last - (int)c + 1, per = (count + kJW - 1) / kJW;
   const int k0 = min(wave * per, count), k1 = min(k0 + per, count);
-  const int col = blockIdx.y * 64 + lane;
-  float s = 0.f;
-  if (col < d)
+  const int first = blockIdx.y * 64 * M, col = first + lane * M;
+  float s[M];
+#pragma unroll
+  for (int j = 0; j < M; ++j) s[j] = 0.f;
+  if (col < d) {
 #pragma unroll 8
-    for (int k = k0; k < k1; ++k) s += part[(2 * (c + k) + (k == 0 ? 1 : 0)) * d + col];
-  quarter[wave][lane] = s;
+    for (int k = k0; k < k1; ++k) {
+      const float* p = part + (2 * (c + k) + (k == 0 ? 1 : 0)) * d + col;
+#pragma unroll
+      for (int j = 0; j < M; ++j) s[j] += p[j];
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < M; ++j) eighth[wave][lane * M + j] = s[j];
   __syncthreads();
-  if (wave == 0 && col < d)
-    Elem<T>::store(dW + (int64_t)token * d + col,
-                   ((quarter[0][lane] + quarter[1][lane]) + (quarter[2][lane] + quarter[3][lane])) * scale);
+  if (tid < 64 * M && first + tid < d) {
+    float x = 0.f;
+#pragma unroll
+    for (int w = 0; w < kJW; ++w) x += eighth[w][tid];
+    Elem<T>::store(dW + (int64_t)token * d + first + tid, x * scale);
+  }
 }
 
 // ---- sizes ----------------------------------------------------------------------------------------------------------
-int range_of(int64_t V) {                  // ids a workgroup of `place` owns: one workgroup a CU, or kMaxRange
-  const int64_t r = (V + 255) / 256;
-  return (int)(r < kMaxRange ? r : kMaxRange);
+Owners owners_of(int64_t V) {              // one workgroup of `place` a CU, or as many as kMaxRange asks for
+  Owners o{8, 0};
+  while (((V + (1 << o.lg) - 1) >> o.lg) > kMaxRange) ++o.lg;
+  o.range = (int)((V + (1 << o.lg) - 1) >> o.lg);
+  return o;
 }
 int chunk_of(int64_t n) {                  // positions a wave adds: 32, or up to 1024 chunks
   int64_t c = 32;
@@ -324,7 +347,7 @@ Layout layout_of(int64_t n, int64_t V, int d) {
   const int c = chunk_of(n);
   l.chunks = (n + c - 1) / c;
   l.starts = 0;
-  l.pairs = align16((V + 1) * 4);
+  l.pairs = align16((owners_of(V).slots() + 1) * 4);
   l.part = l.pairs + align16(n * (int64_t)sizeof(Pair));
   l.bytes = l.part + 2 * l.chunks * d * 4;
   return l;
@@ -350,23 +373,25 @@ int lookup(const void* W, int64_t ldw, int64_t V, int d, const void* ids, int wi
 template <typename T, int N>
 int gradient(const void* dy, int64_t ldy, const void* ids, int wide, int64_t n, int64_t V, int d, float scale, int64_t skip,
              void* dW, char* ws, hipStream_t s) {
-  const int pieces = d / N, range = range_of(V), chunk = chunk_of(n);
+  const int pieces = d / N, chunk = chunk_of(n);
+  const Owners own = owners_of(V);
   const Layout l = layout_of(n, V, d);
   int* starts = (int*)(ws + l.starts);
   Pair* pairs = (Pair*)(ws + l.pairs);
   float* part = (float*)(ws + l.part);
-  place_kernel<T, N><<<dim3((unsigned)((V + range - 1) / range)), dim3(kPT), kPW * range * sizeof(int), s>>>(
-      ids, wide, (int)n, V, range, skip, starts, pairs, (T*)dW, pieces);
+  place_kernel<T, N><<<dim3(1u << own.lg), dim3(kPT), kPW * own.range * sizeof(int), s>>>(
+      ids, wide, (int)n, V, own, skip, starts, pairs, (T*)dW, pieces);
   if (int st = dh_check_launch("dh_embed_bwd")) return st;
   if (n == 0) return 0;
   const int slices = (pieces + 63) / 64;
   const int64_t units = l.chunks * slices;
   sum_kernel<T, N><<<dim3((unsigned)((units + kST / 64 - 1) / (kST / 64))), dim3(kST), 0, s>>>(
-      (const T*)dy, ldy, pairs, starts + V, chunk, slices, scale, (T*)dW, d, pieces, part);
+      (const T*)dy, ldy, pairs, starts + own.slots(), chunk, slices, scale, (T*)dW, d, pieces, part);
   if (int st = dh_check_launch("dh_embed_bwd")) return st;
   if (l.chunks > 1) {
-    join_kernel<T><<<dim3((unsigned)(l.chunks - 1), (unsigned)((d + 63) / 64)), dim3(kJT), 0, s>>>(
-        pairs, starts, V, chunk, scale, part, (T*)dW, d);
+    constexpr int M = N == 1 ? 1 : 4;
+    join_kernel<T, M><<<dim3((unsigned)(l.chunks - 1), (unsigned)((d + 64 * M - 1) / (64 * M))), dim3(kJW * 64), 0, s>>>(
+        pairs, starts, own, chunk, scale, part, (T*)dW, d);
     return dh_check_launch("dh_embed_bwd");
   }
   return 0;

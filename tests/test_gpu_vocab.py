@@ -177,6 +177,23 @@ def test_top_logits_of_awkward_rows(what, rows, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows", [1, 40])
+@pytest.mark.parametrize("V", [50257, 65536, 70001])
+@pytest.mark.parametrize("what", ["few", "masked", "columns", "rising", "equal"])
+def test_top_logits_of_long_awkward_rows(what, V, rows, dtype):
+    """A peaked row among -inf, a masked vocabulary, large values that only every 1024th 16-byte piece holds, a rising row."""
+    say("top long", what, V, rows, dtype)
+    g, i, per = gen(V + rows), torch.arange(V, device=DEV), 8 if dtype == torch.bfloat16 else 4
+    noise = torch.randn(rows, V, device=DEV, generator=g)
+    x = {"few": lambda: torch.where(i % 9001 == 17, noise, -math.inf), "masked": lambda: torch.where(i < 40000, -math.inf, noise),
+         "columns": lambda: torch.where((i // per) % 1024 < 90, noise * 0.1 + 50, noise),
+         "rising": lambda: (i * 0.01 - 100).expand(rows, V).clone(),
+         "equal": lambda: torch.full((rows, V), -math.inf, device=DEV)}[what]().to(dtype)
+    for k in (1, 64, 256):
+        check_top(x, k)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_top_logits_layouts(dtype):
     g = gen(8)
     base = torch.randn(4, 6, 999, device=DEV, generator=g).to(dtype)
@@ -271,7 +288,8 @@ def check_distill(z, t, tok, labels, tau, w, **kw):
     assert abs(total.item() - rows.sum().item()) <= row_bound.sum().item() + 2 * U * abs(total.item())
 
 
-MODES = [(1.0, 1.0, False), (2.0, 0.5, True), (0.7, 1.0, False), (3.0, 0.0, True), (1.0, 0.25, True), (4.0, 1.0, True)]
+MODES = [(1.0, 1.0, False), (2.0, 0.5, True), (0.7, 1.0, False), (3.0, 0.0, True), (1.0, 0.25, True), (4.0, 1.0, True), (4.0, 0.3, True),
+         (1.3, 0.6, True)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
