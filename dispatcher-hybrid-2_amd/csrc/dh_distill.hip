@@ -53,9 +53,10 @@ template <typename T> __device__ __forceinline__ uint4 pack(const float (&x)[kE<
   uint32_t w[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    if constexpr (sizeof(T) == 2)
-      w[j] = (uint32_t)f32_to_bf16(x[2 * j]) | ((uint32_t)f32_to_bf16(x[2 * j + 1]) << 16);
-    else
+    if constexpr (sizeof(T) == 2) {
+      typedef float f2 __attribute__((ext_vector_type(2)));
+      w[j] = __builtin_bit_cast(uint32_t, __builtin_convertvector(f2{x[2 * j], x[2 * j + 1]}, dh_bf16x2));   // one v_cvt_pk
+    } else
       w[j] = __float_as_uint(x[j]);
   }
   return make_uint4(w[0], w[1], w[2], w[3]);
@@ -76,8 +77,7 @@ __device__ __forceinline__ double wave_sum64(double v) {
 struct Rows {
   const void* logits;
   int64_t sb, st;                          // strides of row (b, t), b = r / T
-  int64_t rows;
-  int T, V;
+  int rows, T, V;
   const void* t_logits;
   const void* t_tokens;
   const void* labels;                      // null: none
@@ -89,7 +89,7 @@ struct Rows {
 };
 
 template <typename T>
-__device__ __forceinline__ const T* row_of(const Rows& a, int64_t r) {
+__device__ __forceinline__ const T* row_of(const Rows& a, int r) {
   return reinterpret_cast<const T*>(a.logits) + (r / a.T) * a.sb + (r % a.T) * a.st;
 }
 __device__ __forceinline__ int64_t whole(const void* p, int wide, int64_t i) {
@@ -153,7 +153,7 @@ __device__ __forceinline__ double log_sum(float s) {
 
 // The teacher's probabilities of a row, by one wave: slot lane + 64 i in p[i], token[i] (-1: empty) and t[i]. Returns the log
 // of the sum of exp((t - top) / tau); live: there is a slot that is not empty; bad: a token past the vocabulary.
-__device__ __forceinline__ double teacher_row(const Rows& a, int64_t r, int lane, float (&p)[kSlotsPerLane],
+__device__ __forceinline__ double teacher_row(const Rows& a, int r, int lane, float (&p)[kSlotsPerLane],
                                               int (&token)[kSlotsPerLane], float (&t)[kSlotsPerLane], float& top, bool& live,
                                               bool& bad) {
   float most = -INFINITY;
@@ -164,8 +164,8 @@ __device__ __forceinline__ double teacher_row(const Rows& a, int64_t r, int lane
     token[i] = -1;
     t[i] = -INFINITY;
     if (j < a.K) {
-      const int64_t k = whole(a.t_tokens, a.token_wide, r * a.K + j);
-      const float x = teacher_logit(a, r * a.K + j);
+      const int64_t k = whole(a.t_tokens, a.token_wide, (int64_t)r * a.K + j);
+      const float x = teacher_logit(a, (int64_t)r * a.K + j);
       if (k >= a.V) over = true;
       if (k >= 0 && k < a.V && !(x == -INFINITY)) {
         token[i] = (int)k;
@@ -201,12 +201,12 @@ struct Named {
   int terms;                               // bit 0: the row counts, bit 1: it has live slots, bit 2: out of the vocabulary
 };
 
-__device__ __forceinline__ bool counted(const Rows& a, int64_t r) {
+__device__ __forceinline__ bool counted(const Rows& a, int r) {
   return !a.labels || whole(a.labels, a.label_wide, r) != a.ignore;
 }
 
 template <typename T>
-__device__ __forceinline__ Named named_of(const Rows& a, int64_t r, int lane) {
+__device__ __forceinline__ Named named_of(const Rows& a, int r, int lane) {
   const T* z = row_of<T>(a, r);
   Named n{0.0, 0.0, 0.f, 0.f, 1};
   bool live = false, bad = false;
@@ -245,7 +245,7 @@ __device__ __forceinline__ Named named_of(const Rows& a, int64_t r, int lane) {
 }
 
 // the loss of a row that counts, and what the backward pass keeps of it, by one thread
-__device__ __forceinline__ void finish_row(const Rows& a, int64_t r, const Sums& v, const Named& n, float* losses, Kept* kept) {
+__device__ __forceinline__ void finish_row(const Rows& a, int r, const Sums& v, const Named& n, float* losses, Kept* kept) {
   const float s1 = a.hard && a.soft && a.tau != 1.f ? v.s1 : v.s0;
   const bool live = n.terms & 2, bad = n.terms & 4;
   double row = 0.0;
@@ -258,6 +258,29 @@ __device__ __forceinline__ void finish_row(const Rows& a, int64_t r, const Sums&
   kept[r] = Kept{v.m, bad ? nan : 1.f / v.s0, bad ? nan : 1.f / s1, 1 | (live || bad ? 2 : 0)};
 }
 
+// A row in whole 16-byte pieces from its first 16-byte boundary, a stretch of them for each part, and the logits before and
+// behind them, one by one with the first part.
+struct Cut {
+  int head, p0, p1, singles, tail;
+  __device__ __forceinline__ int single(int i, int V) const { return i < head ? i : V - tail + (i - head); }
+  // the part's elements are [lo, hi) and, with the first part, the singles
+  __device__ __forceinline__ bool holds(int64_t i, int E, int V) const {
+    return (i >= head + p0 * E && i < head + p1 * E) || (singles && i >= 0 && (i < head || (i >= V - tail && i < V)));
+  }
+};
+template <typename T>
+__device__ __forceinline__ Cut cut_row(const T* row, int V, int which, int parts) {
+  constexpr int E = kE<T>;
+  Cut c;
+  c.head = min((int)((16u - (reinterpret_cast<uintptr_t>(row) & 15u)) & 15u) / (int)sizeof(T), V);
+  const int pieces = (V - c.head) / E, per = (pieces + parts - 1) / parts;
+  c.tail = V - c.head - pieces * E;
+  c.p0 = min(which * per, pieces);
+  c.p1 = min(c.p0 + per, pieces);
+  c.singles = which == 0 ? c.head + c.tail : 0;
+  return c;
+}
+
 // ---- forward: a row, or one of its parts ----------------------------------------------------------------------------
 template <typename T, int M>
 __global__ __launch_bounds__(kT + 64) void forward_kernel(Rows a, int parts, Sums* part, Named* named, float* losses,
@@ -266,8 +289,8 @@ __global__ __launch_bounds__(kT + 64) void forward_kernel(Rows a, int parts, Sum
   __shared__ Sums ws[kW];
   __shared__ Named wn;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int64_t r = blockIdx.x / parts;
-  const int which = (int)(blockIdx.x % parts);
+  const int r = (int)blockIdx.x / parts;
+  const int which = (int)blockIdx.x % parts;
   if (!counted(a, r)) {                    // uniform: the row is not read
     if (tid == 0 && which == 0) {
       losses[r] = 0.f;
@@ -287,32 +310,21 @@ __global__ __launch_bounds__(kT + 64) void forward_kernel(Rows a, int parts, Sum
     }
   } else {
     const T* z = row_of<T>(a, r);
-    // 16-byte pieces from the boundary at or below the row (a piece that holds an element of the row is mapped whole);
-    // what the first and last hold of others counts as -inf
-    const int mis = (int)((reinterpret_cast<uintptr_t>(z) & 15u) / sizeof(T));
-    const uint4* base = reinterpret_cast<const uint4*>(z - mis);
-    const int pieces = (mis + a.V + E - 1) / E, per = (pieces + parts - 1) / parts;
-    const int p0 = min(which * per, pieces), p1 = min(p0 + per, pieces);
-    const uint32_t none = sizeof(T) == 2 ? 0xff80ff80u : 0xff800000u;
+    const Cut c = cut_row(z, a.V, which, parts);
+    const uint4* base = reinterpret_cast<const uint4*>(z + c.head);
     Sums v{-INFINITY, 0.f, 0.f};
-    for (int p = p0 + tid; p < p1; p += kT * U) {
-      uint4 q[U];
+    if (tid < c.singles) {                 // a logit outside the whole pieces
+      v.m = Elem<T>::load(z + c.single(tid, a.V));
+      const float d = v.m - finite_ref(v.m);
+      v.s0 = exp2_hw(d * c0);
+      if (M != kOne) v.s1 = exp2_hw(d * c1);
+    }
+    auto add = [&](const auto& q) {        // some pieces
+      constexpr int N = sizeof(q) / sizeof(uint4);
+      float x[N][E], most = v.m;
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        q[u] = make_uint4(none, none, none, none);
-        if (p + u * kT < p1) q[u] = base[p + u * kT];
-      }
-      float x[U][E];
-      float most = v.m;
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
+      for (int u = 0; u < N; ++u) {
         unpack<T>(q[u], x[u]);
-        const int k = p + u * kT;
-        if (k == 0 || k == pieces - 1) {
-#pragma unroll
-          for (int j = 0; j < E; ++j)
-            if (k * E + j < mis || k * E + j >= mis + a.V) x[u][j] = -INFINITY;
-        }
 #pragma unroll
         for (int j = 0; j < E; ++j) most = fmaxf(most, x[u][j]);
       }
@@ -321,13 +333,24 @@ __global__ __launch_bounds__(kT + 64) void forward_kernel(Rows a, int parts, Sum
       if (M != kOne) v.s1 *= exp2_hw((v.m - ref) * c1);
       v.m = most;
 #pragma unroll
-      for (int u = 0; u < U; ++u)
+      for (int u = 0; u < N; ++u)
 #pragma unroll
         for (int j = 0; j < E; ++j) {
           const float d = x[u][j] - ref, e = exp2_hw(d * c0);
           v.s0 += e;
           if (M != kOne) v.s1 += second<M>(e, d, c1);
         }
+    };
+    int p = c.p0 + tid;
+    for (; p + (U - 1) * kT < c.p1; p += U * kT) {
+      uint4 q[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) q[u] = base[p + u * kT];
+      add(q);
+    }
+    for (; p < c.p1; p += kT) {
+      uint4 q[1] = {base[p]};
+      add(q);
     }
     v = wave_join<M>(v, c0, c1);
     if (lane == 0) ws[wave] = v;
@@ -383,10 +406,10 @@ __global__ __launch_bounds__(kRT) void join_kernel(Rows a, int parts, const Sums
   const int lane = threadIdx.x & 63, W = blockDim.x >> 6;
   float c0, c1;
   scales(a, c0, c1);
-  for (int64_t r = (int64_t)blockIdx.x * W + (threadIdx.x >> 6); r < a.rows; r += (int64_t)gridDim.x * W) {
+  for (int r = blockIdx.x * W + (threadIdx.x >> 6); r < a.rows; r += gridDim.x * W) {
     if (!counted(a, r)) continue;          // uniform; the first launch wrote it
     Sums v{-INFINITY, 0.f, 0.f};
-    if (lane < parts) v = part[r * parts + lane];
+    if (lane < parts) v = part[(int64_t)r * parts + lane];
     v = wave_join<M>(v, c0, c1);
     if (lane == 0) finish_row(a, r, v, named[r], losses, kept);
   }
@@ -407,28 +430,21 @@ __global__ __launch_bounds__(kRT) void reduce_kernel(const float* losses, const 
 template <typename T, int M>
 __global__ __launch_bounds__(kT + 64) void backward_kernel(Rows a, int parts, const Kept* kept, const float* dloss,
                                                            int64_t dloss_stride, const float* divisor, T* dz) {
-  constexpr int E = kE<T>, U = 2;
+  constexpr int E = kE<T>, U = 4;
   __shared__ float sp[kMaxSlots];
   __shared__ int stok[kMaxSlots];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int64_t r = a.rows - 1 - blockIdx.x / parts;
-  const int which = (int)(blockIdx.x % parts);
+  const int r = a.rows - 1 - (int)blockIdx.x / parts;
+  const int which = (int)blockIdx.x % parts;
   const T* z = row_of<T>(a, r);
-  T* out = dz + r * a.V;
-  // pieces by the output's 16-byte boundaries
-  const int mis = (int)((reinterpret_cast<uintptr_t>(out) & 15u) / sizeof(T));
-  const int pieces = (mis + a.V + E - 1) / E, per = (pieces + parts - 1) / parts;
-  const int p0 = min(which * per, pieces), p1 = min(p0 + per, pieces);
+  T* out = dz + (int64_t)r * a.V;
+  const Cut c = cut_row(out, a.V, which, parts);               // (by the output's 16-byte boundaries)
+  uint4* to = reinterpret_cast<uint4*>(out + c.head);
   const Kept k = kept[r];
   const bool counts = k.terms & 1, soft = counts && a.soft && (k.terms & 2), hard = counts && a.hard;
   if (!soft && !hard) {                    // uniform: no gradient, whatever the row holds
-    for (int p = p0 + tid; p < p1; p += kT + 64) {
-      const int i = p * E - mis;
-      if (i >= 0 && i + E <= a.V)
-        *reinterpret_cast<uint4*>(out + i) = make_uint4(0u, 0u, 0u, 0u);
-      else
-        for (int j = max(i, 0); j < min(i + E, a.V); ++j) Elem<T>::store(out + j, 0.f);
-    }
+    for (int p = c.p0 + tid; p < c.p1; p += kT + 64) to[p] = make_uint4(0u, 0u, 0u, 0u);
+    if (tid < c.singles) Elem<T>::store(out + c.single(tid, a.V), 0.f);
     return;
   }
   const float g = dloss[dloss_stride * r] / (divisor ? *divisor : 1.f);
@@ -437,13 +453,11 @@ __global__ __launch_bounds__(kT + 64) void backward_kernel(Rows a, int parts, co
   scales(a, c0, c1);
   // dz of a logit without the teacher's and the label's part: f0 exp((z - m) c0) + f1 exp((z - m) c1)
   const float ref = finite_ref(k.m);
-  const float f0 = M != kOne ? gs * k.inv_soft : (gs + gh) * k.inv_soft, f1 = gh * k.inv_hard;
-  const bool use0 = M == kOne || soft;     // (a row without live slots has no soft term, and 0 * inf none either)
+  // (a row without live slots has no soft term, and no 0 * inf)
+  const float f0 = M == kOne ? (gs + gh) * k.inv_soft : soft ? gs * k.inv_soft : 0.f, f1 = gh * k.inv_hard;
   auto value = [&](float x) {
     const float d = x - ref, e = exp2_hw(d * c0);
-    float y = use0 ? f0 * e : 0.f;
-    if (M != kOne) y += f1 * second<M>(e, d, c1);
-    return y;
+    return M == kOne ? f0 * e : M == kSquare ? e * (f0 + f1 * e) : f0 * e + f1 * second<M>(e, d, c1);
   };
   // the named tokens of this part, by the wave beside those that write it: slots lane + 64 i, the label behind them
   const int K = soft ? a.K : 0;
@@ -451,7 +465,6 @@ __global__ __launch_bounds__(kT + 64) void backward_kernel(Rows a, int parts, co
   int64_t at[kSlotsPerLane + 1];
   if (wave == kW) {
     const int64_t label = hard ? whole(a.labels, a.label_wide, r) : -1;
-    const int lo = max(p0 * E - mis, 0), hi = min(p1 * E - mis, a.V);
     float p[kSlotsPerLane], t[kSlotsPerLane], top;
     int token[kSlotsPerLane];
     if (soft) {
@@ -461,7 +474,7 @@ __global__ __launch_bounds__(kT + 64) void backward_kernel(Rows a, int parts, co
 #pragma unroll
     for (int i = 0; i <= kSlotsPerLane; ++i) {
       at[i] = i == kSlotsPerLane ? (lane == 0 ? label : -1) : soft ? token[i] : -1;
-      if (at[i] < lo || at[i] >= hi) at[i] = -1;
+      if (!c.holds(at[i], E, a.V)) at[i] = -1;
       y[i] = at[i] >= 0 ? Elem<T>::load(z + at[i]) : 0.f;
       if (i < kSlotsPerLane && soft) {
         sp[i * 64 + lane] = p[i];
@@ -484,27 +497,26 @@ __global__ __launch_bounds__(kT + 64) void backward_kernel(Rows a, int parts, co
       if (at[i] == label) y[i] -= gh;
     }
   } else {
-    for (int p = p0 + tid; p < p1; p += kT * U) {
+    const T* from = z + c.head;
+    auto put = [&](int p, const uint4& q) {
+      float x[E];
+      unpack<T>(q, x);
+#pragma unroll
+      for (int j = 0; j < E; ++j) x[j] = value(x[j]);
+      to[p] = pack<T>(x);
+    };
+    int p = c.p0 + tid;
+    for (; p + (U - 1) * kT < c.p1; p += U * kT) {
       uint4 q[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int i = (p + u * kT) * E - mis;
-        if (p + u * kT < p1 && i >= 0 && i + E <= a.V) q[u] = load16(z + i);
-      }
+      for (int u = 0; u < U; ++u) q[u] = load16(from + (int64_t)(p + u * kT) * E);
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int i = (p + u * kT) * E - mis;
-        if (p + u * kT >= p1) break;
-        if (i >= 0 && i + E <= a.V) {
-          float x[E];
-          unpack<T>(q[u], x);
-#pragma unroll
-          for (int j = 0; j < E; ++j) x[j] = value(x[j]);
-          *reinterpret_cast<uint4*>(out + i) = pack<T>(x);
-        } else {
-          for (int j = max(i, 0); j < min(i + E, a.V); ++j) Elem<T>::store(out + j, value(Elem<T>::load(z + j)));
-        }
-      }
+      for (int u = 0; u < U; ++u) put(p + u * kT, q[u]);
+    }
+    for (; p < c.p1; p += kT) put(p, load16(from + (int64_t)p * E));
+    if (tid < c.singles) {
+      const int i = c.single(tid, a.V);
+      Elem<T>::store(out + i, value(Elem<T>::load(z + i)));
     }
   }
   __syncthreads();
@@ -531,8 +543,8 @@ int check(const char* who, int dtype, const Rows& a, int t_dtype, int token_bits
   DH_REQUIRE(t_dtype == DH_F32 || t_dtype == DH_BF16, DH_ERR_UNSUPPORTED_DTYPE, "%s: teacher dtype %d", who, t_dtype);
   DH_REQUIRE((token_bits == 32 || token_bits == 64) && (!a.labels || label_bits == 32 || label_bits == 64),
              DH_ERR_UNSUPPORTED_DTYPE, "%s: tokens of %d bits, labels of %d", who, token_bits, label_bits);
-  DH_REQUIRE(a.rows >= 0 && a.rows < ((int64_t)1 << 22) && a.T >= 1 && a.V >= 1 && a.V <= (1 << 24), DH_ERR_UNSUPPORTED_SHAPE,
-             "%s: rows=%lld T=%d V=%d", who, (long long)a.rows, a.T, a.V);
+  DH_REQUIRE(a.rows >= 0 && a.rows < (1 << 22) && a.T >= 1 && a.V >= 1 && a.V <= (1 << 24), DH_ERR_UNSUPPORTED_SHAPE,
+             "%s: %d rows (-1: too many), T=%d V=%d", who, a.rows, a.T, a.V);
   DH_REQUIRE(a.K >= 1 && a.K <= kMaxSlots, DH_ERR_UNSUPPORTED_SHAPE, "%s: K=%d must be in [1, %d]", who, a.K, kMaxSlots);
   DH_REQUIRE(a.tau > 0.f && a.tau < INFINITY && a.weight >= 0.f && a.weight <= 1.f, DH_ERR_INVALID_ARG,
              "%s: temperature %g, weight %g", who, (double)a.tau, (double)a.weight);
@@ -548,7 +560,7 @@ Rows rows_of(const void* logits, int64_t sb, int64_t st, int64_t B, int T, int V
   a.logits = logits;
   a.sb = sb;
   a.st = st;
-  a.rows = B * T;
+  a.rows = B < 0 || T < 0 || (T > 0 && B >= ((int64_t)1 << 22) / T + 1) ? -1 : (int)(B * T);       // -1: too many
   a.T = T;
   a.V = V;
   a.t_logits = t_logits;
@@ -577,7 +589,7 @@ int forward(const Rows& a, int parts, int reduction, float* losses, Kept* kept, 
             hipStream_t s) {
   Named* named = (Named*)ws;
   Sums* part = (Sums*)(ws + a.rows * sizeof(Named));
-  forward_kernel<T, M><<<dim3((unsigned)(a.rows * parts)), dim3(kT + 64), 0, s>>>(a, parts, part, named, losses, kept);
+  forward_kernel<T, M><<<dim3((unsigned)a.rows * parts), dim3(kT + 64), 0, s>>>(a, parts, part, named, losses, kept);
   if (int st = dh_check_launch("dh_distill_fwd")) return st;
   const int mean = reduction == 1;
   if (parts > 1) {
@@ -607,7 +619,7 @@ int forward_mode(const Rows& a, A... rest) {
 template <typename T, int M>
 int backward(const Rows& a, int parts, const Kept* kept, const float* dloss, int64_t stride, const float* divisor, void* dz,
              hipStream_t s) {
-  backward_kernel<T, M><<<dim3((unsigned)(a.rows * parts)), dim3(kT + 64), 0, s>>>(a, parts, kept, dloss, stride, divisor,
+  backward_kernel<T, M><<<dim3((unsigned)a.rows * parts), dim3(kT + 64), 0, s>>>(a, parts, kept, dloss, stride, divisor,
                                                                                   (T*)dz);
   return dh_check_launch("dh_distill_bwd");
 }

@@ -8,10 +8,11 @@
 //   place  every workgroup owns every 256th token id and reads ALL ids itself (8 n bytes from L2, cheaper than the launches
 //          of a sort that shares work between workgroups): it counts the ids of the owners before it (its offset in the
 //          grouped order) and its own per (wave, token), scans, and writes its (token, position) pairs, positions
-//          ascending. The rows of its ids that no position holds it fills with zeros: most of dW's bytes.
+//          ascending.
 //   sum    the grouped list in equal chunks, whatever the distribution of the tokens: a wave adds the dy rows of a chunk and
 //          writes a token's row when the token's positions all lie in the chunk; the sums of a first or last token that
-//          reaches into the neighbouring chunks go to the workspace.
+//          reaches into the neighbouring chunks go to the workspace. Beside it, the rows of tokens without a position are
+//          filled with zeros.
 //   join   adds the chunk sums of every token that lies in more than one chunk.
 // Bytes: n d read, V d written (and the ids). Ids outside [0, V) hold no gradient (their rows of `out` are NaN).
 
@@ -67,24 +68,32 @@ __device__ __forceinline__ int64_t load_id(const void* ids, int wide, int64_t i)
 // ---- lookup ---------------------------------------------------------------------------------------------------------
 constexpr int kLT = 256;                   // threads
 
-// 2^lg lanes hold a row of `pieces` pieces; 2^(8 - lg) rows a workgroup
-template <typename T, int N>
+// 2^lg lanes hold R rows of `pieces` pieces; R 2^(8 - lg) rows a workgroup
+template <typename T, int N, int R>
 __global__ __launch_bounds__(kLT) void lookup_kernel(const T* W, int64_t ldw, int64_t V, const void* ids, int wide, int64_t n,
                                                      float scale, int64_t zero_token, T* out, int64_t ldo, int pieces,
                                                      int lg) {
   typedef Piece<T, N> P;
-  const int64_t row = ((int64_t)blockIdx.x << (8 - lg)) + (threadIdx.x >> lg);
+  const int64_t row = (((int64_t)blockIdx.x << (8 - lg)) + (threadIdx.x >> lg)) * R;
   if (row >= n) return;
-  const int64_t id = load_id(ids, wide, row);
-  const bool ok = id >= 0 && id < V, none = id == zero_token;
-  const typename P::raw* src = reinterpret_cast<const typename P::raw*>(W + (ok ? id : 0) * ldw);
-  typename P::raw* dst = reinterpret_cast<typename P::raw*>(out + row * ldo);
-  for (int c = threadIdx.x & ((1 << lg) - 1); c < pieces; c += 1 << lg) {
-    float v[N];
-    P::unpack(src[c], v);
+  int64_t id[R];
 #pragma unroll
-    for (int j = 0; j < N; ++j) v[j] = none ? 0.f : ok ? v[j] * scale : __builtin_nanf("");
-    dst[c] = P::pack(v);
+  for (int r = 0; r < R; ++r) id[r] = load_id(ids, wide, min(row + r, n - 1));
+  for (int c = threadIdx.x & ((1 << lg) - 1); c < pieces; c += 1 << lg) {
+    typename P::raw q[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+      q[r] = reinterpret_cast<const typename P::raw*>(W + ((uint64_t)id[r] < (uint64_t)V ? id[r] : 0) * ldw)[c];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      if (row + r >= n) break;
+      const bool ok = (uint64_t)id[r] < (uint64_t)V, none = id[r] == zero_token;
+      float v[N];
+      P::unpack(q[r], v);
+#pragma unroll
+      for (int j = 0; j < N; ++j) v[j] = none ? 0.f : ok ? v[j] * scale : __builtin_nanf("");
+      reinterpret_cast<typename P::raw*>(out + (row + r) * ldo)[c] = P::pack(v);
+    }
   }
 }
 
@@ -107,9 +116,8 @@ struct Owners {
   __host__ __device__ int slots() const { return range << lg; }
 };
 
-template <typename T, int N>
 __global__ __launch_bounds__(kPT) void place_kernel(const void* ids, int wide, int n, int64_t V, Owners own, int64_t skip,
-                                                    int* starts, Pair* pairs, T* dW, int pieces) {
+                                                    int* starts, Pair* pairs) {
   extern __shared__ int counts[];          // [wave][id owned]
   __shared__ int wsum[kPW], wbelow[kPW];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -192,25 +200,6 @@ __global__ __launch_bounds__(kPT) void place_kernel(const void* ids, int wide, i
       }
     }
   }
-
-  // rows that no position holds
-  __syncthreads();
-  if (tid < range) counts[tid] = total;
-  __syncthreads();
-  typedef typename Piece<T, N>::raw raw;
-  raw zero;
-  {
-    float z[N];
-#pragma unroll
-    for (int j = 0; j < N; ++j) z[j] = 0.f;
-    zero = Piece<T, N>::pack(z);
-  }
-  for (int r = wave; r < range; r += kPW) {
-    const int64_t token = ((int64_t)r << own.lg) + me;
-    if (counts[r] || token >= V) continue;                     // uniform in the wave
-    raw* row = reinterpret_cast<raw*>(dW) + token * pieces;
-    for (int c = lane; c < pieces; c += 64) row[c] = zero;
-  }
 }
 
 // ---- gradient: sum and join -----------------------------------------------------------------------------------------
@@ -218,18 +207,41 @@ constexpr int kST = 256;                   // threads of `sum`: four waves, a ch
 constexpr int kRows = 32;                  // dy rows in flight a wave: a whole chunk of up to 32768 positions, so that the
                                            // rows cost one round trip (8 in flight: 33 us in place of 2x at 32768 x 1024)
 
+constexpr int kZero = 16;                  // tokens a wave of `sum` looks up that finds rows to fill with zeros
+
+// The first `sums` workgroups add, the others fill the rows that no position holds with zeros: most of dW's bytes, written
+// while the dy rows are read (by `place` before: 28 + 19 us in place of EMBUS at 32768 x 1024, V 50257).
 // partial sums of chunk c: [2 c] of a first token that began in an earlier chunk, [2 c + 1] of a last token that began in
 // this chunk and goes on in the next; d floats each
 template <typename T, int N>
-__global__ __launch_bounds__(kST) void sum_kernel(const T* dy, int64_t ldy, const Pair* pairs, const int* count, int chunk,
-                                                  int slices, float scale, T* dW, int d, int pieces, float* part) {
+__global__ __launch_bounds__(kST) void sum_kernel(const T* dy, int64_t ldy, const Pair* pairs, const int* starts, int64_t V,
+                                                  Owners own, int sums, int chunk, int slices, float scale, T* dW, int d,
+                                                  int pieces, float* part) {
   typedef Piece<T, N> P;
   typedef typename P::raw raw;
-  const int lane = threadIdx.x & 63;
-  const int unit = __builtin_amdgcn_readfirstlane(blockIdx.x * (kST / 64) + (threadIdx.x >> 6));
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  if ((int)blockIdx.x >= sums) {
+    const int64_t first = ((int64_t)((int)blockIdx.x - sums) * (kST / 64) + wave) * kZero;
+    const int64_t mine = first + lane;
+    bool empty = false;
+    if (lane < kZero && mine < V) {
+      const int slot = own.slot((int)mine);
+      empty = starts[slot] == starts[slot + 1];
+    }
+    float z[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) z[j] = 0.f;
+    const raw zero = P::pack(z);
+    for (uint64_t left = __ballot(empty); left; left &= left - 1) {            // uniform in the wave
+      raw* row = reinterpret_cast<raw*>(dW) + (first + __builtin_ctzll(left)) * pieces;
+      for (int c = lane; c < pieces; c += 64) row[c] = zero;
+    }
+    return;
+  }
+  const int unit = __builtin_amdgcn_readfirstlane((int)blockIdx.x * (kST / 64) + wave);
   const int c = unit / slices;
   const int piece = (unit % slices) * 64 + lane;
-  const int m = load_uniform(count);
+  const int m = load_uniform(starts + own.slots());
   const int64_t b64 = (int64_t)c * chunk;
   if (b64 >= m) return;
   const int b = (int)b64, e = min(b + chunk, m);
@@ -363,10 +375,14 @@ int lookup(const void* W, int64_t ldw, int64_t V, int d, const void* ids, int wi
   const int pieces = d / N;
   int lg = 0;
   while (lg < 8 && (1 << lg) < pieces) ++lg;
-  const int64_t per = (int64_t)1 << (8 - lg);
-  const int64_t grid = (n + per - 1) / per;
-  lookup_kernel<T, N><<<dim3((unsigned)grid), dim3(kLT), 0, s>>>((const T*)W, ldw, V, ids, wide, n, scale, zero, (T*)out,
-                                                                 ldo, pieces, lg);
+  // four rows a lane where that still leaves 4096 waves
+  const int R = n * pieces >= (int64_t)4096 * 64 * 4 ? 4 : 1;
+  const int64_t per = (int64_t)R << (8 - lg);
+  const dim3 grid((unsigned)((n + per - 1) / per));
+  if (R == 4)
+    lookup_kernel<T, N, 4><<<grid, dim3(kLT), 0, s>>>((const T*)W, ldw, V, ids, wide, n, scale, zero, (T*)out, ldo, pieces, lg);
+  else
+    lookup_kernel<T, N, 1><<<grid, dim3(kLT), 0, s>>>((const T*)W, ldw, V, ids, wide, n, scale, zero, (T*)out, ldo, pieces, lg);
   return dh_check_launch("dh_embed_fwd");
 }
 
@@ -379,14 +395,14 @@ int gradient(const void* dy, int64_t ldy, const void* ids, int wide, int64_t n, 
   int* starts = (int*)(ws + l.starts);
   Pair* pairs = (Pair*)(ws + l.pairs);
   float* part = (float*)(ws + l.part);
-  place_kernel<T, N><<<dim3(1u << own.lg), dim3(kPT), kPW * own.range * sizeof(int), s>>>(
-      ids, wide, (int)n, V, own, skip, starts, pairs, (T*)dW, pieces);
+  place_kernel<<<dim3(1u << own.lg), dim3(kPT), kPW * own.range * sizeof(int), s>>>(ids, wide, (int)n, V, own, skip, starts,
+                                                                                   pairs);
   if (int st = dh_check_launch("dh_embed_bwd")) return st;
-  if (n == 0) return 0;
   const int slices = (pieces + 63) / 64;
-  const int64_t units = l.chunks * slices;
-  sum_kernel<T, N><<<dim3((unsigned)((units + kST / 64 - 1) / (kST / 64))), dim3(kST), 0, s>>>(
-      (const T*)dy, ldy, pairs, starts + own.slots(), chunk, slices, scale, (T*)dW, d, pieces, part);
+  const int sums = (int)((l.chunks * slices + kST / 64 - 1) / (kST / 64));
+  const int zeros = (int)((V + kZero * (kST / 64) - 1) / (kZero * (kST / 64)));
+  sum_kernel<T, N><<<dim3((unsigned)(sums + zeros)), dim3(kST), 0, s>>>((const T*)dy, ldy, pairs, starts, V, own, sums, chunk,
+                                                                       slices, scale, (T*)dW, d, pieces, part);
   if (int st = dh_check_launch("dh_embed_bwd")) return st;
   if (l.chunks > 1) {
     constexpr int M = N == 1 ? 1 : 4;
