@@ -100,8 +100,9 @@ __global__ __launch_bounds__(kLT) void lookup_kernel(const T* W, int64_t ldw, in
 // ---- gradient: place ------------------------------------------------------------------------------------------------
 constexpr int kPT = 1024;                  // threads of `place`
 constexpr int kPW = kPT / 64;
-constexpr int kMaxRange = 512;             // most ids a workgroup owns: kPW * kMaxRange counters, 32 KB of LDS
+constexpr int kMaxRange = 480;             // most ids a workgroup owns: with the lists below 62 KB of LDS
 constexpr int kBatch = 8;                  // id loads in flight a lane
+constexpr int kList = 256;                 // own ids a wave keeps in LDS; a wave with more of them reads its ids again
 
 struct Pair {
   int32_t token, pos;
@@ -119,39 +120,67 @@ struct Owners {
 __global__ __launch_bounds__(kPT) void place_kernel(const void* ids, int wide, int n, int64_t V, Owners own, int64_t skip,
                                                     int* starts, Pair* pairs) {
   extern __shared__ int counts[];          // [wave][id owned]
+  __shared__ Pair lists[kPW][kList];
   __shared__ int wsum[kPW], wbelow[kPW];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);   // (uniform: masks stay scalar)
   const int me = blockIdx.x, mask = (1 << own.lg) - 1, range = own.range;
   for (int i = tid; i < kPW * range; i += kPT) counts[i] = 0;
   __syncthreads();
 
   // a wave's ids: whole groups of 64, one stretch a wave, so that (wave, group, lane) ascends with the position
-  const int groups = (n + 63) / 64, per = (groups + kPW - 1) / kPW;
+  const int groups = (n + 63) / 64, per = (groups + kPW - 1) / kPW;   // (no group where n is 0: nothing is read)
   const int g0 = min(wave * per, groups), g1 = min(g0 + per, groups);
   int* mine = counts + wave * range;
-  auto load = [&](int g, int (&id)[kBatch]) {                  // -1: no gradient there
-    int64_t v[kBatch];
-#pragma unroll
-    for (int k = 0; k < kBatch; ++k) {
-      const int i = (g + k) * 64 + lane;
-      v[k] = g + k < g1 && i < n ? load_id(ids, wide, i) : -1;
-    }
-#pragma unroll
-    for (int k = 0; k < kBatch; ++k) id[k] = (uint64_t)v[k] < (uint64_t)V && v[k] != skip ? (int)v[k] : -1;
-  };
+  Pair* list = lists[wave];
+  // fn(token, position, mask of the lanes whose token is owned) for every group that has one, in order
   int below = 0;
-  for (int g = g0; g < g1; g += kBatch) {
-    int id[kBatch];
-    load(g, id);
+  auto scan = [&](auto&& fn) {
+    below = 0;
+    for (int g = g0; g < g1; g += kBatch) {
+      uint32_t id[kBatch];
+      bool live[kBatch];
+      if (wide) {
+        int64_t v[kBatch];
 #pragma unroll
-    for (int k = 0; k < kBatch; ++k) {
-      below += id[k] >= 0 && (id[k] & mask) < me;
-      if (id[k] >= 0 && (id[k] & mask) == me) atomicAdd(&mine[id[k] >> own.lg], 1);
+        for (int k = 0; k < kBatch; ++k) v[k] = reinterpret_cast<const int64_t*>(ids)[min((g + k) * 64 + lane, n - 1)];
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) {
+          id[k] = (uint32_t)v[k];
+          live[k] = (uint64_t)v[k] < (uint64_t)V;
+        }
+      } else {
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) id[k] = reinterpret_cast<const uint32_t*>(ids)[min((g + k) * 64 + lane, n - 1)];
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) live[k] = id[k] < (uint32_t)V;
+      }
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k) {
+        if (g + k >= g1) break;                                // uniform
+        const int pos = (g + k) * 64 + lane;
+        uint64_t in = __ballot(live[k] && id[k] != (uint32_t)skip);
+        if (g + k == groups - 1) in &= __ballot(pos < n);
+        below += __popcll(in & __ballot((id[k] & mask) < (uint32_t)me));
+        const uint64_t hits = in & __ballot((id[k] & mask) == (uint32_t)me);
+        if (hits) fn((int)id[k], pos, hits);
+      }
     }
-  }
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) below += __shfl_xor(below, o);
+  };
+  int found = 0;
+  scan([&](int token, int pos, uint64_t hits) {
+    if (found + __popcll(hits) <= kList && ((hits >> lane) & 1))
+      list[found + __popcll(hits & ((1ull << lane) - 1))] = Pair{token, pos};
+    found += __popcll(hits);
+  });
   if (lane == 0) wbelow[wave] = below;
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");       // (the list is the wave's own; LDS answers it in order)
+  if (found <= kList) {
+    for (int i = lane; i < found; i += 64) atomicAdd(&mine[list[i].token >> own.lg], 1);
+  } else {
+    scan([&](int token, int, uint64_t hits) {
+      if ((hits >> lane) & 1) atomicAdd(&mine[token >> own.lg], 1);
+    });
+  }
   __syncthreads();
 
   // exclusive scan: over the ids owned (a thread each), then over an id's waves
@@ -180,25 +209,25 @@ __global__ __launch_bounds__(kPT) void place_kernel(const void* ids, int wide, i
   __syncthreads();
 
   // the pairs, in order of the position within a token: of the lanes that hold one token the first draws their places
-  for (int g = g0; g < g1; g += kBatch) {
-    int id[kBatch];
-    load(g, id);
-#pragma unroll
-    for (int k = 0; k < kBatch; ++k) {
-      const bool hit = id[k] >= 0 && (id[k] & mask) == me;
-      uint64_t left = __ballot(hit);
-      while (left) {                                           // uniform; a token leaves in each turn
-        const int lead = __builtin_ctzll(left);
-        const int token = __builtin_amdgcn_readlane(id[k], lead);
-        const uint64_t same = __ballot(hit && id[k] == token);
-        int base = 0;
-        if (lane == lead) base = atomicAdd(&mine[token >> own.lg], __popcll(same));
-        base = __builtin_amdgcn_readlane(base, lead);
-        if (hit && id[k] == token)
-          pairs[base + __popcll(same & ((1ull << lane) - 1))] = Pair{token, (g + k) * 64 + lane};
-        left &= ~same;
-      }
+  auto place = [&](int token, int pos, uint64_t left) {
+    while (left) {                                             // uniform; a token leaves in each turn
+      const int lead = __builtin_ctzll(left);
+      const int its = __builtin_amdgcn_readlane(token, lead);
+      const uint64_t same = left & __ballot(token == its);
+      int base = 0;
+      if (lane == lead) base = atomicAdd(&mine[its >> own.lg], __popcll(same));
+      base = __builtin_amdgcn_readlane(base, lead);
+      if ((same >> lane) & 1) pairs[base + __popcll(same & ((1ull << lane) - 1))] = Pair{its, pos};
+      left &= ~same;
     }
+  };
+  if (found <= kList) {
+    for (int i = 0; i < found; i += 64) {
+      const Pair p = list[min(i + lane, found - 1)];
+      place(p.token, p.pos, __ballot(i + lane < found));
+    }
+  } else {
+    scan(place);
   }
 }
 

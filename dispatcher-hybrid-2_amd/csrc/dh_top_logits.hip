@@ -24,7 +24,8 @@ namespace {
 
 constexpr int kMaxK = 256;
 constexpr int kSlack = 32;                 // threads more than K that end the bisection
-constexpr int kCap = 4096;                 // keys in LDS
+constexpr int kCap = 9 * kMaxK;            // keys in LDS: ties leave up to E K of them, and K above
+constexpr int kMany = 512;                 // rows from which a row gets 512 threads
 constexpr int kU = 8;                      // 16-byte loads in flight a thread
 
 __device__ __forceinline__ uint32_t image_of(float x) {        // a < b  <=>  image(a) < image(b); NaN above all
@@ -61,15 +62,15 @@ __device__ __forceinline__ V bisect(V lo, V hi, int need, int enough, int& got, 
 
 // The row's whole aligned 16-byte pieces, thread t those of t, t + nt, ... (nt threads), and what stands before the first and
 // behind the last of them, up to 2 (E - 1) logits, one each with the first threads.
-template <typename T>
-__global__ __launch_bounds__(1024, 8) void top_kernel(const T* logits, int64_t stride, int V, int K, T* values,
+template <typename T, int NT>
+__global__ __launch_bounds__(NT, 8) void top_kernel(const T* logits, int64_t stride, int V, int K, T* values,
                                                       int64_t* tokens) {
   constexpr int E = 16 / sizeof(T);
   __shared__ uint64_t keys[kCap];
-  __shared__ uint32_t images[1024], firsts[1024];
-  __shared__ uint16_t list[1024];          // the threads at or above the bound
+  __shared__ uint32_t images[NT], firsts[NT];
+  __shared__ uint16_t list[NT];            // the threads at or above the bound
   __shared__ uint32_t bound[2];            // image; least complement of a token at that image
-  __shared__ int count, listed, part[16];
+  __shared__ int count, listed, part[NT / 64];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, nt = blockDim.x;
   const T* row = logits + (int64_t)blockIdx.x * stride;
   const int head = min((int)((16u - (reinterpret_cast<uintptr_t>(row) & 15u)) & 15u) / (int)sizeof(T), V);
@@ -119,15 +120,15 @@ __global__ __launch_bounds__(1024, 8) void top_kernel(const T* logits, int64_t s
   const bool some = tid < pieces || extra >= 0;                // (a thread that holds nothing has no part in this)
   const uint32_t mine = !some ? 0u : nan ? 0xffffffffu : image_of(most);
   images[tid] = mine;
-  for (int i = nt + tid; i < 1024; i += nt) images[i] = 0u;
+  for (int i = nt + tid; i < NT; i += nt) images[i] = 0u;
   __syncthreads();
 
   if (wave == 0) {
-    uint32_t im[16];
+    uint32_t im[NT / 64];
     uint32_t a = 0xffffffffu, b = 0u;
     int got = 0;
 #pragma unroll
-    for (int j = 0; j < 16; ++j) {
+    for (int j = 0; j < NT / 64; ++j) {
       im[j] = images[j * 64 + lane];
       a = min(a, im[j] - 1u);                                  // (0, nothing, becomes the largest)
       b = max(b, im[j]);
@@ -146,7 +147,7 @@ __global__ __launch_bounds__(1024, 8) void top_kernel(const T* logits, int64_t s
       a = bisect(a, b, K, K + kSlack, got, [&](uint32_t v) {
         int c = 0;
 #pragma unroll
-        for (int j = 0; j < 16; ++j) c += __popcll(__ballot(im[j] >= v));
+        for (int j = 0; j < NT / 64; ++j) c += __popcll(__ballot(im[j] >= v));
         return c;
       });
     }
@@ -165,13 +166,13 @@ __global__ __launch_bounds__(1024, 8) void top_kernel(const T* logits, int64_t s
         if ((uint32_t)(k >> 32) == a) first = max(first, (uint32_t)k);
       });
     firsts[tid] = first;
-    for (int i = nt + tid; i < 1024; i += nt) firsts[i] = 0u;
+    for (int i = nt + tid; i < NT; i += nt) firsts[i] = 0u;
     __syncthreads();
     if (wave == 0) {
-      uint32_t fi[16];
-      int above = 0, got = 1024;
+      uint32_t fi[NT / 64];
+      int above = 0, got = NT;
 #pragma unroll
-      for (int j = 0; j < 16; ++j) {
+      for (int j = 0; j < NT / 64; ++j) {
         fi[j] = firsts[j * 64 + lane];                         // (0 unless the thread's value is the bound)
         above += __popcll(__ballot(images[j * 64 + lane] > a));
       }
@@ -179,7 +180,7 @@ __global__ __launch_bounds__(1024, 8) void top_kernel(const T* logits, int64_t s
       const uint32_t lo = bisect(0u, 0xffffffffu, K - above, K - above, got, [&](uint32_t v) {
         int c = 0;
 #pragma unroll
-        for (int j = 0; j < 16; ++j) c += __popcll(__ballot(fi[j] >= v));
+        for (int j = 0; j < NT / 64; ++j) c += __popcll(__ballot(fi[j] >= v));
         return c;
       });
       if (lane == 0) bound[1] = lo;
@@ -257,9 +258,14 @@ __global__ __launch_bounds__(1024, 8) void top_kernel(const T* logits, int64_t s
 template <typename T>
 int launch(const void* logits, int64_t stride, int64_t rows, int V, int K, void* values, int64_t* tokens, hipStream_t s) {
   constexpr int E = 16 / sizeof(T);
-  const int pieces = (V + E - 1) / E;
-  const dim3 block((unsigned)(pieces >= 1024 ? 1024 : (pieces + 63) / 64 * 64));             // a piece a thread, or more
-  top_kernel<T><<<dim3((unsigned)rows), block, 0, s>>>((const T*)logits, stride, V, K, (T*)values, tokens);
+  const int need = ((V + E - 1) / E + 63) / 64 * 64;           // a piece a thread, or more
+  const dim3 grid((unsigned)rows);
+  if (rows < kMany)
+    top_kernel<T, 1024><<<grid, dim3((unsigned)(need < 1024 ? need : 1024)), 0, s>>>((const T*)logits, stride, V, K,
+                                                                                    (T*)values, tokens);
+  else
+    top_kernel<T, 512><<<grid, dim3((unsigned)(need < 512 ? need : 512)), 0, s>>>((const T*)logits, stride, V, K, (T*)values,
+                                                                                  tokens);
   return dh_check_launch("dh_top_logits");
 }
 
