@@ -16,6 +16,8 @@
 //   join   adds the chunk sums of every token that lies in more than one chunk.
 // Bytes: n d read, V d written (and the ids). Ids outside [0, V) hold no gradient (their rows of `out` are NaN).
 
+#include <type_traits>
+
 #include "dh_common.h"
 
 namespace {
@@ -109,7 +111,7 @@ struct Pair {
 };
 
 // Which ids a workgroup of `place` owns: those equal to its number modulo 2^lg. Low ids are the frequent ones of a
-// vocabulary ordered by frequency, so neighbouring ids go to different workgroups (contiguous ranges: 130 us in place of 27
+// vocabulary ordered by frequency, so neighbouring ids go to different workgroups (contiguous ranges: 130 us in place of 28
 // at 32768 tokens of text, two fifths of them in the first of 256 ranges). The grouped order is by (owner, id).
 struct Owners {
   int lg, range;                           // 2^lg workgroups of `range` ids
@@ -136,51 +138,71 @@ __global__ __launch_bounds__(kPT) void place_kernel(const void* ids, int wide, i
   int below = 0;
   auto scan = [&](auto&& fn) {
     below = 0;
-    for (int g = g0; g < g1; g += kBatch) {
+    auto batch = [&](int g, auto full) {   // kBatch groups; full: all of the wave's stretch and of the ids
       uint32_t id[kBatch];
-      bool live[kBatch];
+      uint64_t live[kBatch];
       if (wide) {
         int64_t v[kBatch];
 #pragma unroll
-        for (int k = 0; k < kBatch; ++k) v[k] = reinterpret_cast<const int64_t*>(ids)[min((g + k) * 64 + lane, n - 1)];
+        for (int k = 0; k < kBatch; ++k) {
+          const int i = (g + k) * 64 + lane;
+          v[k] = reinterpret_cast<const int64_t*>(ids)[full ? i : min(i, n - 1)];
+        }
 #pragma unroll
         for (int k = 0; k < kBatch; ++k) {
           id[k] = (uint32_t)v[k];
-          live[k] = (uint64_t)v[k] < (uint64_t)V;
+          live[k] = __ballot((uint64_t)v[k] < (uint64_t)V);
         }
       } else {
 #pragma unroll
-        for (int k = 0; k < kBatch; ++k) id[k] = reinterpret_cast<const uint32_t*>(ids)[min((g + k) * 64 + lane, n - 1)];
+        for (int k = 0; k < kBatch; ++k) {
+          const int i = (g + k) * 64 + lane;
+          id[k] = reinterpret_cast<const uint32_t*>(ids)[full ? i : min(i, n - 1)];
+        }
 #pragma unroll
-        for (int k = 0; k < kBatch; ++k) live[k] = id[k] < (uint32_t)V;
+        for (int k = 0; k < kBatch; ++k) live[k] = __ballot(id[k] < (uint32_t)V);
       }
 #pragma unroll
       for (int k = 0; k < kBatch; ++k) {
-        if (g + k >= g1) break;                                // uniform
         const int pos = (g + k) * 64 + lane;
-        uint64_t in = __ballot(live[k] && id[k] != (uint32_t)skip);
-        if (g + k == groups - 1) in &= __ballot(pos < n);
-        below += __popcll(in & __ballot((id[k] & mask) < (uint32_t)me));
-        const uint64_t hits = in & __ballot((id[k] & mask) == (uint32_t)me);
+        if (!full) live[k] = g + k < g1 ? live[k] & __ballot(pos < n) : 0ull;
+        const uint64_t in = live[k] & __ballot(id[k] != (uint32_t)skip);
+        const uint32_t owner = id[k] & mask;
+        below += __popcll(in & __ballot(owner < (uint32_t)me));
+        const uint64_t hits = in & __ballot(owner == (uint32_t)me);
         if (hits) fn((int)id[k], pos, hits);
       }
+    };
+    int g = g0;
+    for (; g + kBatch <= g1 && (g + kBatch) * 64 <= n; g += kBatch) batch(g, std::true_type{});
+    for (; g < g1; g += kBatch) batch(g, std::false_type{});
+  };
+  // fn(lane mask of a token, the token, its first lane) for every token among `left`, a token each turn (uniform)
+  auto tokens = [&](int token, uint64_t left, auto&& fn) {
+    while (left) {
+      const int lead = __builtin_ctzll(left), its = __builtin_amdgcn_readlane(token, lead);
+      const uint64_t same = left & __ballot(token == its);
+      fn(same, its, lead);
+      left &= ~same;
     }
   };
-  int found = 0;
+  // the first of them to the list, counted behind it 64 at a time; the others counted as they come
+  int found = 0, listed = 0;
   scan([&](int token, int pos, uint64_t hits) {
-    if (found + __popcll(hits) <= kList && ((hits >> lane) & 1))
-      list[found + __popcll(hits & ((1ull << lane) - 1))] = Pair{token, pos};
-    found += __popcll(hits);
+    const int c = __popcll(hits);
+    if (found == listed && found + c <= kList) {
+      if ((hits >> lane) & 1) list[found + __popcll(hits & ((1ull << lane) - 1))] = Pair{token, pos};
+      listed += c;
+    } else {
+      tokens(token, hits, [&](uint64_t same, int its, int lead) {
+        if (lane == lead) atomicAdd(&mine[its >> own.lg], __popcll(same));
+      });
+    }
+    found += c;
   });
-  if (lane == 0) wbelow[wave] = below;
   __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");       // (the list is the wave's own; LDS answers it in order)
-  if (found <= kList) {
-    for (int i = lane; i < found; i += 64) atomicAdd(&mine[list[i].token >> own.lg], 1);
-  } else {
-    scan([&](int token, int, uint64_t hits) {
-      if ((hits >> lane) & 1) atomicAdd(&mine[token >> own.lg], 1);
-    });
-  }
+  for (int i = lane; i < listed; i += 64) atomicAdd(&mine[list[i].token >> own.lg], 1);
+  if (lane == 0) wbelow[wave] = below;
   __syncthreads();
 
   // exclusive scan: over the ids owned (a thread each), then over an id's waves
@@ -208,20 +230,19 @@ __global__ __launch_bounds__(kPT) void place_kernel(const void* ids, int wide, i
   }
   __syncthreads();
 
-  // the pairs, in order of the position within a token: of the lanes that hold one token the first draws their places
-  auto place = [&](int token, int pos, uint64_t left) {
-    while (left) {                                             // uniform; a token leaves in each turn
-      const int lead = __builtin_ctzll(left);
-      const int its = __builtin_amdgcn_readlane(token, lead);
-      const uint64_t same = left & __ballot(token == its);
+  // the pairs, in order of the position within a token: the first lane that holds a token draws the places of all that do
+  auto place = [&](int token, int pos, uint64_t hits) {
+    tokens(token, hits, [&](uint64_t same, int its, int lead) {
       int base = 0;
-      if (lane == lead) base = atomicAdd(&mine[its >> own.lg], __popcll(same));
+      if (lane == lead) {
+        base = mine[its >> own.lg];
+        mine[its >> own.lg] = base + __popcll(same);
+      }
       base = __builtin_amdgcn_readlane(base, lead);
       if ((same >> lane) & 1) pairs[base + __popcll(same & ((1ull << lane) - 1))] = Pair{its, pos};
-      left &= ~same;
-    }
+    });
   };
-  if (found <= kList) {
+  if (found == listed) {
     for (int i = 0; i < found; i += 64) {
       const Pair p = list[min(i + lane, found - 1)];
       place(p.token, p.pos, __ballot(i + lane < found));
@@ -234,12 +255,12 @@ __global__ __launch_bounds__(kPT) void place_kernel(const void* ids, int wide, i
 // ---- gradient: sum and join -----------------------------------------------------------------------------------------
 constexpr int kST = 256;                   // threads of `sum`: four waves, a chunk and 64 pieces of the row each
 constexpr int kRows = 32;                  // dy rows in flight a wave: a whole chunk of up to 32768 positions, so that the
-                                           // rows cost one round trip (8 in flight: 33 us in place of 2x at 32768 x 1024)
+                                           // rows cost one round trip (8 in flight: 33 us in place of 19 at 32768 x 1024)
 
 constexpr int kZero = 16;                  // tokens a wave of `sum` looks up that finds rows to fill with zeros
 
 // The first `sums` workgroups add, the others fill the rows that no position holds with zeros: most of dW's bytes, written
-// while the dy rows are read (by `place` before: 28 + 19 us in place of EMBUS at 32768 x 1024, V 50257).
+// while the dy rows are read (by `place` instead: 28 us in all in place of 22 at 128 x 1024 bf16, V 50257; the same at 32768).
 // partial sums of chunk c: [2 c] of a first token that began in an earlier chunk, [2 c + 1] of a last token that began in
 // this chunk and goes on in the next; d floats each
 template <typename T, int N>

@@ -5,18 +5,19 @@
 // A value and its token make one 64-bit key, different for every element: an order-preserving 32-bit image of the value
 // above the complement of the token. The K largest keys are the answer, with no case for ties.
 //
-// One workgroup a row, of up to 1024 threads, which read the row once and go back to a few per cent of it:
-//   - each thread keeps the largest of its values (a half instruction a value, and another half for NaN);
+// One workgroup a row, which reads the row once and goes back to a tenth of it or less:
+//   - the largest value of every group of logits, one group a thread: its own 16-byte pieces or, in long rows, one 128-byte
+//     line of each eight pieces that it read with its seven neighbours (whole lines, so that going back costs no more than
+//     the groups themselves hold);
 //   - the K-th largest of those, or a value slightly below it, is a lower bound of the K-th largest logit: bisection over their
-//     images by one wave, ended once K to K + kSlack threads are at least there;
-//   - those threads' 16-byte pieces are read again, by the whole workgroup, and the logits at the bound or above (K and a few
-//     tens more: a thread rarely holds two) go to LDS as keys;
+//     images by one wave, ended once K to K + kSlack groups are at least there;
+//   - those groups are read again, by the whole workgroup, and the logits at the bound or above (K and a few tens more: a
+//     group rarely holds two) go to LDS as keys;
 //   - a key's rank is the number of larger keys; ranks below K write their value and token.
-// Ties at the bound (masked vocabularies, constant rows) take the lower tokens first. Rows whose large values all stand where
-// few threads read them, more than LDS holds, are bisected as a whole, slowly. The first pass is bound by its read, and its
-// two workgroups a CU fill each other's other steps. (Rows kept in registers instead of read again: 130 us in place of
-// TOPUS at 4096 x 50257 bf16, the search for the large values in 64 registers a thread being most of it; a wave a row with a
-// running bound: 219 us.)
+// Ties at the bound (masked vocabularies, constant rows) take the lower tokens first. Rows with a NaN, and rows whose large
+// values all stand in few groups, more than LDS holds, are bisected as a whole, slowly. The first pass is bound by its read.
+// (Rows kept in registers instead of read again: 130 us in place of 92 at 4096 x 50257 bf16; a wave a row with a running
+// bound: 219 us; groups of pieces from eight lines each, which going back reads whole: 106 us.)
 
 #include "dh_common.h"
 
@@ -25,8 +26,11 @@ namespace {
 constexpr int kMaxK = 256;
 constexpr int kSlack = 32;                 // threads more than K that end the bisection
 constexpr int kCap = 9 * kMaxK;            // keys in LDS: ties leave up to E K of them, and K above
-constexpr int kMany = 512;                 // rows from which a row gets 512 threads
-constexpr int kU = 8;                      // 16-byte loads in flight a thread
+// Rows from which a row of fewer than kLong pieces gets 512 threads in place of 1024, so that four rows share a CU
+// (bf16, V 50257: 92 against 102 us at 4096 rows, 31 against 35 at 1024, 21 both at 512; V 8000, 4096 rows: 42 against 74;
+// 16000 pieces, 1024 rows: 56 against 52; fp32, V 50257, 1024 rows: 50 against 45).
+constexpr int kMany = 512, kLong = 8192;
+constexpr int kU = 4;                      // 16-byte loads in flight a thread
 
 __device__ __forceinline__ uint32_t image_of(float x) {        // a < b  <=>  image(a) < image(b); NaN above all
   if (x != x) return 0xffffffffu;
@@ -60,8 +64,9 @@ __device__ __forceinline__ V bisect(V lo, V hi, int need, int enough, int& got, 
   return lo;
 }
 
-// The row's whole aligned 16-byte pieces, thread t those of t, t + nt, ... (nt threads), and what stands before the first and
-// behind the last of them, up to 2 (E - 1) logits, one each with the first threads.
+// The row's whole aligned 16-byte pieces, thread t reads those of t, t + nt, ... (nt threads), and what stands before the first
+// and behind the last of them, up to 2 (E - 1) logits, one each with the first threads' groups. Groups of thread t: the pieces
+// it reads, or (lines) of each stretch of 8 nt pieces the eight from (t mod 8) nt + 8 floor(t / 8).
 template <typename T, int NT>
 __global__ __launch_bounds__(NT, 8) void top_kernel(const T* logits, int64_t stride, int V, int K, T* values,
                                                       int64_t* tokens) {
@@ -70,7 +75,7 @@ __global__ __launch_bounds__(NT, 8) void top_kernel(const T* logits, int64_t str
   __shared__ uint32_t images[NT], firsts[NT];
   __shared__ uint16_t list[NT];            // the threads at or above the bound
   __shared__ uint32_t bound[2];            // image; least complement of a token at that image
-  __shared__ int count, listed, part[NT / 64];
+  __shared__ int count, listed, nans, part[NT / 64];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, nt = blockDim.x;
   const T* row = logits + (int64_t)blockIdx.x * stride;
   const int head = min((int)((16u - (reinterpret_cast<uintptr_t>(row) & 15u)) & 15u) / (int)sizeof(T), V);
@@ -85,42 +90,69 @@ __global__ __launch_bounds__(NT, 8) void top_kernel(const T* logits, int64_t str
   };
   const int extra = tid < head ? tid : tid < head + tail ? V - tail + (tid - head) : -1;   // token of the single logit
   const float ex = extra >= 0 ? Elem<T>::load(row + extra) : -INFINITY;
-  // all keys of this thread, from memory, for the slow paths
+  const bool lines = pieces >= 4 * nt;
+  // fn(piece) for the pieces of thread t's group, part of parts
+  auto group = [&](int t, int part, int parts, auto&& fn) {
+    if (lines) {
+#pragma unroll 1
+      for (int p = (t & 7) * nt + (t & ~7); p < pieces; p += 8 * nt)
+#pragma unroll 1
+        for (int i = part; i < 8; i += parts)
+          if (p + i < pieces) fn(p + i);
+    } else {
+#pragma unroll 1
+      for (int p = t + part * nt; p < pieces; p += parts * nt) fn(p);
+    }
+  };
+  // all keys of the thread's group, for the slow paths
   auto each = [&](auto&& f) {
     if (extra >= 0) f(key_of(ex, extra));
-#pragma unroll 1
-    for (int p = tid; p < pieces; p += nt) {
+    group(tid, 0, 1, [&](int p) {
       uint32_t w[4];
       piece(p, w);
 #pragma unroll
       for (int j = 0; j < E; ++j) f(key_of(element<T>(w, j), head + p * E + j));
-    }
+    });
   };
-  if (tid == 0) count = listed = 0;
+  if (tid == 0) count = listed = nans = 0;
+  for (int i = nt + tid; i < NT; i += nt) images[i] = firsts[i] = 0u;
 
-  // the thread's largest value; a NaN is above it
+  // the group's largest value
   float most = ex;
   bool nan = ex != ex;
-  for (int p = tid; p < pieces; p += nt * kU) {
+  // (whole waves stay in the loop: the lanes exchange below; at: which of eight pieces is this thread's line)
+  for (int p = tid, at = lane & 7; p - lane < pieces; p += nt * kU, at ^= kU) {
     uint32_t w[kU][4];
 #pragma unroll
     for (int u = 0; u < kU; ++u) {
-      const int k = p + u * nt;
-      piece(k < pieces ? k : p, w[u]);     // (behind the row: the first piece again, which changes no maximum)
+      constexpr uint32_t none = sizeof(T) == 2 ? 0xff80ff80u : 0xff800000u;    // -inf
+      w[u][0] = w[u][1] = w[u][2] = w[u][3] = none;
+      if (p + u * nt < pieces) piece(p + u * nt, w[u]);
     }
 #pragma unroll
-    for (int u = 0; u < kU; ++u)
+    for (int u = 0; u < kU; ++u) {
+      float top = -INFINITY;
 #pragma unroll
       for (int j = 0; j < E; j += 2) {
         const float x = element<T>(w[u], j), y = element<T>(w[u], j + 1);
-        most = fmaxf(fmaxf(x, y), most);
+        top = fmaxf(fmaxf(x, y), top);
         nan |= __builtin_isunordered(x, y);
       }
+      if (lines) {                         // uniform: over the line's eight lanes
+        top = fmaxf(top, dpp_move<0xb1, 0xf>(top));            // quad_perm(1,0,3,2)
+        top = fmaxf(top, dpp_move<0x4e, 0xf>(top));            // quad_perm(2,3,0,1)
+        top = fmaxf(top, dpp_move<0x141, 0xf>(top));           // row_half_mirror
+        if (at != u) top = -INFINITY;
+      }
+      most = fmaxf(most, top);
+    }
   }
-  const bool some = tid < pieces || extra >= 0;                // (a thread that holds nothing has no part in this)
-  const uint32_t mine = !some ? 0u : nan ? 0xffffffffu : image_of(most);
+  bool some = extra >= 0;                  // (a thread whose group holds nothing has no part in this)
+  group(tid, 0, 8, [&](int) { some = true; });
+  const uint32_t mine = some ? image_of(most) : 0u;
   images[tid] = mine;
-  for (int i = nt + tid; i < NT; i += nt) images[i] = 0u;
+  firsts[tid] = 0u;
+  if (nan) nans = 1;
   __syncthreads();
 
   if (wave == 0) {
@@ -166,7 +198,6 @@ __global__ __launch_bounds__(NT, 8) void top_kernel(const T* logits, int64_t str
         if ((uint32_t)(k >> 32) == a) first = max(first, (uint32_t)k);
       });
     firsts[tid] = first;
-    for (int i = nt + tid; i < NT; i += nt) firsts[i] = 0u;
     __syncthreads();
     if (wave == 0) {
       uint32_t fi[NT / 64];
@@ -199,29 +230,24 @@ __global__ __launch_bounds__(NT, 8) void top_kernel(const T* logits, int64_t str
   if (extra >= 0) append(key_of(ex, extra));
   __syncthreads();
 
-  // the pieces of the listed threads: 2^lg threads a turn of the list, the others on their further pieces
-  int lg = 0;
-  while ((1 << lg) < min(listed, nt)) ++lg;
-  const float value = a == 0xffffffffu || a == 1u ? -INFINITY   // (a key below `least` may pass this one)
-                                                  : __uint_as_float((a & 0x80000000u) ? (a & 0x7fffffffu) : ~a);
-  const int step = max(nt >> lg, 1);       // (threads past step << lg, of which there are too few for a turn, stay out)
-  if ((tid >> lg) < step && (tid & ((1 << lg) - 1)) < listed) {
-    const int who = list[tid & ((1 << lg) - 1)];
-    for (int p = (tid >> lg) * nt + who; p < pieces; p += step * nt) {
-      uint32_t w[4];
-      piece(p, w);
+  // the listed groups, eight threads each
+  const float value = a == 1u ? -INFINITY : __uint_as_float((a & 0x80000000u) ? (a & 0x7fffffffu) : ~a);
+  if (!nans)
+    for (int i = tid >> 3; i < listed; i += nt >> 3)
+      group(list[i], tid & 7, 8, [&](int p) {
+        uint32_t w[4];
+        piece(p, w);
 #pragma unroll
-      for (int j = 0; j < E; ++j) {
-        const float x = element<T>(w, j);
-        if (!(x < value)) append(key_of(x, head + p * E + j));
-      }
-    }
-  }
+        for (int j = 0; j < E; ++j) {
+          const float x = element<T>(w, j);
+          if (x >= value) append(key_of(x, head + p * E + j));
+        }
+      });
   __syncthreads();
   int n = count;
-  if (n > kCap) {                          // uniform: the exact K-th largest key of the whole row
-    int got = n;
-    const uint64_t lo = bisect(least, (uint64_t)~0ull, K, K, got, [&](uint64_t v) {
+  if (n > kCap || nans) {                  // uniform: the exact K-th largest key of the whole row
+    int got = V;
+    const uint64_t lo = bisect((uint64_t)1, (uint64_t)~0ull, K, K, got, [&](uint64_t v) {
       int c = 0;
       each([&](uint64_t k) { c += k >= v; });
 #pragma unroll
@@ -242,12 +268,15 @@ __global__ __launch_bounds__(NT, 8) void top_kernel(const T* logits, int64_t str
     __syncthreads();
     n = K;
   }
-  for (int i = tid; i < n; i += nt) {
+  for (int i = tid >> 3; i < n; i += nt >> 3) {                // eight threads a key
     const uint64_t k = keys[i];
     int rank = 0;
-#pragma unroll 8
-    for (int j = 0; j < n; ++j) rank += keys[j] > k;
-    if (rank < K) {
+#pragma unroll 4
+    for (int j = tid & 7; j < n; j += 8) rank += keys[j] > k;
+    rank += __shfl_xor(rank, 1);
+    rank += __shfl_xor(rank, 2);
+    rank += __shfl_xor(rank, 4);
+    if (rank < K && (tid & 7) == 0) {
       const int at = (int)~(uint32_t)k;
       values[(int64_t)blockIdx.x * K + rank] = row[at];
       tokens[(int64_t)blockIdx.x * K + rank] = at;
@@ -258,9 +287,9 @@ __global__ __launch_bounds__(NT, 8) void top_kernel(const T* logits, int64_t str
 template <typename T>
 int launch(const void* logits, int64_t stride, int64_t rows, int V, int K, void* values, int64_t* tokens, hipStream_t s) {
   constexpr int E = 16 / sizeof(T);
-  const int need = ((V + E - 1) / E + 63) / 64 * 64;           // a piece a thread, or more
+  const int pieces = (V + E - 1) / E, need = (pieces + 63) / 64 * 64;          // a piece a thread, or more
   const dim3 grid((unsigned)rows);
-  if (rows < kMany)
+  if (rows < kMany || pieces >= kLong)
     top_kernel<T, 1024><<<grid, dim3((unsigned)(need < 1024 ? need : 1024)), 0, s>>>((const T*)logits, stride, V, K,
                                                                                     (T*)values, tokens);
   else

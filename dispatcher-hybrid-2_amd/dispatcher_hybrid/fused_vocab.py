@@ -14,7 +14,6 @@ execution launched without one.
 Importing this module loads the kernel library and raises ImportError if it is missing.
 """
 
-import contextlib
 from typing import List, Optional
 
 import torch
@@ -29,9 +28,14 @@ _INTS = (torch.int32, torch.int64)
 _REDUCTION = {"none": 0, "mean": 1, "sum": 2}
 
 
-def _on(t):
-    """The device of t as the current one (a launch goes to the current device)."""
-    return contextlib.nullcontext() if t.get_device() == torch.cuda.current_device() else torch.cuda.device(t.device)
+def _call(t, what, fn, *args):
+    """fn(*args, the current stream of t's device), with t's device as the current one (a launch goes to that)."""
+    if t.get_device() == torch.cuda.current_device():
+        st = fn(*args, _hip.stream_handle(t.device))
+    else:
+        with torch.cuda.device(t.device):
+            st = fn(*args, _hip.stream_handle(t.device))
+    _hip.check(st, what)
 
 
 def _bits(t):
@@ -54,10 +58,8 @@ def _lookup(weight, tokens, scale, zero_token):
     w = weight if weight.stride(1) == 1 and weight.stride(0) >= d else weight.contiguous()
     ids = tokens.contiguous()
     out = torch.empty(*tokens.shape, d, device=w.device, dtype=w.dtype)
-    with _on(w):
-        st = _hip.lib.dh_embed_fwd(code, _hip.ptr(w), w.stride(0), V, d, _hip.ptr(ids), _bits(ids), ids.numel(), scale,
-                                   zero_token, _hip.ptr(out), d, _hip.stream_handle(w.device))
-    _hip.check(st, what)
+    _call(w, what, _hip.lib.dh_embed_fwd, code, w.data_ptr(), w.stride(0), V, d, ids.data_ptr(), _bits(ids), ids.numel(), scale,
+          zero_token, out.data_ptr(), d)
     return out
 
 
@@ -72,10 +74,8 @@ def _lookup_grad(dy, tokens, rows, scale, skip_token):
     out = torch.empty(rows, d, device=dy.device, dtype=dy.dtype)
     nbytes = _hip.lib.dh_embed_bwd_workspace_bytes(ids.numel(), rows, d)
     ws = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=dy.device)     # refused sizes: the call below says why
-    with _on(dy):
-        st = _hip.lib.dh_embed_bwd(code, _hip.ptr(dy2), dy2.stride(0), _hip.ptr(ids), _bits(ids), ids.numel(), rows, d,
-                                   scale, skip_token, _hip.ptr(out), _hip.ptr(ws), ws.numel(), _hip.stream_handle(dy.device))
-    _hip.check(st, what)
+    _call(dy, what, _hip.lib.dh_embed_bwd, code, dy2.data_ptr(), dy2.stride(0), ids.data_ptr(), _bits(ids), ids.numel(), rows, d,
+          scale, skip_token, out.data_ptr(), ws.data_ptr(), ws.numel())
     return out
 
 
@@ -138,7 +138,8 @@ class _Embed(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dy):
         tokens, = ctx.saved_tensors
-        return _EmbedGrad.apply(dy, tokens, *ctx.args), None, None, None, None
+        grad = _EmbedGrad.apply if torch.is_grad_enabled() else _lookup_grad
+        return grad(dy, tokens, *ctx.args), None, None, None, None
 
 
 class _EmbedGrad(torch.autograd.Function):
@@ -198,10 +199,8 @@ def _top(logits, k):
     rows = _unit_rows(logits.reshape(-1, V))
     values = torch.empty(*logits.shape[:-1], max(k, 0), device=logits.device, dtype=logits.dtype)
     tokens = torch.empty(values.shape, device=logits.device, dtype=torch.int64)
-    with _on(logits):
-        st = _hip.lib.dh_top_logits(code, _hip.ptr(rows), rows.stride(0), rows.shape[0], V, k, _hip.ptr(values),
-                                    _hip.ptr(tokens), _hip.stream_handle(logits.device))
-    _hip.check(st, what)
+    _call(logits, what, _hip.lib.dh_top_logits, code, rows.data_ptr(), rows.stride(0), rows.shape[0], V, k, values.data_ptr(),
+          tokens.data_ptr())
     return [values, tokens]
 
 
@@ -249,12 +248,18 @@ def _rows_of(logits):
 def _distill_args(logits, teacher_logits, teacher_tokens, labels, temperature, weight, ignore_index):
     """The arguments both directions share, and the tensors they point to (held until the launch)."""
     z, sb, st, B, T = _rows_of(logits)
+    if not B * T:
+        B, T = 0, 1
     tl, tt = teacher_logits.contiguous(), teacher_tokens.contiguous()
     lb = None if labels is None else labels.contiguous()
-    p = _hip.ptr
-    return (_hip.dtype_code(z.dtype), p(z), sb, st, B, max(T, 1) if B * T else 1, z.shape[-1], _hip.dtype_code(tl.dtype), p(tl),
-            p(tt), _bits(tt), tl.shape[-1], p(lb), 64 if lb is None else _bits(lb), ignore_index, temperature,
-            weight), (z, tl, tt, lb)
+    return (_hip.dtype_code(z.dtype), z.data_ptr(), sb, st, B, T, z.shape[-1], _hip.dtype_code(tl.dtype), tl.data_ptr(),
+            tt.data_ptr(), _bits(tt), tl.shape[-1], None if lb is None else lb.data_ptr(), 64 if lb is None else _bits(lb),
+            ignore_index, temperature, weight), (z, tl, tt, lb)
+
+
+def _kept_numel(n):
+    """fp32 numbers of what a backward pass keeps of n rows: four a row and, behind them, the divisor (and to 16 bytes)."""
+    return 4 * n + 4
 
 
 def _distill_fwd(logits, teacher_logits, teacher_tokens, labels, temperature, weight, ignore_index, reduction):
@@ -263,34 +268,31 @@ def _distill_fwd(logits, teacher_logits, teacher_tokens, labels, temperature, we
     dev, lead = logits.device, logits.shape[:-1]
     n = lead.numel()
     args, held = _distill_args(logits, teacher_logits, teacher_tokens, labels, temperature, weight, ignore_index)
-    if n == 0:
-        args = (*args[:4], 0, 1, *args[6:])
-    rows = torch.empty(lead, device=dev, dtype=torch.float32)
-    kept = torch.empty(n, 4, device=dev, dtype=torch.float32)
-    # (apart: the loss may be changed in place, and the backward pass reads the divisor)
-    loss, divisor = (torch.empty((), device=dev, dtype=torch.float32) if reduction else None for _ in range(2))
+    # the loss apart (it may be changed in place); in one buffer what is kept, the rows' losses where they are no result, and
+    # the workspace
+    out = torch.empty(() if reduction else lead, device=dev, dtype=torch.float32)
     nbytes = _hip.lib.dh_distill_workspace_bytes(args[0], n, logits.shape[-1])
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-    with _on(logits):
-        st = _hip.lib.dh_distill_fwd(*args, reduction, _hip.ptr(rows), _hip.ptr(kept), _hip.ptr(loss), _hip.ptr(divisor),
-                                     _hip.ptr(ws), nbytes, _hip.stream_handle(dev))
-    _hip.check(st, what)
-    return (rows, kept, None) if reduction == 0 else (loss, kept, divisor)
+    first = _kept_numel(n)
+    rows = -(-n // 4) * 4 if reduction else 0
+    kept = torch.empty(first + rows + -(-nbytes // 4), device=dev, dtype=torch.float32)
+    at = kept.data_ptr()
+    _call(logits, what, _hip.lib.dh_distill_fwd, *args, reduction, at + 4 * first if reduction else out.data_ptr(), at,
+          out.data_ptr() if reduction else None, at + 16 * n if reduction else None, at + 4 * (first + rows), nbytes)
+    return out, kept
 
 
-def _distill_bwd(g, logits, teacher_logits, teacher_tokens, labels, kept, divisor, temperature, weight, ignore_index, reduction):
+def _distill_bwd(g, logits, teacher_logits, teacher_tokens, labels, kept, temperature, weight, ignore_index, reduction):
     what = "distillation_loss gradient"
-    _hip.same_gpu(what, logits, g, teacher_logits, teacher_tokens, labels, kept, divisor)
+    _hip.same_gpu(what, logits, g, teacher_logits, teacher_tokens, labels, kept)
     dz = torch.empty(logits.shape, device=logits.device, dtype=logits.dtype)
     if dz.numel() == 0:
         return dz
     args, held = _distill_args(logits, teacher_logits, teacher_tokens, labels, temperature, weight, ignore_index)
     g = g.float().reshape(-1)
     kept = kept.contiguous()                                                   # (a saved-tensor hook may change the layout)
-    with _on(logits):
-        st = _hip.lib.dh_distill_bwd(*args, _hip.ptr(kept), _hip.ptr(g), g.stride(0) if reduction == 0 else 0,
-                                     _hip.ptr(divisor), _hip.ptr(dz), _hip.stream_handle(logits.device))
-    _hip.check(st, what)
+    at = kept.data_ptr()
+    _call(logits, what, _hip.lib.dh_distill_bwd, *args, at, g.data_ptr(), 0 if reduction else g.stride(0),
+          at + 16 * logits.shape[:-1].numel() if reduction else None, dz.data_ptr())
     return dz
 
 
@@ -298,9 +300,8 @@ def _distill_bwd(g, logits, teacher_logits, teacher_tokens, labels, kept, diviso
 def _distill_op(logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_tokens: torch.Tensor,
                 labels: Optional[torch.Tensor], temperature: float, weight: float, ignore_index: int,
                 reduction: int) -> List[torch.Tensor]:
-    loss, kept, divisor = _distill_fwd(logits, teacher_logits, teacher_tokens, labels, temperature, weight, ignore_index,
-                                       reduction)
-    return [loss, kept, loss.new_empty(0) if divisor is None else divisor]
+    out, kept = _distill_fwd(logits, teacher_logits, teacher_tokens, labels, temperature, weight, ignore_index, reduction)
+    return [out, kept[:_kept_numel(logits.shape[:-1].numel())].clone()]        # (a size that its fake form can say)
 
 
 @_distill_op.register_fake
@@ -310,34 +311,31 @@ def _(logits, teacher_logits, teacher_tokens, labels, temperature, weight, ignor
     n = 1
     for s in lead:
         n = n * s
-    return [logits.new_empty(lead if reduction == 0 else (), dtype=f32), logits.new_empty((n, 4), dtype=f32),
-            logits.new_empty((0,) if reduction == 0 else (), dtype=f32)]
+    return [logits.new_empty(() if reduction else lead, dtype=f32), logits.new_empty((_kept_numel(n),), dtype=f32)]
 
 
 @torch.library.custom_op("dispatcher::distillation_loss_grad", mutates_args=(), device_types="cuda")
 def _distill_grad_op(g: torch.Tensor, logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_tokens: torch.Tensor,
-                     labels: Optional[torch.Tensor], kept: torch.Tensor, divisor: torch.Tensor, temperature: float,
-                     weight: float, ignore_index: int, reduction: int) -> torch.Tensor:
-    return _distill_bwd(g, logits, teacher_logits, teacher_tokens, labels, kept, divisor if reduction else None, temperature,
-                        weight, ignore_index, reduction)
+                     labels: Optional[torch.Tensor], kept: torch.Tensor, temperature: float, weight: float, ignore_index: int,
+                     reduction: int) -> torch.Tensor:
+    return _distill_bwd(g, logits, teacher_logits, teacher_tokens, labels, kept, temperature, weight, ignore_index, reduction)
 
 
 @_distill_grad_op.register_fake
-def _(g, logits, teacher_logits, teacher_tokens, labels, kept, divisor, temperature, weight, ignore_index, reduction):
+def _(g, logits, teacher_logits, teacher_tokens, labels, kept, temperature, weight, ignore_index, reduction):
     return logits.new_empty(logits.shape)
 
 
 def _distill_setup(ctx, inputs, output):
     logits, teacher_logits, teacher_tokens, labels, *args = inputs
-    _, kept, divisor = output
     ctx.set_materialize_grads(False)
-    ctx.save_for_backward(logits, teacher_logits, teacher_tokens, labels, kept, divisor)
+    ctx.save_for_backward(logits, teacher_logits, teacher_tokens, labels, output[1])
     ctx.args = tuple(args)
 
 
 def _again(ctx, g):
     """The gradient in the logits from the formula as torch operations, differentiable itself (create_graph)."""
-    logits, teacher_logits, teacher_tokens, labels, _, _ = ctx.saved_tensors
+    logits, teacher_logits, teacher_tokens, labels, _ = ctx.saved_tensors
     temperature, weight, ignore_index, reduction = ctx.args
     z = logits.view_as(logits)
     loss = plain.distillation_loss(z, teacher_logits, teacher_tokens, labels, temperature, weight, ignore_index,
