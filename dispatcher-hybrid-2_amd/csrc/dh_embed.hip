@@ -119,11 +119,31 @@ struct Owners {
   __host__ __device__ int slots() const { return range << lg; }
 };
 
+// Few positions (SMALL): the owner of a token adds its rows too, in the same launch. A token of few rows is a wave's, one of
+// many (kMany) the workgroup's, each wave a sixteenth of them. Up to kSmallRows rows and kSmallBytes of dy, since one token may
+// hold all of it and a CU reads some 50 GB/s. Against three launches in a graph, bf16: 200 x 64, V 1000 6.0 and 15.3 us;
+// 128 x 1024, V 50257 21.5 and 22.1; 512 x 1024 of one token 29.7 and 23.6, 4096 x 128 of one token 56 and 20. Two launches
+// fewer for the host.
+constexpr int64_t kSmallBytes = 1 << 20;
+constexpr int kSmallRows = 512;
+static_assert(kSmallRows <= kPW * kList, "a wave's ids all fit its list");
+constexpr int kMany = 64;
+constexpr int kFew = 16;                   // dy rows in flight a wave
+
+struct Sink {                              // what SMALL adds to
+  const void* dy;
+  int64_t ldy;
+  void* dW;
+  float scale;
+  int pieces;
+};
+
+template <typename T, int N, bool SMALL>
 __global__ __launch_bounds__(kPT) void place_kernel(const void* ids, int wide, int n, int64_t V, Owners own, int64_t skip,
-                                                    int* starts, Pair* pairs) {
-  extern __shared__ int counts[];          // [wave][id owned]
-  __shared__ Pair lists[kPW][kList];
-  __shared__ int wsum[kPW], wbelow[kPW];
+                                                    int* starts, Pair* pairs, Sink to) {
+  extern __shared__ int counts[];          // [wave][id owned]; SMALL: behind them the starts of the ids and all positions
+  __shared__ __align__(16) Pair lists[kPW][kList];
+  __shared__ int wsum[kPW], wbelow[kPW], many;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);   // (uniform: masks stay scalar)
   const int me = blockIdx.x, mask = (1 << own.lg) - 1, range = own.range;
   for (int i = tid; i < kPW * range; i += kPT) counts[i] = 0;
@@ -218,10 +238,17 @@ __global__ __launch_bounds__(kPT) void place_kernel(const void* ids, int wide, i
   if (lane == 63) wsum[wave] = incl;
   __syncthreads();
   int at = incl - total;
-  for (int w = 0; w < kPW; ++w) at += wbelow[w] + (w < wave ? wsum[w] : 0);
+  for (int w = 0; w < kPW; ++w) at += (SMALL ? 0 : wbelow[w]) + (w < wave ? wsum[w] : 0);
+  int* const from = counts + kPW * range;                      // (SMALL) start of every id, their end
+  int* const order = from + range + 1;                         // (SMALL) positions by id
   if (tid < range) {
-    starts[me * range + tid] = at;
-    if (me == mask && tid == range - 1) starts[own.slots()] = at + total;
+    if (SMALL) {
+      from[tid] = at;
+      if (tid == range - 1) from[range] = at + total;
+    } else {
+      starts[me * range + tid] = at;
+      if (me == mask && tid == range - 1) starts[own.slots()] = at + total;
+    }
     for (int w = 0; w < kPW; ++w) {
       const int c = counts[w * range + tid];
       counts[w * range + tid] = at;
@@ -239,16 +266,90 @@ __global__ __launch_bounds__(kPT) void place_kernel(const void* ids, int wide, i
         mine[its >> own.lg] = base + __popcll(same);
       }
       base = __builtin_amdgcn_readlane(base, lead);
-      if ((same >> lane) & 1) pairs[base + __popcll(same & ((1ull << lane) - 1))] = Pair{its, pos};
+      if ((same >> lane) & 1) {
+        const int i = base + __popcll(same & ((1ull << lane) - 1));
+        if (SMALL)
+          order[i] = pos;
+        else
+          pairs[i] = Pair{its, pos};
+      }
     });
   };
-  if (found == listed) {
+  if (SMALL || found == listed) {
     for (int i = 0; i < found; i += 64) {
       const Pair p = list[min(i + lane, found - 1)];
       place(p.token, p.pos, __ballot(i + lane < found));
     }
   } else {
     scan(place);
+  }
+
+  if constexpr (SMALL) {
+    typedef Piece<T, N> P;
+    typedef typename P::raw raw;
+    const T* dy = reinterpret_cast<const T*>(to.dy);
+    raw* dW = reinterpret_cast<raw*>(to.dW);
+    const int pieces = to.pieces;
+    // the sum of the rows at order[i0, i1), piece c of them (its lanes past the row read its last piece)
+    auto add = [&](int i0, int i1, int c, float (&acc)[N]) {
+#pragma unroll
+      for (int j = 0; j < N; ++j) acc[j] = 0.f;
+      for (int i = i0; i < i1; i += kFew) {
+        const int pos = order[min(i + (lane & (kFew - 1)), i1 - 1)];
+        raw v[kFew];
+#pragma unroll
+        for (int k = 0; k < kFew; ++k)
+          v[k] = reinterpret_cast<const raw*>(dy + (int64_t)__builtin_amdgcn_readlane(pos, k) * to.ldy)[min(c, pieces - 1)];
+#pragma unroll
+        for (int k = 0; k < kFew; ++k) {
+          float x[N];
+          P::unpack(v[k], x);
+#pragma unroll
+          for (int j = 0; j < N; ++j) acc[j] += i + k < i1 ? x[j] : 0.f;
+        }
+      }
+    };
+    if (tid == 0) many = 0;
+    __syncthreads();
+    int* const big = counts;               // (the counters are done with)
+    for (int r = wave; r < range; r += kPW) {
+      const int64_t token = ((int64_t)r << own.lg) + me;
+      if (token >= V) break;
+      const int i0 = __builtin_amdgcn_readfirstlane(from[r]), i1 = __builtin_amdgcn_readfirstlane(from[r + 1]);
+      if (i1 - i0 > kMany) {
+        if (lane == 0) big[atomicAdd(&many, 1)] = r;
+        continue;
+      }
+      for (int c = lane; c - lane < pieces; c += 64) {
+        float acc[N];
+        add(i0, i1, c, acc);
+#pragma unroll
+        for (int j = 0; j < N; ++j) acc[j] = i1 > i0 ? acc[j] * to.scale : 0.f;
+        if (c < pieces) dW[token * pieces + c] = P::pack(acc);
+      }
+    }
+    __syncthreads();
+    float* const parts = reinterpret_cast<float*>(&lists[0][0]);               // [wave][64 N]
+    static_assert(sizeof(lists) >= kPW * 64 * N * sizeof(float), "the partial sums lie over the lists");
+    for (int b = 0; b < many; ++b) {
+      const int r = big[b], i0 = from[r], i1 = from[r + 1], stretch = (i1 - i0 + kPW - 1) / kPW;
+      const int j0 = __builtin_amdgcn_readfirstlane(min(i0 + wave * stretch, i1)), j1 = min(j0 + stretch, i1);
+      for (int first = 0; first < pieces; first += 64) {
+        float acc[N];
+        add(j0, j1, first + lane, acc);
+#pragma unroll
+        for (int j = 0; j < N; ++j) parts[(wave * 64 + lane) * N + j] = acc[j];
+        __syncthreads();
+        const int e = first * N + tid;
+        if (tid < 64 * N && e < pieces * N) {
+          float x = 0.f;
+#pragma unroll
+          for (int w = 0; w < kPW; ++w) x += parts[w * 64 * N + tid];
+          Elem<T>::store(reinterpret_cast<T*>(to.dW) + (((int64_t)r << own.lg) + me) * pieces * N + e, x * to.scale);
+        }
+        __syncthreads();
+      }
+    }
   }
 }
 
@@ -445,8 +546,20 @@ int gradient(const void* dy, int64_t ldy, const void* ids, int wide, int64_t n, 
   int* starts = (int*)(ws + l.starts);
   Pair* pairs = (Pair*)(ws + l.pairs);
   float* part = (float*)(ws + l.part);
-  place_kernel<<<dim3(1u << own.lg), dim3(kPT), kPW * own.range * sizeof(int), s>>>(ids, wide, (int)n, V, own, skip, starts,
-                                                                                   pairs);
+  const Sink to{dy, ldy, dW, scale, pieces};
+  const dim3 owners(1u << own.lg);
+  if (n <= kSmallRows && n * d * (int64_t)sizeof(T) <= kSmallBytes) {
+    const int lds = (kPW * own.range + own.range + 1 + (int)n) * (int)sizeof(int);
+    if (lds > 28 << 10) {                  // (64 KB with the lists)
+      const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&place_kernel<T, N, true>),
+                                               hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+      if (e != hipSuccess) return dh_fail(DH_ERR_LAUNCH_FAILED, "dh_embed_bwd: %d bytes of LDS: %s", lds, hipGetErrorString(e));
+    }
+    place_kernel<T, N, true><<<owners, dim3(kPT), lds, s>>>(ids, wide, (int)n, V, own, skip, starts, pairs, to);
+    return dh_check_launch("dh_embed_bwd");
+  }
+  place_kernel<T, N, false><<<owners, dim3(kPT), kPW * own.range * sizeof(int), s>>>(ids, wide, (int)n, V, own, skip, starts,
+                                                                                    pairs, to);
   if (int st = dh_check_launch("dh_embed_bwd")) return st;
   const int slices = (pieces + 63) / 64;
   const int sums = (int)((l.chunks * slices + kST / 64 - 1) / (kST / 64));

@@ -21,16 +21,16 @@ REDUCTIONS = ("none", "mean", "sum")
 
 def check_targets(logits, teacher_logits, teacher_tokens, labels, temperature, weight, reduction):
     """Raise unless these are a distillation_loss call."""
-    if logits.dim() < 1 or not logits.is_floating_point():
-        raise ValueError(f"distillation_loss: logits (..., vocabulary) expected, got {tuple(logits.shape)} {logits.dtype}")
-    lead = tuple(logits.shape[:-1])
-    if tuple(teacher_logits.shape) != tuple(teacher_tokens.shape) or tuple(teacher_logits.shape[:-1]) != lead \
-            or teacher_logits.dim() != logits.dim():
-        raise ValueError(f"distillation_loss: teacher logits {tuple(teacher_logits.shape)} and tokens "
-                         f"{tuple(teacher_tokens.shape)} must both be {lead + ('k',)}, for logits {tuple(logits.shape)}")
-    if not 1 <= teacher_logits.shape[-1] <= MAX_TARGETS:
-        raise ValueError(f"distillation_loss: {teacher_logits.shape[-1]} targets a position, 1 to {MAX_TARGETS} possible")
-    if logits.shape[-1] < 1:
+    shape, targets = logits.shape, teacher_logits.shape
+    if not shape or not logits.is_floating_point():
+        raise ValueError(f"distillation_loss: logits (..., vocabulary) expected, got {tuple(shape)} {logits.dtype}")
+    lead = shape[:-1]
+    if targets != teacher_tokens.shape or targets[:-1] != lead or len(targets) != len(shape):
+        raise ValueError(f"distillation_loss: teacher logits {tuple(targets)} and tokens {tuple(teacher_tokens.shape)} must both "
+                         f"be {(*lead, 'k')}, for logits {tuple(shape)}")
+    if not 1 <= targets[-1] <= MAX_TARGETS:
+        raise ValueError(f"distillation_loss: {targets[-1]} targets a position, 1 to {MAX_TARGETS} possible")
+    if shape[-1] < 1:
         raise ValueError("distillation_loss: empty vocabulary")
     if teacher_logits.requires_grad:
         raise ValueError("distillation_loss: the teacher's logits are constants; detach them")
@@ -41,8 +41,8 @@ def check_targets(logits, teacher_logits, teacher_tokens, labels, temperature, w
     if labels is not None:
         if labels.dtype not in (torch.int32, torch.int64):
             raise TypeError(f"distillation_loss: labels must be int32 or int64, got {labels.dtype}")
-        if tuple(labels.shape) != lead:
-            raise ValueError(f"distillation_loss: labels {tuple(labels.shape)} for logits {tuple(logits.shape)}")
+        if labels.shape != lead:
+            raise ValueError(f"distillation_loss: labels {tuple(labels.shape)} for logits {tuple(shape)}")
     if not (0.0 < temperature < math.inf):
         raise ValueError(f"distillation_loss: temperature {temperature} must be positive and finite")
     if not 0.0 <= weight <= 1.0:

@@ -76,6 +76,7 @@ def tokens_of(kind, n, V, g):
     (1, 1, 1, "any"), (1, 50257, 1024, "any"), (63, 7, 8, "any"), (64, 300, 64, "text"), (65, 256, 33, "padded"),
     (1025, 257, 128, "one"), (4097, 50257, 1024, "text"), (9001, 1000, 100, "padded"), (40000, 5, 24, "any"),
     (33000, 70001, 72, "text"), (3000, 50257, 1030, "one"), (2048, 140000, 16, "any"), (3001, 512, 2048, "text"),
+    (3000, 120001, 40, "text"), (511, 120001, 40, "text"), (512, 50257, 1024, "one"), (400, 50257, 1024, "padded"), (4096, 300, 128, "text"),
 ])
 def test_embedding_and_gradient(n, V, d, kind, dtype):
     say("embed", n, V, d, kind, dtype)
