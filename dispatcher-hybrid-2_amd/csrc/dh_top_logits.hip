@@ -3,7 +3,8 @@
 //   values are equal (0.0 and -0.0 are), NaN above every number.
 //
 // A value and its token make one 64-bit key, different for every element: an order-preserving 32-bit image of the value
-// above the complement of the token. The K largest keys are the answer, with no case for ties.
+// above the complement of the token. The K largest keys are the answer, with no case for ties; below the token a bit says
+// which zero it was, so that a key has its value whole (NaN apart).
 //
 // One workgroup a row, which reads the row once and goes back to a tenth of it or less:
 //   - the largest value of every group of logits, one group a thread: its own 16-byte pieces or, in long rows, one 128-byte
@@ -19,6 +20,8 @@
 // (Rows kept in registers instead of read again: 130 us in place of 92 at 4096 x 50257 bf16; a wave a row with a running
 // bound: 219 us; groups of pieces from eight lines each, which going back reads whole: 106 us.)
 
+#include <type_traits>
+
 #include "dh_common.h"
 
 namespace {
@@ -30,6 +33,7 @@ constexpr int kCap = 9 * kMaxK;            // keys in LDS: ties leave up to E K 
 // (bf16, V 50257: 92 against 102 us at 4096 rows, 31 against 35 at 1024, 21 both at 512; V 8000, 4096 rows: 42 against 74;
 // 16000 pieces, 1024 rows: 56 against 52; fp32, V 50257, 1024 rows: 50 against 45).
 constexpr int kMany = 512, kLong = 8192;
+constexpr int kFew = 128;                  // keys up to which a thread ranks one (K 64: 95 keys or so, 256: 330)
 constexpr int kU = 4;                      // 16-byte loads in flight a thread
 
 __device__ __forceinline__ uint32_t image_of(float x) {        // a < b  <=>  image(a) < image(b); NaN above all
@@ -37,7 +41,13 @@ __device__ __forceinline__ uint32_t image_of(float x) {        // a < b  <=>  im
   const uint32_t u = __float_as_uint(x + 0.0f);                // -0.0 as 0.0
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
-__device__ __forceinline__ uint64_t key_of(float x, int token) { return ((uint64_t)image_of(x) << 32) | ~(uint32_t)token; }
+__device__ __forceinline__ float value_of(uint32_t image) {
+  return __uint_as_float((image & 0x80000000u) ? (image & 0x7fffffffu) : ~image);
+}
+__device__ __forceinline__ uint64_t key_of(float x, int token) {               // token < 2^24
+  return ((uint64_t)image_of(x) << 32) | (~(uint32_t)token << 8) | (__float_as_uint(x) == 0x80000000u ? 1u : 0u);
+}
+__device__ __forceinline__ int token_of(uint64_t key) { return (int)(~(uint32_t)key >> 8); }
 
 template <typename T>
 __device__ __forceinline__ float element(const uint32_t (&w)[4], int j) {      // element j of 16 bytes
@@ -91,28 +101,19 @@ __global__ __launch_bounds__(NT, 8) void top_kernel(const T* logits, int64_t str
   const int extra = tid < head ? tid : tid < head + tail ? V - tail + (tid - head) : -1;   // token of the single logit
   const float ex = extra >= 0 ? Elem<T>::load(row + extra) : -INFINITY;
   const bool lines = pieces >= 4 * nt;
-  // fn(piece) for the pieces of thread t's group, part of parts
-  auto group = [&](int t, int part, int parts, auto&& fn) {
-    if (lines) {
-#pragma unroll 1
-      for (int p = (t & 7) * nt + (t & ~7); p < pieces; p += 8 * nt)
-#pragma unroll 1
-        for (int i = part; i < 8; i += parts)
-          if (p + i < pieces) fn(p + i);
-    } else {
-#pragma unroll 1
-      for (int p = t + part * nt; p < pieces; p += parts * nt) fn(p);
-    }
-  };
+  const int first_piece = lines ? (tid & 7) * nt + (tid & ~7) : tid;           // of the thread's group
   // all keys of the thread's group, for the slow paths
   auto each = [&](auto&& f) {
     if (extra >= 0) f(key_of(ex, extra));
-    group(tid, 0, 1, [&](int p) {
-      uint32_t w[4];
-      piece(p, w);
+#pragma unroll 1
+    for (int p = first_piece; p < pieces; p += lines ? 8 * nt : nt)
+#pragma unroll 1
+      for (int i = 0; i < (lines ? min(8, pieces - p) : 1); ++i) {
+        uint32_t w[4];
+        piece(p + i, w);
 #pragma unroll
-      for (int j = 0; j < E; ++j) f(key_of(element<T>(w, j), head + p * E + j));
-    });
+        for (int j = 0; j < E; ++j) f(key_of(element<T>(w, j), head + (p + i) * E + j));
+      }
   };
   if (tid == 0) count = listed = nans = 0;
   for (int i = nt + tid; i < NT; i += nt) images[i] = firsts[i] = 0u;
@@ -121,7 +122,7 @@ __global__ __launch_bounds__(NT, 8) void top_kernel(const T* logits, int64_t str
   float most = ex;
   bool nan = ex != ex;
   // (whole waves stay in the loop: the lanes exchange below; at: which of eight pieces is this thread's line)
-  for (int p = tid, at = lane & 7; p - lane < pieces; p += nt * kU, at ^= kU) {
+  for (int p = tid, at = lane & 7; p - lane < pieces; p += nt * kU, at = (at - kU) & 7) {
     uint32_t w[kU][4];
 #pragma unroll
     for (int u = 0; u < kU; ++u) {
@@ -147,8 +148,7 @@ __global__ __launch_bounds__(NT, 8) void top_kernel(const T* logits, int64_t str
       most = fmaxf(most, top);
     }
   }
-  bool some = extra >= 0;                  // (a thread whose group holds nothing has no part in this)
-  group(tid, 0, 8, [&](int) { some = true; });
+  const bool some = extra >= 0 || first_piece < pieces;        // (a thread whose group holds nothing has no part in this)
   const uint32_t mine = some ? image_of(most) : 0u;
   images[tid] = mine;
   firsts[tid] = 0u;
@@ -231,18 +231,41 @@ __global__ __launch_bounds__(NT, 8) void top_kernel(const T* logits, int64_t str
   __syncthreads();
 
   // the listed groups, eight threads each
-  const float value = a == 1u ? -INFINITY : __uint_as_float((a & 0x80000000u) ? (a & 0x7fffffffu) : ~a);
-  if (!nans)
-    for (int i = tid >> 3; i < listed; i += nt >> 3)
-      group(list[i], tid & 7, 8, [&](int p) {
-        uint32_t w[4];
-        piece(p, w);
+  const float value = a == 1u ? -INFINITY : value_of(a);
+  if (!nans) {
+    constexpr int R = 4;                   // groups in flight
+    const int eighth = nt >> 3, stretch = 8 * nt;
+    for (int begin = 0; begin < pieces; begin += stretch)      // (of a group: eight pieces a stretch, one of them here)
+      for (int i = tid >> 3; i < listed; i += R * eighth) {
+        uint32_t w[R][4];
+        int at[R];
 #pragma unroll
-        for (int j = 0; j < E; ++j) {
-          const float x = element<T>(w, j);
-          if (x >= value) append(key_of(x, head + p * E + j));
+        for (int u = 0; u < R; ++u) {
+          at[u] = pieces;
+          w[u][0] = w[u][1] = w[u][2] = w[u][3] = 0u;
+          if (i + u * eighth < listed) {
+            const int t = list[i + u * eighth], j = tid & 7;
+            at[u] = begin + (lines ? (t & 7) * nt + (t & ~7) + j : j * nt + t);
+            if (at[u] < pieces) piece(at[u], w[u]);
+          }
         }
-      });
+#pragma unroll
+        for (int u = 0; u < R; ++u) {
+          uint32_t pass = 0u;              // a bit an element: nearly always one of a wave's turns is enough for all lanes
+#pragma unroll
+          for (int j = 0; j < E; ++j) pass |= element<T>(w[u], j) >= value ? 1u << j : 0u;
+          if (at[u] >= pieces) pass = 0u;
+          while (pass) {
+            const int j = __builtin_ctz(pass);
+            pass &= pass - 1u;
+            const int d = sizeof(T) == 2 ? j >> 1 : j;
+            const uint32_t two = d & 2 ? (d & 1 ? w[u][3] : w[u][2]) : (d & 1 ? w[u][1] : w[u][0]);
+            const float x = __uint_as_float(sizeof(T) == 4 ? two : (j & 1) ? two & 0xffff0000u : two << 16);
+            append(key_of(x, head + at[u] * E + j));
+          }
+        }
+      }
+  }
   __syncthreads();
   int n = count;
   if (n > kCap || nans) {                  // uniform: the exact K-th largest key of the whole row
@@ -268,20 +291,44 @@ __global__ __launch_bounds__(NT, 8) void top_kernel(const T* logits, int64_t str
     __syncthreads();
     n = K;
   }
-  for (int i = tid >> 3; i < n; i += nt >> 3) {                // eight threads a key
-    const uint64_t k = keys[i];
-    int rank = 0;
+  // ranks, eight threads each; four keys a thread where there are many, so that a key read serves four
+  auto ranks = [&](auto many) {
+    constexpr int R = many ? 4 : 1;
+    for (int i = (tid >> 3) * R; i < n; i += (nt >> 3) * R) {
+      uint64_t k[R];
+      int rank[R];
+#pragma unroll
+      for (int u = 0; u < R; ++u) {
+        k[u] = keys[min(i + u, n - 1)];
+        rank[u] = 0;
+      }
 #pragma unroll 4
-    for (int j = tid & 7; j < n; j += 8) rank += keys[j] > k;
-    rank += __shfl_xor(rank, 1);
-    rank += __shfl_xor(rank, 2);
-    rank += __shfl_xor(rank, 4);
-    if (rank < K && (tid & 7) == 0) {
-      const int at = (int)~(uint32_t)k;
-      values[(int64_t)blockIdx.x * K + rank] = row[at];
-      tokens[(int64_t)blockIdx.x * K + rank] = at;
+      for (int j = tid & 7; j < n; j += 8) {
+        const uint64_t other = keys[j];
+#pragma unroll
+        for (int u = 0; u < R; ++u) rank[u] += other > k[u];
+      }
+#pragma unroll
+      for (int u = 0; u < R; ++u) {
+        rank[u] += __shfl_xor(rank[u], 1);
+        rank[u] += __shfl_xor(rank[u], 2);
+        rank[u] += __shfl_xor(rank[u], 4);
+        if (rank[u] < K && i + u < n && (tid & 7) == u) {
+          const int token = token_of(k[u]);
+          T* out = values + (int64_t)blockIdx.x * K + rank[u];
+          if (nans)
+            *out = row[token];
+          else
+            Elem<T>::store(out, (k[u] & 1u) ? -0.0f : value_of((uint32_t)(k[u] >> 32)));
+          tokens[(int64_t)blockIdx.x * K + rank[u]] = token;
+        }
+      }
     }
-  }
+  };
+  if (n > kFew)
+    ranks(std::true_type{});
+  else
+    ranks(std::false_type{});
 }
 
 template <typename T>
