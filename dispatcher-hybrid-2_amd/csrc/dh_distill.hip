@@ -560,6 +560,9 @@ int check(const char* who, int dtype, const Rows& a, int t_dtype, int token_bits
              "%s: temperature %g, weight %g", who, (double)a.tau, (double)a.weight);
   DH_REQUIRE(a.rows == 0 || a.labels || a.weight == 1.f, DH_ERR_INVALID_ARG, "%s: weight %g without labels", who, (double)a.weight);
   DH_REQUIRE(a.rows == 0 || (a.logits && a.t_logits && a.t_tokens), DH_ERR_INVALID_ARG, "%s: null pointer argument", who);
+  DH_REQUIRE((uintptr_t)a.logits % (dtype == DH_BF16 ? 2 : 4) == 0 && (uintptr_t)a.t_logits % (t_dtype == DH_BF16 ? 2 : 4) == 0 &&
+                 (uintptr_t)a.t_tokens % (token_bits / 8) == 0 && (!a.labels || (uintptr_t)a.labels % (label_bits / 8) == 0),
+             DH_ERR_INVALID_ARG, "%s: operands not aligned to their elements", who);
   return 0;
 }
 

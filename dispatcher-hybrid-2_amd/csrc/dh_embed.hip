@@ -516,6 +516,7 @@ Layout layout_of(int64_t n, int64_t V, int d) {
   return l;
 }
 
+bool aligned(int dtype, const void* p) { return (uintptr_t)p % (dtype == DH_BF16 ? 2 : 4) == 0; }
 bool sizes_ok(int64_t n, int64_t V, int d) {
   return n >= 0 && n < ((int64_t)1 << 24) && V >= 1 && V <= ((int64_t)1 << 24) && d >= 1 && d <= (1 << 20);
 }
@@ -588,6 +589,8 @@ extern "C" int dh_embed_fwd(int dtype, const void* W, int64_t ldw, int64_t V, in
              (long long)ldo, d);
   if (n == 0) return 0;
   DH_REQUIRE(W && ids && out, DH_ERR_INVALID_ARG, "%s: null pointer argument", who);
+  DH_REQUIRE(aligned(dtype, W) && aligned(dtype, out) && (uintptr_t)ids % (ids_bits / 8) == 0, DH_ERR_INVALID_ARG,
+             "%s: operands not aligned to their elements", who);
   hipStream_t s = (hipStream_t)stream;
   const int wide = ids_bits == 64;
   const int N = dtype == DH_BF16 ? 8 : 4;
@@ -616,6 +619,8 @@ extern "C" int dh_embed_bwd(int dtype, const void* dy, int64_t ldy, const void* 
   DH_REQUIRE(workspace_bytes >= layout_of(n, V, d).bytes && (uintptr_t)workspace % 16 == 0, DH_ERR_INVALID_ARG,
              "%s: workspace of %lld bytes, 16-byte aligned %lld needed", who, (long long)workspace_bytes,
              (long long)layout_of(n, V, d).bytes);
+  DH_REQUIRE(aligned(dtype, dy) && aligned(dtype, dW) && (uintptr_t)ids % (ids_bits / 8) == 0, DH_ERR_INVALID_ARG,
+             "%s: operands not aligned to their elements", who);
   hipStream_t s = (hipStream_t)stream;
   const int wide = ids_bits == 64;
   const int N = dtype == DH_BF16 ? 8 : 4;

@@ -8,8 +8,8 @@ Kernels: ``dh_embed_fwd`` / ``dh_embed_bwd``, ``dh_top_logits``, ``dh_distill_fw
 under ``model.enable_fused_vocab()``; ``distillation.py`` has the formulas as torch operations. fp32 and bf16; sums are fp32
 or wider, in an order that does not change from call to call.
 
-Each is one registered operation (``dispatcher::embed_tokens``, ...) for compilers and transforms, and in plain eager
-execution launched without one.
+Each is one registered operation (``dispatcher::embed_tokens``, ...) for compilers, which torch.func's transforms refuse, and
+in plain eager execution launched without one.
 
 Importing this module loads the kernel library and raises ImportError if it is missing.
 """
@@ -289,7 +289,8 @@ def _distill_bwd(g, logits, teacher_logits, teacher_tokens, labels, kept, temper
         return dz
     args, held = _distill_args(logits, teacher_logits, teacher_tokens, labels, temperature, weight, ignore_index)
     g = g.float().reshape(-1)
-    kept = kept.contiguous()                                                   # (a saved-tensor hook may change the layout)
+    if not kept.is_contiguous() or kept.data_ptr() % 16:                       # (a saved-tensor hook may change the layout)
+        kept = kept.clone(memory_format=torch.contiguous_format)
     at = kept.data_ptr()
     _call(logits, what, _hip.lib.dh_distill_bwd, *args, at, g.data_ptr(), 0 if reduction else g.stride(0),
           at + 16 * logits.shape[:-1].numel() if reduction else None, dz.data_ptr())

@@ -529,6 +529,91 @@ def test_two_captured_steps_replayed_in_turn():
                 assert torch.equal(a, b), turn
 
 
+def test_under_a_compiler_and_a_transform():
+    z, t, tok, labels = inputs((2, 9), 501, 5, torch.float32, 21)
+    W, ids = torch.randn(50, 16, device=DEV, generator=gen(2)), torch.randint(0, 50, (3, 7), device=DEV, generator=gen(3))
+
+    def step(z, W):
+        values, tokens = ops().top_logits(z * 2, 5)
+        return ops().distillation_loss(z, values, tokens, labels, 2.0, 0.5) + ops().embed_tokens(ids, W, 2.0).square().sum()
+    grads = []
+    for fn in (step, torch.compile(step, backend="aot_eager", fullgraph=True)):
+        a, b = z.clone().requires_grad_(), W.clone().requires_grad_()
+        loss = fn(a, b)
+        grads.append([loss.detach(), *torch.autograd.grad(loss, (a, b))])
+    for x, y in zip(*grads):
+        assert torch.equal(x, y)
+    # a registered operation has no rule for torch.func's transforms: refused, as the other training operations are
+    with pytest.raises(RuntimeError, match="functorch"):
+        torch.func.grad(step, argnums=(0, 1))(z, W)
+
+
+def test_saved_tensors_that_hooks_move():
+    z, t, tok, labels = inputs((2, 9), 501, 5, torch.bfloat16, 22)
+    W, ids = torch.randn(50, 16, device=DEV, generator=gen(2)), torch.randint(0, 50, (3, 7), device=DEV, generator=gen(3))
+
+    def step():
+        a, b = z.clone().requires_grad_(), W.clone().requires_grad_()
+        loss = ops().distillation_loss(a, t, tok, labels, 2.0, 0.5) + ops().embed_tokens(ids, b).sum()
+        return torch.autograd.grad(loss, (a, b))
+
+    def strided(x):                                            # the same values at odd addresses and strides
+        wide = torch.empty(x.numel() * 2 + 1, dtype=x.dtype, device=x.device)[1:].view(*x.shape, 2)[..., 0] if x.dim() else x
+        return wide.copy_(x) if x.dim() else x
+    ref = step()
+    with torch.autograd.graph.save_on_cpu():
+        on_cpu = step()
+    with torch.autograd.graph.saved_tensors_hooks(lambda x: x, strided):
+        moved = step()
+    for other in (on_cpu, moved):
+        assert all(torch.equal(x, y) for x, y in zip(ref, other))
+
+
+def test_captured_gradient_of_a_wide_vocabulary():
+    """The one-launch gradient with more than 64 KB of LDS, in a graph."""
+    V, n, d = 120001, 500, 40
+    ids, dy = torch.randint(0, V, (n,), device=DEV, generator=gen(2)), torch.randn(n, d, device=DEV, generator=gen(3))
+    from dispatcher_hybrid import fused_vocab
+    f = lambda: fused_vocab._lookup_grad(dy, ids, V, 1.0, -1)
+    f()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = f()
+    for seed in range(3):
+        ids.copy_(torch.randint(0, V, (n,), device=DEV, generator=gen(seed)))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, f())
+
+
+def test_two_host_threads():
+    import threading
+    z, t, tok, labels = inputs((40,), 5003, 9, torch.bfloat16, 23)
+
+    def step(z):
+        leaf = z.detach().requires_grad_()
+        loss = ops().distillation_loss(leaf, t, tok, labels, 2.0, 0.5)
+        return [*ops().top_logits(z, 9), loss.detach(), torch.autograd.grad(loss, leaf)[0]]
+    data = [z, z.flip(0)]
+    ref = [step(x) for x in data]
+    got = [None, None]
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(5):
+                got[i] = step(data[i])
+            torch.cuda.current_stream().synchronize()
+    torch.cuda.synchronize()
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join(60)
+    for x, y in zip(got, ref):
+        assert all(torch.equal(p, q) for p, q in zip(x, y))
+
+
 def test_refusals_on_the_gpu():
     W, ids = torch.randn(6, 4, device=DEV), torch.zeros(3, dtype=torch.long, device=DEV)
     tok = torch.zeros(6, 2, dtype=torch.long, device=DEV)
