@@ -120,11 +120,11 @@ struct Owners {
 };
 
 // Few positions (SMALL): the owner of a token adds its rows too, in the same launch. A token of few rows is a wave's, one of
-// many (kMany) the workgroup's, each wave a sixteenth of them. Up to kSmallRows rows and kSmallBytes of dy, since one token may
-// hold all of it and a CU reads some 50 GB/s. Against three launches in a graph, bf16: 200 x 64, V 1000 6.0 and 15.3 us;
-// 128 x 1024, V 50257 21.5 and 22.1; 512 x 1024 of one token 29.7 and 23.6, 4096 x 128 of one token 56 and 20. Two launches
-// fewer for the host.
-constexpr int64_t kSmallBytes = 1 << 20;
+// many (kMany) the workgroup's, each wave a sixteenth of them. Up to kSmallRows rows of kSmallNumbers in all, since one token
+// may hold all of them and a CU reads some 50 GB/s. Against three launches in a graph, bf16: 200 x 64, V 1000 6.0 and 15.3 us;
+// 128 x 1024, V 50257 21.5 and 22.1; 512 x 1024 of one token 29.7 and 23.6, 4096 x 128 of one token 56 and 20. Two launches and
+// the workspace fewer for the host.
+constexpr int64_t kSmallNumbers = 1 << 18;
 constexpr int kSmallRows = 512;
 static_assert(kSmallRows <= kPW * kList, "a wave's ids all fit its list");
 constexpr int kMany = 64;
@@ -516,6 +516,7 @@ Layout layout_of(int64_t n, int64_t V, int d) {
   return l;
 }
 
+bool small(int64_t n, int d) { return n <= kSmallRows && n * d <= kSmallNumbers; }
 bool aligned(int dtype, const void* p) { return (uintptr_t)p % (dtype == DH_BF16 ? 2 : 4) == 0; }
 bool sizes_ok(int64_t n, int64_t V, int d) {
   return n >= 0 && n < ((int64_t)1 << 24) && V >= 1 && V <= ((int64_t)1 << 24) && d >= 1 && d <= (1 << 20);
@@ -549,7 +550,7 @@ int gradient(const void* dy, int64_t ldy, const void* ids, int wide, int64_t n, 
   float* part = (float*)(ws + l.part);
   const Sink to{dy, ldy, dW, scale, pieces};
   const dim3 owners(1u << own.lg);
-  if (n <= kSmallRows && n * d * (int64_t)sizeof(T) <= kSmallBytes) {
+  if (small(n, d)) {
     const int lds = (kPW * own.range + own.range + 1 + (int)n) * (int)sizeof(int);
     if (lds > 28 << 10) {                  // (64 KB with the lists)
       const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&place_kernel<T, N, true>),
@@ -604,7 +605,7 @@ extern "C" int dh_embed_fwd(int dtype, const void* W, int64_t ldw, int64_t V, in
 }
 
 extern "C" int64_t dh_embed_bwd_workspace_bytes(int64_t n, int64_t V, int d) {
-  return sizes_ok(n, V, d) ? layout_of(n, V, d).bytes : -1;
+  return !sizes_ok(n, V, d) ? -1 : small(n, d) ? 0 : layout_of(n, V, d).bytes;
 }
 
 extern "C" int dh_embed_bwd(int dtype, const void* dy, int64_t ldy, const void* ids, int ids_bits, int64_t n, int64_t V, int d,
@@ -615,10 +616,10 @@ extern "C" int dh_embed_bwd(int dtype, const void* dy, int64_t ldy, const void* 
   DH_REQUIRE(ids_bits == 32 || ids_bits == 64, DH_ERR_UNSUPPORTED_DTYPE, "%s: ids of %d bits", who, ids_bits);
   DH_REQUIRE(sizes_ok(n, V, d), DH_ERR_UNSUPPORTED_SHAPE, "%s: n=%lld V=%lld d=%d", who, (long long)n, (long long)V, d);
   DH_REQUIRE(ldy >= d, DH_ERR_INVALID_ARG, "%s: row stride %lld below d=%d", who, (long long)ldy, d);
-  DH_REQUIRE(dW && workspace && (n == 0 || (dy && ids)), DH_ERR_INVALID_ARG, "%s: null pointer argument", who);
-  DH_REQUIRE(workspace_bytes >= layout_of(n, V, d).bytes && (uintptr_t)workspace % 16 == 0, DH_ERR_INVALID_ARG,
-             "%s: workspace of %lld bytes, 16-byte aligned %lld needed", who, (long long)workspace_bytes,
-             (long long)layout_of(n, V, d).bytes);
+  const int64_t need = dh_embed_bwd_workspace_bytes(n, V, d);
+  DH_REQUIRE(dW && (n == 0 || (dy && ids)), DH_ERR_INVALID_ARG, "%s: null pointer argument", who);
+  DH_REQUIRE(workspace_bytes >= need && (need == 0 || workspace) && (uintptr_t)workspace % 16 == 0, DH_ERR_INVALID_ARG,
+             "%s: workspace of %lld bytes, 16-byte aligned %lld needed", who, (long long)workspace_bytes, (long long)need);
   DH_REQUIRE(aligned(dtype, dy) && aligned(dtype, dW) && (uintptr_t)ids % (ids_bits / 8) == 0, DH_ERR_INVALID_ARG,
              "%s: operands not aligned to their elements", who);
   hipStream_t s = (hipStream_t)stream;

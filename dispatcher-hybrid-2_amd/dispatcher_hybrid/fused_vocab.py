@@ -30,12 +30,14 @@ _REDUCTION = {"none": 0, "mean": 1, "sum": 2}
 
 def _call(t, what, fn, *args):
     """fn(*args, the current stream of t's device), with t's device as the current one (a launch goes to that)."""
-    if t.get_device() == torch.cuda.current_device():
-        st = fn(*args, _hip.stream_handle(t.device))
-    else:
-        with torch.cuda.device(t.device):
-            st = fn(*args, _hip.stream_handle(t.device))
-    _hip.check(st, what)
+    index = t.get_device()
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
+            return _call(t, what, fn, *args)
+    # (the raw handle: no stream object, no ctypes object)
+    st = fn(*args, _hip._raw_stream(index) if _hip._raw_stream is not None else _hip.stream_handle(t.device))
+    if st:
+        _hip.check(st, what)
 
 
 def _bits(t):
@@ -73,9 +75,9 @@ def _lookup_grad(dy, tokens, rows, scale, skip_token):
         dy2 = dy2.clone(memory_format=torch.contiguous_format)
     out = torch.empty(rows, d, device=dy.device, dtype=dy.dtype)
     nbytes = _hip.lib.dh_embed_bwd_workspace_bytes(ids.numel(), rows, d)
-    ws = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=dy.device)     # refused sizes: the call below says why
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dy.device) if nbytes > 0 else None  # (refused sizes: the call says why)
     _call(dy, what, _hip.lib.dh_embed_bwd, code, dy2.data_ptr(), dy2.stride(0), ids.data_ptr(), _bits(ids), ids.numel(), rows, d,
-          scale, skip_token, out.data_ptr(), ws.data_ptr(), ws.numel())
+          scale, skip_token, out.data_ptr(), None if ws is None else ws.data_ptr(), nbytes)
     return out
 
 

@@ -577,8 +577,8 @@ int dh_embed_fwd(int dtype, const void* W, int64_t ldw, int64_t V, int d, const 
  * The lookup's gradient: dW[v] = scale * sum of dy[n] over the positions n with ids[n] = v, ascending, for every v (rows of
  * zeros where there is none): fp32 sums in an order that depends on the ids alone, rounded once. Positions that hold
  * skip_token (-1: none) or an id outside [0, V) are left out. dy (n, d) rows ldy apart; dW (V, d) contiguous.
- *   workspace: dh_embed_bwd_workspace_bytes(n, V, d) bytes (-1: sizes outside the limits), 16-byte aligned; contents are
- *   needed during the call only.
+ *   workspace: dh_embed_bwd_workspace_bytes(n, V, d) bytes (0 for few positions, -1: sizes outside the limits), 16-byte
+ *   aligned; contents are needed during the call only.
  */
 int64_t dh_embed_bwd_workspace_bytes(int64_t n, int64_t V, int d);
 int dh_embed_bwd(int dtype, const void* dy, int64_t ldy, const void* ids, int ids_bits, int64_t n, int64_t V, int d,

@@ -186,10 +186,13 @@ def test_c_entry_points_refuse_before_any_launch():
     assert lib.dh_embed_fwd(1, one, 7, 8, 8, one, 64, 1, 1.0, -1, one, 8, N) == 1
     assert lib.dh_embed_fwd(1, N, 8, 8, 8, one, 64, 1, 1.0, -1, one, 8, N) == 1
     assert lib.dh_embed_bwd_workspace_bytes(1 << 24, 8, 8) == -1
-    need = lib.dh_embed_bwd_workspace_bytes(100, 50, 8)
+    assert lib.dh_embed_bwd_workspace_bytes(100, 50, 8) == 0     # few positions: one launch
+    need = lib.dh_embed_bwd_workspace_bytes(1000, 50, 8)
     assert need > 0
-    assert lib.dh_embed_bwd(1, one, 8, one, 64, 100, 50, 8, 1.0, -1, one, one, need - 1, N) == 1
+    assert lib.dh_embed_bwd(1, one, 8, one, 64, 1000, 50, 8, 1.0, -1, one, one, need - 1, N) == 1
     assert b"workspace" in lib.dh_last_error()
+    assert lib.dh_embed_bwd(1, one + 1, 8, one, 64, 100, 50, 8, 1.0, -1, one, N, 0, N) == 1
+    assert b"aligned" in lib.dh_last_error()
     assert lib.dh_embed_bwd(1, one, 8, one, 64, 100, 0, 8, 1.0, -1, one, one, need, N) == 2
     assert lib.dh_top_logits(1, one, 8, 1, 8, 9, one, one, N) == 2 and b"K=9" in lib.dh_last_error()
     assert lib.dh_top_logits(1, one, 8, 1, 8, 0, one, one, N) == 2
