@@ -12,6 +12,8 @@
 // tokens that the teacher or the label names are written again after the row, from fp32, by a wave that has them ready by then;
 // a token named twice gets the sum of its slots in their order.
 //
+// 4096 x 50257 bf16, K 64, an eighth of the rows ignored: forward 73 us (360 MB, 4.9 TB/s), backward 154 us (772 MB, 5.0 TB/s).
+//
 // Exponents are taken of z - m (exact for bf16 inputs near m), never of z times a constant: rows of the type's lowest value
 // stay finite. The few operations on a row's sums are in fp64: log p - log q is a small difference of larger numbers.
 
@@ -428,7 +430,7 @@ __global__ __launch_bounds__(kRT) void reduce_kernel(const float* losses, const 
 // ---- backward -------------------------------------------------------------------------------------------------------
 // Gradients of kPast bytes or more are stored past the caches: what reads them next would find little of them there (the last
 // level holds 256 MB), and unwritten lines no longer stand in the way of reading the logits (forward and backward of
-// 4096 x 50257 bf16, 412 MB: 242 -> 227 us). Smaller ones stay for the product that takes them.
+// 4096 x 50257 bf16, 412 MB: 244 -> 227 us). Smaller ones stay for the product that takes them.
 constexpr int64_t kPast = (int64_t)256 << 20;
 
 // Rows in descending order: the forward pass read the last rows last, and what the caches still hold of them is read first.

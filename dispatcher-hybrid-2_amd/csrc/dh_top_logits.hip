@@ -17,8 +17,8 @@
 //   - a key's rank is the number of larger keys; ranks below K write their value and token.
 // Ties at the bound (masked vocabularies, constant rows) take the lower tokens first. Rows with a NaN, and rows whose large
 // values all stand in few groups, more than LDS holds, are bisected as a whole, slowly. The first pass is bound by its read.
-// (Rows kept in registers instead of read again: 130 us in place of 92 at 4096 x 50257 bf16; a wave a row with a running
-// bound: 219 us; groups of pieces from eight lines each, which going back reads whole: 106 us.)
+// 4096 x 50257 bf16, K 64: 84 us, 4.9 TB/s. (Rows kept in registers instead of read again: 130 us; a wave a row with a
+// running bound: 219 us; groups of pieces from eight lines each, which going back reads whole: 106 us.)
 
 #include <type_traits>
 
@@ -29,9 +29,9 @@ namespace {
 constexpr int kMaxK = 256;
 constexpr int kSlack = 32;                 // threads more than K that end the bisection
 constexpr int kCap = 9 * kMaxK;            // keys in LDS: ties leave up to E K of them, and K above
-// Rows from which a row of fewer than kLong pieces gets 512 threads in place of 1024, so that four rows share a CU
-// (bf16, V 50257: 92 against 102 us at 4096 rows, 31 against 35 at 1024, 21 both at 512; V 8000, 4096 rows: 42 against 74;
-// 16000 pieces, 1024 rows: 56 against 52; fp32, V 50257, 1024 rows: 50 against 45).
+// Rows from which a row of fewer than kLong pieces gets 512 threads in place of 1024, so that four rows share a CU (K 64, in a
+// graph; bf16, V 50257: 90 against 105 us at 4096 rows, 32 against 34 at 1024, 20 against 21 at 512; V 8000, 4096 rows: 40
+// against 75; 16000 pieces, 1024 rows: 60 against 53; fp32, V 50257, 1024 rows: 48 against 45).
 constexpr int kMany = 512, kLong = 8192;
 constexpr int kFew = 128;                  // keys up to which a thread ranks one (K 64: 95 keys or so, 256: 330)
 constexpr int kU = 4;                      // 16-byte loads in flight a thread
