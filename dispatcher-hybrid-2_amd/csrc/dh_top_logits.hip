@@ -17,7 +17,7 @@
 //   - a key's rank is the number of larger keys; ranks below K write their value and token.
 // Ties at the bound (masked vocabularies, constant rows) take the lower tokens first. Rows with a NaN, and rows whose large
 // values all stand in few groups, more than LDS holds, are bisected as a whole, slowly. The first pass is bound by its read.
-// 4096 x 50257 bf16, K 64: 84 us, 4.9 TB/s. (Rows kept in registers instead of read again: 130 us; a wave a row with a
+// 4096 x 50257 bf16, K 64: 79 us, 5.2 TB/s. (Rows kept in registers instead of read again: 130 us; a wave a row with a
 // running bound: 219 us; groups of pieces from eight lines each, which going back reads whole: 106 us.)
 
 #include <type_traits>
@@ -57,6 +57,9 @@ __device__ __forceinline__ float element(const uint32_t (&w)[4], int j) {      /
     return __uint_as_float(w[j]);
 }
 
+// The larger one, NaN if one is: v_maximum3_f32 takes a pair more, and asks for no canonical input.
+__device__ __forceinline__ float larger(float x, float y) { return __builtin_elementwise_maximum(x, y); }
+
 // The largest v in [lo, hi] with count(v) >= need, given count(lo) >= need; ends early once the count is at most `enough`.
 // got: the count at the result. All uniform in the wave.
 template <typename V, typename F>
@@ -76,7 +79,7 @@ __device__ __forceinline__ V bisect(V lo, V hi, int need, int enough, int& got, 
 
 // The row's whole aligned 16-byte pieces, thread t reads those of t, t + nt, ... (nt threads), and what stands before the first
 // and behind the last of them, up to 2 (E - 1) logits, one each with the first threads' groups. Groups of thread t: the pieces
-// it reads, or (lines) of each stretch of 8 nt pieces the eight from (t mod 8) nt + 8 floor(t / 8).
+// it reads, or (lines) of each stretch of 8 nt pieces the eight from line(t) nt + 8 floor(t / 8).
 template <typename T, int NT>
 __global__ __launch_bounds__(NT, 8) void top_kernel(const T* logits, int64_t stride, int V, int K, T* values,
                                                       int64_t* tokens) {
@@ -101,7 +104,9 @@ __global__ __launch_bounds__(NT, 8) void top_kernel(const T* logits, int64_t str
   const int extra = tid < head ? tid : tid < head + tail ? V - tail + (tid - head) : -1;   // token of the single logit
   const float ex = extra >= 0 ? Elem<T>::load(row + extra) : -INFINITY;
   const bool lines = pieces >= 4 * nt;
-  const int first_piece = lines ? (tid & 7) * nt + (tid & ~7) : tid;           // of the thread's group
+  // which of a stretch's eight pieces is on the line of thread t, as the exchange below leaves them
+  auto line = [](int t) { return (t & 1) << 2 | (t & 4) >> 1 | (t & 2) >> 1; };
+  const int first_piece = lines ? line(tid) * nt + (tid & ~7) : tid;           // of the thread's group
   // all keys of the thread's group, for the slow paths
   auto each = [&](auto&& f) {
     if (extra >= 0) f(key_of(ex, extra));
@@ -118,36 +123,45 @@ __global__ __launch_bounds__(NT, 8) void top_kernel(const T* logits, int64_t str
   if (tid == 0) count = listed = nans = 0;
   for (int i = nt + tid; i < NT; i += nt) images[i] = firsts[i] = 0u;
 
-  // the group's largest value
+  // the group's largest value (NaN where it has one: the maxima propagate it)
   float most = ex;
-  bool nan = ex != ex;
-  // (whole waves stay in the loop: the lanes exchange below; at: which of eight pieces is this thread's line)
-  for (int p = tid, at = lane & 7; p - lane < pieces; p += nt * kU, at = (at - kU) & 7) {
+  bool odd = false;                        // of a stretch's eight pieces: the first or the last four
+  auto four = [&](int p, auto whole) {     // whole: none of the wave's four pieces is behind the last
     uint32_t w[kU][4];
 #pragma unroll
     for (int u = 0; u < kU; ++u) {
       constexpr uint32_t none = sizeof(T) == 2 ? 0xff80ff80u : 0xff800000u;    // -inf
-      w[u][0] = w[u][1] = w[u][2] = w[u][3] = none;
-      if (p + u * nt < pieces) piece(p + u * nt, w[u]);
+      if constexpr (whole) {
+        piece(p + u * nt, w[u]);
+      } else {
+        w[u][0] = w[u][1] = w[u][2] = w[u][3] = none;
+        if (p + u * nt < pieces) piece(p + u * nt, w[u]);
+      }
     }
+    float top[kU];
 #pragma unroll
     for (int u = 0; u < kU; ++u) {
-      float top = -INFINITY;
+      top[u] = larger(element<T>(w[u], 0), element<T>(w[u], 1));
 #pragma unroll
-      for (int j = 0; j < E; j += 2) {
-        const float x = element<T>(w[u], j), y = element<T>(w[u], j + 1);
-        top = fmaxf(fmaxf(x, y), top);
-        nan |= __builtin_isunordered(x, y);
-      }
-      if (lines) {                         // uniform: over the line's eight lanes
-        top = fmaxf(top, dpp_move<0xb1, 0xf>(top));            // quad_perm(1,0,3,2)
-        top = fmaxf(top, dpp_move<0x4e, 0xf>(top));            // quad_perm(2,3,0,1)
-        top = fmaxf(top, dpp_move<0x141, 0xf>(top));           // row_half_mirror
-        if (at != u) top = -INFINITY;
-      }
-      most = fmaxf(most, top);
+      for (int j = 2; j < E; j += 2) top[u] = larger(larger(element<T>(w[u], j), element<T>(w[u], j + 1)), top[u]);
     }
-  }
+    if (lines) {                           // uniform: each lane gives away what it is not to keep, four values in three steps
+      const bool b2 = lane & 4, b1 = lane & 2;
+      const float x = larger(b2 ? top[2] : top[0], dpp_move<0x141, 0xf>(b2 ? top[0] : top[2]));    // row_half_mirror
+      const float y = larger(b2 ? top[3] : top[1], dpp_move<0x141, 0xf>(b2 ? top[1] : top[3]));
+      float z = larger(b1 ? y : x, dpp_move<0x4e, 0xf>(b1 ? x : y));           // quad_perm(2,3,0,1)
+      z = larger(z, dpp_move<0xb1, 0xf>(z));                                   // quad_perm(1,0,3,2)
+      if ((bool)(lane & 1) == odd) most = larger(most, z);
+    } else {
+      most = larger(larger(larger(top[0], top[1]), larger(top[2], top[3])), most);
+    }
+    odd = !odd;
+  };
+  static_assert(kU == 4, "");
+  int at = tid;                            // (whole waves stay in the loops: the lanes exchange above)
+  for (; at - lane + 63 + (kU - 1) * nt < pieces; at += nt * kU) four(at, std::true_type{});
+  for (; at - lane < pieces; at += nt * kU) four(at, std::false_type{});
+  const bool nan = most != most;
   const bool some = extra >= 0 || first_piece < pieces;        // (a thread whose group holds nothing has no part in this)
   const uint32_t mine = some ? image_of(most) : 0u;
   images[tid] = mine;
@@ -234,37 +248,48 @@ __global__ __launch_bounds__(NT, 8) void top_kernel(const T* logits, int64_t str
   const float value = a == 1u ? -INFINITY : value_of(a);
   if (!nans) {
     constexpr int R = 4;                   // groups in flight
-    const int eighth = nt >> 3, stretch = 8 * nt;
-    for (int begin = 0; begin < pieces; begin += stretch)      // (of a group: eight pieces a stretch, one of them here)
-      for (int i = tid >> 3; i < listed; i += R * eighth) {
-        uint32_t w[R][4];
-        int at[R];
+    const int eighth = nt >> 3, stretch = 8 * nt, heard = listed;
+    // pairs of a group and a stretch (eight pieces of the group, one of them here), group by group in each stretch
+    int i = tid >> 3, begin = 0;
+    auto settle = [&] {
+      while (i >= heard && begin < pieces) {
+        i -= heard;
+        begin += stretch;
+      }
+    };
+    settle();
+    while (__any(begin < pieces)) {        // (a wave's lanes leave together; nothing below waits for other waves)
+      uint32_t w[R][4];
+      int at[R];
 #pragma unroll
-        for (int u = 0; u < R; ++u) {
-          at[u] = pieces;
-          w[u][0] = w[u][1] = w[u][2] = w[u][3] = 0u;
-          if (i + u * eighth < listed) {
-            const int t = list[i + u * eighth], j = tid & 7;
-            at[u] = begin + (lines ? (t & 7) * nt + (t & ~7) + j : j * nt + t);
-            if (at[u] < pieces) piece(at[u], w[u]);
-          }
+      for (int u = 0; u < R; ++u) {
+        at[u] = pieces;
+        w[u][0] = w[u][1] = w[u][2] = w[u][3] = 0u;
+        if (begin < pieces) {
+          const int t = list[i], j = tid & 7;
+          at[u] = begin + (lines ? line(t) * nt + (t & ~7) + j : j * nt + t);
+          if (at[u] < pieces) piece(at[u], w[u]);
         }
+        i += eighth;
+        settle();
+      }
 #pragma unroll
-        for (int u = 0; u < R; ++u) {
-          uint32_t pass = 0u;              // a bit an element: nearly always one of a wave's turns is enough for all lanes
+      for (int u = 0; u < R; ++u) {
+        if (!__any(at[u] < pieces)) continue;                  // (often one or two of the four are taken)
+        uint32_t pass = 0u;                // a bit an element: nearly always one of a wave's turns is enough for all lanes
 #pragma unroll
-          for (int j = 0; j < E; ++j) pass |= element<T>(w[u], j) >= value ? 1u << j : 0u;
-          if (at[u] >= pieces) pass = 0u;
-          while (pass) {
-            const int j = __builtin_ctz(pass);
-            pass &= pass - 1u;
-            const int d = sizeof(T) == 2 ? j >> 1 : j;
-            const uint32_t two = d & 2 ? (d & 1 ? w[u][3] : w[u][2]) : (d & 1 ? w[u][1] : w[u][0]);
-            const float x = __uint_as_float(sizeof(T) == 4 ? two : (j & 1) ? two & 0xffff0000u : two << 16);
-            append(key_of(x, head + at[u] * E + j));
-          }
+        for (int j = 0; j < E; ++j) pass |= element<T>(w[u], j) >= value ? 1u << j : 0u;
+        if (at[u] >= pieces) pass = 0u;
+        while (pass) {
+          const int j = __builtin_ctz(pass);
+          pass &= pass - 1u;
+          const int d = sizeof(T) == 2 ? j >> 1 : j;
+          const uint32_t two = d & 2 ? (d & 1 ? w[u][3] : w[u][2]) : (d & 1 ? w[u][1] : w[u][0]);
+          const float x = __uint_as_float(sizeof(T) == 4 ? two : (j & 1) ? two & 0xffff0000u : two << 16);
+          append(key_of(x, head + at[u] * E + j));
         }
       }
+    }
   }
   __syncthreads();
   int n = count;
