@@ -30,8 +30,8 @@ constexpr int kMaxK = 256;
 constexpr int kSlack = 32;                 // threads more than K that end the bisection
 constexpr int kCap = 9 * kMaxK;            // keys in LDS: ties leave up to E K of them, and K above
 // Rows from which a row of fewer than kLong pieces gets 512 threads in place of 1024, so that four rows share a CU (K 64, in a
-// graph; bf16, V 50257: 90 against 105 us at 4096 rows, 32 against 34 at 1024, 20 against 21 at 512; V 8000, 4096 rows: 40
-// against 75; 16000 pieces, 1024 rows: 60 against 53; fp32, V 50257, 1024 rows: 48 against 45).
+// graph; bf16, V 50257: 85 against 95 us at 4096 rows, 29 against 33 at 1024, 19 against 20 at 512; V 8000, 4096 rows: 38
+// against 73; 16000 pieces, 1024 rows: 56 against 50; fp32, V 50257, 1024 rows: 48 against 43).
 constexpr int kMany = 512, kLong = 8192;
 constexpr int kFew = 128;                  // keys up to which a thread ranks one (K 64: 95 keys or so, 256: 330)
 constexpr int kU = 4;                      // 16-byte loads in flight a thread
