@@ -79,6 +79,7 @@ __global__ __launch_bounds__(kLT) void lookup_kernel(const T* W, int64_t ldw, in
   typedef Piece<T, N> P;
   const int64_t row = (((int64_t)blockIdx.x << (8 - lg)) + (threadIdx.x >> lg)) * R;
   if (row >= n) return;
+  const float stray = zero_token < 0 ? __builtin_nanf("") : 0.f;
   int64_t id[R];
 #pragma unroll
   for (int r = 0; r < R; ++r) id[r] = load_id(ids, wide, min(row + r, n - 1));
@@ -94,7 +95,7 @@ __global__ __launch_bounds__(kLT) void lookup_kernel(const T* W, int64_t ldw, in
       float v[N];
       P::unpack(q[r], v);
 #pragma unroll
-      for (int j = 0; j < N; ++j) v[j] = none ? 0.f : ok ? v[j] * scale : __builtin_nanf("");
+      for (int j = 0; j < N; ++j) v[j] = !ok ? stray : none ? 0.f : v[j] * scale;
       reinterpret_cast<typename P::raw*>(out + (row + r) * ldo)[c] = P::pack(v);
     }
   }
@@ -587,6 +588,7 @@ extern "C" int dh_embed_fwd(int dtype, const void* W, int64_t ldw, int64_t V, in
   DH_REQUIRE(dtype == DH_F32 || dtype == DH_BF16, DH_ERR_UNSUPPORTED_DTYPE, "%s: dtype %d", who, dtype);
   DH_REQUIRE(ids_bits == 32 || ids_bits == 64, DH_ERR_UNSUPPORTED_DTYPE, "%s: ids of %d bits", who, ids_bits);
   DH_REQUIRE(sizes_ok(n, V, d), DH_ERR_UNSUPPORTED_SHAPE, "%s: n=%lld V=%lld d=%d", who, (long long)n, (long long)V, d);
+  DH_REQUIRE(zero_token >= -1 && zero_token <= V, DH_ERR_INVALID_ARG, "%s: zero_token %lld", who, (long long)zero_token);
   DH_REQUIRE(ldw >= d && ldo >= d, DH_ERR_INVALID_ARG, "%s: row strides %lld, %lld below d=%d", who, (long long)ldw,
              (long long)ldo, d);
   if (n == 0) return 0;

@@ -118,11 +118,16 @@ def _embed_grad_setup(ctx, inputs, output):
     ctx.args = (scale, skip_token)
 
 
+def _zero_token(g, skip_token):
+    """zero_token of the lookup that undoes a gradient by tokens: the left-out token, or one past the vocabulary (none)."""
+    return skip_token if skip_token >= 0 else g.shape[0]
+
+
 def _embed_grad_backward(ctx, g):
     # the gradient is linear in dy: its own gradient looks the rows of g up, zeros where positions were left out
     tokens, = ctx.saved_tensors
     scale, skip_token = ctx.args
-    return torch.ops.dispatcher.embed_tokens(g, tokens, scale, skip_token, skip_token), None, None, None, None
+    return torch.ops.dispatcher.embed_tokens(g, tokens, scale, _zero_token(g, skip_token), skip_token), None, None, None, None
 
 
 torch.library.register_autograd("dispatcher::embed_tokens", _embed_backward, setup_context=_embed_setup)
@@ -154,7 +159,7 @@ class _EmbedGrad(torch.autograd.Function):
     def backward(ctx, g):
         tokens, = ctx.saved_tensors
         scale, skip_token = ctx.args
-        return _Embed.apply(g, tokens, scale, skip_token, skip_token), None, None, None, None
+        return _Embed.apply(g, tokens, scale, _zero_token(g, skip_token), skip_token), None, None, None, None
 
 
 def embed_tokens(tokens, weight, scale=1.0, padding_idx=None):

@@ -567,8 +567,9 @@ int dh_decode_persistent_status(const void* scratch, uint32_t* out2, void* strea
  * Embedding rows: out[n] = scale * W[ids[n]], rounded once. The parallel forward's lookup (reference
  * dispatcher_hybrid/modeling_dispatcher.py:340).
  *   W (V, d) rows ldw apart; out (n, d) rows ldo apart; any d (rows that start on 16-byte boundaries with d * size a
- *   multiple of 16 move in 16-byte pieces). ids: n integers of ids_bits (32 or 64) bits. An id outside [0, V) gives a row of
- *   NaN and is not read; positions that hold zero_token (-1: none) give a row of zeros.
+ *   multiple of 16 move in 16-byte pieces). ids: n integers of ids_bits (32 or 64) bits; one outside [0, V) is not read.
+ *   zero_token -1: rows of ids outside are NaN (a lookup). In [0, V]: rows of that token and of ids outside (V: of these
+ *   alone) are zeros, the transpose of dh_embed_bwd with that skip_token.
  *   Limits of both: n < 2^24, V <= 2^24, d <= 2^20.
  */
 int dh_embed_fwd(int dtype, const void* W, int64_t ldw, int64_t V, int d, const void* ids, int ids_bits, int64_t n,

@@ -132,6 +132,36 @@ def test_embedding_gradient_of_the_gradient():
     assert torch.equal(got, (v * 2.0)[ids] * (ids != 3).unsqueeze(-1))
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", [(2, 5), (7, 150), (40, 1001)])                 # one launch, three, four rows a lane
+@pytest.mark.parametrize("wide", [False, True])
+def test_tokens_outside_the_vocabulary(wide, shape, dtype):
+    g = gen(7)
+    V, d = 90, 2048 if shape[0] == 40 else 40
+    ids = torch.randint(0, V, shape, device=DEV, generator=g)
+    strays = [-1, V, -7, -2 ** 31, 2 ** 31 - 1] + ([2 ** 40 + 3, 2 ** 32, -2 ** 32 + 5] if wide else [])
+    flat = ids.view(-1)
+    for i, s in enumerate(strays[:flat.numel() - 1]):
+        flat[(i * 37 + 1) % flat.numel()] = s
+    ids = ids if wide else ids.int()
+    ok = (ids >= 0) & (ids < V)
+    assert int((~ok).sum()) >= min(len(strays), 5)
+    for skip in (None, 3):
+        W = torch.randn(V, d, device=DEV, generator=g).to(dtype).requires_grad_()
+        dy = torch.randn(*shape, d, device=DEV, generator=g).to(dtype).requires_grad_()
+        y = ops().embed_tokens(ids, W, 1.0, skip)
+        assert torch.equal(y[ok], W[ids[ok].long()]) and bool(y[~ok].isnan().all())
+        dW, = torch.autograd.grad(y, W, dy, create_graph=True)
+        check_grad(dW.detach(), dy.detach(), ids, V, 1.0, skip)
+        v = torch.randn(V, d, device=DEV, generator=g).to(dtype)
+        again, = torch.autograd.grad(dW, dy, v)
+        used = ok if skip is None else ok & (ids != skip)
+        assert torch.equal(again[used], v[ids[used].long()]) and bool((again[~used] == 0).all())
+        x = dy.detach().requires_grad_()                                          # the registered forms
+        two = torch.ops.dispatcher.embed_tokens_grad(x, ids, V, 1.0, -1 if skip is None else skip)
+        assert torch.equal(two, dW) and torch.equal(torch.autograd.grad(two, x, v)[0], again)
+
+
 # ---- top logits -----------------------------------------------------------------------------------------------------
 
 def check_top(x, k):
