@@ -57,7 +57,8 @@ def _lookup(weight, tokens, scale, zero_token):
     _hip.same_gpu(what, weight, tokens)
     V, d = weight.shape
     code = _hip.dtype_code(weight.dtype)
-    w = weight if weight.stride(1) == 1 and weight.stride(0) >= d else weight.contiguous()
+    # (contiguous() would leave one row of any stride as it is)
+    w = weight if weight.stride(1) == 1 and weight.stride(0) >= d else weight.clone(memory_format=torch.contiguous_format)
     ids = tokens.contiguous()
     out = torch.empty(*tokens.shape, d, device=w.device, dtype=w.dtype)
     _call(w, what, _hip.lib.dh_embed_fwd, code, w.data_ptr(), w.stride(0), V, d, ids.data_ptr(), _bits(ids), ids.numel(), scale,

@@ -133,6 +133,22 @@ def test_embedding_gradient_of_the_gradient():
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d", [1, 5, 16])
+def test_a_vocabulary_of_one(d, dtype):
+    g = gen(9)
+    ids = torch.zeros(3, 7, dtype=torch.long, device=DEV)
+    for W in (torch.randn(d, device=DEV, generator=g).to(dtype).expand(1, d),     # a row stride of 0
+              torch.randn(d, 1, device=DEV, generator=g).to(dtype).t(),
+              torch.randn(1, d, device=DEV, generator=g).to(dtype)):
+        w = W.detach().requires_grad_()
+        y = ops().embed_tokens(ids, w)
+        assert torch.equal(y, W.expand(3, 7, d))
+        dy = torch.randn(d, device=DEV, generator=g).to(dtype).expand(1, d)
+        dW, = torch.autograd.grad(ops().embed_tokens(ids[0, :1], w), w, dy)       # one row, of stride 0 too
+        assert torch.equal(dW, dy)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("shape", [(2, 5), (7, 150), (40, 1001)])                 # one launch, three, four rows a lane
 @pytest.mark.parametrize("wide", [False, True])
 def test_tokens_outside_the_vocabulary(wide, shape, dtype):
