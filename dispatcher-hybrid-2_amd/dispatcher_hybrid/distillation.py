@@ -93,5 +93,8 @@ def top_logits(logits, k):
     """fused_vocab.top_logits as a stable sort."""
     if not 1 <= k <= min(MAX_TARGETS, logits.shape[-1]):
         raise ValueError(f"top_logits: k={k} must be in [1, min({MAX_TARGETS}, vocabulary {logits.shape[-1]})]")
-    values, tokens = torch.sort(logits.detach(), dim=-1, descending=True, stable=True)
-    return values[..., :k].contiguous(), tokens[..., :k].contiguous()
+    logits = logits.detach()
+    # (NaN of one sign: the GPU's sort puts one whose sign bit is set below every number)
+    order = torch.where(logits.isnan(), math.nan, logits)
+    tokens = torch.sort(order, dim=-1, descending=True, stable=True).indices[..., :k].contiguous()
+    return logits.gather(-1, tokens), tokens

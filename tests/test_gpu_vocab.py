@@ -182,7 +182,8 @@ def test_tokens_outside_the_vocabulary(wide, shape, dtype):
 
 def check_top(x, k):
     values, tokens = ops().top_logits(x, k)
-    ref, at = torch.sort(x.double(), dim=-1, descending=True, stable=True)
+    # (NaN of one sign: the GPU's sort puts one whose sign bit is set below every number, the CPU's above)
+    ref, at = torch.sort(torch.where(x.isnan(), math.nan, x.double()), dim=-1, descending=True, stable=True)
     assert torch.equal(tokens, at[..., :k])
     picked = x.gather(-1, tokens)
     assert values.dtype == x.dtype and bool(((values == picked) | (values.isnan() & picked.isnan())).all())
@@ -238,6 +239,24 @@ def test_top_logits_of_long_awkward_rows(what, V, rows, dtype):
          "equal": lambda: torch.full((rows, V), -math.inf, device=DEV)}[what]().to(dtype)
     for k in (1, 64, 256):
         check_top(x, k)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,V", [(120, 50257), (600, 50257), (600, 1501), (90, 40)])
+def test_top_logits_of_rows_with_one_nan(rows, V, dtype):
+    """One NaN a row, of either sign, in every stretch of the row and at both ends; a row in eight without."""
+    x = torch.randn(rows, V + 3, device=DEV, generator=gen(rows + V)).to(dtype)[:, 3:]      # rows of every alignment
+    at = torch.arange(rows, device=DEV) * 7919 % V
+    at[:6] = torch.tensor([0, 1, 7, V - 1, V - 2, V - 8], device=DEV)
+    bits = torch.tensor([0x7fc00000, -0x400000], dtype=torch.int32, device=DEV).view(torch.float32).to(dtype)
+    i = torch.arange(rows, device=DEV)
+    has = i % 8 != 7
+    x[i[has], at[has]] = bits[i[has] % 2]
+    assert int(x.isnan().sum()) == int(has.sum())
+    for k in (1, 33):
+        check_top(x, k)
+    for a, b in zip(plain.top_logits(x, 9), ops().top_logits(x, 9)):              # the formula sorts them as the kernel does
+        assert torch.equal(a.nan_to_num(123.0), b.nan_to_num(123.0)) if a.is_floating_point() else torch.equal(a, b)
 
 
 @pytest.mark.parametrize("dtype", TYPES)
