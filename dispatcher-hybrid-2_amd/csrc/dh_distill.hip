@@ -558,7 +558,8 @@ int check(const char* who, int dtype, const Rows& a, int t_dtype, int token_bits
   DH_REQUIRE(a.rows >= 0 && a.rows < (1 << 22) && a.T >= 1 && a.V >= 1 && a.V <= (1 << 24), DH_ERR_UNSUPPORTED_SHAPE,
              "%s: %d rows (-1: too many), T=%d V=%d", who, a.rows, a.T, a.V);
   DH_REQUIRE(a.K >= 1 && a.K <= kMaxSlots, DH_ERR_UNSUPPORTED_SHAPE, "%s: K=%d must be in [1, %d]", who, a.K, kMaxSlots);
-  DH_REQUIRE(a.tau > 0.f && a.tau < INFINITY && a.weight >= 0.f && a.weight <= 1.f, DH_ERR_INVALID_ARG,
+  // (below the least normal number its reciprocal overflows)
+  DH_REQUIRE(a.tau >= 0x1p-126f && a.tau < INFINITY && a.weight >= 0.f && a.weight <= 1.f, DH_ERR_INVALID_ARG,
              "%s: temperature %g, weight %g", who, (double)a.tau, (double)a.weight);
   DH_REQUIRE(a.rows == 0 || a.labels || a.weight == 1.f, DH_ERR_INVALID_ARG, "%s: weight %g without labels", who, (double)a.weight);
   DH_REQUIRE(a.rows == 0 || (a.logits && a.t_logits && a.t_tokens), DH_ERR_INVALID_ARG, "%s: null pointer argument", who);

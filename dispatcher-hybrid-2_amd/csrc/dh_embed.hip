@@ -618,6 +618,7 @@ extern "C" int dh_embed_bwd(int dtype, const void* dy, int64_t ldy, const void* 
   DH_REQUIRE(dtype == DH_F32 || dtype == DH_BF16, DH_ERR_UNSUPPORTED_DTYPE, "%s: dtype %d", who, dtype);
   DH_REQUIRE(ids_bits == 32 || ids_bits == 64, DH_ERR_UNSUPPORTED_DTYPE, "%s: ids of %d bits", who, ids_bits);
   DH_REQUIRE(sizes_ok(n, V, d), DH_ERR_UNSUPPORTED_SHAPE, "%s: n=%lld V=%lld d=%d", who, (long long)n, (long long)V, d);
+  DH_REQUIRE(skip_token >= -1 && skip_token < V, DH_ERR_INVALID_ARG, "%s: skip_token %lld", who, (long long)skip_token);
   DH_REQUIRE(ldy >= d, DH_ERR_INVALID_ARG, "%s: row stride %lld below d=%d", who, (long long)ldy, d);
   const int64_t need = dh_embed_bwd_workspace_bytes(n, V, d);
   DH_REQUIRE(dW && (n == 0 || (dy && ids)), DH_ERR_INVALID_ARG, "%s: null pointer argument", who);

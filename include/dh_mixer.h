@@ -607,7 +607,7 @@ int dh_top_logits(int dtype, const void* logits, int64_t row_stride, int64_t row
  *   none), divisor = their number; 2: loss = the sum, divisor = 1. row_loss (B * T) fp32; row_kept: 16 bytes a row, 16-byte
  *   aligned, for the backward pass; loss, divisor: one fp32 each.
  *   workspace: dh_distill_workspace_bytes(dtype, B * T, V) bytes (0 for many rows), needed during the call only.
- *   1 <= K <= 256, V <= 2^24, B * T < 2^22, 0 < tau, 0 <= w <= 1.
+ *   1 <= K <= 256, V <= 2^24, B * T < 2^22, 2^-126 <= tau < inf, 0 <= w <= 1.
  */
 int64_t dh_distill_workspace_bytes(int dtype, int64_t rows, int V);
 int dh_distill_fwd(int dtype, const void* logits, int64_t stride_b, int64_t stride_t, int64_t B, int T, int V,

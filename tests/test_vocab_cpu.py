@@ -185,6 +185,10 @@ def test_c_entry_points_refuse_before_any_launch():
     assert lib.dh_embed_fwd(1, one, 8, 8, 8, one, 64, 1 << 24, 1.0, -1, one, 8, N) == 2
     assert lib.dh_embed_fwd(1, one, 7, 8, 8, one, 64, 1, 1.0, -1, one, 8, N) == 1
     assert lib.dh_embed_fwd(1, N, 8, 8, 8, one, 64, 1, 1.0, -1, one, 8, N) == 1
+    for zero in (-2, 9, 1 << 40):                                # -1, a token, or one past them
+        assert lib.dh_embed_fwd(1, one, 8, 8, 8, one, 64, 1, 1.0, zero, one, 8, N) == 1 and b"zero_token" in lib.dh_last_error()
+    for skip in (-2, 8, (1 << 32) + 3):
+        assert lib.dh_embed_bwd(1, one, 8, one, 64, 100, 8, 8, 1.0, skip, one, N, 0, N) == 1 and b"skip_token" in lib.dh_last_error()
     assert lib.dh_embed_bwd_workspace_bytes(1 << 24, 8, 8) == -1
     assert lib.dh_embed_bwd_workspace_bytes(100, 50, 8) == 0     # few positions: one launch
     need = lib.dh_embed_bwd_workspace_bytes(1000, 50, 8)
@@ -205,7 +209,7 @@ def test_c_entry_points_refuse_before_any_launch():
         a.update(kw)
         return lib.dh_distill_fwd(*a.values(), N)
     for kw, code in ((dict(dtype=5), 3), (dict(td=5), 3), (dict(bits=8), 3), (dict(lb=one, lbits=8), 3), (dict(K=0), 2),
-                     (dict(K=257), 2), (dict(V=0), 2), (dict(B=1 << 22), 2), (dict(tau=0.0), 1), (dict(tau=math.nan), 1),
+                     (dict(K=257), 2), (dict(V=0), 2), (dict(B=1 << 22), 2), (dict(tau=0.0), 1), (dict(tau=1e-40), 1), (dict(tau=math.nan), 1),
                      (dict(w=0.5), 1), (dict(w=-1.0), 1), (dict(red=3), 1), (dict(rows=N), 1), (dict(kept=one + 4), 1),
                      (dict(loss=N), 1), (dict(z=N), 1), (dict(V=1 << 20, ws=N), 1)):
         assert fwd(**kw) == code, kw
