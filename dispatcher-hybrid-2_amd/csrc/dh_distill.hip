@@ -671,8 +671,8 @@ extern "C" int dh_distill_fwd(int dtype, const void* logits, int64_t stride_b, i
              "%s: null or unaligned pointer argument", who);
   DH_REQUIRE(reduction == 0 || (loss && divisor), DH_ERR_INVALID_ARG, "%s: null pointer argument", who);
   const int64_t need = dh_distill_workspace_bytes(dtype, a.rows, V);
-  DH_REQUIRE(workspace_bytes >= need && (need == 0 || (workspace && (uintptr_t)workspace % 8 == 0)), DH_ERR_INVALID_ARG, "%s: workspace of %lld bytes, %lld needed",
-             who, (long long)workspace_bytes, (long long)need);
+  DH_REQUIRE(workspace_bytes >= need && (need == 0 || (workspace && (uintptr_t)workspace % 8 == 0)), DH_ERR_INVALID_ARG,
+             "%s: workspace of %lld bytes, %lld needed", who, (long long)workspace_bytes, (long long)need);
   hipStream_t s = (hipStream_t)stream;
   Kept* kept = (Kept*)row_kept;
   if (a.rows == 0) {

@@ -1,4 +1,4 @@
-"""Build libdh_mixer.so (gfx950) in-tree from ``csrc/*.hip``.
+"""Build libdh_mixer.so (gfx950) in-tree from ``csrc/*.hip``, and the torch extension of ``csrc/host`` beside it.
 
     python -m dispatcher_hybrid._build
 
@@ -21,6 +21,8 @@ REPO_DIR = os.path.dirname(PROJECT_DIR)
 INCLUDE_DIRS = [os.path.join(REPO_DIR, "include"), CSRC_DIR]
 OUT_DIR = os.path.join(PKG_DIR, "_lib")
 LIB = os.path.join(OUT_DIR, "libdh_mixer.so")
+NODES_SRC = os.path.join(CSRC_DIR, "host", "vocab_nodes.cpp")
+NODES_LIB = os.path.join(OUT_DIR, "_vocab_nodes.so")
 
 ARCH = os.environ.get("DH_OFFLOAD_ARCH", "gfx950")
 HIPCC = os.environ.get("HIPCC", shutil.which("hipcc") or "/opt/rocm/bin/hipcc")
@@ -35,6 +37,22 @@ def sources():
     return sorted(glob.glob(os.path.join(CSRC_DIR, "*.hip")))
 
 
+def nodes_command(out):
+    """The host compiler's command for the torch extension (no device code; it finds the kernels at run time)."""
+    import sysconfig
+
+    import torch
+    root = os.path.dirname(torch.__file__)
+    rocm = os.path.dirname(os.path.dirname(os.path.realpath(HIPCC)))
+    system = [os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
+              os.path.join(rocm, "include"), "/opt/rocm/include", sysconfig.get_paths()["include"]]
+    return ([os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-Wall",
+             "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
+            + [a for d in system for a in ("-isystem", d)] + [f"-I{d}" for d in INCLUDE_DIRS]
+            + [NODES_SRC, "-o", out, f"-L{os.path.join(root, 'lib')}"]
+            + [f"-l{n}" for n in ("c10", "c10_hip", "torch_cpu", "torch_hip", "torch", "torch_python")])
+
+
 def build(verbose=False):
     srcs = sources()
     if not srcs:
@@ -42,7 +60,8 @@ def build(verbose=False):
     os.makedirs(OUT_DIR, exist_ok=True)
     inc = [f"-I{d}" for d in INCLUDE_DIRS]
     with tempfile.TemporaryDirectory(prefix="dh_build_") as tmp:
-        procs = []
+        nodes = nodes_command(NODES_LIB + ".tmp")
+        procs = [(nodes, subprocess.Popen(nodes, stdout=subprocess.PIPE, stderr=subprocess.STDOUT))]
         objs = []
         for src in srcs:
             obj = os.path.join(tmp, os.path.basename(src) + ".o")
@@ -59,13 +78,14 @@ def build(verbose=False):
             elif verbose and out.strip():
                 print(out)
         if failed:
-            raise RuntimeError("hipcc failed:\n" + "\n".join(failed))
+            raise RuntimeError("compilation failed:\n" + "\n".join(failed))
         tmp_lib = LIB + ".tmp"
         cmd = [HIPCC, f"--offload-arch={ARCH}", "-shared", "-fPIC", "-o", tmp_lib] + objs
         p = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT)
         if p.returncode != 0:
             raise RuntimeError(f"link failed:\n$ {' '.join(cmd)}\n{p.stdout.decode(errors='replace')}")
         os.replace(tmp_lib, LIB)
+        os.replace(NODES_LIB + ".tmp", NODES_LIB)
     return LIB
 
 

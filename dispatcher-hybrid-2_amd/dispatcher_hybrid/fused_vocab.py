@@ -8,10 +8,11 @@ Kernels: ``dh_embed_fwd`` / ``dh_embed_bwd``, ``dh_top_logits``, ``dh_distill_fw
 under ``model.enable_fused_vocab()``; ``distillation.py`` has the formulas as torch operations. fp32 and bf16; sums are fp32
 or wider, in an order that does not change from call to call.
 
-Each is one registered operation (``dispatcher::embed_tokens``, ...) for compilers, which torch.func's transforms refuse, and
-in plain eager execution launched without one.
+Each is one registered operation (``dispatcher::embed_tokens``, ...) for compilers, which torch.func's transforms refuse. In
+plain eager execution the launches and the autograd nodes are C++ (``csrc/host/vocab_nodes.cpp``): a backward pass runs on
+autograd's thread for the device, and a node in Python costs it several times the small kernels' own time.
 
-Importing this module loads the kernel library and raises ImportError if it is missing.
+Importing this module loads the kernel library and that extension, and raises ImportError if one is missing.
 """
 
 from typing import List, Optional
@@ -19,7 +20,7 @@ from typing import List, Optional
 import torch
 import torch.nn as nn
 
-from . import _hip
+from . import _hip, _nodes
 from . import distillation as plain
 from .fused_gates import _function_mode, _has_any_global_hook, plain_eager
 
@@ -28,60 +29,21 @@ _INTS = (torch.int32, torch.int64)
 _REDUCTION = {"none": 0, "mean": 1, "sum": 2}
 
 
-def _call(t, what, fn, *args):
-    """fn(*args, the current stream of t's device), with t's device as the current one (a launch goes to that)."""
-    index = t.get_device()
-    if index != torch.cuda.current_device():
-        with torch.cuda.device(index):
-            return _call(t, what, fn, *args)
-    # (the raw handle: no stream object, no ctypes object)
-    st = fn(*args, _hip._raw_stream(index) if _hip._raw_stream is not None else _hip.stream_handle(t.device))
-    if st:
-        _hip.check(st, what)
+def _again(logits, teacher_logits, teacher_tokens, labels, temperature, weight, ignore_index, reduction, g):
+    """The loss's gradient in the logits from the formula as torch operations, differentiable itself (create_graph)."""
+    z = logits.view_as(logits)
+    loss = plain.distillation_loss(z, teacher_logits, teacher_tokens, labels, temperature, weight, ignore_index,
+                                   plain.REDUCTIONS[reduction])
+    return torch.autograd.grad(loss, z, g, create_graph=True)[0]
 
 
-def _bits(t):
-    return 32 if t.dtype == torch.int32 else 64
-
-
-def _unit_rows(t):
-    """t with unit-stride rows (any other layout copied); broadcast rows stay."""
-    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+_native = _nodes.load(_again)
+_lookup, _lookup_grad = _native.lookup, _native.lookup_grad
 
 
 # ---------------------------------------------------------------------------------------------
 # embedding
 # ---------------------------------------------------------------------------------------------
-def _lookup(weight, tokens, scale, zero_token):
-    what = "embed_tokens"
-    _hip.same_gpu(what, weight, tokens)
-    V, d = weight.shape
-    code = _hip.dtype_code(weight.dtype)
-    # (contiguous() would leave one row of any stride as it is)
-    w = weight if weight.stride(1) == 1 and weight.stride(0) >= d else weight.clone(memory_format=torch.contiguous_format)
-    ids = tokens.contiguous()
-    out = torch.empty(*tokens.shape, d, device=w.device, dtype=w.dtype)
-    _call(w, what, _hip.lib.dh_embed_fwd, code, w.data_ptr(), w.stride(0), V, d, ids.data_ptr(), _bits(ids), ids.numel(), scale,
-          zero_token, out.data_ptr(), d)
-    return out
-
-
-def _lookup_grad(dy, tokens, rows, scale, skip_token):
-    what = "embed_tokens gradient"
-    _hip.same_gpu(what, dy, tokens)
-    d = dy.shape[-1]
-    code = _hip.dtype_code(dy.dtype)
-    dy2, ids = dy.reshape(-1, d), tokens.contiguous()
-    if not (dy2.stride(1) == 1 and dy2.stride(0) >= d):
-        dy2 = dy2.clone(memory_format=torch.contiguous_format)
-    out = torch.empty(rows, d, device=dy.device, dtype=dy.dtype)
-    nbytes = _hip.lib.dh_embed_bwd_workspace_bytes(ids.numel(), rows, d)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dy.device) if nbytes > 0 else None  # (refused sizes: the call says why)
-    _call(dy, what, _hip.lib.dh_embed_bwd, code, dy2.data_ptr(), dy2.stride(0), ids.data_ptr(), _bits(ids), ids.numel(), rows, d,
-          scale, skip_token, out.data_ptr(), None if ws is None else ws.data_ptr(), nbytes)
-    return out
-
-
 @torch.library.custom_op("dispatcher::embed_tokens", mutates_args=(), device_types="cuda")
 def _embed_op(weight: torch.Tensor, tokens: torch.Tensor, scale: float, zero_token: int, skip_token: int) -> torch.Tensor:
     return _lookup(weight, tokens, scale, zero_token)
@@ -135,34 +97,6 @@ torch.library.register_autograd("dispatcher::embed_tokens", _embed_backward, set
 torch.library.register_autograd("dispatcher::embed_tokens_grad", _embed_grad_backward, setup_context=_embed_grad_setup)
 
 
-class _Embed(torch.autograd.Function):
-    """dispatcher::embed_tokens without the registered operation's per-call bookkeeping."""
-
-    @staticmethod
-    def forward(ctx, weight, tokens, scale, zero_token, skip_token):
-        _embed_setup(ctx, (weight, tokens, scale, zero_token, skip_token), None)
-        return _lookup(weight, tokens, scale, zero_token)
-
-    @staticmethod
-    def backward(ctx, dy):
-        tokens, = ctx.saved_tensors
-        grad = _EmbedGrad.apply if torch.is_grad_enabled() else _lookup_grad
-        return grad(dy, tokens, *ctx.args), None, None, None, None
-
-
-class _EmbedGrad(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, dy, tokens, rows, scale, skip_token):
-        _embed_grad_setup(ctx, (dy, tokens, rows, scale, skip_token), None)
-        return _lookup_grad(dy, tokens, rows, scale, skip_token)
-
-    @staticmethod
-    def backward(ctx, g):
-        tokens, = ctx.saved_tensors
-        scale, skip_token = ctx.args
-        return _Embed.apply(g, tokens, scale, _zero_token(g, skip_token), skip_token), None, None, None, None
-
-
 def embed_tokens(tokens, weight, scale=1.0, padding_idx=None):
     """weight[tokens] * scale, (*tokens.shape, d), differentiable in weight; rounded once.
 
@@ -181,7 +115,7 @@ def embed_tokens(tokens, weight, scale=1.0, padding_idx=None):
             raise ValueError(f"embed_tokens: padding_idx {padding_idx} outside a vocabulary of {V}")
         skip = padding_idx % V
     if type(weight) in _PLAIN and weight.is_cuda and plain_eager():
-        return _Embed.apply(weight, tokens, float(scale), -1, skip)
+        return _native.embed_tokens(weight, tokens, scale, -1, skip)
     _hip.require_gpu(weight, "embed_tokens")
     return torch.ops.dispatcher.embed_tokens(weight, tokens, float(scale), -1, skip)
 
@@ -199,22 +133,9 @@ def embedding_fits(module):
 # ---------------------------------------------------------------------------------------------
 # a teacher's targets
 # ---------------------------------------------------------------------------------------------
-def _top(logits, k):
-    what = "top_logits"
-    _hip.require_gpu(logits, what)
-    V = logits.shape[-1]
-    code = _hip.dtype_code(logits.dtype)
-    rows = _unit_rows(logits.reshape(-1, V))
-    values = torch.empty(*logits.shape[:-1], max(k, 0), device=logits.device, dtype=logits.dtype)
-    tokens = torch.empty(values.shape, device=logits.device, dtype=torch.int64)
-    _call(logits, what, _hip.lib.dh_top_logits, code, rows.data_ptr(), rows.stride(0), rows.shape[0], V, k, values.data_ptr(),
-          tokens.data_ptr())
-    return [values, tokens]
-
-
 @torch.library.custom_op("dispatcher::top_logits", mutates_args=(), device_types="cuda")
 def _top_op(logits: torch.Tensor, k: int) -> List[torch.Tensor]:
-    return _top(logits, k)
+    return list(_native.top_logits(logits, k))
 
 
 @_top_op.register_fake
@@ -231,85 +152,26 @@ def top_logits(logits, k):
         raise ValueError(f"top_logits: logits (..., vocabulary) expected, got {tuple(logits.shape)}")
     if not 1 <= k <= min(plain.MAX_TARGETS, logits.shape[-1]):
         raise ValueError(f"top_logits: k={k} must be in [1, min({plain.MAX_TARGETS}, vocabulary {logits.shape[-1]})]")
-    logits = logits.detach()
     if type(logits) in _PLAIN and logits.is_cuda and plain_eager():
-        return tuple(_top(logits, k))
+        return _native.top_logits(logits, k)
     _hip.require_gpu(logits, "top_logits")
-    values, tokens = torch.ops.dispatcher.top_logits(logits, k)
+    values, tokens = torch.ops.dispatcher.top_logits(logits.detach(), k)
     return values, tokens
 
 
 # ---------------------------------------------------------------------------------------------
 # distillation loss
 # ---------------------------------------------------------------------------------------------
-def _rows_of(logits):
-    """(tensor, stride_b, stride_t, B, T): the rows of logits (..., V) by two strides."""
-    V = logits.shape[-1]
-    z = _unit_rows(logits)
-    if z.dim() > 3:
-        z = _unit_rows(z.reshape(-1, V))
-    B, T = (1, z.shape[0]) if z.dim() == 2 else tuple(z.shape[:2]) if z.dim() == 3 else (1, 1)
-    sb, st = (0, z.stride(0)) if z.dim() == 2 else tuple(z.stride()[:2]) if z.dim() == 3 else (0, 0)
-    return z, sb, st, B, T
-
-
-def _distill_args(logits, teacher_logits, teacher_tokens, labels, temperature, weight, ignore_index):
-    """The arguments both directions share, and the tensors they point to (held until the launch)."""
-    z, sb, st, B, T = _rows_of(logits)
-    if not B * T:
-        B, T = 0, 1
-    tl, tt = teacher_logits.contiguous(), teacher_tokens.contiguous()
-    lb = None if labels is None else labels.contiguous()
-    return (_hip.dtype_code(z.dtype), z.data_ptr(), sb, st, B, T, z.shape[-1], _hip.dtype_code(tl.dtype), tl.data_ptr(),
-            tt.data_ptr(), _bits(tt), tl.shape[-1], None if lb is None else lb.data_ptr(), 64 if lb is None else _bits(lb),
-            ignore_index, temperature, weight), (z, tl, tt, lb)
-
-
 def _kept_numel(n):
     """fp32 numbers of what a backward pass keeps of n rows: four a row and, behind them, the divisor (and to 16 bytes)."""
     return 4 * n + 4
-
-
-def _distill_fwd(logits, teacher_logits, teacher_tokens, labels, temperature, weight, ignore_index, reduction):
-    what = "distillation_loss"
-    _hip.same_gpu(what, logits, teacher_logits, teacher_tokens, labels)
-    dev, lead = logits.device, logits.shape[:-1]
-    n = lead.numel()
-    args, held = _distill_args(logits, teacher_logits, teacher_tokens, labels, temperature, weight, ignore_index)
-    # the loss apart (it may be changed in place); in one buffer what is kept, the rows' losses where they are no result, and
-    # the workspace
-    out = torch.empty(() if reduction else lead, device=dev, dtype=torch.float32)
-    nbytes = _hip.lib.dh_distill_workspace_bytes(args[0], n, logits.shape[-1])
-    first = _kept_numel(n)
-    rows = -(-n // 4) * 4 if reduction else 0
-    kept = torch.empty(first + rows + -(-nbytes // 4), device=dev, dtype=torch.float32)
-    at = kept.data_ptr()
-    _call(logits, what, _hip.lib.dh_distill_fwd, *args, reduction, at + 4 * first if reduction else out.data_ptr(), at,
-          out.data_ptr() if reduction else None, at + 16 * n if reduction else None, at + 4 * (first + rows), nbytes)
-    return out, kept
-
-
-def _distill_bwd(g, logits, teacher_logits, teacher_tokens, labels, kept, temperature, weight, ignore_index, reduction):
-    what = "distillation_loss gradient"
-    _hip.same_gpu(what, logits, g, teacher_logits, teacher_tokens, labels, kept)
-    dz = torch.empty(logits.shape, device=logits.device, dtype=logits.dtype)
-    if dz.numel() == 0:
-        return dz
-    args, held = _distill_args(logits, teacher_logits, teacher_tokens, labels, temperature, weight, ignore_index)
-    g = g.float().reshape(-1)
-    if not kept.is_contiguous() or kept.data_ptr() % 16:                       # (a saved-tensor hook may change the layout)
-        kept = kept.clone(memory_format=torch.contiguous_format)
-    at = kept.data_ptr()
-    _call(logits, what, _hip.lib.dh_distill_bwd, *args, at, g.data_ptr(), 0 if reduction else g.stride(0),
-          at + 16 * logits.shape[:-1].numel() if reduction else None, dz.data_ptr())
-    return dz
 
 
 @torch.library.custom_op("dispatcher::distillation_loss", mutates_args=(), device_types="cuda")
 def _distill_op(logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_tokens: torch.Tensor,
                 labels: Optional[torch.Tensor], temperature: float, weight: float, ignore_index: int,
                 reduction: int) -> List[torch.Tensor]:
-    out, kept = _distill_fwd(logits, teacher_logits, teacher_tokens, labels, temperature, weight, ignore_index, reduction)
+    out, kept = _native.distill(logits, teacher_logits, teacher_tokens, labels, temperature, weight, ignore_index, reduction)
     return [out, kept[:_kept_numel(logits.shape[:-1].numel())].clone()]        # (a size that its fake form can say)
 
 
@@ -327,7 +189,7 @@ def _(logits, teacher_logits, teacher_tokens, labels, temperature, weight, ignor
 def _distill_grad_op(g: torch.Tensor, logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_tokens: torch.Tensor,
                      labels: Optional[torch.Tensor], kept: torch.Tensor, temperature: float, weight: float, ignore_index: int,
                      reduction: int) -> torch.Tensor:
-    return _distill_bwd(g, logits, teacher_logits, teacher_tokens, labels, kept, temperature, weight, ignore_index, reduction)
+    return _native.distill_grad(g, logits, teacher_logits, teacher_tokens, labels, kept, temperature, weight, ignore_index, reduction)
 
 
 @_distill_grad_op.register_fake
@@ -342,43 +204,15 @@ def _distill_setup(ctx, inputs, output):
     ctx.args = tuple(args)
 
 
-def _again(ctx, g):
-    """The gradient in the logits from the formula as torch operations, differentiable itself (create_graph)."""
-    logits, teacher_logits, teacher_tokens, labels, _ = ctx.saved_tensors
-    temperature, weight, ignore_index, reduction = ctx.args
-    z = logits.view_as(logits)
-    loss = plain.distillation_loss(z, teacher_logits, teacher_tokens, labels, temperature, weight, ignore_index,
-                                   plain.REDUCTIONS[reduction])
-    return torch.autograd.grad(loss, z, g, create_graph=True)[0]
-
-
 def _distill_backward(ctx, grads):
     if grads[0] is None:
         return (None,) * 8
     if torch.is_grad_enabled():
-        return (_again(ctx, grads[0]), *(None,) * 7)
+        return (_again(*ctx.saved_tensors[:4], *ctx.args, grads[0]), *(None,) * 7)
     return (torch.ops.dispatcher.distillation_loss_grad(grads[0], *ctx.saved_tensors, *ctx.args), *(None,) * 7)
 
 
 torch.library.register_autograd("dispatcher::distillation_loss", _distill_backward, setup_context=_distill_setup)
-
-
-class _Distill(torch.autograd.Function):
-    """dispatcher::distillation_loss without the registered operation's per-call bookkeeping."""
-
-    @staticmethod
-    def forward(ctx, *inputs):
-        output = _distill_fwd(*inputs)
-        _distill_setup(ctx, inputs, output)
-        return output[0]
-
-    @staticmethod
-    def backward(ctx, g):
-        if g is None:
-            return (None,) * 8
-        if torch.is_grad_enabled():
-            return (_again(ctx, g), *(None,) * 7)
-        return (_distill_bwd(g, *ctx.saved_tensors, *ctx.args), *(None,) * 7)
 
 
 def distillation_loss(logits, teacher_logits, teacher_tokens, labels=None, temperature=1.0, weight=1.0, ignore_index=-100,
@@ -400,6 +234,6 @@ def distillation_loss(logits, teacher_logits, teacher_tokens, labels=None, tempe
     args = (logits, teacher_logits, teacher_tokens, labels, float(temperature), float(weight), int(ignore_index),
             _REDUCTION[reduction])
     if type(logits) in _PLAIN and logits.is_cuda and plain_eager():
-        return _Distill.apply(*args)
+        return _native.distillation_loss(*args)
     _hip.require_gpu(logits, "distillation_loss")
     return torch.ops.dispatcher.distillation_loss(*args)[0]
