@@ -1,8 +1,8 @@
 // The vocabulary-end operators as autograd nodes in C++: what fused_vocab.py calls in plain eager execution.
 //
-// Their backward passes run on autograd's thread for the device. In Python they would hand the interpreter over twice a
-// pass: with nodes in Python the gradient of 200 embedding rows takes 90 us from end to end, of which the kernel is 6. The
-// kernels are the C entry points of libdh_mixer.so, bound by address by the module that loads that library; nothing here
+// Their backward passes run on autograd's thread for the device, and nodes in Python hand the interpreter over twice a pass:
+// lookup and gradient of 200 embedding rows took 90 us with them, of which the kernels are 9, and take 48 with these (torch's
+// own 52 in the same process). The kernels are the C entry points of libdh_mixer.so, bound by address by the module that loads that library; nothing here
 // computes.
 
 #include <ATen/ATen.h>
@@ -67,7 +67,17 @@ void same_gpu(const char* what, const Tensor& x, std::initializer_list<const Ten
 // the current stream of a device; made with that device as the current one
 void* stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.get_device()).stream(); }
 
-int bits(const Tensor& t) { return t.scalar_type() == at::kInt ? 32 : 64; }
+int bits(const char* what, const Tensor& t) {
+  if (t.scalar_type() == at::kInt) return 32;
+  TORCH_CHECK_TYPE(t.scalar_type() == at::kLong, what, ": integers must be int32 or int64, got torch.",
+                   c10::toString(t.scalar_type()));
+  return 64;
+}
+// A kernel reads as much as the sizes say, so every launch checks them, whoever calls it (a registered operation by its name,
+// a saved-tensor hook that hands back another tensor).
+void same_count(const char* what, const char* which, int64_t has, int64_t needs) {
+  TORCH_CHECK_VALUE(has == needs, what, ": ", which, " of ", has, " elements, ", needs, " needed");
+}
 
 Tensor fresh(const Tensor& t) { return t.clone(at::MemoryFormat::Contiguous); }
 // unit-stride rows (any other layout copied); broadcast rows stay
@@ -78,6 +88,7 @@ Tensor lookup(const Tensor& weight, const Tensor& tokens, double scale, int64_t 
   const char* what = "embed_tokens";
   same_gpu(what, weight, {&tokens});
   const int code = dtype_code(weight);
+  TORCH_CHECK_VALUE(weight.dim() == 2, what, ": weight (V, d) expected, got ", weight.sizes());
   const int64_t V = weight.size(0), d = weight.size(1);
   const c10::DeviceGuard guard(weight.device());
   const Tensor w = weight.stride(1) == 1 && weight.stride(0) >= d ? weight : fresh(weight);
@@ -85,8 +96,9 @@ Tensor lookup(const Tensor& weight, const Tensor& tokens, double scale, int64_t 
   auto shape = tokens.sizes().vec();
   shape.push_back(d);
   Tensor out = at::empty(shape, weight.options());
+  const int id_bits = bits(what, ids);
   // (a width past an int is refused by the entry point, as -1)
-  check(lib.dh_embed_fwd(code, w.data_ptr(), w.stride(0), V, d <= INT32_MAX ? (int)d : -1, ids.data_ptr(), bits(ids), ids.numel(),
+  check(lib.dh_embed_fwd(code, w.data_ptr(), w.stride(0), V, d <= INT32_MAX ? (int)d : -1, ids.data_ptr(), id_bits, ids.numel(),
                          (float)scale, zero_token, out.data_ptr(), d, stream_of(w)),
         what);
   return out;
@@ -99,6 +111,9 @@ Tensor lookup_grad(const Tensor& dy, const Tensor& tokens, int64_t rows, double 
   const int64_t d = dy.size(-1);
   const c10::DeviceGuard guard(dy.device());
   const Tensor ids = tokens.contiguous();
+  const int id_bits = bits(what, ids);
+  same_count(what, "dy", dy.numel(), ids.numel() * d);
+  TORCH_CHECK_VALUE(rows >= 1, what, ": a vocabulary of ", rows);
   Tensor y = dy.dim() == 2 ? dy : dy.reshape({-1, d});
   if (y.stride(1) != 1 || y.stride(0) < d) y = fresh(y);
   Tensor out = at::empty({rows, d}, dy.options());
@@ -106,7 +121,7 @@ Tensor lookup_grad(const Tensor& dy, const Tensor& tokens, int64_t rows, double 
   const int64_t bytes = lib.dh_embed_bwd_workspace_bytes(ids.numel(), rows, width);
   Tensor ws;                                                   // (refused sizes: the call says why)
   if (bytes > 0) ws = at::empty({bytes}, dy.options().dtype(at::kByte));
-  check(lib.dh_embed_bwd(code, y.data_ptr(), y.stride(0), ids.data_ptr(), bits(ids), ids.numel(), rows, width, (float)scale,
+  check(lib.dh_embed_bwd(code, y.data_ptr(), y.stride(0), ids.data_ptr(), id_bits, ids.numel(), rows, width, (float)scale,
                          skip_token, out.data_ptr(), ws.defined() ? ws.data_ptr() : nullptr, bytes, stream_of(dy)),
         what);
   return out;
@@ -178,9 +193,9 @@ struct Mix {                               // what the loss is mixed from
 // the arguments both directions share, and the tensors they point to
 struct Rows {
   Tensor z, t_logits, t_tokens, labels;
-  int64_t sb = 0, st = 0, B = 1, T = 1;
-  int code, t_code, V;
-  Rows(const Tensor& logits, const Tensor& teacher_logits, const Tensor& teacher_tokens, const Tensor& lb)
+  int64_t sb = 0, st = 0, B = 1, T = 1, n = 1;
+  int code, t_code, V, token_bits, label_bits = 64;
+  Rows(const char* what, const Tensor& logits, const Tensor& teacher_logits, const Tensor& teacher_tokens, const Tensor& lb)
       : z(unit_rows(logits)),
         t_logits(teacher_logits.contiguous()),
         t_tokens(teacher_tokens.contiguous()),
@@ -194,18 +209,20 @@ struct Rows {
     } else if (z.dim() == 2) {
       T = z.size(0), st = z.stride(0);
     }
-    if (B * T == 0) B = 0, T = 1;
-    TORCH_CHECK_VALUE(B * T < (1 << 22), "distillation_loss: ", B * T, " rows, fewer than ", 1 << 22, " possible");
+    n = B * T;
+    if (n == 0) B = 0, T = 1;
+    TORCH_CHECK_VALUE(n < (1 << 22), what, ": ", n, " rows, fewer than ", 1 << 22, " possible");
+    token_bits = bits(what, t_tokens);
+    same_count(what, "teacher logits", t_logits.numel(), n * K());
+    same_count(what, "teacher tokens", t_tokens.numel(), n * K());
+    if (labels.defined()) {
+      label_bits = bits(what, labels);
+      same_count(what, "labels", labels.numel(), n);
+    }
   }
+  int64_t K() const { return t_logits.size(-1); }
   void* label_ptr() const { return labels.defined() ? labels.data_ptr() : nullptr; }
-  int label_bits() const { return labels.defined() ? bits(labels) : 64; }
 };
-
-int64_t rows_of(const Tensor& logits) {
-  int64_t n = 1;
-  for (int64_t i = 0; i + 1 < logits.dim(); ++i) n *= logits.size(i);
-  return n;
-}
 
 // (loss, kept): kept holds four numbers a row and the divisor, and behind them the rows' losses where they are no result and
 // the workspace
@@ -214,8 +231,8 @@ std::tuple<Tensor, Tensor> distill(const Tensor& logits, const Tensor& teacher_l
   const char* what = "distillation_loss";
   same_gpu(what, logits, {&teacher_logits, &teacher_tokens, &labels});
   const c10::DeviceGuard guard(logits.device());
-  const Rows a(logits, teacher_logits, teacher_tokens, labels);
-  const int64_t n = rows_of(logits);
+  const Rows a(what, logits, teacher_logits, teacher_tokens, labels);
+  const int64_t n = a.n;
   const auto f32 = logits.options().dtype(at::kFloat);
   // the loss apart: it may be changed in place
   Tensor out = m.reduction ? at::empty({}, f32) : at::empty(logits.sizes().slice(0, logits.dim() - 1), f32);
@@ -224,7 +241,7 @@ std::tuple<Tensor, Tensor> distill(const Tensor& logits, const Tensor& teacher_l
   Tensor kept = at::empty({first + rows + (bytes + 3) / 4}, f32);
   float* at_ = kept.data_ptr<float>();
   check(lib.dh_distill_fwd(a.code, a.z.data_ptr(), a.sb, a.st, a.B, (int)a.T, a.V, a.t_code, a.t_logits.data_ptr(),
-                           a.t_tokens.data_ptr(), bits(a.t_tokens), (int)a.t_logits.size(-1), a.label_ptr(), a.label_bits(),
+                           a.t_tokens.data_ptr(), a.token_bits, (int)a.K(), a.label_ptr(), a.label_bits,
                            m.ignore_index, (float)m.temperature, (float)m.weight, (int)m.reduction,
                            m.reduction ? at_ + first : out.data_ptr<float>(), at_, m.reduction ? out.data_ptr<float>() : nullptr,
                            m.reduction ? at_ + 4 * n : nullptr, at_ + first + rows, bytes, stream_of(logits)),
@@ -239,15 +256,17 @@ Tensor distill_grad(const Tensor& grad, const Tensor& logits, const Tensor& teac
   const c10::DeviceGuard guard(logits.device());
   Tensor dz = at::empty(logits.sizes(), logits.options());
   if (dz.numel() == 0) return dz;
-  const Rows a(logits, teacher_logits, teacher_tokens, labels);
+  const Rows a(what, logits, teacher_logits, teacher_tokens, labels);
   const Tensor g = grad.to(at::kFloat).reshape({-1});
+  same_count(what, "the loss's gradient", g.numel(), m.reduction ? 1 : a.n);
+  TORCH_CHECK_VALUE(kept_.numel() >= 4 * a.n + 4, what, ": ", kept_.numel(), " numbers kept of ", a.n, " rows");
   Tensor kept = kept_;                                         // (a saved-tensor hook may change the layout)
   if (!kept.is_contiguous() || reinterpret_cast<uintptr_t>(kept.data_ptr()) % 16) kept = fresh(kept);
   const float* at_ = kept.data_ptr<float>();
   check(lib.dh_distill_bwd(a.code, a.z.data_ptr(), a.sb, a.st, a.B, (int)a.T, a.V, a.t_code, a.t_logits.data_ptr(),
-                           a.t_tokens.data_ptr(), bits(a.t_tokens), (int)a.t_logits.size(-1), a.label_ptr(), a.label_bits(),
+                           a.t_tokens.data_ptr(), a.token_bits, (int)a.K(), a.label_ptr(), a.label_bits,
                            m.ignore_index, (float)m.temperature, (float)m.weight, at_, g.data_ptr<float>(),
-                           m.reduction ? 0 : g.stride(0), m.reduction ? at_ + 4 * rows_of(logits) : nullptr, dz.data_ptr(),
+                           m.reduction ? 0 : g.stride(0), m.reduction ? at_ + 4 * a.n : nullptr, dz.data_ptr(),
                            stream_of(logits)),
         what);
   return dz;

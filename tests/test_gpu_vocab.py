@@ -693,6 +693,44 @@ def test_refusals_on_the_gpu():
             call()
 
 
+def test_launches_refuse_sizes_that_do_not_fit():
+    """The registered operations by name, and tensors that a hook hands back smaller: nothing is launched."""
+    o, n = torch.ops.dispatcher, fused_native()
+    W, ids = torch.randn(6, 4, device=DEV), torch.zeros(3, dtype=torch.long, device=DEV)
+    z, t, tok, labels = inputs((4,), 50, 3, torch.float32, 31)
+    out, kept = o.distillation_loss(z, t, tok, labels, 2.0, 0.5, -100, 1)
+    assert kept.numel() == 4 * 4 + 4
+    for exc, call in (
+            (TypeError, lambda: o.embed_tokens(W, ids.byte(), 1.0, -1, -1)),
+            (TypeError, lambda: o.embed_tokens_grad(W[:3], ids.short(), 6, 1.0, -1)),
+            (ValueError, lambda: o.embed_tokens_grad(W[:2], ids, 6, 1.0, -1)),
+            (ValueError, lambda: o.embed_tokens_grad(W[:3], ids, 0, 1.0, -1)),
+            (ValueError, lambda: o.embed_tokens(W, ids, 1.0, 7, -1)),
+            (ValueError, lambda: n.lookup(W[0], ids, 1.0, -1)),
+            (TypeError, lambda: o.distillation_loss(z, t, tok.byte(), labels, 2.0, 0.5, -100, 1)),
+            (ValueError, lambda: o.distillation_loss(z, t, tok[:3], labels, 2.0, 0.5, -100, 1)),
+            (ValueError, lambda: o.distillation_loss(z, t[:, :2], tok, labels, 2.0, 0.5, -100, 1)),
+            (ValueError, lambda: o.distillation_loss(z, t, tok, labels[:3], 2.0, 0.5, -100, 1)),
+            (ValueError, lambda: o.distillation_loss(z, t, tok, None, 2.0, 0.5, -100, 1)),
+            (ValueError, lambda: o.distillation_loss_grad(out, z, t, tok, labels, kept[:19], 2.0, 0.5, -100, 1)),
+            (ValueError, lambda: o.distillation_loss_grad(z[:3, 0], z, t, tok, labels, kept, 2.0, 0.5, -100, 0)),
+            (ValueError, lambda: o.top_logits(z, 51))):
+        with pytest.raises(exc):
+            call()
+    leaf, w = z.clone().requires_grad_(), W.clone().requires_grad_()
+    with torch.autograd.graph.saved_tensors_hooks(lambda x: x, lambda x: x[:2]):
+        loss, rows = ops().distillation_loss(leaf, t, tok, labels, 2.0, 0.5), ops().embed_tokens(ids, w)
+        with pytest.raises((ValueError, RuntimeError)):
+            torch.autograd.grad(loss, leaf)
+        with pytest.raises((ValueError, RuntimeError), match="elements"):
+            torch.autograd.grad(rows.sum(), w)
+    torch.cuda.synchronize()
+
+
+def fused_native():
+    return ops()._native
+
+
 # ---- the model ------------------------------------------------------------------------------------------------------
 
 def test_model_step_against_torch():
