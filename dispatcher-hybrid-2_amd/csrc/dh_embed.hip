@@ -13,8 +13,8 @@
 //          writes a token's row when the token's positions all lie in the chunk; the sums of a first or last token that
 //          reaches into the neighbouring chunks go to the workspace. Beside it, the rows of tokens without a position are
 //          filled with zeros.
-//   join   adds the chunk sums of every token that lies in more than one chunk.
-// Bytes: n d read, V d written (and the ids): 32768 x 1024 bf16, V 50257: place 13, sum 30 (5.7 TB/s), join 7 us. Ids outside
+//   join   adds the chunk sums of every token that lies in more than one chunk, as `sum` noted them.
+// Bytes: n d read, V d written (and the ids): 32768 x 1024 bf16, V 50257: place 13, sum 29 (5.9 TB/s), join 5 us. Ids outside
 // [0, V) hold no gradient (their rows of `out` are NaN).
 
 #include <type_traits>
@@ -131,6 +131,10 @@ constexpr int kSmallRows = 512;
 static_assert(kSmallRows <= kPW * kList, "a wave's ids all fit its list");
 constexpr int kMany = 64;
 constexpr int kFew = 16;                   // dy rows in flight a wave
+
+struct Starter {
+  int32_t token, last;
+};
 
 struct Sink {                              // what SMALL adds to
   const void* dy;
@@ -364,12 +368,13 @@ constexpr int kZero = 16;                  // tokens a wave of `sum` looks up th
 
 // The first `sums` workgroups add, the others fill the rows that no position holds with zeros: most of dW's bytes, written
 // while the dy rows are read (by `place` instead: 28 us in all in place of 22 at 128 x 1024 bf16, V 50257; the same at 32768).
+// starter[c]: the token that began in chunk c and goes on behind it, and the last chunk that holds it (token -1: none).
 // partial sums of chunk c: [2 c] of a first token that began in an earlier chunk, [2 c + 1] of a last token that began in
 // this chunk and goes on in the next; d floats each
 template <typename T, int N>
 __global__ __launch_bounds__(kST) void sum_kernel(const T* dy, int64_t ldy, const Pair* pairs, const int* starts, int64_t V,
                                                   Owners own, int sums, int chunk, int slices, float scale, T* dW, int d,
-                                                  int pieces, float* part) {
+                                                  int pieces, float* part, Starter* starter) {
   typedef Piece<T, N> P;
   typedef typename P::raw raw;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -396,7 +401,11 @@ __global__ __launch_bounds__(kST) void sum_kernel(const T* dy, int64_t ldy, cons
   const int piece = (unit % slices) * 64 + lane;
   const int m = load_uniform(starts + own.slots());
   const int64_t b64 = (int64_t)c * chunk;
-  if (b64 >= m) return;
+  const bool notes = unit % slices == 0 && lane == 0;          // (one of the chunk's waves)
+  if (b64 >= m) {
+    if (notes) starter[c] = Starter{-1, 0};
+    return;
+  }
   const int b = (int)b64, e = min(b + chunk, m);
   const int col = min(piece, pieces - 1);                      // (lanes past the row read its last piece and write nothing)
   const bool in = piece < pieces;
@@ -446,26 +455,24 @@ __global__ __launch_bounds__(kST) void sum_kernel(const T* dy, int64_t ldy, cons
       }
     }
   }
+  if (notes) {
+    const bool starts_here = !open && token == after;
+    starter[c] = Starter{starts_here ? token : -1, starts_here ? (starts[own.slot(token) + 1] - 1) / chunk : 0};
+  }
   flush(token != after);
 }
 
 constexpr int kJW = 8;                     // waves of `join`: each an eighth of a token's chunks, 64 lanes of M columns
 
 template <typename T, int M>
-__global__ __launch_bounds__(kJW * 64) void join_kernel(const Pair* pairs, const int* starts, Owners own, int chunk,
-                                                        float scale, const float* part, T* dW, int d) {
+__global__ __launch_bounds__(kJW * 64) void join_kernel(const Starter* starter, float scale, const float* part, T* dW, int d) {
   __shared__ float eighth[kJW][64 * M];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int m = load_uniform(starts + own.slots());
   const int64_t c = blockIdx.x;
-  const int64_t e = (c + 1) * chunk;
-  if (e >= m) return;                                          // uniform: the last chunk, or none
-  const int token = pairs[e - 1].token;
-  if (pairs[e].token != token) return;
-  const int slot = own.slot(token);
-  if (starts[slot] < c * chunk) return;                        // began earlier: that chunk joins it
-  const int last = (starts[slot + 1] - 1) / chunk;             // chunks c .. last hold the token
-  const int count = last - (int)c + 1, per = (count + kJW - 1) / kJW;
+  const Starter s0 = starter[c];
+  const int token = s0.token;
+  if (token < 0) return;                                       // uniform
+  const int count = s0.last - (int)c + 1, per = (count + kJW - 1) / kJW;      // chunks c .. last hold the token
   const int k0 = min(wave * per, count), k1 = min(k0 + per, count);
   const int first = blockIdx.y * 64 * M, col = first + lane * M;
   float s[M];
@@ -505,7 +512,7 @@ int chunk_of(int64_t n) {                  // positions a wave adds: 32, or up t
 int64_t align16(int64_t b) { return (b + 15) / 16 * 16; }
 
 struct Layout {
-  int64_t starts, pairs, part, bytes, chunks;
+  int64_t starts, pairs, starter, part, bytes, chunks;
 };
 Layout layout_of(int64_t n, int64_t V, int d) {
   Layout l;
@@ -513,7 +520,9 @@ Layout layout_of(int64_t n, int64_t V, int d) {
   l.chunks = (n + c - 1) / c;
   l.starts = 0;
   l.pairs = align16((owners_of(V).slots() + 1) * 4);
-  l.part = l.pairs + align16(n * (int64_t)sizeof(Pair));
+  l.starter = l.pairs + align16(n * (int64_t)sizeof(Pair));
+  // (waves of the last workgroup past the chunks note too)
+  l.part = l.starter + align16((l.chunks + kST / 64) * (int64_t)sizeof(Starter));
   l.bytes = l.part + 2 * l.chunks * d * 4;
   return l;
 }
@@ -549,6 +558,7 @@ int gradient(const void* dy, int64_t ldy, const void* ids, int wide, int64_t n, 
   const Layout l = layout_of(n, V, d);
   int* starts = (int*)(ws + l.starts);
   Pair* pairs = (Pair*)(ws + l.pairs);
+  Starter* starter = (Starter*)(ws + l.starter);
   float* part = (float*)(ws + l.part);
   const Sink to{dy, ldy, dW, scale, pieces};
   const dim3 owners(1u << own.lg);
@@ -569,12 +579,12 @@ int gradient(const void* dy, int64_t ldy, const void* ids, int wide, int64_t n, 
   const int sums = (int)((l.chunks * slices + kST / 64 - 1) / (kST / 64));
   const int zeros = (int)((V + kZero * (kST / 64) - 1) / (kZero * (kST / 64)));
   sum_kernel<T, N><<<dim3((unsigned)(sums + zeros)), dim3(kST), 0, s>>>((const T*)dy, ldy, pairs, starts, V, own, sums, chunk,
-                                                                       slices, scale, (T*)dW, d, pieces, part);
+                                                                       slices, scale, (T*)dW, d, pieces, part, starter);
   if (int st = dh_check_launch("dh_embed_bwd")) return st;
   if (l.chunks > 1) {
     constexpr int M = N == 1 ? 1 : 4;
     join_kernel<T, M><<<dim3((unsigned)(l.chunks - 1), (unsigned)((d + 64 * M - 1) / (64 * M))), dim3(kJW * 64), 0, s>>>(
-        pairs, starts, own, chunk, scale, part, (T*)dW, d);
+        starter, scale, part, (T*)dW, d);
     return dh_check_launch("dh_embed_bwd");
   }
   return 0;
