@@ -200,8 +200,8 @@ struct Named {
   double cross, mass;                      // sum_j p_j (log p_j - (z_{k_j} - ref) / tau), sum_j p_j
   float ref;                               // the largest of those z: near the row's own maximum, or as far below it as all
   float label;                             // the label's logit
-  int terms;                               // bit 0: the row counts, bit 1: it has live slots, bit 2: out of the vocabulary
-};
+  int terms;                               // bit 0: the row counts, bit 1: it has live slots, bit 2: its loss and gradient are
+};                                         // NaN: a token or label past the vocabulary, a live slot of NaN or +inf
 
 __device__ __forceinline__ bool counted(const Rows& a, int r) {
   return !a.labels || whole(a.labels, a.label_wide, r) != a.ignore;
@@ -241,6 +241,7 @@ __device__ __forceinline__ Named named_of(const Rows& a, int r, int lane) {
       }
     n.cross = wave_sum64(cross);
     n.mass = wave_sum64(mass);
+    bad |= n.mass != n.mass;               // (a softmax without a value: no logit of the row has a gradient either)
   }
   n.terms |= (live ? 2 : 0) | (bad ? 4 : 0);
   return n;

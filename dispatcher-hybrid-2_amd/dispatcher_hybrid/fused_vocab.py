@@ -228,8 +228,9 @@ def distillation_loss(logits, teacher_logits, teacher_tokens, labels=None, tempe
 
     without the first term where every slot is empty. weight < 1 needs labels. A position whose label is ignore_index counts
     for nothing: no loss, a gradient of zeros, whatever its logits hold. reduction: "mean" over the other positions (NaN when
-    there is none, as the cross-entropy's mean), "sum" or "none". A teacher token past the vocabulary, or a label outside it,
-    makes its position's loss and gradient NaN. The teacher's logits are constants."""
+    there is none, as the cross-entropy's mean), "sum" or "none". A teacher token past the vocabulary or a live teacher logit
+    of NaN or +inf (with weight > 0; the teacher is not read otherwise), or a label outside the vocabulary, makes its position's
+    loss and all of its gradient NaN. The teacher's logits are constants."""
     plain.check_targets(logits, teacher_logits, teacher_tokens, labels, temperature, weight, reduction)
     args = (logits, teacher_logits, teacher_tokens, labels, float(temperature), float(weight), int(ignore_index),
             _REDUCTION[reduction])

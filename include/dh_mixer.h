@@ -599,8 +599,9 @@ int dh_top_logits(int dtype, const void* logits, int64_t row_stride, int64_t row
  *   p = softmax of t / tau over the live slots (k_j >= 0 and t_j > -inf), q = softmax(z / tau), P = softmax(z)
  *   row_loss[r] = w tau^2 sum_j p_j (log p_j - log q_{k_j}) - (1 - w) log P_y
  * A row without live slots has no first term; with labels, a row whose label is ignore_index has loss 0 and is not read; a
- * teacher token past the vocabulary, or another label outside it, makes its row NaN. The sums over V are fp32, a row's few
- * other operations fp64.
+ * teacher token past the vocabulary, a live t_j of NaN or +inf (neither is looked at where w is 0), or another label outside
+ * the vocabulary makes its row NaN, the whole row of its gradient too. The sums over V are fp32, a row's few other operations
+ * fp64.
  *   teacher_logits (B * T, K) of teacher_dtype; teacher_tokens (B * T, K) of token_bits (32 or 64) bits; labels (B * T) of
  *   label_bits bits, null: none (weight must be 1). All contiguous.
  *   reduction 0: rows only (loss, divisor unused); 1: loss = the mean over the rows that are not ignored (NaN if there is
