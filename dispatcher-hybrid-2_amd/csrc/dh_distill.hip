@@ -15,7 +15,7 @@
 // 4096 x 50257 bf16, K 64, an eighth of the rows ignored: forward 73 us (360 MB, 4.9 TB/s), backward 154 us (772 MB, 5.0 TB/s).
 //
 // Exponents are taken of z - m (exact for bf16 inputs near m), never of z times a constant: rows of the type's lowest value
-// stay finite. The few operations on a row's sums are in fp64: log p - log q is a small difference of larger numbers.
+// stay finite. Exponentials of fp32 logits are good to fp32 (exp_of). The few operations on a row's sums are in fp64: log p - log q is a small difference of larger numbers.
 
 #include "dh_common.h"
 
@@ -26,10 +26,36 @@ constexpr int kW = kT / 64;
 constexpr int kMaxSlots = 256;
 constexpr int kSlotsPerLane = kMaxSlots / 64;
 constexpr int kMaxParts = 32;
-constexpr float kLog2e = 1.4426950408889634f;
+constexpr double kLog2e = 1.4426950408889634;
 constexpr double kLn2 = 0.6931471805599453;
 
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// log2(e) over a temperature in two fp32 numbers
+struct Scale {
+  float hi, lo;
+};
+// An exponent in base 2, d times a scale: h rounded to fp32 and, in l, what the rounding left. h alone costs the result |h| half
+// steps: nothing beside a bf16 gradient, 63 half steps at exponents of -80 beside an fp32 one. FULL puts l back, 2^h (1 + l ln 2),
+// for five instructions (four in the forward's sums): 3 half steps whatever the exponent. fp32, V 50257, without and with it, in a
+// graph: one exp 777 rows forward 33 and 35, backward 71 and 72 us, 2048 rows 81 and 82, 189 and 190; two exps 35 and 38, 75 and
+// 76; 81 and 90, 189 and 193.
+struct Exponent {
+  float h, l;
+};
+template <bool FULL> __device__ __forceinline__ Exponent exponent_of(float d, Scale c) {
+  const float h = d * c.hi;
+  if constexpr (!FULL) return Exponent{h, 0.f};
+  // (where h is infinite l would be too, or NaN: the median leaves a number, for 0 times it to be 0)
+  return Exponent{h, __builtin_amdgcn_fmed3f(__builtin_fmaf(d, c.lo, __builtin_fmaf(d, c.hi, -h)), -1.f, 1.f)};
+}
+// 2 to the exponent's `times`, a power of two
+template <bool FULL> __device__ __forceinline__ float exp_of(Exponent x, float times = 1.f) {
+  const float e = exp2_hw(x.h * times);
+  return FULL ? __builtin_fmaf(e * x.l, (float)kLn2 * times, e) : e;
+}
+template <bool FULL> __device__ __forceinline__ float exp_of(float d, Scale c) { return exp_of<FULL>(exponent_of<FULL>(d, c)); }
+template <typename T> constexpr bool kFull = sizeof(T) == 4;
 __device__ __forceinline__ float finite_ref(float m) { return m == -INFINITY ? 0.f : m; }
 
 template <typename T> constexpr int kE = 16 / (int)sizeof(T);
@@ -88,6 +114,7 @@ struct Rows {
   float tau, weight;
   double inv_tau;
   int soft, hard;                          // which terms there are
+  Scale c0, c1;                            // of the exponents: the soft term's (or, without one, the hard term's); the hard term's
 };
 
 template <typename T>
@@ -107,41 +134,45 @@ struct Kept {
   int terms;                               // bit 0: the row counts, bit 1: it has live slots
 };
 
-// How the two sums of exponentials are had: one alone (only one term, or tau = 1), both, or, where tau is 2 or 4, the
-// second from powers of the first's terms: exp(z - m) = exp((z - m) / tau)^tau in one or two products in place of an exp,
-// which takes as long as four (forward of 2048 x 50257 bf16: 38 -> 34 us).
+// How the two sums of exponentials are had: one alone (only one term, or tau = 1), both, or, where tau is 2 or 4, the second
+// with the first's help, exp(z - m) = exp((z - m) / tau)^tau: for bf16 logits as one or two products in place of an exp, which
+// takes as long as four (forward of 2048 x 50257 bf16: 38 -> 34 us); for fp32, since a power multiplies the relative error by
+// tau, as the exp of tau times the first's exponent, rounded part included (forward of 2048 x 50257: 90 -> 86 us).
 enum Mode { kOne = 1, kTwo = 2, kSquare = 3, kFourth = 4 };
 
 struct Sums {
-  float m, s0, s1;                         // s0: of exp((z - m) c0), s1: of exp((z - m) c1), c as in scales()
+  float m, s0, s1;                         // s0: of exp(z - m) to the scale c0, s1: to c1
 };
-// c0: the soft term's (or, without one, the hard term's) scale of the exponent in base 2; c1: the hard term's
-__device__ __forceinline__ void scales(const Rows& a, float& c0, float& c1) {
-  c0 = a.soft ? kLog2e / a.tau : kLog2e;
-  c1 = kLog2e;
-}
-template <int M> __device__ __forceinline__ float second(float e, float d, float c1) {
-  if (M == kSquare) return e * e;
-  if (M == kFourth) {
-    const float f = e * e;
-    return f * f;
+// exp(d) to the scale c0 and, unless M is kOne, to c1
+template <int M, bool FULL> __device__ __forceinline__ void exps(float d, Scale c0, Scale c1, float& e0, float& e1) {
+  const Exponent x = exponent_of<FULL>(d, c0);
+  e0 = exp_of<FULL>(x);
+  if constexpr (M == kTwo) {
+    e1 = exp_of<FULL>(d, c1);
+  } else if constexpr (M == kOne) {
+    e1 = 0.f;
+  } else if constexpr (FULL) {
+    e1 = exp_of<FULL>(x, M == kSquare ? 2.f : 4.f);
+  } else {
+    e1 = e0 * e0;
+    if constexpr (M == kFourth) e1 *= e1;
   }
-  return exp2_hw(d * c1);
 }
+// (a few a row: FULL whatever the logits' type)
 template <int M>
-__device__ __forceinline__ Sums join(const Sums& a, const Sums& b, float c0, float c1) {
+__device__ __forceinline__ Sums join(const Sums& a, const Sums& b, Scale c0, Scale c1) {
   Sums r;
   r.m = fmaxf(a.m, b.m);
   const float ref = finite_ref(r.m);
-  r.s0 = a.s0 * exp2_hw((a.m - ref) * c0) + b.s0 * exp2_hw((b.m - ref) * c0);
-  r.s1 = M != kOne ? a.s1 * exp2_hw((a.m - ref) * c1) + b.s1 * exp2_hw((b.m - ref) * c1) : 0.f;
+  r.s0 = a.s0 * exp_of<true>(a.m - ref, c0) + b.s0 * exp_of<true>(b.m - ref, c0);
+  r.s1 = M != kOne ? a.s1 * exp_of<true>(a.m - ref, c1) + b.s1 * exp_of<true>(b.m - ref, c1) : 0.f;
   return r;
 }
 template <int M>
-__device__ __forceinline__ Sums wave_join(Sums v, float c0, float c1) {
+__device__ __forceinline__ Sums wave_join(Sums v, Scale c0, Scale c1) {
   const float m = wave_max(v.m), ref = finite_ref(m);
-  v.s0 = wave_sum(v.s0 * exp2_hw((v.m - ref) * c0));
-  v.s1 = M != kOne ? wave_sum(v.s1 * exp2_hw((v.m - ref) * c1)) : 0.f;
+  v.s0 = wave_sum(v.s0 * exp_of<true>(v.m - ref, c0));
+  v.s1 = M != kOne ? wave_sum(v.s1 * exp_of<true>(v.m - ref, c1)) : 0.f;
   v.m = m;
   return v;
 }
@@ -181,11 +212,10 @@ __device__ __forceinline__ double teacher_row(const Rows& a, int r, int lane, fl
   bad = __ballot(over) != 0;
   most = wave_max(most);
   top = finite_ref(most);
-  const float c = kLog2e / a.tau;
   float s = 0.f;
 #pragma unroll
   for (int i = 0; i < kSlotsPerLane; ++i) {
-    p[i] = token[i] >= 0 ? exp2_hw((t[i] - top) * c) : 0.f;
+    p[i] = token[i] >= 0 ? exp_of<true>(t[i] - top, a.c0) : 0.f;               // (there is a soft term: c0 is its scale)
     s += p[i];
   }
   s = wave_sum(s);
@@ -301,8 +331,7 @@ __global__ __launch_bounds__(kT + 64) void forward_kernel(Rows a, int parts, Sum
     }
     return;
   }
-  float c0, c1;
-  scales(a, c0, c1);
+  const Scale c0 = a.c0, c1 = a.c1;
   if (wave == kW) {
     if (which == 0) {
       const Named n = named_of<T>(a, r, lane);
@@ -319,8 +348,8 @@ __global__ __launch_bounds__(kT + 64) void forward_kernel(Rows a, int parts, Sum
     if (tid < c.singles) {                 // a logit outside the whole pieces
       v.m = Elem<T>::load(z + c.single(tid, a.V));
       const float d = v.m - finite_ref(v.m);
-      v.s0 = exp2_hw(d * c0);
-      if (M != kOne) v.s1 = exp2_hw(d * c1);
+      v.s0 = exp_of<kFull<T>>(d, c0);
+      if (M != kOne) v.s1 = exp_of<kFull<T>>(d, c1);
     }
     auto add = [&](const auto& q) {        // some pieces
       constexpr int N = sizeof(q) / sizeof(uint4);
@@ -332,17 +361,36 @@ __global__ __launch_bounds__(kT + 64) void forward_kernel(Rows a, int parts, Sum
         for (int j = 0; j < E; ++j) most = fmaxf(most, x[u][j]);
       }
       const float ref = finite_ref(most);
-      v.s0 *= exp2_hw((v.m - ref) * c0);
-      if (M != kOne) v.s1 *= exp2_hw((v.m - ref) * c1);
+      v.s0 *= exp_of<kFull<T>>(v.m - ref, c0);
+      if (M != kOne) v.s1 *= exp_of<kFull<T>>(v.m - ref, c1);
       v.m = most;
+      constexpr float kTimes = M == kFourth ? 4.f : 2.f;
+      float k0 = 0.f, k1 = 0.f;
 #pragma unroll
       for (int u = 0; u < N; ++u)
 #pragma unroll
         for (int j = 0; j < E; ++j) {
-          const float d = x[u][j] - ref, e = exp2_hw(d * c0);
-          v.s0 += e;
-          if (M != kOne) v.s1 += second<M>(e, d, c1);
+          float e0, e1;
+          const float d = x[u][j] - ref;
+          if constexpr (kFull<T>) {        // the left parts' sum apart, put back after the loop
+            const Exponent a0 = exponent_of<true>(d, c0);
+            e0 = exp2_hw(a0.h);
+            k0 = __builtin_fmaf(e0, a0.l, k0);
+            if constexpr (M != kOne) {
+              const Exponent a1 = M == kTwo ? exponent_of<true>(d, c1) : Exponent{a0.h * kTimes, a0.l * kTimes};
+              e1 = exp2_hw(a1.h);
+              k1 = __builtin_fmaf(e1, a1.l, k1);
+            }
+          } else {
+            exps<M, false>(d, c0, c1, e0, e1);
+          }
+          v.s0 += e0;
+          if (M != kOne) v.s1 += e1;
         }
+      if constexpr (kFull<T>) {
+        v.s0 = __builtin_fmaf(k0, (float)kLn2, v.s0);
+        if (M != kOne) v.s1 = __builtin_fmaf(k1, (float)kLn2, v.s1);
+      }
     };
     int p = c.p0 + tid;
     for (; p + (U - 1) * kT < c.p1; p += U * kT) {
@@ -407,8 +455,7 @@ __global__ __launch_bounds__(kRT) void join_kernel(Rows a, int parts, const Sums
   __shared__ double red[kRT / 64];
   __shared__ int cnt[kRT / 64];
   const int lane = threadIdx.x & 63, W = blockDim.x >> 6;
-  float c0, c1;
-  scales(a, c0, c1);
+  const Scale c0 = a.c0, c1 = a.c1;
   for (int r = blockIdx.x * W + (threadIdx.x >> 6); r < a.rows; r += gridDim.x * W) {
     if (!counted(a, r)) continue;          // uniform; the first launch wrote it
     Sums v{-INFINITY, 0.f, 0.f};
@@ -458,15 +505,15 @@ __global__ __launch_bounds__(kT + 64) void backward_kernel(Rows a, int parts, co
   }
   const float g = dloss[dloss_stride * r] / (divisor ? *divisor : 1.f);
   const float gs = soft ? g * a.weight * a.tau : 0.f, gh = hard ? g * (1.f - a.weight) : 0.f;
-  float c0, c1;
-  scales(a, c0, c1);
-  // dz of a logit without the teacher's and the label's part: f0 exp((z - m) c0) + f1 exp((z - m) c1)
+  const Scale c0 = a.c0, c1 = a.c1;
+  // dz of a logit without the teacher's and the label's part: f0 exp(z - m) to the scale c0, and f1 exp(z - m) to c1
   const float ref = finite_ref(k.m);
   // (a row without live slots has no soft term, and no 0 * inf)
   const float f0 = M == kOne ? (gs + gh) * k.inv_soft : soft ? gs * k.inv_soft : 0.f, f1 = gh * k.inv_hard;
   auto value = [&](float x) {
-    const float d = x - ref, e = exp2_hw(d * c0);
-    return M == kOne ? f0 * e : M == kSquare ? e * (f0 + f1 * e) : f0 * e + f1 * second<M>(e, d, c1);
+    float e0, e1;
+    exps<M, kFull<T>>(x - ref, c0, c1, e0, e1);
+    return M == kOne ? f0 * e0 : M == kSquare && !kFull<T> ? e0 * (f0 + f1 * e0) : f0 * e0 + f1 * e1;
   };
   // the named tokens of this part, by the wave beside those that write it: slots lane + 64 i, the label behind them
   const int K = soft ? a.K : 0;
@@ -593,6 +640,9 @@ Rows rows_of(const void* logits, int64_t sb, int64_t st, int64_t B, int T, int V
   a.inv_tau = 1.0 / (double)tau;
   a.soft = weight > 0.f;
   a.hard = labels != nullptr && weight < 1.f;
+  auto scale = [](double c) { return Scale{(float)c, (float)(c - (double)(float)c)}; };
+  a.c1 = scale(kLog2e);
+  a.c0 = a.soft ? scale(kLog2e / (double)tau) : a.c1;
   return a;
 }
 

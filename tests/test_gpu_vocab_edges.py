@@ -51,3 +51,44 @@ def test_a_teacher_without_probabilities_makes_its_whole_row_nan(with_labels, va
         bad = torch.arange(rows, device=DEV) == 1
         assert torch.equal(each.isnan(), bad)
         assert torch.equal(grad.isnan(), bad.unsqueeze(1).expand(rows, V))
+
+
+@pytest.mark.parametrize("rows", [4, 600])
+@pytest.mark.parametrize("tau,w", [(1.0, 1.0), (2.0, 0.0), (3.0, 1.0), (4.0, 0.5), (2.0, 0.5), (0.75, 0.5)])
+def test_fp32_probabilities_far_below_the_maximum(tau, w, rows):
+    """Rows of one logit at 0 and the others at exponents of -20 to -80, all multiples of 2^-10 (their differences are exact).
+
+    Every exp: one unit of exp2 (2 u) and the rounding of its correction, 3 u. The sum is 1 and some 1e-6: at most four roundings
+    in the thread that holds the 1, six in its wave, three over the waves, 13 u. Then 1 / sum 1 u, the factor of the term
+    (weight, temperature, 1 / sum) 3 u, its product 1 u, the two terms' sum 1 u: 22 u in all."""
+    say("far", tau, w, rows)
+    V, g = 1000, gen(rows)
+    soft = tau if w > 0 else 1.0
+    x = (-20 - 60 * torch.rand(rows, V, device=DEV, generator=g)) * soft
+    x = (x * 1024).round() / 1024
+    x[:, 17] = 0
+    t, tok = torch.zeros(rows, 1, device=DEV), torch.full((rows, 1), 17, device=DEV)
+    labels = tok[:, 0].clone()
+    leaf, wide = x.clone().requires_grad_(), x.double().requires_grad_()
+    grad, = torch.autograd.grad(ops().distillation_loss(leaf, t, tok, labels, tau, w, reduction="sum"), leaf)
+    ref, = torch.autograd.grad(plain.distillation_loss(wide, t.double(), tok, labels, tau, w, reduction="sum"), wide)
+    far = torch.arange(V, device=DEV) != 17
+    worst = ((grad.double() - ref).abs() / ref.abs())[:, far].max().item() / U
+    assert worst <= 22, worst
+
+
+@pytest.mark.parametrize("tau", [1e-30, 0.5, 3.0, 1e30])
+@pytest.mark.parametrize("rows", [2, 600])
+def test_fp32_infinite_and_lowest_logits_at_any_temperature(rows, tau):
+    """What a mask leaves of a vocabulary, at temperatures at both ends: no exponent becomes NaN, masked tokens get zeros."""
+    say("masked", rows, tau)
+    V, low = 2003, torch.finfo(torch.float32).min
+    z = torch.randn(rows, V, device=DEV, generator=gen(rows))
+    z[0, 5:], z[1, 5:] = -math.inf, low
+    t, tok = torch.zeros(rows, 2, device=DEV), torch.randint(0, 5, (rows, 2), device=DEV, generator=gen(1))
+    labels = tok[:, 0].clone()
+    for w in (1.0, 0.5):
+        leaf = z.clone().requires_grad_()
+        each = ops().distillation_loss(leaf, t, tok, labels, tau, w, reduction="none")
+        grad, = torch.autograd.grad(each[:2].sum(), leaf)
+        assert bool(grad.isfinite().all()) and bool((grad[:2, 5:] == 0).all()) and not bool(each.isnan().any())
