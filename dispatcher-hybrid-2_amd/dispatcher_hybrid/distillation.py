@@ -64,10 +64,10 @@ def distillation_loss(logits, teacher_logits, teacher_tokens, labels=None, tempe
     z = torch.where(kept.unsqueeze(-1), z, torch.zeros((), dtype=wide, device=z.device))
     zero = torch.zeros((), dtype=wide, device=z.device)
     rows = torch.zeros(z.shape[:-1], dtype=wide, device=z.device)
-    bad = torch.zeros_like(kept)
+    bad = torch.zeros_like(kept) if labels is None else (labels < 0) | (labels >= V)
     if weight > 0.0:
         t = teacher_logits.to(wide)
-        bad = (teacher_tokens >= V).any(-1)
+        bad = bad | (teacher_tokens >= V).any(-1)
         live = (teacher_tokens >= 0) & (teacher_tokens < V) & (t != -math.inf)
         # (an all-dead row goes through the softmax as zeros, and is masked behind it)
         t = torch.where(live, t / temperature, torch.where(live.any(-1, keepdim=True), -math.inf, 0.0).to(wide))
@@ -75,12 +75,11 @@ def distillation_loss(logits, teacher_logits, teacher_tokens, labels=None, tempe
         use = live & (p != 0)
         log_q = torch.log_softmax(z / temperature, -1).gather(-1, teacher_tokens.long().clamp(0, V - 1))
         terms = torch.where(use, p, zero) * (torch.where(use, log_p, zero) - torch.where(use, log_q, zero))
-        rows = rows + weight * temperature ** 2 * terms.sum(-1)
-    if labels is not None:
-        bad = bad | (labels < 0) | (labels >= V)
-        if weight < 1.0:
-            picked = torch.log_softmax(z, -1).gather(-1, labels.long().clamp(0, V - 1).unsqueeze(-1)).squeeze(-1)
-            rows = rows - (1.0 - weight) * picked
+        # (a bad row without a live slot: a term for the factor of NaN below to reach the gradient through)
+        rows = rows + weight * temperature ** 2 * terms.sum(-1) + torch.where(bad, log_q[..., 0], zero)
+    if labels is not None and weight < 1.0:
+        picked = torch.log_softmax(z, -1).gather(-1, labels.long().clamp(0, V - 1).unsqueeze(-1)).squeeze(-1)
+        rows = rows - (1.0 - weight) * picked
     # (a factor of NaN: the row's gradient is NaN too)
     rows = rows * torch.where(bad, math.nan, 1.0).to(wide)
     rows = torch.where(kept, rows, zero)

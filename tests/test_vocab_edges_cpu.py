@@ -1,0 +1,32 @@
+"""Corners of the vocabulary-end operators that need no GPU: the formula's rows without a value, the entry points' refusals, the
+library and the extension beside it."""
+
+import math
+
+import pytest
+import torch
+
+from dispatcher_hybrid import distillation as plain
+
+
+@pytest.mark.parametrize("weight,with_labels", [(1.0, False), (1.0, True), (0.5, True), (0.0, True)])
+def test_a_bad_row_without_live_slots_has_a_gradient_of_nan(weight, with_labels):
+    """A token or label past the vocabulary, whatever the row's other slots hold: loss and gradient are NaN together."""
+    g = torch.Generator().manual_seed(1)
+    z = torch.randn(5, 9, dtype=torch.float64, generator=g)
+    t = torch.randn(5, 3, dtype=torch.float64, generator=g)
+    tok = torch.tensor([[1, 2, 3], [9, -1, -1], [-1, -1, -1], [9, 2, -1], [-1, -1, -1]])
+    labels = torch.tensor([0, 1, 99, 2, 3]) if with_labels else None
+    leaf = z.clone().requires_grad_()
+    rows = plain.distillation_loss(leaf, t, tok, labels, 2.0, weight, reduction="none")
+    grad, = torch.autograd.grad(rows.sum(), leaf)
+    bad = [False, weight > 0, with_labels, weight > 0, False]  # (the teacher is not read where weight is 0)
+    assert rows.isnan().tolist() == bad
+    assert torch.equal(grad.isnan(), torch.tensor(bad).unsqueeze(1).expand(5, 9))
+    if weight == 1.0:
+        assert rows[4] == 0 and bool((grad[4] == 0).all())
+    if with_labels:                                            # an ignored row is not bad
+        labels[2] = -100
+        rows = plain.distillation_loss(leaf, t, tok, labels, 2.0, weight, reduction="none")
+        grad, = torch.autograd.grad(rows.sum(), leaf)
+        assert rows[2] == 0 and bool((grad[2] == 0).all()) and math.isnan(rows[1]) == (weight > 0)
