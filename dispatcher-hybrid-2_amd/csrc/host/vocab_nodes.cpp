@@ -35,7 +35,9 @@ struct Entries {
 } lib;
 #undef MEMBER
 
-py::object* again = nullptr;               // the differentiable gradient as torch operations (never freed: it outlives us)
+// never freed: they outlive us
+py::object* again = nullptr;               // the differentiable gradient as torch operations
+py::object* out_of_memory = nullptr;       // torch.OutOfMemoryError
 
 void check(int status, const char* what) {
   if (status == 0) return;
@@ -317,6 +319,10 @@ auto guarded(F&& f) {
     throw py::value_error(e.what_without_backtrace());
   } catch (const c10::TypeError& e) {
     throw py::type_error(e.what_without_backtrace());
+  } catch (const c10::OutOfMemoryError& e) {                   // (what a training loop catches to try a smaller batch)
+    const py::gil_scoped_acquire gil;
+    PyErr_SetString(out_of_memory->ptr(), e.what_without_backtrace());
+    throw py::error_already_set();
   } catch (const c10::Error& e) {
     throw std::runtime_error(e.what_without_backtrace());
   }
@@ -330,6 +336,7 @@ PYBIND11_MODULE(_vocab_nodes, m) {
     ENTRIES(ENTRY)
 #undef ENTRY
     again = new py::object(std::move(differentiable));
+    out_of_memory = new py::object(py::module_::import("torch").attr("OutOfMemoryError"));
   });
   using release = py::call_guard<py::gil_scoped_release>;
   // the launches alone, for the registered operations

@@ -92,3 +92,23 @@ def test_fp32_infinite_and_lowest_logits_at_any_temperature(rows, tau):
         each = ops().distillation_loss(leaf, t, tok, labels, tau, w, reduction="none")
         grad, = torch.autograd.grad(each[:2].sum(), leaf)
         assert bool(grad.isfinite().all()) and bool((grad[:2, 5:] == 0).all()) and not bool(each.isnan().any())
+
+
+# ---- errors and foreign tensors -------------------------------------------------------------------------------------
+
+def test_an_allocation_that_fails_is_torchs_error():
+    """torch.OutOfMemoryError, as torch's own operations raise it, from the direct calls and the registered operations. The
+    allocator refuses by its own limit: nothing is asked of the device."""
+    W = torch.zeros(1, 1 << 20, device=DEV)
+    ids = torch.zeros(1, dtype=torch.long, device=DEV).expand(1 << 20)
+    z = torch.zeros(1, 1, 1, device=DEV).expand(1 << 10, 1 << 10, 1 << 22)
+    t, tok = torch.zeros(1 << 10, 1 << 10, 1, device=DEV), torch.zeros(1 << 10, 1 << 10, 1, dtype=torch.long, device=DEV)
+    torch.cuda.synchronize()
+    torch.cuda.set_per_process_memory_fraction(0.05)
+    try:
+        for call in (lambda: ops().embed_tokens(ids, W), lambda: torch.ops.dispatcher.embed_tokens(W, ids, 1.0, -1, -1),
+                     lambda: ops().top_logits(z, 1), lambda: ops().distillation_loss(z, t, tok)):
+            with pytest.raises(torch.OutOfMemoryError, match="out of memory"):
+                call()
+    finally:
+        torch.cuda.set_per_process_memory_fraction(1.0)
