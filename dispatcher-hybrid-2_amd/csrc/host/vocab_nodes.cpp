@@ -274,6 +274,9 @@ Tensor distill_grad(const Tensor& grad, const Tensor& logits, const Tensor& teac
   return dz;
 }
 
+// targets and labels made under inference mode (a teacher's, say) cannot be saved for a backward pass: copies of them can
+Tensor savable(const Tensor& t) { return t.defined() && t.is_inference() ? t.clone() : t; }
+
 struct Distill : torch::autograd::Function<Distill> {
   static Tensor forward(AutogradContext* ctx, const Tensor& logits, const Tensor& teacher_logits, const Tensor& teacher_tokens,
                         const std::optional<Tensor>& labels, double temperature, double weight, int64_t ignore_index,
@@ -281,7 +284,8 @@ struct Distill : torch::autograd::Function<Distill> {
     const Tensor lb = labels ? *labels : Tensor();
     auto [out, kept] = distill(logits, teacher_logits, teacher_tokens, lb, Mix{temperature, weight, ignore_index, reduction});
     ctx->set_materialize_grads(false);
-    ctx->save_for_backward({logits, teacher_logits, teacher_tokens, lb, kept});
+    if (logits.requires_grad())
+      ctx->save_for_backward({logits, savable(teacher_logits), savable(teacher_tokens), savable(lb), kept});
     ctx->saved_data["temperature"] = temperature;
     ctx->saved_data["weight"] = weight;
     ctx->saved_data["ignore"] = ignore_index;

@@ -198,10 +198,11 @@ def _(g, logits, teacher_logits, teacher_tokens, labels, kept, temperature, weig
 
 
 def _distill_setup(ctx, inputs, output):
-    logits, teacher_logits, teacher_tokens, labels, *args = inputs
+    logits, *constants = inputs[:4]
     ctx.set_materialize_grads(False)
-    ctx.save_for_backward(logits, teacher_logits, teacher_tokens, labels, output[1])
-    ctx.args = tuple(args)
+    # (what was made under inference mode, as a teacher's targets may be, cannot be saved: a copy can)
+    ctx.save_for_backward(logits, *(t.clone() if t is not None and t.is_inference() else t for t in constants), output[1])
+    ctx.args = tuple(inputs[4:])
 
 
 def _distill_backward(ctx, grads):

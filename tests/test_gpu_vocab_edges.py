@@ -112,3 +112,24 @@ def test_an_allocation_that_fails_is_torchs_error():
                 call()
     finally:
         torch.cuda.set_per_process_memory_fraction(1.0)
+
+
+def test_targets_of_inference_mode():
+    """A teacher run under torch.inference_mode sets targets for a training step; labels of that mode too."""
+    g = gen(41)
+    z, teacher = torch.randn(2, 7, 90, device=DEV, generator=g), torch.randn(2, 7, 90, device=DEV, generator=g)
+    with torch.inference_mode():
+        targets = ops().top_logits(teacher, 5)
+        labels = torch.randint(0, 90, (2, 7), device=DEV, generator=g)
+        frozen = ops().distillation_loss(z, *targets, labels, 2.0, 0.5)
+    normal = [x.clone() for x in (*targets, labels)]
+    losses, grads = [], []
+    for t, tok, lb in ((*targets, labels), normal):
+        for fn in (lambda *a: ops().distillation_loss(*a), lambda *a: torch.ops.dispatcher.distillation_loss(*a, -100, 1)[0]):
+            leaf = z.clone().requires_grad_()
+            losses.append(fn(leaf, t, tok, lb, 2.0, 0.5))
+            grads.append(torch.autograd.grad(losses[-1], leaf)[0])
+    assert all(torch.equal(x, losses[0]) for x in [*losses, frozen]) and all(torch.equal(x, grads[0]) for x in grads)
+    leaf = z.clone().requires_grad_()
+    one, = torch.autograd.grad(ops().distillation_loss(leaf, *targets, labels, 2.0, 0.5), leaf, create_graph=True)
+    assert torch.autograd.grad(one.square().sum(), leaf)[0].isfinite().all()
