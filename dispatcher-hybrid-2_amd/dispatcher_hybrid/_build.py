@@ -53,6 +53,36 @@ def nodes_command(out):
             + [f"-l{n}" for n in ("c10", "c10_hip", "torch_cpu", "torch_hip", "torch", "torch_python")])
 
 
+def _quiet(out):
+    return "\n".join(l for l in out.decode(errors="replace").splitlines() if "packed-fp32-ops" not in l)
+
+
+def _start_nodes():
+    """(command, process) of the extension's compilation, the process None and the reason in the command's place where it cannot
+    begin (no torch, no host compiler)."""
+    try:
+        cmd = nodes_command(NODES_LIB + ".tmp")
+        return " ".join(cmd), subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT)
+    except (ImportError, OSError) as e:
+        return f"{type(e).__name__}: {e}", None
+
+
+def _end_nodes(cmd, process, verbose):
+    """Put the extension in place. Where it does not compile (no Python or torch headers, say) the kernel library stays as it
+    is: importing fused_vocab raises ImportError, and nothing else needs the extension."""
+    out = "" if process is None else _quiet(process.communicate()[0])
+    if process is not None and process.returncode == 0 and "warning:" not in out:
+        os.replace(NODES_LIB + ".tmp", NODES_LIB)
+        if verbose and out.strip():
+            print(out)
+        return
+    for path in (NODES_LIB, NODES_LIB + ".tmp"):               # (an older one would be of other sources)
+        if os.path.exists(path):
+            os.remove(path)
+    print(f"the torch extension of csrc/host was not built; dispatcher_hybrid.fused_vocab needs it:\n$ {cmd}\n{out}",
+          file=sys.stderr, flush=True)
+
+
 def build(verbose=False):
     srcs = sources()
     if not srcs:
@@ -60,8 +90,8 @@ def build(verbose=False):
     os.makedirs(OUT_DIR, exist_ok=True)
     inc = [f"-I{d}" for d in INCLUDE_DIRS]
     with tempfile.TemporaryDirectory(prefix="dh_build_") as tmp:
-        nodes = nodes_command(NODES_LIB + ".tmp")
-        procs = [(nodes, subprocess.Popen(nodes, stdout=subprocess.PIPE, stderr=subprocess.STDOUT))]
+        nodes = _start_nodes()
+        procs = []
         objs = []
         for src in srcs:
             obj = os.path.join(tmp, os.path.basename(src) + ".o")
@@ -70,22 +100,24 @@ def build(verbose=False):
             procs.append((cmd, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT)))
         failed = []
         for cmd, p in procs:
-            out = p.communicate()[0].decode(errors="replace")
-            out = "\n".join(l for l in out.splitlines() if "packed-fp32-ops" not in l)
+            out = _quiet(p.communicate()[0])
             if p.returncode != 0 or "warning:" in out:
                 # warnings fail the build too (an inline-asm clobber of a reserved register is one)
                 failed.append(f"$ {' '.join(cmd)}\n{out}")
             elif verbose and out.strip():
                 print(out)
         if failed:
-            raise RuntimeError("compilation failed:\n" + "\n".join(failed))
+            if nodes[1] is not None:
+                nodes[1].kill()
+                nodes[1].communicate()
+            raise RuntimeError("hipcc failed:\n" + "\n".join(failed))
         tmp_lib = LIB + ".tmp"
         cmd = [HIPCC, f"--offload-arch={ARCH}", "-shared", "-fPIC", "-o", tmp_lib] + objs
         p = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT)
         if p.returncode != 0:
             raise RuntimeError(f"link failed:\n$ {' '.join(cmd)}\n{p.stdout.decode(errors='replace')}")
         os.replace(tmp_lib, LIB)
-        os.replace(NODES_LIB + ".tmp", NODES_LIB)
+        _end_nodes(*nodes, verbose)
     return LIB
 
 

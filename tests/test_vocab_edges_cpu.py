@@ -30,3 +30,22 @@ def test_a_bad_row_without_live_slots_has_a_gradient_of_nan(weight, with_labels)
         rows = plain.distillation_loss(leaf, t, tok, labels, 2.0, weight, reduction="none")
         grad, = torch.autograd.grad(rows.sum(), leaf)
         assert rows[2] == 0 and bool((grad[2] == 0).all()) and math.isnan(rows[1]) == (weight > 0)
+
+
+@pytest.mark.parametrize("host", ["/nonexistent/g++", "/bin/false"])
+def test_the_kernel_library_is_built_where_the_extension_does_not_compile(host, tmp_path, monkeypatch, capsys):
+    """With a stand-in for hipcc that leaves empty outputs: a host compiler that is missing, or one that fails."""
+    from dispatcher_hybrid import _build
+    hipcc = tmp_path / "hipcc"
+    hipcc.write_text('#!/bin/sh\nwhile [ $# -gt 0 ]; do [ "$1" = -o ] && : > "$2"; shift; done\nexit 0\n')
+    hipcc.chmod(0o755)
+    out = tmp_path / "lib"
+    out.mkdir()
+    for name, value in (("HIPCC", str(hipcc)), ("OUT_DIR", str(out)), ("LIB", str(out / "lib.so")),
+                        ("NODES_LIB", str(out / "nodes.so"))):
+        monkeypatch.setattr(_build, name, value)
+    (out / "nodes.so").write_text("of other sources")
+    monkeypatch.setenv("CXX", host)
+    assert _build.build() == str(out / "lib.so")
+    assert [f.name for f in out.iterdir()] == ["lib.so"]
+    assert "fused_vocab needs it" in capsys.readouterr().err
