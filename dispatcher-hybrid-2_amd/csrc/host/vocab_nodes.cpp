@@ -335,6 +335,9 @@ auto guarded(F&& f) {
 }  // namespace
 
 PYBIND11_MODULE(_vocab_nodes, m) {
+  // what this was compiled against, for the loader to compare before anything is called
+  m.attr("abi_version") = DH_ABI_VERSION;
+  m.attr("torch_version") = DH_TORCH_VERSION;
   m.def("bind", [](const std::map<std::string, uintptr_t>& at, py::object differentiable) {
 #define ENTRY(name) lib.name = reinterpret_cast<decltype(&::name)>(at.at(#name));
     ENTRIES(ENTRY)

@@ -47,7 +47,8 @@ def nodes_command(out):
     system = [os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
               os.path.join(rocm, "include"), "/opt/rocm/include", sysconfig.get_paths()["include"]]
     return ([os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-Wall",
-             "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
+             "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", f'-DDH_TORCH_VERSION="{torch.__version__}"',
+             f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
             + [a for d in system for a in ("-isystem", d)] + [f"-I{d}" for d in INCLUDE_DIRS]
             + [NODES_SRC, "-o", out, f"-L{os.path.join(root, 'lib')}"]
             + [f"-l{n}" for n in ("c10", "c10_hip", "torch_cpu", "torch_hip", "torch", "torch_python")])

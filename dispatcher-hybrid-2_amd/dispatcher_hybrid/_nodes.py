@@ -1,13 +1,15 @@
 """The C++ side of ``fused_vocab``: launches and autograd nodes over libdh_mixer's entry points (``csrc/host/vocab_nodes.cpp``).
 
-Bound to the library that ``_hip`` loaded, by address. Importing this module raises ImportError if the extension is missing or
-was built for another torch.
+Bound to the library that ``_hip`` loaded, by address. Loading it raises ImportError if the extension is missing, or was built
+for another torch or another version of the library's interface.
 """
 
 import ctypes
 import importlib.machinery
 import importlib.util
 import os
+
+import torch
 
 from . import _hip
 
@@ -23,5 +25,10 @@ def load(differentiable):
     loader = importlib.machinery.ExtensionFileLoader("_vocab_nodes", _PATH)
     module = importlib.util.module_from_spec(importlib.util.spec_from_loader("_vocab_nodes", loader))
     loader.exec_module(module)
+    # (it calls bare addresses: with another interface it would hand the kernels shifted arguments)
+    built = getattr(module, "abi_version", None), getattr(module, "torch_version", None)
+    if built != (_hip.ABI_VERSION, str(torch.__version__)):
+        raise ImportError(f"{_PATH} was built for ABI version {built[0]} and torch {built[1]}, not {_hip.ABI_VERSION} and "
+                          f"{torch.__version__}; rebuild it")
     module.bind({name: ctypes.cast(getattr(_hip.lib, name), ctypes.c_void_p).value for name in _ENTRIES}, differentiable)
     return module

@@ -1,8 +1,6 @@
 """Corners of the vocabulary-end operators that need no GPU: the formula's rows without a value, the entry points' refusals, the
 library and the extension beside it."""
 
-import math
-
 import pytest
 import torch
 
@@ -29,7 +27,7 @@ def test_a_bad_row_without_live_slots_has_a_gradient_of_nan(weight, with_labels)
         labels[2] = -100
         rows = plain.distillation_loss(leaf, t, tok, labels, 2.0, weight, reduction="none")
         grad, = torch.autograd.grad(rows.sum(), leaf)
-        assert rows[2] == 0 and bool((grad[2] == 0).all()) and math.isnan(rows[1]) == (weight > 0)
+        assert rows[2] == 0 and bool((grad[2] == 0).all()) and bool(rows[1].isnan()) == (weight > 0)
 
 
 @pytest.mark.parametrize("host", ["/nonexistent/g++", "/bin/false"])
@@ -49,3 +47,36 @@ def test_the_kernel_library_is_built_where_the_extension_does_not_compile(host, 
     assert _build.build() == str(out / "lib.so")
     assert [f.name for f in out.iterdir()] == ["lib.so"]
     assert "fused_vocab needs it" in capsys.readouterr().err
+
+
+def test_an_extension_built_for_something_else_is_not_bound(monkeypatch):
+    """Another version of the C interface, another torch, one that says neither."""
+    from dispatcher_hybrid import _hip, _nodes
+    bound = []
+
+    class Loader:
+        def __init__(self, *a):
+            pass
+
+        def create_module(self, spec):
+            return None
+
+        def exec_module(self, module):
+            module.bind = lambda *a: bound.append(a)
+            for name, value in says.items():
+                setattr(module, name, value)
+    monkeypatch.setattr(_nodes.importlib.machinery, "ExtensionFileLoader", Loader)
+    right = dict(abi_version=_hip.ABI_VERSION, torch_version=str(torch.__version__))
+    for says in (dict(right, abi_version=_hip.ABI_VERSION - 1), dict(right, torch_version="1.0"), {}):
+        with pytest.raises(ImportError, match="rebuild"):
+            _nodes.load(None)
+    assert not bound
+    says = right
+    _nodes.load(None)
+    assert len(bound) == 1
+
+
+def test_the_extension_says_what_it_was_built_for():
+    from dispatcher_hybrid import _hip, fused_vocab
+    native = fused_vocab._native
+    assert (native.abi_version, native.torch_version) == (_hip.ABI_VERSION, str(torch.__version__))
