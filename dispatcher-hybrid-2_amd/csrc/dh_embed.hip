@@ -132,6 +132,9 @@ static_assert(kSmallRows <= kPW * kList, "a wave's ids all fit its list");
 constexpr int kMany = 64;
 constexpr int kFew = 16;                   // dy rows in flight a wave
 
+// bytes of dynamic LDS: counters, starts of the ids and their end, positions
+constexpr int small_lds(int range, int n) { return (kPW * range + range + 1 + n) * (int)sizeof(int); }
+
 struct Starter {
   int32_t token, last;
 };
@@ -563,11 +566,13 @@ int gradient(const void* dy, int64_t ldy, const void* ids, int wide, int64_t n, 
   const Sink to{dy, ldy, dW, scale, pieces};
   const dim3 owners(1u << own.lg);
   if (small(n, d)) {
-    const int lds = (kPW * own.range + own.range + 1 + (int)n) * (int)sizeof(int);
+    const int lds = small_lds(own.range, (int)n);
     if (lds > 28 << 10) {                  // (64 KB with the lists)
+      // the kernel's limit is the process's: always the same, so that no host thread lowers it before another's launch
+      constexpr int most = small_lds(kMaxRange, kSmallRows);
       const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&place_kernel<T, N, true>),
-                                               hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-      if (e != hipSuccess) return dh_fail(DH_ERR_LAUNCH_FAILED, "dh_embed_bwd: %d bytes of LDS: %s", lds, hipGetErrorString(e));
+                                               hipFuncAttributeMaxDynamicSharedMemorySize, most);
+      if (e != hipSuccess) return dh_fail(DH_ERR_LAUNCH_FAILED, "dh_embed_bwd: %d bytes of LDS: %s", most, hipGetErrorString(e));
     }
     place_kernel<T, N, true><<<owners, dim3(kPT), lds, s>>>(ids, wide, (int)n, V, own, skip, starts, pairs, to);
     return dh_check_launch("dh_embed_bwd");

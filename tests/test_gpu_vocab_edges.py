@@ -133,3 +133,32 @@ def test_targets_of_inference_mode():
     leaf = z.clone().requires_grad_()
     one, = torch.autograd.grad(ops().distillation_loss(leaf, *targets, labels, 2.0, 0.5), leaf, create_graph=True)
     assert torch.autograd.grad(one.square().sum(), leaf)[0].isfinite().all()
+
+
+def test_two_host_threads_with_wide_vocabularies_of_their_own():
+    """The one-launch gradient at more than 64 KB of LDS, at two sizes at once."""
+    import threading
+    data = []
+    for V, n in ((122001, 512), (105001, 300)):
+        g = gen(V)
+        data.append((torch.randn(n, 24, device=DEV, generator=g), torch.randint(0, V, (n,), device=DEV, generator=g), V))
+    f = lambda dy, ids, V: ops()._lookup_grad(dy, ids, V, 1.0, -1)
+    ref = [f(*d) for d in data]
+    for (dy, ids, V), x in zip(data, ref):
+        assert (x.double() - torch.zeros(V, 24, dtype=torch.float64, device=DEV).index_add_(0, ids, dy.double())).abs().max() < 1e-4
+    torch.cuda.synchronize()
+    got, begin = [[], []], threading.Barrier(2)
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            begin.wait(60)
+            for _ in range(20):
+                got[i].append(f(*data[i]))
+            torch.cuda.current_stream().synchronize()
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join(60)
+    for outs, x in zip(got, ref):
+        assert len(outs) == 20 and all(torch.equal(o, x) for o in outs)
