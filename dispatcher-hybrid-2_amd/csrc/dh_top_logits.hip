@@ -35,6 +35,11 @@ constexpr int kCap = 9 * kMaxK;            // keys in LDS: ties leave up to E K 
 constexpr int kMany = 512, kLong = 8192;
 constexpr int kFew = 128;                  // keys up to which a thread ranks one (K 64: 95 keys or so, 256: 330)
 constexpr int kU = 4;                      // 16-byte loads in flight a thread
+// Groups are lines where there are kLines times as many lines as the bisection may leave, or one for every thread: with few more
+// groups than that the bound falls to the lowest of their maxima, and the whole row is above it.
+// Lines and, by this rule, pieces, 2048 rows of bf16, K 256, us: 256 lines 614 and 53, 320 lines 94 and 55, 448 lines 61 and 58;
+// K 160, 256 lines 42 and 33, 320 lines 40 and 35.
+constexpr int kLines = 2;
 
 __device__ __forceinline__ uint32_t image_of(float x) {        // a < b  <=>  image(a) < image(b); NaN above all
   if (x != x) return 0xffffffffu;
@@ -103,7 +108,7 @@ __global__ __launch_bounds__(NT, 8) void top_kernel(const T* logits, int64_t str
   };
   const int extra = tid < head ? tid : tid < head + tail ? V - tail + (tid - head) : -1;   // token of the single logit
   const float ex = extra >= 0 ? Elem<T>::load(row + extra) : -INFINITY;
-  const bool lines = pieces >= 4 * nt;
+  const bool lines = pieces >= 4 * nt && (pieces >= 8 * nt || pieces / 8 >= kLines * (K + kSlack));
   // which of a stretch's eight pieces is on the line of thread t, as the exchange below leaves them
   auto line = [](int t) { return (t & 1) << 2 | (t & 4) >> 1 | (t & 2) >> 1; };
   const int first_piece = lines ? line(tid) * nt + (tid & ~7) : tid;           // of the thread's group

@@ -162,3 +162,37 @@ def test_two_host_threads_with_wide_vocabularies_of_their_own():
         th.join(60)
     for outs, x in zip(got, ref):
         assert len(outs) == 20 and all(torch.equal(o, x) for o in outs)
+
+
+# ---- top logits -----------------------------------------------------------------------------------------------------
+
+def us(fn, turns=9):
+    """Median time of a call among calls, in microseconds."""
+    for _ in range(3):
+        fn()
+    marks = [torch.cuda.Event(enable_timing=True) for _ in range(turns + 1)]
+    marks[0].record()
+    for m in marks[1:]:
+        fn()
+        m.record()
+    torch.cuda.synchronize()
+    return sorted(a.elapsed_time(b) * 1e3 for a, b in zip(marks, marks[1:]))[turns // 2]
+
+
+def check_top(x, k):
+    values, tokens = ops().top_logits(x, k)
+    ref, at = torch.sort(x.double(), dim=-1, descending=True, stable=True)
+    assert torch.equal(tokens, at[..., :k]) and torch.equal(values, x.gather(-1, tokens))
+
+
+@pytest.mark.parametrize("dtype,V", [(torch.bfloat16, 16384), (torch.float32, 8192)])
+def test_many_targets_of_a_vocabulary_with_few_lines(V, dtype):
+    """Just above where a row's groups may be whole lines there are as many lines as targets: neighbouring vocabularies cost
+    alike (they were 8 to 15 times apart)."""
+    times = []
+    for v in (V - 8, V, V + 8, V + 600):
+        x = (torch.randn(2048, v, device=DEV, generator=gen(v)) * 2).to(dtype)
+        check_top(x[:600], 256)
+        times.append(us(lambda: ops().top_logits(x, 256)))
+    say("lines", dtype, V, times)
+    assert max(times) < 3 * times[0]
