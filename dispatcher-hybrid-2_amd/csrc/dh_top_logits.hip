@@ -6,7 +6,8 @@
 // above the complement of the token. The K largest keys are the answer, with no case for ties; below the token a bit says
 // which zero it was, so that a key has its value whole (NaN apart).
 //
-// One workgroup a row, which reads the row once and goes back to a tenth of it or less:
+// One workgroup a row, which reads the row once and goes back to a part of it, about (K + kSlack) of its groups (a fifth of a
+// long row at K 64 with 512 groups, half of it at K 256):
 //   - the largest value of every group of logits, one group a thread: its own 16-byte pieces or, in long rows, one 128-byte
 //     line of each eight pieces that it read with its seven neighbours (whole lines, so that going back costs no more than
 //     the groups themselves hold);
@@ -15,10 +16,13 @@
 //   - those groups are read again, by the whole workgroup, and the logits at the bound or above (K and a few tens more: a
 //     group rarely holds two) go to LDS as keys;
 //   - a key's rank is the number of larger keys; ranks below K write their value and token.
-// Ties at the bound (masked vocabularies, constant rows) take the lower tokens first. Rows with a NaN, and rows whose large
-// values all stand in few groups, more than LDS holds, are bisected as a whole, slowly. The first pass is bound by its read.
-// 4096 x 50257 bf16, K 64: 79 us, 5.2 TB/s. (Rows kept in registers instead of read again: 130 us; a wave a row with a
-// running bound: 219 us; groups of pieces from eight lines each, which going back reads whole: 106 us.)
+// Ties at the bound take the lower tokens first. Where more keys pass than LDS holds (masked vocabularies and constant rows,
+// whose ties fill whole lines; large values in few groups), the K-th largest of the keys that it does hold is the next bound
+// and the row is read again, nearly always once: 1024 x 50257, masked to 40 tokens, bf16 K 64 211 us where bisecting the row
+// took 3916, fp32 K 256 420 where it took 6512, beside 27 and 56 of ordinary rows. Rows with a NaN are bisected, slowly.
+// The first pass is bound by its read. 4096 x 50257 bf16, K 64: 79 us, 5.2 TB/s. (Rows kept in registers instead of read
+// again: 130 us; a wave a row with a running bound: 219 us; groups of pieces from eight lines each, which going back reads
+// whole: 106 us.)
 
 #include <type_traits>
 
@@ -28,7 +32,8 @@ namespace {
 
 constexpr int kMaxK = 256;
 constexpr int kSlack = 32;                 // threads more than K that end the bisection
-constexpr int kCap = 9 * kMaxK;            // keys in LDS: ties leave up to E K of them, and K above
+constexpr int kCap = 9 * kMaxK;            // keys in LDS: where groups are pieces, ties leave up to E K of them, and K above
+constexpr int kTurns = 4;                  // reads of a row whose keys do not fit, each by a higher bound, before the bisection
 // Rows from which a row of fewer than kLong pieces gets 512 threads in place of 1024, so that four rows share a CU (K 64, in a
 // graph; bf16, V 50257: 85 against 95 us at 4096 rows, 29 against 33 at 1024, 19 against 20 at 512; V 8000, 4096 rows: 38
 // against 73; 16000 pieces, 1024 rows: 56 against 50; fp32, V 50257, 1024 rows: 48 against 43).
@@ -298,28 +303,47 @@ __global__ __launch_bounds__(NT, 8) void top_kernel(const T* logits, int64_t str
   }
   __syncthreads();
   int n = count;
-  if (n > kCap || nans) {                  // uniform: the exact K-th largest key of the whole row
-    int got = V;
-    const uint64_t lo = bisect((uint64_t)1, (uint64_t)~0ull, K, K, got, [&](uint64_t v) {
-      int c = 0;
-      each([&](uint64_t k) { c += k >= v; });
+  auto total = [&](int c) {                // over the workgroup
 #pragma unroll
-      for (int o = 32; o > 0; o >>= 1) c += __shfl_xor(c, o);
-      __syncthreads();
-      if (lane == 0) part[wave] = c;
-      __syncthreads();
-      c = 0;
-      for (int i = 0; i < nt / 64; ++i) c += part[i];
-      return c;
-    });
+    for (int o = 32; o > 0; o >>= 1) c += __shfl_xor(c, o);
+    __syncthreads();
+    if (lane == 0) part[wave] = c;
+    __syncthreads();
+    c = 0;
+    for (int i = 0; i < nt / 64; ++i) c += part[i];
+    return c;
+  };
+  auto gather = [&](uint64_t lo) {         // the row's keys from lo on, or kCap of them; how many there are
     __syncthreads();
     if (tid == 0) count = 0;
     __syncthreads();
     each([&](uint64_t k) {
-      if (k >= lo) keys[atomicAdd(&count, 1)] = k;             // K of them: keys differ
+      if (k < lo) return;
+      const int at = atomicAdd(&count, 1);
+      if (at < kCap) keys[at] = k;
     });
     __syncthreads();
-    n = K;
+    return count;
+  };
+  // more keys than LDS holds: the K-th largest of those that it does is a higher bound
+  uint64_t lo = nans ? (uint64_t)1 : least;
+  for (int turn = 0; turn < kTurns && n > kCap && !nans; ++turn) {             // uniform
+    int got = kCap;
+    lo = bisect(lo, (uint64_t)~0ull, K, K, got, [&](uint64_t v) {
+      int c = 0;
+      for (int i = tid; i < kCap; i += nt) c += keys[i] >= v;
+      return total(c);
+    });
+    n = gather(lo);
+  }
+  if (n > kCap || nans) {                  // uniform: the exact K-th largest key of the whole row; keys differ
+    int got = V;
+    lo = bisect(lo, (uint64_t)~0ull, K, K, got, [&](uint64_t v) {
+      int c = 0;
+      each([&](uint64_t k) { c += k >= v; });
+      return total(c);
+    });
+    n = gather(lo);
   }
   // ranks, eight threads each; four keys a thread where there are many, so that a key read serves four
   auto ranks = [&](auto many) {

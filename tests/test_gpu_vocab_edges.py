@@ -196,3 +196,35 @@ def test_many_targets_of_a_vocabulary_with_few_lines(V, dtype):
         times.append(us(lambda: ops().top_logits(x, 256)))
     say("lines", dtype, V, times)
     assert max(times) < 3 * times[0]
+
+
+ROWS = {"equal": lambda i, x: torch.full_like(x, 1.5),
+        "masked": lambda i, x: torch.where(i < 40, x, -math.inf),                 # fewer tokens than targets
+        "low": lambda i, x: torch.where((i < 30) | (i >= i.numel() - 9), x, torch.finfo(x.dtype).min),
+        "steps": lambda i, x: (i // 512).to(x.dtype).expand_as(x),                # large values in few groups
+        "falling steps": lambda i, x: (-(i // 5000)).to(x.dtype).expand_as(x),
+        "halves": lambda i, x: torch.where(i % 2 == 0, 2.0, x.clamp(max=1.0)),    # ties in every piece
+        "teeth": lambda i, x: ((i * 7919) % 4099 // 512).to(x.dtype).expand_as(x)}
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,V", [(1, 50257), (600, 50257), (3, 400001), (700, 9001)])
+@pytest.mark.parametrize("what", list(ROWS))
+def test_top_logits_of_rows_with_more_candidates_than_fit(what, rows, V, dtype):
+    say("top", what, rows, V, dtype)
+    x = torch.randn(rows, V, device=DEV, generator=gen(rows + V)).to(dtype)
+    x = ROWS[what](torch.arange(V, device=DEV), x)
+    for k in (1, 20, 64, 256):
+        check_top(x, k)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("what", ["equal", "masked", "steps"])
+def test_what_a_masked_vocabulary_costs(what, dtype):
+    """Rows of ties and few live tokens against ordinary ones: a few more reads (they took 70 to 150 times as long)."""
+    x = (torch.randn(1024, 50257, device=DEV, generator=gen(3)) * 2).to(dtype)
+    y = ROWS[what](torch.arange(50257, device=DEV), x).contiguous()
+    for k in (64, 256):
+        usual, odd = us(lambda: ops().top_logits(x, k)), us(lambda: ops().top_logits(y, k))
+        say("cost", what, dtype, k, usual, odd)
+        assert odd < 20 * usual
