@@ -721,6 +721,8 @@ extern "C" int dh_distill_fwd(int dtype, const void* logits, int64_t stride_b, i
   DH_REQUIRE(a.rows == 0 || (row_loss && row_kept && (uintptr_t)row_kept % 16 == 0), DH_ERR_INVALID_ARG,
              "%s: null or unaligned pointer argument", who);
   DH_REQUIRE(reduction == 0 || (loss && divisor), DH_ERR_INVALID_ARG, "%s: null pointer argument", who);
+  DH_REQUIRE((uintptr_t)row_loss % 4 == 0 && (uintptr_t)loss % 4 == 0 && (uintptr_t)divisor % 4 == 0, DH_ERR_INVALID_ARG,
+             "%s: results not aligned to their elements", who);
   const int64_t need = dh_distill_workspace_bytes(dtype, a.rows, V);
   DH_REQUIRE(workspace_bytes >= need && (need == 0 || (workspace && (uintptr_t)workspace % 8 == 0)), DH_ERR_INVALID_ARG,
              "%s: workspace of %lld bytes, %lld needed", who, (long long)workspace_bytes, (long long)need);
@@ -748,6 +750,8 @@ extern "C" int dh_distill_bwd(int dtype, const void* logits, int64_t stride_b, i
   if (a.rows == 0) return 0;
   DH_REQUIRE(row_kept && (uintptr_t)row_kept % 16 == 0 && dloss && dlogits && dloss_stride >= 0, DH_ERR_INVALID_ARG,
              "%s: null or unaligned pointer argument", who);
+  DH_REQUIRE((uintptr_t)dloss % 4 == 0 && (uintptr_t)divisor % 4 == 0 && (uintptr_t)dlogits % (dtype == DH_BF16 ? 2 : 4) == 0,
+             DH_ERR_INVALID_ARG, "%s: operands not aligned to their elements", who);
   const int parts = parts_of(a.rows, V, dtype);
   const Kept* kept = (const Kept*)row_kept;
   hipStream_t s = (hipStream_t)stream;

@@ -80,3 +80,24 @@ def test_the_extension_says_what_it_was_built_for():
     from dispatcher_hybrid import _hip, fused_vocab
     native = fused_vocab._native
     assert (native.abi_version, native.torch_version) == (_hip.ABI_VERSION, str(torch.__version__))
+
+
+def test_the_loss_entry_points_refuse_results_off_their_elements():
+    from dispatcher_hybrid import _hip
+    lib, one, N = _hip.lib, 256, None                          # never dereferenced: every call is refused
+
+    def fwd(**kw):
+        a = dict(dtype=1, z=one, sb=8, st=8, B=1, T=2, V=8, td=1, tl=one, tt=one, bits=64, K=2, lb=N, lbits=64, ignore=-100,
+                 tau=1.0, w=1.0, red=1, rows=one, kept=one, loss=one, div=one, ws=N, nb=0)
+        a.update(kw)
+        return lib.dh_distill_fwd(*a.values(), N)
+
+    def bwd(**kw):
+        a = dict(dtype=1, z=one, sb=8, st=8, B=1, T=2, V=8, td=1, tl=one, tt=one, bits=64, K=2, lb=N, lbits=64, ignore=-100,
+                 tau=1.0, w=1.0, kept=one, dl=one, ds=0, div=one, dz=one)
+        a.update(kw)
+        return lib.dh_distill_bwd(*a.values(), N)
+    for kw in (dict(rows=one + 2), dict(loss=one + 1), dict(div=one + 2)):
+        assert fwd(**kw) == 1 and b"aligned" in lib.dh_last_error(), kw
+    for kw in (dict(dl=one + 2), dict(div=one + 2), dict(dz=one + 1), dict(dtype=0, dz=one + 2)):
+        assert bwd(**kw) == 1 and b"aligned" in lib.dh_last_error(), kw
