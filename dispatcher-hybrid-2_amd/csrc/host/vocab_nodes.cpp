@@ -81,6 +81,9 @@ void same_count(const char* what, const char* which, int64_t has, int64_t needs)
   TORCH_CHECK_VALUE(has == needs, what, ": ", which, " of ", has, " elements, ", needs, " needed");
 }
 
+// for the entry points' ints: what does not fit is -1, which they refuse
+int narrow(int64_t v) { return v >= 0 && v <= INT32_MAX ? (int)v : -1; }
+
 Tensor fresh(const Tensor& t) { return t.clone(at::MemoryFormat::Contiguous); }
 // unit-stride rows (any other layout copied); broadcast rows stay
 Tensor unit_rows(const Tensor& t) { return t.stride(-1) == 1 || t.size(-1) == 1 ? t : t.contiguous(); }
@@ -99,8 +102,7 @@ Tensor lookup(const Tensor& weight, const Tensor& tokens, double scale, int64_t 
   shape.push_back(d);
   Tensor out = at::empty(shape, weight.options());
   const int id_bits = bits(what, ids);
-  // (a width past an int is refused by the entry point, as -1)
-  check(lib.dh_embed_fwd(code, w.data_ptr(), w.stride(0), V, d <= INT32_MAX ? (int)d : -1, ids.data_ptr(), id_bits, ids.numel(),
+  check(lib.dh_embed_fwd(code, w.data_ptr(), w.stride(0), V, narrow(d), ids.data_ptr(), id_bits, ids.numel(),
                          (float)scale, zero_token, out.data_ptr(), d, stream_of(w)),
         what);
   return out;
@@ -119,7 +121,7 @@ Tensor lookup_grad(const Tensor& dy, const Tensor& tokens, int64_t rows, double 
   Tensor y = dy.dim() == 2 ? dy : dy.reshape({-1, d});
   if (y.stride(1) != 1 || y.stride(0) < d) y = fresh(y);
   Tensor out = at::empty({rows, d}, dy.options());
-  const int width = d <= INT32_MAX ? (int)d : -1;
+  const int width = narrow(d);
   const int64_t bytes = lib.dh_embed_bwd_workspace_bytes(ids.numel(), rows, width);
   Tensor ws;                                                   // (refused sizes: the call says why)
   if (bytes > 0) ws = at::empty({bytes}, dy.options().dtype(at::kByte));
@@ -180,7 +182,7 @@ std::tuple<Tensor, Tensor> top_logits(const Tensor& logits, int64_t k) {
   shape.back() = k;
   Tensor values = at::empty(shape, logits.options().requires_grad(false)),
          tokens = at::empty(shape, logits.options().dtype(at::kLong).requires_grad(false));
-  check(lib.dh_top_logits(code, rows.data_ptr(), rows.stride(0), rows.size(0), V <= INT32_MAX ? (int)V : -1, (int)k,
+  check(lib.dh_top_logits(code, rows.data_ptr(), rows.stride(0), rows.size(0), narrow(V), narrow(k),
                           values.data_ptr(), tokens.data_ptr<int64_t>(), stream_of(logits)),
         what);
   return {values, tokens};
@@ -204,7 +206,7 @@ struct Rows {
         labels(lb.defined() ? lb.contiguous() : lb),
         code(dtype_code(logits)),
         t_code(dtype_code(teacher_logits)),
-        V(logits.size(-1) <= INT32_MAX ? (int)logits.size(-1) : -1) {
+        V(narrow(logits.size(-1))) {
     if (z.dim() > 3) z = unit_rows(z.reshape({-1, z.size(-1)}));
     if (z.dim() == 3) {
       B = z.size(0), T = z.size(1), sb = z.stride(0), st = z.stride(1);
@@ -243,8 +245,8 @@ std::tuple<Tensor, Tensor> distill(const Tensor& logits, const Tensor& teacher_l
   Tensor kept = at::empty({first + rows + (bytes + 3) / 4}, f32);
   float* at_ = kept.data_ptr<float>();
   check(lib.dh_distill_fwd(a.code, a.z.data_ptr(), a.sb, a.st, a.B, (int)a.T, a.V, a.t_code, a.t_logits.data_ptr(),
-                           a.t_tokens.data_ptr(), a.token_bits, (int)a.K(), a.label_ptr(), a.label_bits,
-                           m.ignore_index, (float)m.temperature, (float)m.weight, (int)m.reduction,
+                           a.t_tokens.data_ptr(), a.token_bits, narrow(a.K()), a.label_ptr(), a.label_bits,
+                           m.ignore_index, (float)m.temperature, (float)m.weight, narrow(m.reduction),
                            m.reduction ? at_ + first : out.data_ptr<float>(), at_, m.reduction ? out.data_ptr<float>() : nullptr,
                            m.reduction ? at_ + 4 * n : nullptr, at_ + first + rows, bytes, stream_of(logits)),
         what);
@@ -266,7 +268,7 @@ Tensor distill_grad(const Tensor& grad, const Tensor& logits, const Tensor& teac
   if (!kept.is_contiguous() || reinterpret_cast<uintptr_t>(kept.data_ptr()) % 16) kept = fresh(kept);
   const float* at_ = kept.data_ptr<float>();
   check(lib.dh_distill_bwd(a.code, a.z.data_ptr(), a.sb, a.st, a.B, (int)a.T, a.V, a.t_code, a.t_logits.data_ptr(),
-                           a.t_tokens.data_ptr(), a.token_bits, (int)a.K(), a.label_ptr(), a.label_bits,
+                           a.t_tokens.data_ptr(), a.token_bits, narrow(a.K()), a.label_ptr(), a.label_bits,
                            m.ignore_index, (float)m.temperature, (float)m.weight, at_, g.data_ptr<float>(),
                            m.reduction ? 0 : g.stride(0), m.reduction ? at_ + 4 * a.n : nullptr, dz.data_ptr(),
                            stream_of(logits)),

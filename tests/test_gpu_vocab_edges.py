@@ -228,3 +228,13 @@ def test_what_a_masked_vocabulary_costs(what, dtype):
         usual, odd = us(lambda: ops().top_logits(x, k)), us(lambda: ops().top_logits(y, k))
         say("cost", what, dtype, k, usual, odd)
         assert odd < 20 * usual
+
+
+def test_numbers_past_32_bits_are_refused():
+    """By the registered operations' names, where nothing else checks them; no rows, so that nothing needs memory."""
+    o, far = torch.ops.dispatcher, 2 ** 32
+    z, tok = torch.zeros(0, 50, device=DEV), torch.zeros(0, 3, dtype=torch.long, device=DEV)
+    for call in (lambda: o.top_logits(z, far + 1), lambda: o.distillation_loss(z, z[:, :3], tok, None, 1.0, 1.0, -100, far),
+                 lambda: o.distillation_loss(z, z[:, :1].expand(0, far + 3), tok[:, :1].expand(0, far + 3), None, 1.0, 1.0, -100, 1)):
+        with pytest.raises(ValueError):
+            call()
