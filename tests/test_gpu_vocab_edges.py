@@ -94,6 +94,33 @@ def test_fp32_infinite_and_lowest_logits_at_any_temperature(rows, tau):
         assert bool(grad.isfinite().all()) and bool((grad[:2, 5:] == 0).all()) and not bool(each.isnan().any())
 
 
+@pytest.mark.parametrize("dtype,rows,V", [(torch.bfloat16, 1100, 130001), (torch.float32, 1100, 65001),
+                                          (torch.bfloat16, 40, 4000001)])         # odd rows; the last over several workgroups
+def test_gradients_past_the_caches(dtype, rows, V):
+    """A gradient of more than 256 MiB, stored past the caches with the named tokens written behind, against the same rows in two
+    calls of less: the same bits."""
+    say("past", dtype, rows, V)
+    g, size, K = gen(V), 2 if dtype == torch.bfloat16 else 4, 64
+    assert rows * V * size >= 256 << 20 > (rows // 2) * V * size
+    z = torch.randn(rows, V, device=DEV, generator=g, dtype=torch.bfloat16).to(dtype)
+    t = torch.randn(rows, K, device=DEV, generator=g)
+    tok = torch.randint(0, V, (rows, K), device=DEV, generator=g)
+    tok[:, :10] = torch.arange(10, device=DEV)                                    # the ends of a row, where its pieces begin
+    tok[:, 10:20] = V - 1 - torch.arange(10, device=DEV)
+    tok[:, 40:] = tok[:, 20:21]                                                   # the same token again and again
+    labels = tok[:, 5].clone()
+    labels[::7], labels[3] = -100, tok[3, 20]
+    f = torch.rand(rows, device=DEV, generator=g) + 0.5
+    ops()                                                      # registers them
+    o, half = torch.ops.dispatcher, rows // 2
+    _, kept = o.distillation_loss(z, t, tok, labels, 2.0, 0.5, -100, 0)
+    whole = o.distillation_loss_grad(f, z, t, tok, labels, kept, 2.0, 0.5, -100, 0)
+    for a, b in ((0, half), (half, rows)):
+        part = o.distillation_loss_grad(f[a:b], z[a:b], t[a:b], tok[a:b], labels[a:b], kept[4 * a:4 * b + 4], 2.0, 0.5, -100, 0)
+        assert torch.equal(part, whole[a:b])
+    assert bool((whole[::7] == 0).all()) and bool((whole[1, tok[1]] != 0).all())
+
+
 # ---- errors and foreign tensors -------------------------------------------------------------------------------------
 
 def test_an_allocation_that_fails_is_torchs_error():
@@ -232,6 +259,7 @@ def test_what_a_masked_vocabulary_costs(what, dtype):
 
 def test_numbers_past_32_bits_are_refused():
     """By the registered operations' names, where nothing else checks them; no rows, so that nothing needs memory."""
+    ops()
     o, far = torch.ops.dispatcher, 2 ** 32
     z, tok = torch.zeros(0, 50, device=DEV), torch.zeros(0, 3, dtype=torch.long, device=DEV)
     for call in (lambda: o.top_logits(z, far + 1), lambda: o.distillation_loss(z, z[:, :3], tok, None, 1.0, 1.0, -100, far),
