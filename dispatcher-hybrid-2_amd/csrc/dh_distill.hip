@@ -364,10 +364,13 @@ __global__ __launch_bounds__(kT + 64) void forward_kernel(Rows a, int parts, Sum
       v.s0 *= exp_of<kFull<T>>(v.m - ref, c0);
       if (M != kOne) v.s1 *= exp_of<kFull<T>>(v.m - ref, c1);
       v.m = most;
+      // sums of a piece, of the pieces, of all: a thread's sum is rounded once for N E exponentials (each added to it alone, the
+      // rest of a row beside its largest logit was off by up to half a step for every one of them)
       constexpr float kTimes = M == kFourth ? 4.f : 2.f;
-      float k0 = 0.f, k1 = 0.f;
+      float t0 = 0.f, t1 = 0.f, k0 = 0.f, k1 = 0.f;
 #pragma unroll
-      for (int u = 0; u < N; ++u)
+      for (int u = 0; u < N; ++u) {
+        float p0 = 0.f, p1 = 0.f;
 #pragma unroll
         for (int j = 0; j < E; ++j) {
           float e0, e1;
@@ -384,13 +387,14 @@ __global__ __launch_bounds__(kT + 64) void forward_kernel(Rows a, int parts, Sum
           } else {
             exps<M, false>(d, c0, c1, e0, e1);
           }
-          v.s0 += e0;
-          if (M != kOne) v.s1 += e1;
+          p0 = j ? p0 + e0 : e0;
+          if (M != kOne) p1 = j ? p1 + e1 : e1;
         }
-      if constexpr (kFull<T>) {
-        v.s0 = __builtin_fmaf(k0, (float)kLn2, v.s0);
-        if (M != kOne) v.s1 = __builtin_fmaf(k1, (float)kLn2, v.s1);
+        t0 = u ? t0 + p0 : p0;
+        if (M != kOne) t1 = u ? t1 + p1 : p1;
       }
+      v.s0 += kFull<T> ? __builtin_fmaf(k0, (float)kLn2, t0) : t0;
+      if (M != kOne) v.s1 += kFull<T> ? __builtin_fmaf(k1, (float)kLn2, t1) : t1;
     };
     int p = c.p0 + tid;
     for (; p + (U - 1) * kT < c.p1; p += U * kT) {

@@ -77,6 +77,40 @@ def test_fp32_probabilities_far_below_the_maximum(tau, w, rows):
     assert worst <= 22, worst
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("tau,w", [(1.0, 1.0), (2.0, 0.5), (1.0, 0.0)])
+def test_many_small_exponentials_beside_a_large_one(tau, w, dtype):
+    """A logit of 0 and 400000 of about -15 (times the temperature), each some 2.5 steps of the numbers from 1 on: added to the 1
+    one by one, every rounding is off by nearly half a step to the same side.
+
+    Bounds: a thread reads V / 256 logits, 16 fp32 or 32 bf16 between two roundings of its sum, so the one that holds the 1 is
+    off by at most V / 4096 (V / 8192) u; 7 u in a wave, 9 over the waves; the other terms, an eighth of the sum, by 11 u in
+    their sums and by 3 u (fp32) or 25 u (bf16: an exponent of 22 rounded twice) each: 5 u of the whole. The loss is the log of
+    that sum, a term of it the exponent of the hard one at temperature 2, where all of it is smaller; the gradient's factors
+    and its exp 9 u, or 31 u and the type's half step."""
+    rows, V = 520, 400001
+    x0 = -15.03125 if dtype == torch.float32 else -15.0
+    say("small", dtype, tau, w)
+    z = torch.full((rows, V), x0 * (tau if w > 0 else 1.0), device=DEV, dtype=dtype)
+    z[:, 0] = 0
+    t, tok = torch.zeros(rows, 1, device=DEV), torch.zeros(rows, 1, dtype=torch.long, device=DEV)
+    labels = tok[:, 0].clone()
+    leaf = z.clone().requires_grad_()
+    each = ops().distillation_loss(leaf, t, tok, labels, tau, w, reduction="none")
+    grad, = torch.autograd.grad(each.sum(), leaf)
+    at = float(z[0, 1])
+    sums = lambda s: 1 + (V - 1) * math.exp(at / s)
+    loss = w * tau * tau * math.log(sums(tau)) + (1 - w) * math.log(sums(1.0))
+    dz = w * tau * math.exp(at / tau) / sums(tau) + (1 - w) * math.exp(at) / sums(1.0)
+    full = dtype == torch.float32
+    bound = V / (4096 if full else 8192) + 7 + 9 + 5 + 2
+    scale = w * tau * tau + (1 - w)
+    worst = (each.double() - loss).abs().max().item() / U
+    assert worst <= bound * scale, (worst, bound * scale)
+    worst = (grad[:, 1:].double() - dz).abs().max().item() / dz
+    assert worst <= (bound + (9 if full else 31)) * U + (0 if full else 2.0 ** -8), (worst / U, bound)
+
+
 @pytest.mark.parametrize("tau", [1e-30, 0.5, 3.0, 1e30])
 @pytest.mark.parametrize("rows", [2, 600])
 def test_fp32_infinite_and_lowest_logits_at_any_temperature(rows, tau):
