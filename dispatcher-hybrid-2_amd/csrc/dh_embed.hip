@@ -3,8 +3,9 @@
 //   dW[v]  = rnd(scale sum_{n: id_n = v} dy[n])       (dh_embed_bwd; every row of dW is written)
 // The parallel forward's embedding (reference dispatcher_hybrid/modeling_dispatcher.py:340) and its autograd gradient.
 //
-// The gradient groups the positions by token: sums in fp32 over a token's positions in ascending order, split at fixed
-// places, so the same call gives the same bits whatever the launch order. Three launches:
+// The gradient groups the positions by token: sums in fp32 over stretches of a token's positions in ascending order, split and
+// joined as the ids and the sizes say (chunks, eighths of a token's chunks, sixteenths in the one launch), so the same call gives
+// the same bits whatever the launch order. Three launches:
 //   place  every workgroup owns every 256th token id and reads ALL ids itself (8 n bytes from L2, cheaper than the launches
 //          of a sort that shares work between workgroups): it counts the ids of the owners before it (its offset in the
 //          grouped order) and its own per (wave, token), scans, and writes its (token, position) pairs, positions

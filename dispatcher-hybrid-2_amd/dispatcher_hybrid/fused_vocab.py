@@ -102,8 +102,8 @@ def embed_tokens(tokens, weight, scale=1.0, padding_idx=None):
 
     tokens: int32 or int64 of any shape; weight (V, d) fp32 or bf16 of any width. A token outside [0, V) gives a row of NaN
     (it is neither read nor reported) and no gradient. padding_idx: this token's row gets no gradient, as nn.Embedding's. The
-    gradient is dense: (V, d) in weight's dtype, every token's positions summed in fp32 in ascending order and rounded once,
-    the same bits on every call."""
+    gradient is dense: (V, d) in weight's dtype, every token's positions summed in fp32, by stretches joined in an order
+    that the tokens and sizes fix, and rounded once: the same bits on every call."""
     if tokens.dtype not in _INTS:
         raise TypeError(f"embed_tokens: tokens must be int32 or int64, got {tokens.dtype}")
     if weight.dim() != 2 or weight.shape[0] < 1 or weight.shape[1] < 1:

@@ -575,9 +575,10 @@ int dh_decode_persistent_status(const void* scratch, uint32_t* out2, void* strea
 int dh_embed_fwd(int dtype, const void* W, int64_t ldw, int64_t V, int d, const void* ids, int ids_bits, int64_t n,
                  float scale, int64_t zero_token, void* out, int64_t ldo, void* stream);
 /*
- * The lookup's gradient: dW[v] = scale * sum of dy[n] over the positions n with ids[n] = v, ascending, for every v (rows of
- * zeros where there is none): fp32 sums in an order that depends on the ids alone, rounded once. Positions that hold
- * skip_token (-1: none) or an id outside [0, V) are left out. dy (n, d) rows ldy apart; dW (V, d) contiguous.
+ * The lookup's gradient: dW[v] = scale * sum of dy[n] over the positions n with ids[n] = v, for every v (rows of zeros where
+ * there is none): fp32 sums over stretches of a token's positions, ascending, joined in an order that the ids and the sizes fix
+ * (one token's last bits depend on the other ids), rounded once. Positions that hold skip_token (-1: none) or an id outside
+ * [0, V) are left out. dy (n, d) rows ldy apart; dW (V, d) contiguous.
  *   workspace: dh_embed_bwd_workspace_bytes(n, V, d) bytes (0 for few positions, -1: sizes outside the limits), 16-byte
  *   aligned; contents are needed during the call only.
  */
