@@ -15,7 +15,8 @@
 // 4096 x 50257 bf16, K 64, an eighth of the rows ignored: forward 73 us (360 MB, 4.9 TB/s), backward 154 us (772 MB, 5.0 TB/s).
 //
 // Exponents are taken of z - m (exact for bf16 inputs near m), never of z times a constant: rows of the type's lowest value
-// stay finite. Exponentials of fp32 logits are good to fp32 (exp_of). The few operations on a row's sums are in fp64: log p - log q is a small difference of larger numbers.
+// stay finite. Exponentials of fp32 logits are good to fp32 (exp_of). The few operations on a row's sums are in fp64: log p - log q
+// is a small difference of larger numbers.
 
 #include "dh_common.h"
 
