@@ -1,0 +1,725 @@
+// Log-probabilities of given tokens and the losses made of them, forward and backward, for gfx950. A row of V logits z, a
+// temperature tau, the row's token y:
+//   p = softmax(z / tau),  lp = log p_y,  H = - sum_v p_v log p_v
+//   dz_v = (a ([v = y] - p_v) - e p_v (log p_v + H)) / tau            with a, e the gradients in lp and H
+// A row whose token is ignore_index is not read: lp = H = 0, a gradient of zeros. Three operators share the passes over z:
+//   log-probabilities   lp and, wanted, H of every row; a, e are the caller's gradients
+//   preference loss     sequences i and i + n are a pair. S = the sum (or mean) of a sequence's lp, R a reference's,
+//                       D = (S - R)_i - (S - R)_{i+n}, x = beta D - margin, and of a pair
+//                         sigmoid   - (1 - eps) log sigma(x) - eps log sigma(-x)
+//                         hinge     max(0, 1 - x)
+//                         squared   (D - 1 / (2 beta))^2
+//   policy loss         r = exp(lp - old), an advantage A, d = reference - lp, and of a row
+//                         - min(r A, clip(r, 1 - low, 1 + high) A) + kl (exp(d) - d - 1) - w H
+//                       over the rows, their number, or each sequence's number and the number of sequences
+//
+// Forward: one pass over the row with the running maximum m and the sums of E = exp((z - m) / tau) and, for H, of E times its
+// exponent; the read of z bounds it. Few rows are split over several workgroups, whose sums a second launch joins. The losses
+// add one launch over the rows' lp (and one that adds their parts), which also leaves a and e. Backward: z once more, and dz;
+// m, 1 / sum and the mean exponent are all it needs of a row. A row with a = e = 0 (a clipped ratio, a pair behind the hinge)
+// is not read.
+//
+// Sums over V are fp32 (a thread's over 4 pieces at a time), what follows from a row's sums is fp64, lp included until it is
+// returned: sequence sums, ratios and their comparison with the clip are of unrounded lp.
+
+#include "dh_rows.h"
+
+namespace {
+
+constexpr int kT = 256;
+constexpr int kW = kT / 64;
+constexpr int kMaxParts = 32;
+constexpr float kFar = -200.f;             // an exponent in base 2 whose power is 0: stands in for -inf where it is a factor
+
+struct Rows {
+  const void* logits;
+  int64_t sb, st;                          // strides of row (b, t), b = r / T
+  int rows, T, V;
+  const void* tokens;
+  int wide;
+  int64_t ignore;
+  double inv_tau;
+  Scale c;                                 // log2(e) / tau
+};
+
+template <typename T>
+__device__ __forceinline__ const T* row_of(const Rows& a, int r) {
+  return reinterpret_cast<const T*>(a.logits) + (r / a.T) * a.sb + (r % a.T) * a.st;
+}
+
+// kept of a row for the backward pass
+struct Kept {
+  float m, inv;                            // the maximum, 1 / sum of E (NaN: the row's token is outside the vocabulary)
+  float lean;                              // sum of p (z - m) / tau: log p_v + H = (z_v - m) / tau - lean
+  int live;
+};
+// where a row's results go (null: not wanted)
+struct Results {
+  float *lp, *ent;
+  double *lp64, *ent64;
+  Kept* kept;
+};
+
+struct Sums {
+  float m, s, t;                           // t: the sum of E times its exponent in base 2
+};
+template <bool ENT>
+__device__ __forceinline__ void move_to(Sums& v, float ref, Scale c) {
+  const Exponent x = exponent_of<true>(v.m - ref, c);
+  const float f = exp_of<true>(x);
+  if constexpr (ENT) v.t = f * __builtin_fmaf(v.s, fmaxf(x.h, kFar), v.t);     // (no sum yet: 0 (0 kFar + 0))
+  v.s *= f;
+}
+template <bool ENT>
+__device__ __forceinline__ Sums join(Sums a, Sums b, Scale c) {
+  const float m = fmaxf(a.m, b.m), ref = finite_ref(m);
+  move_to<ENT>(a, ref, c);
+  move_to<ENT>(b, ref, c);
+  return Sums{m, a.s + b.s, ENT ? a.t + b.t : 0.f};
+}
+template <bool ENT>
+__device__ __forceinline__ Sums wave_join(Sums v, Scale c) {
+  const float m = wave_max(v.m);
+  move_to<ENT>(v, finite_ref(m), c);
+  return Sums{m, wave_sum(v.s), ENT ? wave_sum(v.t) : 0.f};
+}
+
+// the results of a row that is not ignored, by one thread; zy: its token's logit, unless the token is outside the vocabulary
+template <bool ENT>
+__device__ __forceinline__ void finish_row(const Rows& a, int r, const Sums& v, float zy, bool bad, const Results& o) {
+  const double nan = __builtin_nan("");
+  const double ls = log((double)v.s), lean = ENT ? (double)v.t * kLn2 / (double)v.s : 0.0;
+  const double lp = bad ? nan : ((double)zy - (double)v.m) * a.inv_tau - ls, ent = bad ? nan : ls - lean;
+  if (o.lp) o.lp[r] = (float)lp;
+  if (o.lp64) o.lp64[r] = lp;
+  if (ENT && o.ent) o.ent[r] = (float)ent;
+  if (ENT && o.ent64) o.ent64[r] = ent;
+  if (o.kept) o.kept[r] = Kept{v.m, bad ? (float)nan : 1.f / v.s, (float)lean, 1};
+}
+__device__ __forceinline__ void skip_row(int r, const Results& o) {
+  if (o.lp) o.lp[r] = 0.f;
+  if (o.lp64) o.lp64[r] = 0.0;
+  if (o.ent) o.ent[r] = 0.f;
+  if (o.ent64) o.ent64[r] = 0.0;
+  if (o.kept) o.kept[r] = Kept{0.f, 0.f, 0.f, 0};
+}
+
+// ---- forward: a row, or one of its parts, by N threads ----------------------------------------------------------------
+template <typename T, bool ENT, int N>
+__device__ __forceinline__ Sums row_sums(const T* z, int V, int which, int parts, int tid, Scale c) {
+  constexpr int E = kE<T>, U = 4;
+  const Cut cut = cut_row(z, V, which, parts);
+  const uint4* base = reinterpret_cast<const uint4*>(z + cut.head);
+  Sums v{-INFINITY, 0.f, 0.f};
+  if (tid < cut.singles) {                 // a logit outside the whole pieces
+    v.m = Elem<T>::load(z + cut.single(tid, V));
+    v.s = exp_of<kFull<T>>(v.m - finite_ref(v.m), c);          // (1, or 0 of -inf: its exponent is 0 or no term)
+    if (ENT && v.s != v.s) v.t = v.s;
+  }
+  auto add = [&](const auto& q) {          // some pieces
+    constexpr int P = sizeof(q) / sizeof(uint4);
+    float x[P][E], most = v.m;
+#pragma unroll
+    for (int u = 0; u < P; ++u) {
+      unpack<T>(q[u], x[u]);
+#pragma unroll
+      for (int j = 0; j < E; ++j) most = fmaxf(most, x[u][j]);
+    }
+    const float ref = finite_ref(most);
+    const Exponent by = exponent_of<kFull<T>>(v.m - ref, c);
+    const float f = exp_of<kFull<T>>(by);
+    if (ENT) v.t = f * __builtin_fmaf(v.s, fmaxf(by.h, kFar), v.t);
+    v.s *= f;
+    v.m = most;
+    // sums of a piece, of the pieces, of all: a thread's sum is rounded once for P E exponentials
+    float s = 0.f, t = 0.f, left = 0.f, left_t = 0.f;
+#pragma unroll
+    for (int u = 0; u < P; ++u) {
+      float p = 0.f, pt = 0.f;
+#pragma unroll
+      for (int j = 0; j < E; ++j) {
+        const Exponent h = exponent_of<kFull<T>>(x[u][j] - ref, c);
+        const float e = exp2_hw(h.h);
+        p = j ? p + e : e;
+        if constexpr (kFull<T>) left = __builtin_fmaf(e, h.l, left);           // (put back after the loop)
+        if constexpr (ENT) {
+          const float eh = e * fmaxf(h.h, kFar);
+          pt = j ? pt + eh : eh;
+          if constexpr (kFull<T>) left_t = __builtin_fmaf(eh, h.l, left_t);
+        }
+      }
+      s = u ? s + p : p;
+      if (ENT) t = u ? t + pt : pt;
+    }
+    v.s += kFull<T> ? __builtin_fmaf(left, (float)kLn2, s) : s;
+    if (ENT) v.t += kFull<T> ? __builtin_fmaf(left_t, (float)kLn2, t) : t;
+  };
+  int p = cut.p0 + tid;
+  for (; p + (U - 1) * N < cut.p1; p += U * N) {
+    uint4 q[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) q[u] = base[p + u * N];
+    add(q);
+  }
+  for (; p < cut.p1; p += N) {
+    uint4 q[1] = {base[p]};
+    add(q);
+  }
+  return wave_join<ENT>(v, c);
+}
+
+// N = 256: a workgroup a row or part of one. N = 64: a wave a row, four to a workgroup, parts 1
+template <typename T, bool ENT, int N>
+__global__ __launch_bounds__(kT) void forward_kernel(Rows a, int parts, Sums* part, Results o) {
+  const int tid = threadIdx.x % N, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int r = N == kT ? (int)blockIdx.x / parts : (int)blockIdx.x * (kT / N) + wave;
+  const int which = N == kT ? (int)blockIdx.x % parts : 0;
+  if (r >= a.rows) return;                 // (N = 64: no barrier follows)
+  const int64_t y = whole(a.tokens, a.wide, r);
+  if (y == a.ignore) {                     // uniform: the row is not read
+    if (tid == 0 && which == 0) skip_row(r, o);
+    return;
+  }
+  const T* z = row_of<T>(a, r);
+  const bool bad = y < 0 || y >= a.V;
+  float zy = 0.f;
+  if (tid == 0 && !bad) zy = Elem<T>::load(z + y);
+  Sums v = row_sums<T, ENT, N>(z, a.V, which, parts, tid, a.c);
+  if constexpr (N == kT) {
+    __shared__ Sums ws[kW];
+    if (lane == 0) ws[wave] = v;
+    __syncthreads();
+    if (tid) return;
+    v = ws[0];
+#pragma unroll
+    for (int w = 1; w < kW; ++w) v = join<ENT>(v, ws[w], a.c);
+    if (parts > 1) {
+      part[blockIdx.x] = v;
+      return;
+    }
+  }
+  if (tid == 0) finish_row<ENT>(a, r, v, zy, bad, o);
+}
+
+// rows split over workgroups: their sums joined, a wave a row
+template <typename T, bool ENT>
+__global__ __launch_bounds__(kT) void join_kernel(Rows a, int parts, const Sums* part, Results o) {
+  const int lane = threadIdx.x & 63;
+  const int r = blockIdx.x * kW + (threadIdx.x >> 6);
+  if (r >= a.rows) return;
+  const int64_t y = whole(a.tokens, a.wide, r);
+  if (y == a.ignore) return;               // the first launch wrote it
+  const bool bad = y < 0 || y >= a.V;
+  float zy = 0.f;
+  if (lane == 0 && !bad) zy = Elem<T>::load(row_of<T>(a, r) + y);
+  Sums v{-INFINITY, 0.f, 0.f};
+  if (lane < parts) v = part[(int64_t)r * parts + lane];
+  v = wave_join<ENT>(v, a.c);
+  if (lane == 0) finish_row<ENT>(a, r, v, zy, bad, o);
+}
+
+// ---- the losses on the rows' log-probabilities ------------------------------------------------------------------------
+// one workgroup's part of a loss: a sum, and what the mean divides it by
+struct Part {
+  double sum;
+  int64_t n;
+};
+
+__device__ __forceinline__ Part wave_part(Part p) {
+  p.sum = wave_sum64(p.sum);
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) p.n += __shfl_xor(p.n, o);
+  return p;
+}
+__device__ __forceinline__ void write_loss(const Part& p, int mean, float* loss, float* divisor) {
+  *loss = (float)(mean ? p.sum / (double)p.n : p.sum);         // (the mean of none is NaN)
+  *divisor = mean ? (float)p.n : 1.f;
+}
+// the parts in a fixed order, by one workgroup
+__global__ __launch_bounds__(1024) void reduce_kernel(const Part* part, int64_t parts, int mean, float* loss, float* divisor) {
+  __shared__ Part red[16];
+  Part p{0.0, 0};
+  for (int64_t i = threadIdx.x; i < parts; i += blockDim.x) {
+    p.sum += part[i].sum;
+    p.n += part[i].n;
+  }
+  p = wave_part(p);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = p;
+  __syncthreads();
+  if (threadIdx.x) return;
+  for (int w = 1; w < (int)blockDim.x / 64; ++w) {
+    p.sum += red[w].sum;
+    p.n += red[w].n;
+  }
+  write_loss(p, mean, loss, divisor);
+}
+
+struct Preference {
+  int pairs, T, kind, average;
+  double beta, margin, eps;
+  const void* reference;                   // null: none
+  int wide;                                // fp64
+};
+
+__device__ __forceinline__ double log1p_exp(double x) {        // log(1 + e^x)
+  return x > 0.0 ? x + log1p(exp(-x)) : log1p(exp(x));
+}
+
+// a workgroup a pair: half of its waves a sequence
+__global__ __launch_bounds__(kT) void preference_kernel(Preference f, const double* lp, const Kept* kept, float* losses,
+                                                        float* sums, float* coef, Part* part, int mean, float* loss,
+                                                        float* divisor) {
+  __shared__ Part red[kW];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = blockIdx.x, half = wave / (kW / 2);
+  const int64_t first = (int64_t)(half ? f.pairs + i : i) * f.T;
+  Part p{0.0, 0};
+  for (int t = threadIdx.x % (kT / 2); t < f.T; t += kT / 2) {
+    p.sum += lp[first + t];
+    p.n += kept[first + t].live;
+  }
+  p = wave_part(p);
+  if (lane == 0) red[wave] = p;
+  __syncthreads();
+  if (threadIdx.x) return;
+  double gain[2], count[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    Part q = red[h * (kW / 2)];
+#pragma unroll
+    for (int w = 1; w < kW / 2; ++w) {
+      q.sum += red[h * (kW / 2) + w].sum;
+      q.n += red[h * (kW / 2) + w].n;
+    }
+    const int s = h ? f.pairs + i : i;
+    count[h] = f.average && q.n > 1 ? (double)q.n : 1.0;
+    const double S = q.sum / count[h];
+    sums[s] = (float)S;
+    gain[h] = S;
+    if (f.reference)
+      gain[h] -= f.wide ? reinterpret_cast<const double*>(f.reference)[s] : (double)reinterpret_cast<const float*>(f.reference)[s];
+  }
+  const double D = gain[0] - gain[1], x = f.beta * D - f.margin;
+  double l, slope;                         // the pair's loss, and its derivative in D
+  if (f.kind == 0) {
+    l = (1.0 - f.eps) * log1p_exp(-x) + (f.eps > 0.0 ? f.eps * log1p_exp(x) : 0.0);
+    slope = f.beta * (f.eps / (1.0 + exp(-x)) - (1.0 - f.eps) / (1.0 + exp(x)));
+  } else if (f.kind == 1) {
+    l = x < 1.0 ? 1.0 - x : x >= 1.0 ? 0.0 : x;                // (NaN stays)
+    slope = x < 1.0 ? -f.beta : x >= 1.0 ? 0.0 : x;
+  } else {
+    l = D - 0.5 / f.beta;
+    slope = 2.0 * l;
+    l *= l;
+  }
+  if (losses) losses[i] = (float)l;
+  coef[i] = (float)(slope / count[0]);
+  coef[f.pairs + i] = (float)(-slope / count[1]);
+  if (!loss) return;
+  const Part one{l, 1};
+  if (gridDim.x == 1)
+    write_loss(one, mean, loss, divisor);
+  else
+    part[i] = one;
+}
+
+struct Policy {
+  int64_t rows;
+  int T;
+  int unit;                                // rows a workgroup: a sequence's T, or any number
+  int by_sequence;                         // divide by a sequence's rows and the number of sequences
+  const float *old, *advantage, *reference;                    // reference null: no third term
+  int adv_div;                             // rows an advantage holds for
+  double low, high, kl, ent;               // 1 - clip, 1 + clip_high, the weights
+};
+
+// by_lp, by_ent: the loss's derivatives in lp and H without the divisor
+__global__ __launch_bounds__(kT) void policy_kernel(Policy f, const double* lp, const double* ent, const Kept* kept,
+                                                    float* losses, float* by_lp, float* by_ent, Part* part, int mean,
+                                                    float* loss, float* divisor) {
+  __shared__ Part red[kW];
+  __shared__ int counts[kW];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t lo = (int64_t)blockIdx.x * f.unit, hi = lo + f.unit < f.rows ? lo + f.unit : f.rows;
+  double share = 1.0;
+  int length = 0;
+  if (f.by_sequence) {
+    for (int64_t r = lo + threadIdx.x; r < hi; r += kT) length += kept[r].live;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) length += __shfl_xor(length, o);
+    if (lane == 0) counts[wave] = length;
+    __syncthreads();
+    length = 0;
+#pragma unroll
+    for (int w = 0; w < kW; ++w) length += counts[w];
+    share = 1.0 / (double)(length > 0 ? length : 1);
+  }
+  Part p{0.0, 0};
+  for (int64_t r = lo + threadIdx.x; r < hi; r += kT) {
+    const bool live = kept[r].live;
+    double l = 0.0, slope = 0.0;
+    if (live) {
+      const double A = (double)f.advantage[r / f.adv_div], x = lp[r];
+      const double ratio = exp(x - (double)f.old[r]);
+      const bool off = (A > 0.0 && ratio > f.high) || (A < 0.0 && ratio < f.low);
+      // (a ratio of NaN stays, as does an advantage of NaN)
+      l = off ? -(A > 0.0 ? f.high : f.low) * A : -ratio * A;
+      slope = off ? 0.0 : -ratio * A;
+      if (f.reference) {
+        const double d = (double)f.reference[r] - x, more = expm1(d);
+        l += f.kl * (more - d);
+        slope -= f.kl * more;
+      }
+      if (by_ent) l -= f.ent * ent[r];
+      ++p.n;
+    }
+    p.sum += l;
+    if (losses) losses[r] = (float)l;
+    by_lp[r] = (float)(slope * share);
+    if (by_ent) by_ent[r] = live ? (float)(-f.ent * share) : 0.f;
+  }
+  if (!loss) return;
+  p = wave_part(p);
+  if (lane == 0) red[wave] = p;
+  __syncthreads();
+  if (threadIdx.x) return;
+#pragma unroll
+  for (int w = 1; w < kW; ++w) {
+    p.sum += red[w].sum;
+    p.n += red[w].n;
+  }
+  if (f.by_sequence) {
+    p.sum *= share;
+    p.n = p.n > 0;
+  }
+  if (gridDim.x == 1)
+    write_loss(p, mean, loss, divisor);
+  else
+    part[blockIdx.x] = p;
+}
+
+// ---- backward ---------------------------------------------------------------------------------------------------------
+// a row's gradients in lp and H
+struct Upstream {
+  const float* by_lp;                      // [r / lp_div * lp_stride]
+  const float* by_ent;                     // [r * ent_stride]; null: none
+  int64_t lp_div, lp_stride, ent_stride;
+  const float* g;                          // a factor of both: [(r / g_div) % g_mod * g_stride]; null: 1
+  int64_t g_div, g_mod, g_stride;
+  const float* divisor;                    // of that factor
+};
+
+// Rows in descending order: the forward pass read the last rows last, and what the caches still hold of them is read first.
+template <typename T, bool ENT, int N>
+__global__ __launch_bounds__(kT) void backward_kernel(Rows a, int parts, const Kept* kept, Upstream up, T* dz, int past) {
+  typedef uint32_t words __attribute__((ext_vector_type(4)));
+  constexpr int E = kE<T>, U = 4;
+  const int tid = threadIdx.x % N;
+  const int at = N == kT ? (int)blockIdx.x / parts : (int)blockIdx.x * (kT / N) + (int)(threadIdx.x >> 6);
+  const int which = N == kT ? (int)blockIdx.x % parts : 0;
+  if (at >= a.rows) return;
+  const int r = a.rows - 1 - at;
+  T* out = dz + (int64_t)r * a.V;
+  const Cut c = cut_row(out, a.V, which, parts);               // (by the output's 16-byte boundaries)
+  uint4* to = reinterpret_cast<uint4*>(out + c.head);
+  auto store = [&](int p, const uint4& o) {
+    if (past)
+      __builtin_nontemporal_store(words{o.x, o.y, o.z, o.w}, reinterpret_cast<words*>(to + p));
+    else
+      to[p] = o;
+  };
+  const Kept k = kept[r];
+  float ga = 0.f, ge = 0.f;
+  if (k.live) {                            // uniform
+    const float g = up.g ? up.g[(r / up.g_div) % up.g_mod * up.g_stride] / (up.divisor ? *up.divisor : 1.f) : 1.f;
+    ga = g * up.by_lp[r / up.lp_div * up.lp_stride];
+    if (ENT) ge = g * up.by_ent[r * up.ent_stride];
+  }
+  // no gradient, whatever the row holds; or none in a row whose probabilities are numbers
+  if (!k.live || (ga == 0.f && ge == 0.f && k.inv <= 3.4028234e38f)) {
+    for (int p = c.p0 + tid; p < c.p1; p += N) store(p, make_uint4(0u, 0u, 0u, 0u));
+    if (tid < c.singles) Elem<T>::store(out + c.single(tid, a.V), 0.f);
+    return;
+  }
+  const T* z = row_of<T>(a, r);
+  const int64_t y = whole(a.tokens, a.wide, r);
+  const float ref = finite_ref(k.m), inv_tau = (float)a.inv_tau;
+  const float gy = ga * inv_tau;
+  // dz of a logit that is not the token's: E (f0 + f1 times its exponent in base 2)
+  const float f0 = -(ga - ge * k.lean) * k.inv * inv_tau, f1 = -ge * (float)kLn2 * k.inv * inv_tau;
+  auto value = [&](float x) {
+    const Exponent h = exponent_of<kFull<T>>(x - ref, a.c);
+    const float e = exp_of<kFull<T>>(h);
+    return ENT ? e * __builtin_fmaf(f1, fmaxf(h.h, kFar), f0) : e * f0;
+  };
+  const int yp = y >= c.head && y < a.V ? (int)(y - c.head) / E : -1, yj = (int)(y - c.head) % E;
+  const T* from = z + c.head;
+  auto put = [&](int p, const uint4& q) {
+    float x[E];
+    unpack<T>(q, x);
+#pragma unroll
+    for (int j = 0; j < E; ++j) x[j] = value(x[j]);
+    if (p == yp) {
+#pragma unroll
+      for (int j = 0; j < E; ++j) x[j] += j == yj ? gy : 0.f;
+    }
+    store(p, pack<T>(x));
+  };
+  int p = c.p0 + tid;
+  for (; p + (U - 1) * N < c.p1; p += U * N) {
+    uint4 q[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) q[u] = load16(from + (int64_t)(p + u * N) * E);
+#pragma unroll
+    for (int u = 0; u < U; ++u) put(p + u * N, q[u]);
+  }
+  for (; p < c.p1; p += N) put(p, load16(from + (int64_t)p * E));
+  if (tid < c.singles) {
+    const int i = c.single(tid, a.V);
+    Elem<T>::store(out + i, value(Elem<T>::load(z + i)) + (i == y ? gy : 0.f));
+  }
+}
+
+// ---- sizes ------------------------------------------------------------------------------------------------------------
+// workgroups a row: enough for 1024 in all, each with at least two pieces a thread
+int parts_of(int64_t rows, int V, int dtype) {
+  const int64_t pieces = ((int64_t)V * (dtype == DH_BF16 ? 2 : 4) + 15) / 16;
+  int64_t p = 1024 / (rows > 0 ? rows : 1);
+  const int64_t most = pieces / (2 * kT);
+  if (p > most) p = most;
+  if (p > kMaxParts) p = kMaxParts;
+  return p < 1 ? 1 : (int)p;
+}
+// a wave a row: short rows, as many as fill the card so
+bool by_waves(int64_t rows, int V, int dtype) { return (int64_t)V * (dtype == DH_BF16 ? 2 : 4) <= 8192 && rows >= 1024; }
+
+int check(const char* who, int dtype, const Rows& a, int token_bits, double tau) {
+  DH_REQUIRE(dtype == DH_F32 || dtype == DH_BF16, DH_ERR_UNSUPPORTED_DTYPE, "%s: dtype %d", who, dtype);
+  DH_REQUIRE(token_bits == 32 || token_bits == 64, DH_ERR_UNSUPPORTED_DTYPE, "%s: tokens of %d bits", who, token_bits);
+  DH_REQUIRE(a.rows >= 0 && a.rows < (1 << 22) && a.T >= 1 && a.V >= 1 && a.V <= (1 << 24), DH_ERR_UNSUPPORTED_SHAPE,
+             "%s: %d rows (-1: too many), T=%d V=%d", who, a.rows, a.T, a.V);
+  DH_REQUIRE(tau >= 0x1p-126 && tau <= 0x1p126, DH_ERR_INVALID_ARG, "%s: temperature %g", who, tau);
+  DH_REQUIRE(a.rows == 0 || (a.logits && a.tokens), DH_ERR_INVALID_ARG, "%s: null pointer argument", who);
+  DH_REQUIRE((uintptr_t)a.logits % (dtype == DH_BF16 ? 2 : 4) == 0 && (uintptr_t)a.tokens % (token_bits / 8) == 0,
+             DH_ERR_INVALID_ARG, "%s: operands not aligned to their elements", who);
+  return 0;
+}
+
+Rows rows_of(const void* logits, int64_t sb, int64_t st, int64_t B, int T, int V, const void* tokens, int token_bits,
+             int64_t ignore, double tau) {
+  Rows a;
+  a.logits = logits;
+  a.sb = sb;
+  a.st = st;
+  a.rows = B < 0 || T < 0 || (T > 0 && B >= ((int64_t)1 << 22) / T + 1) ? -1 : (int)(B * T);       // -1: too many
+  a.T = T;
+  a.V = V;
+  a.tokens = tokens;
+  a.wide = token_bits == 64;
+  a.ignore = ignore;
+  a.inv_tau = 1.0 / tau;
+  const double c = kLog2e / tau;
+  a.c = Scale{(float)c, (float)(c - (double)(float)c)};
+  return a;
+}
+
+template <typename T, bool ENT>
+int forward(const char* who, int dtype, const Rows& a, const Results& o, void* ws, hipStream_t s) {
+  if (by_waves(a.rows, a.V, dtype)) {
+    forward_kernel<T, ENT, 64><<<dim3((unsigned)((a.rows + kW - 1) / kW)), dim3(kT), 0, s>>>(a, 1, nullptr, o);
+    return dh_check_launch(who);
+  }
+  const int parts = parts_of(a.rows, a.V, dtype);
+  forward_kernel<T, ENT, kT><<<dim3((unsigned)a.rows * parts), dim3(kT), 0, s>>>(a, parts, (Sums*)ws, o);
+  if (int st = dh_check_launch(who)) return st;
+  if (parts == 1) return 0;
+  join_kernel<T, ENT><<<dim3((unsigned)((a.rows + kW - 1) / kW)), dim3(kT), 0, s>>>(a, parts, (const Sums*)ws, o);
+  return dh_check_launch(who);
+}
+int forward(const char* who, int dtype, const Rows& a, bool ent, const Results& o, void* ws, hipStream_t s) {
+  if (a.rows == 0) return 0;
+  if (dtype == DH_BF16) return ent ? forward<bf16_t, true>(who, dtype, a, o, ws, s) : forward<bf16_t, false>(who, dtype, a, o, ws, s);
+  return ent ? forward<float, true>(who, dtype, a, o, ws, s) : forward<float, false>(who, dtype, a, o, ws, s);
+}
+
+template <typename T, bool ENT>
+int backward(const char* who, int dtype, const Rows& a, const Kept* kept, const Upstream& up, void* dz, hipStream_t s) {
+  const int past = (int64_t)a.rows * a.V * (int)sizeof(T) >= kPast;
+  if (by_waves(a.rows, a.V, dtype)) {
+    backward_kernel<T, ENT, 64><<<dim3((unsigned)((a.rows + kW - 1) / kW)), dim3(kT), 0, s>>>(a, 1, kept, up, (T*)dz, past);
+    return dh_check_launch(who);
+  }
+  const int parts = parts_of(a.rows, a.V, dtype);
+  backward_kernel<T, ENT, kT><<<dim3((unsigned)a.rows * parts), dim3(kT), 0, s>>>(a, parts, kept, up, (T*)dz, past);
+  return dh_check_launch(who);
+}
+
+// the workspace of a call: the sums of split rows, lp (and H) in fp64, a loss's parts
+struct Layout {
+  int64_t lp64, ent64, part, bytes;
+};
+constexpr int64_t kUnit = 256;             // rows a workgroup of the policy loss where sequences do not matter
+Layout layout_of(int op, int64_t rows, int64_t units, int V, int dtype, bool ent) {
+  Layout l;
+  const int parts = parts_of(rows, V, dtype);
+  l.lp64 = parts > 1 ? (rows * parts * (int64_t)sizeof(Sums) + 7) / 8 * 8 : 0;
+  l.ent64 = l.lp64 + (op ? rows * 8 : 0);
+  l.part = l.ent64 + (op && ent ? rows * 8 : 0);
+  l.bytes = l.part + (op ? units * (int64_t)sizeof(Part) : 0);
+  return l;
+}
+bool fits(int64_t rows, int V) { return rows >= 0 && rows < (1 << 22) && V >= 1 && V <= (1 << 24); }
+
+}  // namespace
+
+extern "C" int64_t dh_logprob_workspace_bytes(int dtype, int64_t rows, int V) {
+  return fits(rows, V) ? layout_of(0, rows, 0, V, dtype, false).bytes : -1;
+}
+
+extern "C" int dh_logprob_fwd(int dtype, const void* logits, int64_t stride_b, int64_t stride_t, int64_t B, int T, int V,
+                              const void* tokens, int token_bits, int64_t ignore_index, double temperature, float* logprob,
+                              float* entropy, void* row_kept, void* workspace, int64_t workspace_bytes, void* stream) {
+  const char* who = "dh_logprob_fwd";
+  const Rows a = rows_of(logits, stride_b, stride_t, B, T, V, tokens, token_bits, ignore_index, temperature);
+  if (int st = check(who, dtype, a, token_bits, temperature)) return st;
+  DH_REQUIRE(a.rows == 0 || logprob, DH_ERR_INVALID_ARG, "%s: null pointer argument", who);
+  DH_REQUIRE((uintptr_t)logprob % 4 == 0 && (uintptr_t)entropy % 4 == 0 && (uintptr_t)row_kept % 16 == 0, DH_ERR_INVALID_ARG,
+             "%s: results not aligned to their elements", who);
+  const int64_t need = dh_logprob_workspace_bytes(dtype, a.rows, V);
+  DH_REQUIRE(workspace_bytes >= need && (need == 0 || (workspace && (uintptr_t)workspace % 8 == 0)), DH_ERR_INVALID_ARG,
+             "%s: workspace of %lld bytes, %lld needed", who, (long long)workspace_bytes, (long long)need);
+  return forward(who, dtype, a, entropy != nullptr, Results{logprob, entropy, nullptr, nullptr, (Kept*)row_kept}, workspace,
+                 (hipStream_t)stream);
+}
+
+extern "C" int dh_logprob_bwd(int dtype, const void* logits, int64_t stride_b, int64_t stride_t, int64_t B, int T, int V,
+                              const void* tokens, int token_bits, int64_t ignore_index, double temperature, const void* row_kept,
+                              const float* by_logprob, int64_t logprob_div, int64_t logprob_stride, const float* by_entropy,
+                              int64_t entropy_stride, const float* dloss, int64_t dloss_div, int64_t dloss_mod,
+                              int64_t dloss_stride, const float* divisor, void* dlogits, void* stream) {
+  const char* who = "dh_logprob_bwd";
+  const Rows a = rows_of(logits, stride_b, stride_t, B, T, V, tokens, token_bits, ignore_index, temperature);
+  if (int st = check(who, dtype, a, token_bits, temperature)) return st;
+  if (a.rows == 0) return 0;
+  DH_REQUIRE(row_kept && (uintptr_t)row_kept % 16 == 0 && by_logprob && dlogits, DH_ERR_INVALID_ARG,
+             "%s: null or unaligned pointer argument", who);
+  DH_REQUIRE(logprob_div >= 1 && logprob_stride >= 0 && entropy_stride >= 0 &&
+                 (!dloss || (dloss_div >= 1 && dloss_mod >= 1 && dloss_stride >= 0)),
+             DH_ERR_INVALID_ARG, "%s: strides and divisors of the gradients", who);
+  DH_REQUIRE((uintptr_t)by_logprob % 4 == 0 && (uintptr_t)by_entropy % 4 == 0 && (uintptr_t)dloss % 4 == 0 &&
+                 (uintptr_t)divisor % 4 == 0 && (uintptr_t)dlogits % (dtype == DH_BF16 ? 2 : 4) == 0,
+             DH_ERR_INVALID_ARG, "%s: operands not aligned to their elements", who);
+  const Upstream up{by_logprob, by_entropy, logprob_div, logprob_stride, entropy_stride, dloss, dloss_div, dloss_mod,
+                    dloss_stride, divisor};
+  const Kept* kept = (const Kept*)row_kept;
+  hipStream_t s = (hipStream_t)stream;
+  if (dtype == DH_BF16)
+    return by_entropy ? backward<bf16_t, true>(who, dtype, a, kept, up, dlogits, s)
+                      : backward<bf16_t, false>(who, dtype, a, kept, up, dlogits, s);
+  return by_entropy ? backward<float, true>(who, dtype, a, kept, up, dlogits, s)
+                    : backward<float, false>(who, dtype, a, kept, up, dlogits, s);
+}
+
+extern "C" int64_t dh_preference_workspace_bytes(int dtype, int64_t pairs, int T, int V) {
+  if (pairs < 0 || pairs >= (1 << 21) || T < 0 || (T > 0 && pairs > (1 << 21) / T) || !fits(2 * pairs * T, V)) return -1;
+  return layout_of(1, 2 * pairs * T, pairs, V, dtype, false).bytes;
+}
+
+extern "C" int dh_preference_fwd(int dtype, const void* logits, int64_t stride_b, int64_t stride_t, int64_t pairs, int T, int V,
+                                 const void* tokens, int token_bits, int64_t ignore_index, const void* reference,
+                                 int reference_bits, int kind, int average, double beta, double margin, double label_smoothing,
+                                 int reduction, float* pair_loss, float* sums, float* coef, void* row_kept, float* loss,
+                                 float* divisor, void* workspace, int64_t workspace_bytes, void* stream) {
+  const char* who = "dh_preference_fwd";
+  DH_REQUIRE(pairs >= 0 && T >= 0, DH_ERR_UNSUPPORTED_SHAPE, "%s: %lld pairs of %d", who, (long long)pairs, T);
+  const int64_t need = dh_preference_workspace_bytes(dtype, pairs, T, V);
+  DH_REQUIRE(need >= 0, DH_ERR_UNSUPPORTED_SHAPE, "%s: %lld pairs of %d rows, V=%d", who, (long long)pairs, T, V);
+  const Rows a = rows_of(logits, stride_b, stride_t, T ? 2 * pairs : 0, T ? T : 1, V, tokens, token_bits, ignore_index, 1.0);
+  if (int st = check(who, dtype, a, token_bits, 1.0)) return st;
+  DH_REQUIRE(kind >= 0 && kind <= 2 && reduction >= 0 && reduction <= 2, DH_ERR_INVALID_ARG, "%s: kind %d, reduction %d", who, kind,
+             reduction);
+  DH_REQUIRE(beta > 0.0 && beta < INFINITY && margin > -INFINITY && margin < INFINITY && label_smoothing >= 0.0 &&
+                 label_smoothing <= 0.5, DH_ERR_INVALID_ARG, "%s: beta %g, margin %g, label smoothing %g", who, beta, margin, label_smoothing);
+  DH_REQUIRE(!reference || reference_bits == 32 || reference_bits == 64, DH_ERR_UNSUPPORTED_DTYPE, "%s: reference of %d bits",
+             who, reference_bits);
+  DH_REQUIRE(pairs == 0 || (sums && coef), DH_ERR_INVALID_ARG, "%s: null pointer argument", who);
+  DH_REQUIRE((a.rows == 0 || row_kept) && (uintptr_t)row_kept % 16 == 0, DH_ERR_INVALID_ARG, "%s: null or unaligned pointer argument", who);
+  DH_REQUIRE(reduction ? loss && divisor : pairs == 0 || pair_loss, DH_ERR_INVALID_ARG, "%s: null pointer argument", who);
+  DH_REQUIRE((uintptr_t)pair_loss % 4 == 0 && (uintptr_t)sums % 4 == 0 && (uintptr_t)coef % 4 == 0 && (uintptr_t)loss % 4 == 0 &&
+                 (uintptr_t)divisor % 4 == 0 && (!reference || (uintptr_t)reference % (reference_bits / 8) == 0),
+             DH_ERR_INVALID_ARG, "%s: operands not aligned to their elements", who);
+  DH_REQUIRE(workspace_bytes >= need && (need == 0 || (workspace && (uintptr_t)workspace % 8 == 0)), DH_ERR_INVALID_ARG,
+             "%s: workspace of %lld bytes, %lld needed", who, (long long)workspace_bytes, (long long)need);
+  hipStream_t s = (hipStream_t)stream;
+  const Layout l = layout_of(1, a.rows, pairs, V, dtype, false);
+  char* ws = (char*)workspace;
+  double* lp = (double*)(ws + l.lp64);
+  Part* part = (Part*)(ws + l.part);
+  Kept* kept = (Kept*)row_kept;
+  if (int st = forward(who, dtype, a, false, Results{nullptr, nullptr, lp, nullptr, kept}, ws, s)) return st;
+  if (pairs) {
+    const Preference f{(int)pairs, T, kind, average, beta, margin, label_smoothing, reference, reference_bits == 64};
+    preference_kernel<<<dim3((unsigned)pairs), dim3(kT), 0, s>>>(f, lp, kept, reduction ? nullptr : pair_loss, sums, coef, part,
+                                                                 reduction == 1, reduction ? loss : nullptr, divisor);
+    if (int st = dh_check_launch(who)) return st;
+  }
+  if (!reduction || pairs == 1) return 0;
+  reduce_kernel<<<dim3(1), dim3(pairs > 64 ? 1024 : 64), 0, s>>>(part, pairs, reduction == 1, loss, divisor);
+  return dh_check_launch(who);
+}
+
+extern "C" int64_t dh_policy_workspace_bytes(int dtype, int64_t B, int T, int V, int entropy) {
+  if (B < 0 || T < 0 || (T > 0 && B > ((int64_t)1 << 22) / T) || !fits(B * T, V)) return -1;
+  const int64_t rows = B * T, units = (rows + kUnit - 1) / kUnit;
+  return layout_of(1, rows, T && B > units ? B : units, V, dtype, entropy != 0).bytes;
+}
+
+extern "C" int dh_policy_fwd(int dtype, const void* logits, int64_t stride_b, int64_t stride_t, int64_t B, int T, int V,
+                             const void* tokens, int token_bits, int64_t ignore_index, double temperature,
+                             const float* old_logprob, const float* advantage, int per_sequence,
+                             const float* reference_logprob, double clip, double clip_high, double kl_weight,
+                             double entropy_weight, int reduction, float* row_loss, float* logprob, float* by_logprob,
+                             float* by_entropy, void* row_kept, float* loss, float* divisor, void* workspace,
+                             int64_t workspace_bytes, void* stream) {
+  const char* who = "dh_policy_fwd";
+  DH_REQUIRE(B >= 0 && T >= 0, DH_ERR_UNSUPPORTED_SHAPE, "%s: B=%lld T=%d", who, (long long)B, T);
+  const int64_t need = dh_policy_workspace_bytes(dtype, B, T, V, by_entropy != nullptr);
+  DH_REQUIRE(need >= 0, DH_ERR_UNSUPPORTED_SHAPE, "%s: B=%lld T=%d V=%d", who, (long long)B, T, V);
+  const Rows a = rows_of(logits, stride_b, stride_t, T ? B : 0, T ? T : 1, V, tokens, token_bits, ignore_index, temperature);
+  if (int st = check(who, dtype, a, token_bits, temperature)) return st;
+  DH_REQUIRE(reduction >= 0 && reduction <= 3, DH_ERR_INVALID_ARG, "%s: reduction %d", who, reduction);
+  DH_REQUIRE(clip >= 0.0 && clip <= 1.0 && clip_high >= 0.0 && clip_high < INFINITY && kl_weight >= 0.0 && kl_weight < INFINITY &&
+                 entropy_weight > -INFINITY && entropy_weight < INFINITY,
+             DH_ERR_INVALID_ARG, "%s: clip %g and %g, weights %g and %g", who, clip, clip_high, kl_weight, entropy_weight);
+  DH_REQUIRE(by_entropy || entropy_weight == 0.0, DH_ERR_INVALID_ARG, "%s: an entropy weight of %g, and no by_entropy", who, entropy_weight);
+  DH_REQUIRE(reference_logprob || kl_weight == 0.0, DH_ERR_INVALID_ARG, "%s: a KL weight of %g without a reference", who, kl_weight);
+  DH_REQUIRE(a.rows == 0 || (old_logprob && advantage && logprob && by_logprob && row_kept), DH_ERR_INVALID_ARG,
+             "%s: null pointer argument", who);
+  DH_REQUIRE(reduction ? loss && divisor : a.rows == 0 || row_loss, DH_ERR_INVALID_ARG, "%s: null pointer argument", who);
+  DH_REQUIRE((uintptr_t)old_logprob % 4 == 0 && (uintptr_t)advantage % 4 == 0 && (uintptr_t)reference_logprob % 4 == 0 &&
+                 (uintptr_t)row_loss % 4 == 0 && (uintptr_t)logprob % 4 == 0 && (uintptr_t)by_logprob % 4 == 0 &&
+                 (uintptr_t)by_entropy % 4 == 0 && (uintptr_t)row_kept % 16 == 0 && (uintptr_t)loss % 4 == 0 &&
+                 (uintptr_t)divisor % 4 == 0,
+             DH_ERR_INVALID_ARG, "%s: operands not aligned to their elements", who);
+  DH_REQUIRE(workspace_bytes >= need && (need == 0 || (workspace && (uintptr_t)workspace % 8 == 0)), DH_ERR_INVALID_ARG,
+             "%s: workspace of %lld bytes, %lld needed", who, (long long)workspace_bytes, (long long)need);
+  hipStream_t s = (hipStream_t)stream;
+  const bool ent = by_entropy != nullptr, by_sequence = reduction == 3, mean = reduction == 1 || by_sequence;
+  const int64_t units = by_sequence ? (T ? B : 0) : (a.rows + kUnit - 1) / kUnit;
+  const Layout l = layout_of(1, a.rows, units, V, dtype, ent);
+  char* ws = (char*)workspace;
+  double *lp = (double*)(ws + l.lp64), *h = ent ? (double*)(ws + l.ent64) : nullptr;
+  Part* part = (Part*)(ws + l.part);
+  Kept* kept = (Kept*)row_kept;
+  if (int st = forward(who, dtype, a, ent, Results{logprob, nullptr, lp, h, kept}, ws, s)) return st;
+  if (units) {
+    const Policy f{a.rows, T, by_sequence ? T : (int)kUnit, by_sequence, old_logprob, advantage,
+                   kl_weight > 0.0 ? reference_logprob : nullptr, per_sequence ? T : 1, 1.0 - clip, 1.0 + clip_high, kl_weight,
+                   entropy_weight};
+    policy_kernel<<<dim3((unsigned)units), dim3(kT), 0, s>>>(f, lp, h, kept, reduction ? nullptr : row_loss, by_logprob, by_entropy,
+                                                             part, mean, reduction ? loss : nullptr, divisor);
+    if (int st = dh_check_launch(who)) return st;
+  }
+  if (!reduction || units == 1) return 0;
+  reduce_kernel<<<dim3(1), dim3(units > 64 ? 1024 : 64), 0, s>>>(part, units, mean, loss, divisor);
+  return dh_check_launch(who);
+}

@@ -21,7 +21,7 @@ REPO_DIR = os.path.dirname(PROJECT_DIR)
 INCLUDE_DIRS = [os.path.join(REPO_DIR, "include"), CSRC_DIR]
 OUT_DIR = os.path.join(PKG_DIR, "_lib")
 LIB = os.path.join(OUT_DIR, "libdh_mixer.so")
-NODES_SRC = os.path.join(CSRC_DIR, "host", "vocab_nodes.cpp")
+NODES_SRCS = sorted(glob.glob(os.path.join(CSRC_DIR, "host", "*.cpp")))
 NODES_LIB = os.path.join(OUT_DIR, "_vocab_nodes.so")
 
 ARCH = os.environ.get("DH_OFFLOAD_ARCH", "gfx950")
@@ -50,7 +50,7 @@ def nodes_command(out):
              "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", f'-DDH_TORCH_VERSION="{torch.__version__}"',
              f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
             + [a for d in system for a in ("-isystem", d)] + [f"-I{d}" for d in INCLUDE_DIRS]
-            + [NODES_SRC, "-o", out, f"-L{os.path.join(root, 'lib')}"]
+            + [*NODES_SRCS, "-o", out, f"-L{os.path.join(root, 'lib')}"]
             + [f"-l{n}" for n in ("c10", "c10_hip", "torch_cpu", "torch_hip", "torch", "torch_python")])
 
 

@@ -15,7 +15,7 @@ import os
 
 import torch
 
-ABI_VERSION = 21
+ABI_VERSION = 22
 _LIB_NAME = "libdh_mixer.so"
 
 DH_F32, DH_BF16 = 0, 1
@@ -47,7 +47,7 @@ def _load():
         lib = ctypes.CDLL(path)
     except OSError as e:  # pragma: no cover - depends on the host
         raise ImportError(f"cannot load {path}: {e}") from e
-    vp, i32, i64 = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64
+    vp, i32, i64, f64 = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_double
     sigs = {
         "dh_abi_version": ([], i32),
         "dh_last_error": ([], ctypes.c_char_p),
@@ -117,6 +117,16 @@ def _load():
                             ctypes.c_float, i32, vp, vp, vp, vp, vp, i64, vp], i32),
         "dh_distill_bwd": ([i32, vp, i64, i64, i64, i32, i32, i32, vp, vp, i32, i32, vp, i32, i64, ctypes.c_float,
                             ctypes.c_float, vp, vp, i64, vp, vp, vp], i32),
+        "dh_logprob_workspace_bytes": ([i32, i64, i32], i64),
+        "dh_logprob_fwd": ([i32, vp, i64, i64, i64, i32, i32, vp, i32, i64, f64, vp, vp, vp, vp, i64, vp], i32),
+        "dh_logprob_bwd": ([i32, vp, i64, i64, i64, i32, i32, vp, i32, i64, f64, vp, vp, i64, i64, vp, i64, vp, i64, i64, i64,
+                            vp, vp, vp], i32),
+        "dh_preference_workspace_bytes": ([i32, i64, i32, i32], i64),
+        "dh_preference_fwd": ([i32, vp, i64, i64, i64, i32, i32, vp, i32, i64, vp, i32, i32, i32, f64, f64, f64, i32]
+                              + [vp] * 7 + [i64, vp], i32),
+        "dh_policy_workspace_bytes": ([i32, i64, i32, i32, i32], i64),
+        "dh_policy_fwd": ([i32, vp, i64, i64, i64, i32, i32, vp, i32, i64, f64, vp, vp, i32, vp, f64, f64, f64, f64, i32]
+                          + [vp] * 8 + [i64, vp], i32),
         "dh_add_rmsnorm": ([i32, vp, vp, vp, ctypes.c_float, vp, vp, i64, i32, vp], i32),
     }
     for name, (argtypes, restype) in sigs.items():

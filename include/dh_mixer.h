@@ -29,7 +29,7 @@
 extern "C" {
 #endif
 
-#define DH_ABI_VERSION 21
+#define DH_ABI_VERSION 22
 
 enum dh_status {
   DH_OK = 0,
@@ -628,6 +628,75 @@ int dh_distill_bwd(int dtype, const void* logits, int64_t stride_b, int64_t stri
                    const void* labels, int label_bits, int64_t ignore_index, float temperature, float weight,
                    const void* row_kept, const float* dloss, int64_t dloss_stride, const float* divisor, void* dlogits,
                    void* stream);
+
+/*
+ * Log-probabilities of given tokens; no counterpart in the reference. Row r = b * T + t of the logits z (V of unit stride at
+ * b * stride_b + t * stride_t), its token y, temperature tau, p = softmax(z / tau):
+ *   logprob[r] = log p_y,   entropy[r] = - sum_v p_v log p_v (null: not wanted)
+ * A row whose token is ignore_index is not read: zeros; a token outside [0, V) otherwise makes its row NaN, the whole row of its
+ * gradient too. Sums over V are fp32, a row's few other operations fp64.
+ *   tokens (B * T) of token_bits (32 or 64) bits, contiguous; logprob, entropy (B * T) fp32; row_kept: 16 bytes a row, 16-byte
+ *   aligned, for the backward pass (null: none).
+ *   workspace: dh_logprob_workspace_bytes(dtype, B * T, V) bytes (0 for many rows), 8-byte aligned, needed during the call only.
+ *   V <= 2^24, B * T < 2^22, 2^-126 <= tau <= 2^126.
+ */
+int64_t dh_logprob_workspace_bytes(int dtype, int64_t rows, int V);
+int dh_logprob_fwd(int dtype, const void* logits, int64_t stride_b, int64_t stride_t, int64_t B, int T, int V,
+                   const void* tokens, int token_bits, int64_t ignore_index, double temperature, float* logprob,
+                   float* entropy, void* row_kept, void* workspace, int64_t workspace_bytes, void* stream);
+/*
+ * Gradient in z from those in the rows' log-probabilities and entropies, of this call and of the two losses below:
+ * dlogits (B * T, V) contiguous, every element written,
+ *   dz_v = (a ([v = y] - p_v) - e p_v (log p_v + H)) / tau,   zeros where the row is ignored,
+ *   a = g by_logprob[r / logprob_div * logprob_stride],  e = g by_entropy[r * entropy_stride] (null: 0),
+ *   g = dloss[(r / dloss_div) % dloss_mod * dloss_stride] / *divisor (dloss null: 1; divisor null: 1).
+ * All of them fp32 on the device. A row with a = e = 0 is not read (zeros, unless its probabilities are NaN). The other arguments
+ * are the forward call's, where entropies are asked for if by_entropy is given; row_kept as it wrote it.
+ */
+int dh_logprob_bwd(int dtype, const void* logits, int64_t stride_b, int64_t stride_t, int64_t B, int T, int V,
+                   const void* tokens, int token_bits, int64_t ignore_index, double temperature, const void* row_kept,
+                   const float* by_logprob, int64_t logprob_div, int64_t logprob_stride, const float* by_entropy,
+                   int64_t entropy_stride, const float* dloss, int64_t dloss_div, int64_t dloss_mod, int64_t dloss_stride,
+                   const float* divisor, void* dlogits, void* stream);
+/*
+ * Preference loss on pairs of sequences; no counterpart in the reference. Logits of 2 pairs sequences of T rows, as above at
+ * temperature 1: sequence i is preferred to sequence pairs + i. S = the sum of a sequence's log-probabilities (average: over
+ * their number; a sequence without any has 0), R the reference's (null: 0), D = (S - R)_i - (S - R)_{pairs + i},
+ * x = beta D - margin:
+ *   kind 0: - (1 - s) log sigma(x) - s log sigma(-x), s = label_smoothing;  1: max(0, 1 - x);  2: (D - 1 / (2 beta))^2
+ *   reduction 0: pair_loss (pairs) alone; 1: loss = their mean (NaN of none), divisor = pairs; 2: loss = their sum, divisor = 1.
+ *   reference (2 pairs) fp32 or fp64 (reference_bits); sums (2 pairs): S; coef (2 pairs): the derivative of a pair's loss in a
+ *   log-probability of the sequence, the by_logprob of dh_logprob_bwd (logprob_div T, stride 1; dloss_div T and dloss_mod pairs
+ *   for reduction 0). All fp32 but the reference. S and all that follows are fp64 inside.
+ *   workspace: dh_preference_workspace_bytes(dtype, pairs, T, V) bytes, 8-byte aligned.
+ *   0 < beta < inf, finite margin, 0 <= label_smoothing <= 1/2; 2 pairs T < 2^22, fewer than 2^21 pairs.
+ */
+int64_t dh_preference_workspace_bytes(int dtype, int64_t pairs, int T, int V);
+int dh_preference_fwd(int dtype, const void* logits, int64_t stride_b, int64_t stride_t, int64_t pairs, int T, int V,
+                      const void* tokens, int token_bits, int64_t ignore_index, const void* reference, int reference_bits,
+                      int kind, int average, double beta, double margin, double label_smoothing, int reduction,
+                      float* pair_loss, float* sums, float* coef, void* row_kept, float* loss, float* divisor,
+                      void* workspace, int64_t workspace_bytes, void* stream);
+/*
+ * Clipped policy loss with a KL term and an entropy bonus; no counterpart in the reference. Rows as above, x = log p_y of a row,
+ * ratio = exp(x - old_logprob[r]), A = advantage[r] (per_sequence: advantage[b]), d = reference_logprob[r] - x:
+ *   row_loss[r] = - min(ratio A, clip(ratio, 1 - clip, 1 + clip_high) A) + kl_weight (exp(d) - d - 1) - entropy_weight H
+ * 0 where the row is ignored (its old log-probability, advantage and reference are not looked at). No KL term where kl_weight is
+ * 0 (reference_logprob may be null then) and no entropies without by_entropy (entropy_weight must be 0 then).
+ *   reduction 0: rows only; 1: loss = the mean over the rows that are not ignored (NaN of none), divisor = their number; 2: the
+ *   sum, divisor = 1; 3: the mean over the sequences that have such a row of each one's mean, divisor = their number.
+ *   logprob (B * T): x; by_logprob, by_entropy (B * T): the derivatives of the loss times the divisor, for dh_logprob_bwd.
+ *   old_logprob, reference_logprob (B * T), advantage (B * T or B), fp32. The ratio and what follows are fp64 inside.
+ *   workspace: dh_policy_workspace_bytes(dtype, B, T, V, by_entropy given) bytes, 8-byte aligned.
+ *   0 <= clip <= 1, 0 <= clip_high < inf, 0 <= kl_weight < inf, finite entropy_weight.
+ */
+int64_t dh_policy_workspace_bytes(int dtype, int64_t B, int T, int V, int entropy);
+int dh_policy_fwd(int dtype, const void* logits, int64_t stride_b, int64_t stride_t, int64_t B, int T, int V,
+                  const void* tokens, int token_bits, int64_t ignore_index, double temperature, const float* old_logprob,
+                  const float* advantage, int per_sequence, const float* reference_logprob, double clip, double clip_high,
+                  double kl_weight, double entropy_weight, int reduction, float* row_loss, float* logprob, float* by_logprob,
+                  float* by_entropy, void* row_kept, float* loss, float* divisor, void* workspace, int64_t workspace_bytes,
+                  void* stream);
 
 #ifdef __cplusplus
 }
