@@ -143,6 +143,36 @@ struct TokenLogprobs : torch::autograd::Function<TokenLogprobs> {
   }
 };
 
+// the same from hidden states and the head's weight
+variable_list head_logprobs(const Tensor& hidden, const Tensor& weight, const Tensor& tokens_, double temperature,
+                            int64_t ignore_index, bool entropy, bool round_logits) {
+  const char* what = "head_logprobs";
+  same_gpu(what, hidden, {&weight, &tokens_});
+  const int code = dtype_code(hidden);
+  TORCH_CHECK_TYPE(weight.scalar_type() == hidden.scalar_type(), what, ": weight of another type");
+  const at::NoGradGuard no_grad;
+  const c10::DeviceGuard guard(hidden.device());
+  TORCH_CHECK_VALUE(weight.dim() == 2 && hidden.dim() >= 1 && weight.size(1) == hidden.size(-1), what, ": hidden states ",
+                    hidden.sizes(), " and weight ", weight.sizes());
+  const Tensor h = unit_rows(hidden.dim() == 2 ? hidden : hidden.dim() == 1 ? hidden.unsqueeze(0) : hidden.flatten(0, -2)),
+               w = unit_rows(weight), tokens = tokens_.contiguous();
+  const int64_t n = h.size(0);
+  const int token_bits = bits(what, tokens);
+  same_count(what, "tokens", tokens.numel(), n);
+  const auto f32 = hidden.options().dtype(at::kFloat).requires_grad(false);
+  const auto shape = hidden.sizes().slice(0, hidden.dim() - 1);
+  variable_list out{at::empty(shape, f32)};
+  if (entropy) out.push_back(at::empty(shape, f32));
+  const int V = narrow(w.size(0));
+  const int64_t bytes = lib.dh_head_logprob_workspace_bytes(code, n, V);
+  const Tensor ws = workspace(bytes, hidden);
+  check(lib.dh_head_logprob(code, h.data_ptr(), h.stride(0), n, narrow(h.size(1)), w.data_ptr(), w.stride(0), V, tokens.data_ptr(),
+                            token_bits, ignore_index, temperature, round_logits, floats(out[0]), entropy ? floats(out[1]) : nullptr,
+                            at_(ws), bytes, stream_of(hidden)),
+        what);
+  return out;
+}
+
 // ---- preference loss ----------------------------------------------------------------------------------------------------
 struct Preference {
   int64_t kind;                            // 0 sigmoid, 1 hinge, 2 squared
@@ -352,6 +382,10 @@ void bind_logprobs(py::module_& m) {
     return guarded([&] {
       return logprobs_grad(g_lp.value_or(Tensor()), g_ent.value_or(Tensor()), logits, tokens, kept, temperature, ignore_index);
     });
+  }, release());
+  m.def("head_logprobs", [](const Tensor& hidden, const Tensor& weight, const Tensor& tokens, double temperature,
+                            int64_t ignore_index, bool entropy, bool round_logits) {
+    return guarded([&] { return head_logprobs(hidden, weight, tokens, temperature, ignore_index, entropy, round_logits); });
   }, release());
   m.def("preference", [](const Tensor& logits, const Tensor& tokens, const Maybe& reference, int64_t kind, bool average, double beta,
                          double margin, double smoothing, int64_t ignore_index, int64_t reduction) {

@@ -24,7 +24,7 @@ using torch::autograd::variable_list;
   X(dh_embed_fwd) X(dh_embed_bwd) X(dh_embed_bwd_workspace_bytes) X(dh_top_logits) X(dh_distill_fwd) X(dh_distill_bwd)   \
       X(dh_distill_workspace_bytes) X(dh_logprob_fwd) X(dh_logprob_bwd) X(dh_logprob_workspace_bytes)                    \
           X(dh_preference_fwd) X(dh_preference_workspace_bytes) X(dh_policy_fwd) X(dh_policy_workspace_bytes)            \
-              X(dh_last_error)
+              X(dh_head_logprob) X(dh_head_logprob_workspace_bytes) X(dh_last_error)
 #define MEMBER(name) decltype(&::name) name = nullptr;
 struct Entries {
   ENTRIES(MEMBER)

@@ -127,6 +127,8 @@ def _load():
         "dh_policy_workspace_bytes": ([i32, i64, i32, i32, i32], i64),
         "dh_policy_fwd": ([i32, vp, i64, i64, i64, i32, i32, vp, i32, i64, f64, vp, vp, i32, vp, f64, f64, f64, f64, i32]
                           + [vp] * 8 + [i64, vp], i32),
+        "dh_head_logprob_workspace_bytes": ([i32, i64, i32], i64),
+        "dh_head_logprob": ([i32, vp, i64, i64, i32, vp, i64, i32, vp, i32, i64, f64, i32, vp, vp, vp, i64, vp], i32),
         "dh_add_rmsnorm": ([i32, vp, vp, vp, ctypes.c_float, vp, vp, i64, i32, vp], i32),
     }
     for name, (argtypes, restype) in sigs.items():

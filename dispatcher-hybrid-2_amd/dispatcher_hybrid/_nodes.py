@@ -17,7 +17,8 @@ from . import _hip
 _PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_lib", "_vocab_nodes.so")
 _ENTRIES = ("dh_embed_fwd", "dh_embed_bwd", "dh_embed_bwd_workspace_bytes", "dh_top_logits", "dh_distill_fwd", "dh_distill_bwd",
             "dh_distill_workspace_bytes", "dh_logprob_fwd", "dh_logprob_bwd", "dh_logprob_workspace_bytes", "dh_preference_fwd",
-            "dh_preference_workspace_bytes", "dh_policy_fwd", "dh_policy_workspace_bytes", "dh_last_error")
+            "dh_preference_workspace_bytes", "dh_policy_fwd", "dh_policy_workspace_bytes", "dh_head_logprob", "dh_head_logprob_workspace_bytes",
+            "dh_last_error")
 
 
 def load(differentiable):

@@ -131,6 +131,34 @@ def token_logprobs(logits, tokens, temperature=1.0, ignore_index=-100, entropy=F
     return (out[0], out[1]) if entropy else out[0]
 
 
+@torch.library.custom_op("dispatcher::head_logprobs", mutates_args=(), device_types="cuda")
+def _head_op(hidden: torch.Tensor, weight: torch.Tensor, tokens: torch.Tensor, temperature: float, ignore_index: int, entropy: bool,
+             round_logits: bool) -> List[torch.Tensor]:
+    return _native.head_logprobs(hidden, weight, tokens, temperature, ignore_index, entropy, round_logits)
+
+
+@_head_op.register_fake
+def _(hidden, weight, tokens, temperature, ignore_index, entropy, round_logits):
+    return [hidden.new_empty(hidden.shape[:-1], dtype=_f32) for _ in range(2 if entropy else 1)]
+
+
+def head_logprobs(hidden, weight, tokens, temperature=1.0, ignore_index=-100, entropy=False, round_logits=False):
+    """token_logprobs of the logits hidden . weight^T without those logits in memory; no gradient (raises where one is wanted of
+    `hidden` or `weight`).
+
+    hidden (..., d) and weight (V, d) of one type, fp32 or bf16; tokens (...) int32 or int64. The logits are fp32 sums; with
+    round_logits they are rounded to the operands' type first, as a head that stores them does. Positions whose token is
+    ignore_index cost nothing where there are many (zeros); another token outside the vocabulary gives NaN."""
+    plain.check_head(hidden, weight, tokens, temperature)
+    args = (hidden, weight, tokens, float(temperature), int(ignore_index), bool(entropy), bool(round_logits))
+    if type(hidden) in _PLAIN and type(weight) in _PLAIN and hidden.is_cuda and plain_eager():
+        out = _native.head_logprobs(*args)
+    else:
+        _hip.require_gpu(hidden, "head_logprobs")
+        out = torch.ops.dispatcher.head_logprobs(hidden.detach(), weight.detach(), *args[2:])
+    return (out[0], out[1]) if entropy else out[0]
+
+
 # ---- preference loss --------------------------------------------------------------------------------------------------
 @torch.library.custom_op("dispatcher::preference_loss", mutates_args=(), device_types="cuda")
 def _preference_op(logits: torch.Tensor, tokens: torch.Tensor, reference: Optional[torch.Tensor], kind: int, average: bool,

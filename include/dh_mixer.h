@@ -698,6 +698,20 @@ int dh_policy_fwd(int dtype, const void* logits, int64_t stride_b, int64_t strid
                   float* by_entropy, void* row_kept, float* loss, float* divisor, void* workspace, int64_t workspace_bytes,
                   void* stream);
 
+/*
+ * Log-probabilities (and entropies; null: not wanted) of given tokens from hidden states and the vocabulary head's weight, without
+ * the logits in memory: z = hidden . weight^T in fp32 sums (round_logits: rounded to bf16 then, as a bf16 head stores them), and
+ * the rest as in dh_logprob_fwd. Rows whose token is ignore_index are not computed, but where there are few rows.
+ *   hidden (rows, d) of row stride hidden_stride, weight (V, d) of row stride weight_stride, both of dtype and of unit stride inside
+ *   a row; any d, alignment and (not negative) strides, the fast kernels at d a multiple of 64 and 16-byte aligned rows of bf16.
+ *   workspace: dh_head_logprob_workspace_bytes(dtype, rows, V) bytes, 16-byte aligned, needed during the call only.
+ *   rows < 2^22, d <= 2^20, V <= 2^24, 2^-126 <= tau <= 2^126.
+ */
+int64_t dh_head_logprob_workspace_bytes(int dtype, int64_t rows, int V);
+int dh_head_logprob(int dtype, const void* hidden, int64_t hidden_stride, int64_t rows, int d, const void* weight,
+                    int64_t weight_stride, int V, const void* tokens, int token_bits, int64_t ignore_index, double temperature,
+                    int round_logits, float* logprob, float* entropy, void* workspace, int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -253,6 +253,141 @@ def test_gradient_against_differences():
             break
 
 
+# ---- from the hidden states ---------------------------------------------------------------------------------------------
+
+def head_inputs(lead, V, d, dtype, seed, ignored=0.3):
+    g = gen(seed)
+    tokens = torch.randint(0, V, lead, device=DEV, generator=g)
+    w = torch.randn(V, d, device=DEV, generator=g) * (2.0 / math.sqrt(d))
+    h = torch.randn(*lead, d, device=DEV, generator=g) + w[tokens]
+    if len(lead):
+        tokens = torch.where(torch.rand(lead, device=DEV, generator=g) < ignored, IGNORE, tokens)
+    return h.to(dtype), w.to(dtype), tokens
+
+
+def check_head(got, h, w, tokens, tau, round_logits=False, exact=False):
+    """Against the logits in 64 bits. A logit is a sum of d products: off by at most (d + 2) u of the sum of their magnitudes (and
+    where it is rounded, by half a step of bf16, or a whole one if that error crosses a rounding border)."""
+    V, d = w.shape
+    rows = h.reshape(-1, d)
+    lp, ent = got if isinstance(got, tuple) else (got, None)
+    for r in range(0, rows.shape[0], 256):
+        x = rows[r:r + 256].double()
+        z, size = x @ w.double().t(), x.abs() @ w.double().abs().t()
+        off = (d + 2) * U * size * (0 if exact else 1)
+        if round_logits:
+            z = z.to(torch.bfloat16).double()
+            off = off + 2.0 ** -7 * (z.abs() + off)
+        tok = tokens.reshape(-1)[r:r + 256]
+        ref = Rows(z, tok, tau)
+        ref.rel = U * (4 * ref.near.abs() + 3)                   # (fp32 logits, exponents rounded as bf16 ones' are)
+        ref.rel_s = (ref.p * ref.rel).sum(1) + 200 * U           # 128 columns a tile and lane, tiles, lanes, slots
+        mean_off = (ref.p * off).sum(1) / tau
+        if round_logits:                                         # few logits cross a border, here bounded by all of them
+            own = off.gather(1, ref.at).squeeze(1) / tau
+        else:
+            own = off.gather(1, ref.at).squeeze(1) / tau
+        # with every logit off by at most off: log of the sum by mean_off e^most, the mean exponent by off (1 + |d| + mean |d|)
+        most = (off / tau).max(1).values.exp()
+        err = (ref.rel_s + mean_off + own) * most + U * (ref.lp.abs() + 30) + 1e-12
+        bad = (lp.reshape(-1)[r:r + 256].double() - ref.lp).abs() - torch.where(ref.live, err, 0.0)
+        assert bool((bad <= 0).all()), bad.max()
+        if ent is not None:
+            spread = (ref.p * (off / tau) * (1 + ref.near.abs() + ref.lean.abs().unsqueeze(1))).sum(1) * 2 * most
+            err = ref.rel_s * (1 + ref.lean.abs()) + spread + (ref.p * ref.near.abs() * (ref.rel + 4 * U)).sum(1) \
+                + U * (ref.ent + 30) + 200 * U * ref.lean.abs()
+            bad = (ent.reshape(-1)[r:r + 256].double() - ref.ent).abs() - torch.where(ref.live, err, 0.0)
+            assert bool((bad <= 0).all()), bad.max()
+
+
+HEADS = [((), 7, 3), ((1,), 50257, 1024), ((16,), 50257, 1024), ((3, 7), 1003, 64), ((50,), 130, 200), ((64,), 5003, 320),
+         ((65,), 5003, 128), ((2, 100), 257, 1), ((300,), 4097, 72), ((700,), 777, 512), ((2, 400), 2049, 1024), ((1030,), 130, 2048),
+         ((4500,), 300, 64), ((130,), 50257, 256)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("lead,V,d", HEADS)
+def test_head_logprobs(lead, V, d, dtype):
+    for i, (tau, entropy, rounded) in enumerate([(1.0, False, False), (0.7, True, False), (2.0, True, True)]):
+        say("head", lead, V, d, dtype, tau)
+        h, w, tokens = head_inputs(lead, V, d, dtype, 60 + i)
+        if i == 1:
+            tokens = tokens.int()
+        got = ops().head_logprobs(h, w, tokens, temperature=tau, entropy=entropy, round_logits=rounded)
+        check_head(got, h, w, tokens, tau, rounded and dtype == torch.bfloat16)
+        first = got[0] if entropy else got
+        assert first.shape == lead and first.dtype == torch.float32
+        again = ops().head_logprobs(h, w, tokens, temperature=tau, entropy=entropy, round_logits=rounded)
+        assert torch.equal(first, again[0] if entropy else again)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,V,d", [(9, 50257, 1024), (64, 1003, 2048), (90, 5003, 1024), (700, 2049, 320), (700, 2049, 77), (2600, 514, 64)])
+def test_head_of_exact_products(rows, V, d, dtype):
+    """Eighths and whole numbers: every sum of products is a number of fp32, whatever its order."""
+    g = gen(75)
+    h = torch.randint(-3, 4, (rows, d), device=DEV, generator=g).to(dtype)
+    w = (torch.randint(-2, 3, (V, d), device=DEV, generator=g) / 8).to(dtype)
+    tokens = torch.randint(0, V, (rows,), device=DEV, generator=g)
+    tokens[::7] = IGNORE
+    for tau in (1.0, 2.0):
+        check_head(ops().head_logprobs(h, w, tokens, temperature=tau, entropy=True), h, w, tokens, tau, exact=True)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("lead", [(2, 9), (3, 100)])
+def test_head_layouts(lead, dtype):
+    V, d = 1003, 128
+    h, w, tokens = head_inputs(lead, V, d, dtype, 70)
+    wide_h, wide_w = torch.randn(*lead, d + 3, device=DEV).to(dtype), torch.randn(V, d + 5, device=DEV).to(dtype)
+    wide_h[..., 1:d + 1], wide_w[:, 2:d + 2] = h, w
+    for x, y in ((wide_h[..., 1:d + 1], wide_w[:, 2:d + 2]), (h.transpose(0, 1).contiguous().transpose(0, 1), w.t().contiguous().t()),
+                 (h.flip(0).flip(0), w), (h, wide_w[:, 2:d + 2])):
+        say("head layout", x.stride(), y.stride())
+        check_head(ops().head_logprobs(x, y, tokens, entropy=True), h, w, tokens, 1.0)
+    one = ops().head_logprobs(h[:1, :1].expand(*lead, d), w, tokens.flatten()[:1].clamp(min=0).expand(lead), entropy=True)
+    for x in one:
+        assert bool((x == x.flatten()[0]).all())
+    none = ops().head_logprobs(h[:0], w, tokens[:0], entropy=True)
+    assert none[0].shape == none[1].shape == (0, lead[1])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,d", [(20, 128), (400, 128), (400, 100)])
+def test_head_of_awkward_rows(rows, d, dtype):
+    V = 2100
+    h, w, tokens = head_inputs((rows,), V, d, dtype, 71, ignored=0.0)
+    h[3], tokens[3] = math.nan, IGNORE
+    h[5] = math.nan
+    h[6, 0] = math.inf
+    tokens[7], tokens[8] = V, -5
+    h[9] = 0
+    lp, ent = ops().head_logprobs(h, w, tokens, entropy=True)
+    assert lp[3] == 0 and ent[3] == 0
+    for r in (5, 6, 7, 8):
+        assert lp[r].isnan() and ent[r].isnan(), r
+    assert abs(lp[9].item() + math.log(V)) < 1e-5 and abs(ent[9].item() - math.log(V)) < 1e-5
+    ok = torch.ones(rows, dtype=torch.bool, device=DEV)
+    ok[[5, 6, 7, 8]] = False
+    check_head((lp[ok], ent[ok]), h[ok].nan_to_num(), w, tokens[ok], 1.0)
+    none = torch.full_like(tokens, IGNORE)                       # no row at all
+    lp, ent = ops().head_logprobs(h, w, none, entropy=True)
+    assert not bool(lp.any()) and not bool(ent.any())
+    w[V // 2] = math.inf                                         # a weight without value: no row has one
+    h[3] = 1.0
+    assert bool(ops().head_logprobs(h, w, tokens).isnan()[[5, 6, 9]].all())
+
+
+def test_head_agrees_with_stored_logits():
+    h, w, tokens = head_inputs((2, 300), 5003, 256, torch.bfloat16, 72)
+    z = torch.nn.functional.linear(h, w)
+    stored = ops().token_logprobs(z, tokens)
+    rounded = ops().head_logprobs(h, w, tokens, round_logits=True)
+    # equal but where a rounding of a logit falls the other way (the library sums in another order): at most a step of the largest
+    assert (stored - rounded).abs().max() <= 2.0 ** -7 * z.abs().max()
+    assert ((stored - rounded).abs() < 1e-4).double().mean() > 0.9
+
+
 # ---- preference loss --------------------------------------------------------------------------------------------------
 
 def preference_ref(rows, n, T, reference, beta, kind, average, margin, eps):
