@@ -136,11 +136,10 @@ __global__ __launch_bounds__(kCT) void compact_kernel(Args a, int bm, int groups
   }
   // rounds of the workgroups times the tiles of a part (and half a tile that beginning and ending one takes)
   int64_t mine = INT64_MAX;
-  const int most = max(1, min(a.nt, 2 * groups / mt));
+  const int most = max(1, min(a.nt, 2 * groups / mt));         // (mt p and the cost: at most some 2^27)
   for (int p = tid + 1; p <= most; p += kCT) {
-    const int64_t per = (a.nt + p - 1) / p, rounds = ((int64_t)mt * p + groups - 1) / groups;
-    const int64_t cost = rounds * (2 * per + 1);
-    mine = min(mine, cost << 20 | p);
+    const uint32_t per = (uint32_t)(a.nt + p - 1) / (uint32_t)p, rounds = (uint32_t)(mt * p + groups - 1) / (uint32_t)groups;
+    mine = min(mine, (int64_t)(rounds * (2 * per + 1)) << 20 | p);
   }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) {
@@ -166,6 +165,12 @@ __device__ __forceinline__ void item_at(const Plan& q, int i, int& m, int& p) {
 // item of a workgroup in a round: XCD id % 8 takes a contiguous eighth
 __device__ __forceinline__ int item_of(int id, int groups) { return (id & 7) * (groups >> 3) + (id >> 3); }
 
+// the token of a compact row as a column, -1: none
+__device__ __forceinline__ int token_at(const Args& a, int row, int live) {
+  const int64_t k = row < live ? whole(a.tokens, a.wide, row_at(a, row)) : -1;
+  return k >= 0 && k < a.V ? (int)k : -1;
+}
+
 // ---- the rows' results ------------------------------------------------------------------------------------------------
 template <bool ENT>
 __device__ __forceinline__ void finish(const Args& a, int r, const State& v, float zy, bool bad) {
@@ -175,37 +180,59 @@ __device__ __forceinline__ void finish(const Args& a, int r, const State& v, flo
   if (ENT) a.ent[r] = (float)(bad ? nan : ls - (double)v.t * kLn2 / (double)v.s);
 }
 
-// a wave a live row: its slots joined in their order
+// a wave a live row: its slots in their order, kAhead a lane at a time
 template <bool ENT>
 __global__ __launch_bounds__(256) void join_kernel(Args a, int slots_a_part, int slots_if_all) {
+  constexpr int kAhead = 4;
   const int lane = threadIdx.x & 63;
-  const int i = blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int i = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int live = a.plan ? a.plan->live : a.rows;
   if (i >= live) return;
   const int slots = a.plan ? a.plan->parts * slots_a_part : slots_if_all;
   const int r = row_at(a, i);
   const int64_t y = whole(a.tokens, a.wide, r);
+  const bool bad = y < 0 || y >= a.V;
+  const float zy = bad ? 0.f : a.zy[i];
+  const State* part = a.part + (int64_t)i * slots;
   State v{-INFINITY, 0.f, 0.f};
-  for (int k = lane; k < slots; k += 64) v = join(v, a.part[(int64_t)i * slots + k], a.c);
+  for (int k = lane; k < slots; k += 64 * kAhead) {
+    State q[kAhead];
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1)
-    v = join(v, State{__shfl_xor(v.m, o), __shfl_xor(v.s, o), __shfl_xor(v.t, o)}, a.c);
+    for (int u = 0; u < kAhead; ++u) q[u] = k + 64 * u < slots ? part[k + 64 * u] : State{-INFINITY, 0.f, 0.f};
+    float m = v.m;
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) m = fmaxf(m, q[u].m);
+    const float ref = finite_ref(m);
+    move_to(v, ref, a.c);
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      move_to(q[u], ref, a.c);
+      v.s += q[u].s;
+      v.t += q[u].t;
+    }
+    v.m = m;
+  }
+  const float m = wave_max(v.m);
+  move_to(v, finite_ref(m), a.c);
+  v = State{m, wave_sum(v.s), ENT ? wave_sum(v.t) : 0.f};
   if (lane) return;
   if (y == a.ignore) {                     // (rows that were not sorted out)
     a.lp[r] = 0.f;
     if (ENT) a.ent[r] = 0.f;
     return;
   }
-  const bool bad = y < 0 || y >= a.V;
-  finish<ENT>(a, r, v, bad ? 0.f : a.zy[i], bad);
+  finish<ENT>(a, r, v, zy, bad);
 }
 
 // ---- a workgroup's tiles ------------------------------------------------------------------------------------------------
 // acc[j][i] of lane (r, g): columns n + 16 j + 4 g .. + 3 of row 16 i + r, n the wave's first column
+// ys: the tokens of the wave's rows, -1: none; zs: their logits, written as they are met
 template <bool ENT, int TM, int TN>
-__device__ __forceinline__ void take_tile(const Args& a, f32x4 (&acc)[TN][TM], State (&st)[TM], const int (&y)[TM], int n, int row0,
-                                          int live) {
+__device__ __forceinline__ void take_tile(const Args& a, f32x4 (&acc)[TN][TM], State (&st)[TM], const int* ys, float* zs, int n) {
   const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+  int y[TM];
+#pragma unroll
+  for (int i = 0; i < TM; ++i) y[i] = ys[16 * i + r];
   if (a.round) {                           // uniform
 #pragma unroll
     for (int j = 0; j < TN; ++j)
@@ -223,12 +250,12 @@ __device__ __forceinline__ void take_tile(const Args& a, f32x4 (&acc)[TN][TM], S
     for (int i = 0; i < TM; ++i)
 #pragma unroll
       for (int j = 0; j < TN; ++j) {
-        const int k = y[i] - (n + 16 * j + 4 * g), row = row0 + 16 * i + r;
-        if (k >= 0 && k < 4 && row < live) {
+        const int k = y[i] - (n + 16 * j + 4 * g);
+        if (k >= 0 && k < 4) {
           float z = acc[j][i][0];
 #pragma unroll
           for (int e = 1; e < 4; ++e) z = k == e ? acc[j][i][e] : z;
-          a.zy[row] = z;
+          zs[16 * i + r] = z;
         }
       }
   }
@@ -263,6 +290,11 @@ __device__ __forceinline__ void leave_rows(const Args& a, State (&st)[TM], int r
     const int row = row0 + 16 * i + (lane & 15);
     if (lane < 16 && row < live) a.part[(int64_t)row * slots + slot] = v;
   }
+}
+
+// a row's token among the columns [lo, hi) that a workgroup took: its logit
+__device__ __forceinline__ void leave_token(const Args& a, int y, float z, int row, int64_t lo, int64_t hi) {
+  if (y >= lo && y < hi) a.zy[row] = z;
 }
 
 // ---- any type, width, alignment -----------------------------------------------------------------------------------------
@@ -300,6 +332,8 @@ template <typename T, bool ENT, int TM, int TN>
 __global__ __launch_bounds__(256) void staged_kernel(Args a) {
   constexpr int BM = 32 * TM, BN = 32 * TN, E = kE<T>, kRS = kRowBytes + 16;
   __shared__ __align__(16) unsigned char sw[2][BN * kRS], sx[2][BM * kRS];
+  __shared__ int sy[BM];
+  __shared__ float sz[BM];
   const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave & 1, wn = wave >> 1;
   const Plan q = *a.plan;
@@ -312,15 +346,11 @@ __global__ __launch_bounds__(256) void staged_kernel(Args a) {
 #pragma unroll
     for (int i = 0; i < TM; ++i)
       xp[i] = (const T*)a.h + (int64_t)row_at(a, min(m0 + (tid >> 3) + 32 * i, q.live - 1)) * a.ldh;
-    int y[TM];
     State st[TM];
 #pragma unroll
-    for (int i = 0; i < TM; ++i) {
-      const int row = row0 + 16 * i + r;
-      const int64_t k = row < q.live ? whole(a.tokens, a.wide, row_at(a, row)) : -1;
-      y[i] = k >= 0 && k < a.V ? (int)k : -1;
-      st[i] = State{-INFINITY, 0.f, 0.f};
-    }
+    for (int i = 0; i < TM; ++i) st[i] = State{-INFINITY, 0.f, 0.f};
+    __syncthreads();                       // the item before has read its tokens
+    if (tid < BM) sy[tid] = token_at(a, m0 + tid, q.live);
     const int n_end = min((part + 1) * q.per, a.nt);
     for (int nt = part * q.per; nt < n_end; ++nt) {
       const int n0 = nt * BN;
@@ -370,29 +400,293 @@ __global__ __launch_bounds__(256) void staged_kernel(Args a) {
         if (kt + 1 < nk) stage(cur ^ 1);
         __syncthreads();
       }
-      take_tile<ENT>(a, acc, st, y, n0 + wn * 16 * TN, row0, q.live);
+      take_tile<ENT>(a, acc, st, sy + wm * 16 * TM, sz + wm * 16 * TM, n0 + wn * 16 * TN);
     }
     leave_rows(a, st, row0, q.live, q.parts * 2, part * 2 + wn);
+    __syncthreads();
+    if (tid < BM) leave_token(a, sy[tid], sz[tid], m0 + tid, (int64_t)part * q.per * BN, (int64_t)n_end * BN);
   }
 }
 
+// ---- bf16 with rows of 16-byte pieces, d a multiple of 64 ---------------------------------------------------------------
+// LDS byte address of a __shared__ pointer (the M0 operand of global_load_lds)
+__device__ __forceinline__ uint32_t lds_addr(const void* p) {
+  return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)p;
+}
+// 16 bytes a lane from base + voff into LDS at lds + 16 lane. M0 is an input operand bound to the register itself, so the compiler
+// writes it and knows that its value is live across the statement.
+__device__ __forceinline__ void dma16(const void* base, uint32_t voff, uint32_t lds) {
+  asm volatile("global_load_lds_dwordx4 %0, %1" ::"v"(voff), "s"(base), "{m0}"(lds) : "memory");
+}
+template <int N>
+__device__ __forceinline__ void wait_vm() {  // s_waitcnt vmcnt(N), other counters untouched
+  static_assert(N >= 0 && N < 64, "vmcnt range");
+  __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | (7 << 4) | (15 << 8));
+}
+
+// Operands through LDS by the DMA path, S stages (S - 1 K tiles on their way while one is multiplied); the fragments of a K tile's
+// two halves in two register sets, one read while the other is multiplied. The K tiles of a workgroup's column tiles follow each
+// other without a pause: the next column tile's first are on their way while the sums of the last take its accumulators. Slot p of
+// LDS row R holds the row's chunk p ^ (R & 7), which makes the fragment reads free of bank conflicts.
+template <typename T, bool ENT, int TM, int TN, int WGM, int WGN, int S>
+__global__ __launch_bounds__(64 * WGM * WGN) void dma_kernel(Args a) {
+  constexpr int NW = WGM * WGN, BM = 16 * TM * WGM, BN = 16 * TN * WGN, GX = BM / 8 / NW, GW = BN / 8 / NW;
+  static_assert(GX * 8 * NW == BM && GW * 8 * NW == BN, "tile rows must split into 8-row groups per wave");
+  constexpr int PER = GX + GW, E = kE<T>;
+  __shared__ __align__(1024) unsigned char sw[S][BN * kRowBytes], sx[S][BM * kRowBytes];
+  __shared__ int sy[BM];
+  __shared__ float sz[BM];
+  const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave % WGM, wn = wave / WGM;
+  const Plan q = *a.plan;
+  const int nk = a.K / (8 * E);
+  const int fw = (wn * 16 * TN + r) * kRowBytes, fx = (wm * 16 * TM + r) * kRowBytes;
+  const int c0 = (g ^ (r & 7)) << 4, c1 = ((4 + g) ^ (r & 7)) << 4;
+  auto read = [&](uint4 (&wf)[TN], uint4 (&xf)[TM], int st, int c) {
+#pragma unroll
+    for (int j = 0; j < TN; ++j) wf[j] = *reinterpret_cast<const uint4*>(&sw[st][fw + j * 16 * kRowBytes + c]);
+#pragma unroll
+    for (int i = 0; i < TM; ++i) xf[i] = *reinterpret_cast<const uint4*>(&sx[st][fx + i * 16 * kRowBytes + c]);
+  };
+  f32x4 acc[TN][TM];
+  auto mma_all = [&](const uint4 (&wf)[TN], const uint4 (&xf)[TM]) {
+#pragma unroll
+    for (int j = 0; j < TN; ++j)
+#pragma unroll
+      for (int i = 0; i < TM; ++i) Frag<T>::mma(acc[j][i], wf[j], xf[i]);
+  };
+  for (int item = item_of(blockIdx.x, gridDim.x); item < q.mt * q.parts; item += gridDim.x) {
+    int mt, part;
+    item_at(q, item, mt, part);
+    const int m0 = mt * BM, row0 = m0 + wm * 16 * TM;
+    const int n_first = part * q.per, n_end = min(n_first + q.per, a.nt);
+    // load group u of this wave: rows 8 G .. 8 G + 7, G = NW u + wave; lane -> row 8 G + lane / 8, slot lane % 8
+    uint32_t xo[GX], wo[GW];
+#pragma unroll
+    for (int u = 0; u < GX; ++u) {
+      const int R = 8 * (NW * u + wave) + (lane >> 3);
+      xo[u] = ((uint32_t)row_at(a, min(m0 + R, q.live - 1)) * (uint32_t)a.ldh + (uint32_t)(((lane & 7) ^ (R & 7)) * E)) * (uint32_t)sizeof(T);
+    }
+    int next_n = n_first, next_k = 0;      // what is loaded next
+    const char* wbase = nullptr;
+    auto columns = [&]() {                 // the offsets of column tile next_n
+      const int n0 = next_n * BN;
+      wbase = (const char*)a.w + (int64_t)n0 * a.ldw * (int)sizeof(T);
+#pragma unroll
+      for (int u = 0; u < GW; ++u) {
+        const int R = 8 * (NW * u + wave) + (lane >> 3);
+        wo[u] = ((uint32_t)min(R, a.V - 1 - n0) * (uint32_t)a.ldw + (uint32_t)(((lane & 7) ^ (R & 7)) * E)) * (uint32_t)sizeof(T);
+      }
+    };
+    auto issue = [&](int st) {
+      const int kb = next_k * kRowBytes;
+#pragma unroll
+      for (int u = 0; u < GW; ++u) dma16(wbase + kb, wo[u], lds_addr(&sw[st][(NW * u + wave) * 1024]));
+#pragma unroll
+      for (int u = 0; u < GX; ++u) dma16((const char*)a.h + kb, xo[u], lds_addr(&sx[st][(NW * u + wave) * 1024]));
+      if (++next_k == nk) {                // (behind the last tile its own again: read by nobody)
+        next_k = 0;
+        next_n = min(next_n + 1, n_end - 1);
+        columns();
+      }
+    };
+    State sums[TM];
+#pragma unroll
+    for (int i = 0; i < TM; ++i) sums[i] = State{-INFINITY, 0.f, 0.f};
+    columns();
+    __syncthreads();                       // the item before has been read
+    if (tid < BM) sy[tid] = token_at(a, m0 + tid, q.live);
+#pragma unroll
+    for (int u = 0; u < S - 1; ++u) issue(u);
+    wait_vm<(S - 2) * PER>();              // loads return in their order
+    __syncthreads();
+    issue(S - 1);
+    uint4 aw[TN], ax[TM], bw[TN], bx[TM];
+    read(aw, ax, 0, c0);
+    int st = 0;
+    for (int nt = n_first; nt < n_end; ++nt) {
+#pragma unroll
+      for (int j = 0; j < TN; ++j)
+#pragma unroll
+        for (int i = 0; i < TM; ++i) acc[j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int kt = 0; kt < nk; ++kt) {
+        read(bw, bx, st, c1);              // step 1 of the K tile ...
+        mma_all(aw, ax);                   // ... under step 0's products
+        __builtin_amdgcn_sched_barrier(0);
+        wait_vm<(S - 2) * PER>();          // the next K tile is there (nothing else was stored or loaded since)
+        __syncthreads();                   // for everyone, and this one has been read
+        issue(st);
+        st = st + 1 == S ? 0 : st + 1;
+        read(aw, ax, st, c0);              // its step 0 ...
+        __builtin_amdgcn_sched_barrier(0);
+        mma_all(bw, bx);                   // ... under step 1's products
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      take_tile<ENT>(a, acc, sums, sy + wm * 16 * TM, sz + wm * 16 * TM, nt * BN + wn * 16 * TN);
+    }
+    leave_rows(a, sums, row0, q.live, q.parts * WGN, part * WGN + wn);
+    __syncthreads();
+    if (tid < BM) leave_token(a, sy[tid], sz[tid], m0 + tid, (int64_t)n_first * BN, (int64_t)n_end * BN);
+    wait_vm<0>();                          // also the loads that nobody reads
+  }
+}
+
+// ---- few rows -----------------------------------------------------------------------------------------------------------
+// The weight's bytes are what counts: every wave streams column tiles of 16 weight rows by DMA through a ring of its own of kRing K
+// tiles (whole 128-byte lines, kRing - 1 of them on their way; no barrier) against all rows, which lie in LDS: K tiles of 128 bytes a
+// row, chunk p of row R at p ^ (R & 7), as those of the ring. Rows of 16-byte pieces, d a multiple of 128 bytes.
+constexpr int kFewWaves = 8, kFewGroups = 256, kFewLds = 64 * 1024, kRing = 5;
+
+template <typename T, bool ENT, int TM>
+__global__ __launch_bounds__(64 * kFewWaves) void few_kernel(Args a) {
+  constexpr int BM = 16 * TM, E = kE<T>, kTile = 16 * kRowBytes;
+  extern __shared__ __align__(1024) unsigned char lds[];
+  __shared__ int sy[BM];
+  __shared__ float sz[BM];
+  __shared__ State red[kFewWaves][BM];
+  const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), id = blockIdx.x * kFewWaves + wave;
+  const int nk = a.K / (8 * E);            // K tiles
+  const int tiles = (a.V + 15) / 16, waves = gridDim.x * kFewWaves, per = (tiles + waves - 1) / waves;
+  const int first = min(id * per, tiles), end = min(first + per, tiles), total = (end - first) * nk;
+  unsigned char *ring = lds + wave * kRing * kTile, *sx = lds + kFewWaves * kRing * kTile;
+  const uint32_t slot = (uint32_t)(((lane & 7) ^ (lane >> 3)) * 16);           // (8 rows a load: their chunks' places)
+  for (int c = wave; c < nk * 2 * TM; c += kFewWaves) {        // the rows: first, as loads return in their order
+    const int kt = c / (2 * TM), R = 8 * (c - kt * 2 * TM) + (lane >> 3);
+    const uint32_t at = (uint32_t)min(R, a.rows - 1) * (uint32_t)a.ldh * (uint32_t)sizeof(T) + slot;
+    dma16((const char*)a.h + kt * kRowBytes, at, lds_addr(sx) + (uint32_t)(c * 1024));
+  }
+  int tile = first, kt = 0;                // what is loaded next
+  uint32_t wo[2];
+  const char* wbase = nullptr;
+  auto columns = [&] {
+    wbase = (const char*)a.w + (int64_t)tile * 16 * a.ldw * (int)sizeof(T);
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+      wo[u] = (uint32_t)min(8 * u + (lane >> 3), a.V - 1 - tile * 16) * (uint32_t)a.ldw * (uint32_t)sizeof(T) + slot;
+  };
+  auto issue = [&](int place) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) dma16(wbase + kt * kRowBytes, wo[u], lds_addr(ring + place * kTile + u * 1024));
+    if (++kt == nk) {
+      kt = 0;
+      tile = min(tile + 1, tiles - 1);
+      columns();
+    }
+  };
+  if (total) {                             // uniform
+    columns();
+    for (int u = 0; u < min(kRing, total); ++u) issue(u);
+  }
+  State sums[TM];
+#pragma unroll
+  for (int i = 0; i < TM; ++i) sums[i] = State{-INFINITY, 0.f, 0.f};
+  f32x4 acc[1][TM];
+  if (total >= kRing)
+    wait_vm<2 * kRing>();
+  else
+    wait_vm<0>();
+  __builtin_amdgcn_sched_barrier(0);
+  if (tid < BM) sy[tid] = token_at(a, tid, a.rows);
+  __syncthreads();
+  int t = 0, place = 0;
+  for (int at = first; at < end; ++at) {
+#pragma unroll
+    for (int i = 0; i < TM; ++i) acc[0][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int k = 0; k < nk; ++k, ++t) {
+      if (t + kRing <= total)
+        wait_vm<2 * (kRing - 1)>();        // the oldest of kRing tiles
+      else
+        wait_vm<0>();
+      __builtin_amdgcn_sched_barrier(0);
+      uint4 w[2], x[2][TM];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int c = ((4 * h + g) ^ (r & 7)) << 4;
+        w[h] = *reinterpret_cast<const uint4*>(ring + place * kTile + r * kRowBytes + c);
+#pragma unroll
+        for (int i = 0; i < TM; ++i) x[h][i] = *reinterpret_cast<const uint4*>(sx + (k * BM + 16 * i + r) * kRowBytes + c);
+      }
+      __builtin_amdgcn_s_waitcnt(15 | (3 << 14) | (7 << 4));   // s_waitcnt lgkmcnt(0): the tile has been read
+      __builtin_amdgcn_sched_barrier(0);
+      if (t + kRing < total) issue(place);
+      place = place + 1 == kRing ? 0 : place + 1;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < TM; ++i) Frag<T>::mma(acc[0][i], w[h], x[h][i]);
+    }
+    take_tile<ENT>(a, acc, sums, sy, sz, at * 16);
+  }
+#pragma unroll
+  for (int i = 0; i < TM; ++i) {
+    State v = sums[i];
+#pragma unroll
+    for (int o = 16; o <= 32; o <<= 1) v = join(v, State{__shfl_xor(v.m, o), __shfl_xor(v.s, o), __shfl_xor(v.t, o)}, a.c);
+    if (lane < 16) red[wave][16 * i + r] = v;
+  }
+  __syncthreads();
+  if (tid >= BM || tid >= a.rows) return;
+  State v = red[0][tid];
+#pragma unroll
+  for (int u = 1; u < kFewWaves; ++u) v = join(v, red[u][tid], a.c);
+  a.part[(int64_t)tid * gridDim.x + blockIdx.x] = v;
+  const int64_t lo = (int64_t)blockIdx.x * kFewWaves * per * 16;
+  leave_token(a, sy[tid], sz[tid], tid, lo, lo + (int64_t)kFewWaves * per * 16);
+}
+
 // ---- sizes ------------------------------------------------------------------------------------------------------------
-struct Tile {
-  int bm, bn, groups, slots;
+// A form of the product. kind 0: staged through registers, 1: by DMA, 2: few rows. groups: workgroups; slots: a part's slots
+struct Form {
+  int kind, bm, bn, groups, slots, id;
 };
-Tile tile_of(int dtype, int64_t rows) {
-  if (dtype == DH_F32 && rows <= 512) return Tile{64, 64, 1024, 2};
-  return Tile{128, 128, 512, 2};
+// The forms of the DMA kernel, and what a tile of each takes at K = 1024, microseconds on a full card: the form whose rounds of tiles
+// take least. bf16, V 50257, d 1024, us of a call by rows, 256 x 256 / 128 x 256 / 64 x 256 / 64 x 64: 64 46 / 34 / 32 / 36; 128 46 / 34
+// / 36 / 41; 256 46 / 47 / 54 / 57; 512 70 / 75 / 81 / 90; 1024 117 / 116 / 136 / 155; 5300 440 / 500 / 607 / 732. (A tile's share of a
+// full card falls with its size; a few large tiles leave most of the card idle: 2000 rows of V 1000 are 32 of 256 x 256.) fp32 is
+// bound by its products whatever the tile, and 32 x 128 tiles have the fewest empty rows: us at 200, 329, 501, 4096 rows 205, 292,
+// 413, 3090; 64 x 64 236, 321, 412, 3055; 128 x 128 255, 372, 491, 2995.
+struct Timed {
+  Form form;
+  float us;
+};
+constexpr Timed kBf16[] = {{{1, 256, 256, 256, 2, 0}, 25.5f}, {{1, 128, 256, 256, 2, 1}, 15.f}, {{1, 64, 256, 256, 2, 2}, 9.4f},
+                           {{1, 64, 64, 512, 2, 3}, 5.7f}};
+constexpr Form kFp32 = {1, 32, 128, 512, 2, 0};
+// up to 32 rows (as many as LDS holds beside the rings) the form for few: 16 rows 23 us, the 64 x 256 tiles 32; fp32 38 and 51
+Form form_of(int dtype, int64_t rows, int d, int V, bool fast) {
+  if (!fast) return dtype == DH_F32 && rows <= 512 ? Form{0, 64, 64, 1024, 2, 0} : Form{0, 128, 128, 512, 2, 1};
+  if (rows <= 32 && (rows <= 16 ? 16 : 32) * (int64_t)d * (dtype == DH_BF16 ? 2 : 4) <= kFewLds)
+    return Form{2, 0, 0, kFewGroups, 1, 0};
+  if (dtype == DH_F32) return kFp32;
+  int best = 0;
+  double least = 1e30;
+  for (int i = 0; i < 4; ++i) {
+    const Form& f = kBf16[i].form;
+    const int64_t tiles = ((rows + f.bm - 1) / f.bm) * ((V + f.bn - 1) / f.bn);
+    const double us = (double)((tiles + f.groups - 1) / f.groups) * kBf16[i].us;
+    if (us < least) {
+      least = us;
+      best = i;
+    }
+  }
+  return kBf16[best].form;
 }
 struct Layout {
   int64_t index, part, zy, bytes;
 };
-Layout layout_of(int dtype, int64_t rows) {
-  const Tile t = tile_of(dtype, rows);
+Layout layout_of(const Form& t, int64_t rows) {
+  Layout l;
+  if (t.kind == 2) {
+    l.index = 0;
+    l.part = 0;
+    l.zy = rows * t.groups * (int64_t)sizeof(State);
+    l.bytes = l.zy + rows * 4;
+    return l;
+  }
   // a row tile has at most max(1, 2 groups / row tiles) parts
   const int64_t mt = (rows + t.bm - 1) / t.bm, padded = mt * t.bm;
   const int64_t slots = (padded > 2 * (int64_t)t.groups * t.bm ? padded : 2 * (int64_t)t.groups * t.bm) * t.slots;
-  Layout l;
   l.index = 256;
   l.part = l.index + (rows * 4 + 255) / 256 * 256;
   l.zy = l.part + slots * (int64_t)sizeof(State);
@@ -400,21 +694,53 @@ Layout layout_of(int dtype, int64_t rows) {
   return l;
 }
 
+template <typename T, bool ENT, int TM>
+int run_few(Args& a, int groups, hipStream_t s, const char* who) {
+  const size_t lds = (size_t)16 * TM * a.K * sizeof(T) + kFewWaves * kRing * 16 * kRowBytes;
+  // (the same on every call, so that no host thread lowers it before another's launch)
+  if (hipFuncSetAttribute((const void*)few_kernel<T, ENT, TM>, hipFuncAttributeMaxDynamicSharedMemorySize,
+                          kFewLds + kFewWaves * kRing * 16 * kRowBytes) != hipSuccess)
+    return dh_fail(DH_ERR_LAUNCH_FAILED, "%s: %d bytes of LDS", who, kFewLds);
+  few_kernel<T, ENT, TM><<<dim3((unsigned)groups), dim3(64 * kFewWaves), lds, s>>>(a);
+  return dh_check_launch(who);
+}
+
 template <typename T, bool ENT>
-int run(Args& a, int dtype, char* ws, const Layout& l, hipStream_t s, const char* who) {
-  const Tile t = tile_of(dtype, a.rows);
+int run(Args& a, const Form& t, char* ws, const Layout& l, hipStream_t s, const char* who) {
+  a.part = (State*)(ws + l.part);
+  a.zy = (float*)(ws + l.zy);
+  if (t.kind == 2) {
+    // as few workgroups as have every wave take the same number of column tiles
+    const int tiles = (a.V + 15) / 16, per = (tiles + t.groups * kFewWaves - 1) / (t.groups * kFewWaves);
+    const int groups = (tiles + per * kFewWaves - 1) / (per * kFewWaves);
+    const int st = a.rows <= 16 ? run_few<T, ENT, 1>(a, groups, s, who) : run_few<T, ENT, 2>(a, groups, s, who);
+    if (st) return st;
+    join_kernel<ENT><<<dim3((unsigned)((a.rows + 3) / 4)), dim3(256), 0, s>>>(a, 0, groups);
+    return dh_check_launch(who);
+  }
   a.nt = (a.V + t.bn - 1) / t.bn;
   a.plan = (Plan*)ws;
   a.index = (int*)(ws + l.index);
-  a.part = (State*)(ws + l.part);
-  a.zy = (float*)(ws + l.zy);
   compact_kernel<<<dim3((unsigned)((a.rows + kChunk - 1) / kChunk)), dim3(kCT), 0, s>>>(a, t.bm, t.groups, (int*)(ws + l.index),
                                                                                        (Plan*)ws);
   if (int st = dh_check_launch(who)) return st;
-  if (t.bm == 64)
-    staged_kernel<T, ENT, 2, 2><<<dim3((unsigned)t.groups), dim3(256), 0, s>>>(a);
-  else
-    staged_kernel<T, ENT, 4, 4><<<dim3((unsigned)t.groups), dim3(256), 0, s>>>(a);
+  const dim3 grid((unsigned)t.groups);
+  if (t.kind == 1) {
+    if (sizeof(T) == 4) {
+      dma_kernel<float, ENT, 1, 4, 2, 2, 3><<<grid, dim3(256), 0, s>>>(a);
+    } else {
+      switch (t.id) {
+        case 0: dma_kernel<bf16_t, ENT, 4, 8, 4, 2, 2><<<grid, dim3(512), 0, s>>>(a); break;
+        case 1: dma_kernel<bf16_t, ENT, 2, 8, 4, 2, 3><<<grid, dim3(512), 0, s>>>(a); break;
+        case 2: dma_kernel<bf16_t, ENT, 1, 8, 4, 2, 3><<<grid, dim3(512), 0, s>>>(a); break;
+        default: dma_kernel<bf16_t, ENT, 2, 2, 2, 2, 4><<<grid, dim3(256), 0, s>>>(a); break;
+      }
+    }
+  } else if (t.id == 0) {
+    staged_kernel<T, ENT, 2, 2><<<grid, dim3(256), 0, s>>>(a);
+  } else {
+    staged_kernel<T, ENT, 4, 4><<<grid, dim3(256), 0, s>>>(a);
+  }
   if (int st = dh_check_launch(who)) return st;
   join_kernel<ENT><<<dim3((unsigned)((a.rows + 3) / 4)), dim3(256), 0, s>>>(a, t.slots, 0);
   return dh_check_launch(who);
@@ -424,7 +750,13 @@ int run(Args& a, int dtype, char* ws, const Layout& l, hipStream_t s, const char
 
 extern "C" int64_t dh_head_logprob_workspace_bytes(int dtype, int64_t rows, int V) {
   if ((dtype != DH_F32 && dtype != DH_BF16) || rows < 0 || rows >= (1 << 22) || V < 1 || V > (1 << 24)) return -1;
-  return layout_of(dtype, rows).bytes;
+  // (whatever form d and the operands' alignment allow)
+  int64_t most = layout_of(form_of(dtype, rows, 0, V, false), rows).bytes;
+  for (int d : {0, 1 << 20}) {
+    const int64_t bytes = layout_of(form_of(dtype, rows, d, V, true), rows).bytes;
+    if (bytes > most) most = bytes;
+  }
+  return most;
 }
 
 extern "C" int dh_head_logprob(int dtype, const void* hidden, int64_t hidden_stride, int64_t rows, int d, const void* weight,
@@ -445,9 +777,15 @@ extern "C" int dh_head_logprob(int dtype, const void* hidden, int64_t hidden_str
                  (uintptr_t)logprob % 4 == 0 && (uintptr_t)entropy % 4 == 0,
              DH_ERR_INVALID_ARG, "%s: operands not aligned to their elements", who);
   if (rows == 0) return 0;
-  const Layout l = layout_of(dtype, rows);
-  DH_REQUIRE(workspace_bytes >= l.bytes && workspace && (uintptr_t)workspace % 16 == 0, DH_ERR_INVALID_ARG,
-             "%s: workspace of %lld bytes, %lld needed", who, (long long)workspace_bytes, (long long)l.bytes);
+  const int64_t need = dh_head_logprob_workspace_bytes(dtype, rows, V);
+  DH_REQUIRE(workspace_bytes >= need && workspace && (uintptr_t)workspace % 16 == 0, DH_ERR_INVALID_ARG,
+             "%s: workspace of %lld bytes, %lld needed", who, (long long)workspace_bytes, (long long)need);
+  // (offsets of a lane in 32 bits)
+  const int e = 16 / size;
+  const bool fast = d % (8 * e) == 0 && hidden_stride % e == 0 && weight_stride % e == 0 && (uintptr_t)hidden % 16 == 0 &&
+                    (uintptr_t)weight % 16 == 0 && (rows - 1) * hidden_stride + d < (int64_t)1 << 30 && weight_stride < (1 << 21);
+  const Form t = form_of(dtype, rows, d, V, fast);
+  const Layout l = layout_of(t, rows);
   Args a{};
   a.h = hidden;
   a.ldh = hidden_stride;
@@ -466,6 +804,6 @@ extern "C" int dh_head_logprob(int dtype, const void* hidden, int64_t hidden_str
   a.ent = entropy;
   hipStream_t s = (hipStream_t)stream;
   char* ws = (char*)workspace;
-  if (dtype == DH_BF16) return entropy ? run<bf16_t, true>(a, dtype, ws, l, s, who) : run<bf16_t, false>(a, dtype, ws, l, s, who);
-  return entropy ? run<float, true>(a, dtype, ws, l, s, who) : run<float, false>(a, dtype, ws, l, s, who);
+  if (dtype == DH_BF16) return entropy ? run<bf16_t, true>(a, t, ws, l, s, who) : run<bf16_t, false>(a, t, ws, l, s, who);
+  return entropy ? run<float, true>(a, t, ws, l, s, who) : run<float, false>(a, t, ws, l, s, who);
 }
