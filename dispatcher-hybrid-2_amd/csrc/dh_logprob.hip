@@ -513,8 +513,11 @@ int parts_of(int64_t rows, int V, int dtype) {
   if (p > kMaxParts) p = kMaxParts;
   return p < 1 ? 1 : (int)p;
 }
-// a wave a row: short rows, as many as fill the card so
-bool by_waves(int64_t rows, int V, int dtype) { return (int64_t)V * (dtype == DH_BF16 ? 2 : 4) <= 8192 && rows >= 1024; }
+// A wave a row: rows of up to this many bytes, as many as fill the card so. us with a wave and with a workgroup a row, 16384 rows of
+// bf16: V 6000 forward 42 and 58, backward 82 and 98; 8000 51 and 64, 114 and 110; 12000 74 and 95, 169 and 147; 16000 93 and 105, 224
+// and 206. fp32, V 4000 49 and 63, 112 and 134; 8000 91 and 100, 222 and 212.
+constexpr int kWaveForward = 32768, kWaveBackward = 16384;
+bool by_waves(int64_t rows, int V, int dtype, int bytes) { return (int64_t)V * (dtype == DH_BF16 ? 2 : 4) <= bytes && rows >= 1024; }
 
 int check(const char* who, int dtype, const Rows& a, int token_bits, double tau) {
   DH_REQUIRE(dtype == DH_F32 || dtype == DH_BF16, DH_ERR_UNSUPPORTED_DTYPE, "%s: dtype %d", who, dtype);
@@ -548,7 +551,7 @@ Rows rows_of(const void* logits, int64_t sb, int64_t st, int64_t B, int T, int V
 
 template <typename T, bool ENT>
 int forward(const char* who, int dtype, const Rows& a, const Results& o, void* ws, hipStream_t s) {
-  if (by_waves(a.rows, a.V, dtype)) {
+  if (by_waves(a.rows, a.V, dtype, kWaveForward)) {
     forward_kernel<T, ENT, 64><<<dim3((unsigned)((a.rows + kW - 1) / kW)), dim3(kT), 0, s>>>(a, 1, nullptr, o);
     return dh_check_launch(who);
   }
@@ -571,7 +574,7 @@ int forward(const char* who, int dtype, const Rows& a, bool ent, const Results& 
 template <typename T, bool ENT>
 int backward(const char* who, int dtype, const Rows& a, const Kept* kept, const Upstream& up, void* dz, hipStream_t s) {
   const int past = (int64_t)a.rows * a.V * (int)sizeof(T) >= kPast;
-  if (by_waves(a.rows, a.V, dtype)) {
+  if (by_waves(a.rows, a.V, dtype, kWaveBackward)) {
     backward_kernel<T, ENT, 64><<<dim3((unsigned)((a.rows + kW - 1) / kW)), dim3(kT), 0, s>>>(a, 1, kept, up, (T*)dz, past);
     return dh_check_launch(who);
   }

@@ -196,7 +196,7 @@ def policy_loss(logits, tokens, old_logprobs, advantages, reference_logprobs=Non
     moved = lp - known(old_logprobs)
     ratio, low, high = moved.detach().exp(), 1.0 - clip, 1.0 + clip_high
     off = ((A > 0) & (ratio > high)) | ((A < 0) & (ratio < low))
-    clipped = -torch.where(A > 0, high, low).to(lp.dtype) * A
+    clipped = -torch.where(A > 0, torch.full_like(A, high), torch.full_like(A, low)) * A
     # (a clipped ratio may be infinite: no 0 * inf in its gradient)
     rows = torch.where(off, clipped, -torch.exp(torch.where(off, zero, moved)) * A)
     if kl_weight:

@@ -20,6 +20,8 @@ Two implementations of the mixer, selected per module by `use_fused_gates`:
 """
 
 import math
+from dataclasses import dataclass
+from typing import Optional
 
 import torch
 import torch.nn as nn
@@ -28,8 +30,15 @@ from transformers import PreTrainedModel
 from transformers.generation import GenerationMixin
 from transformers.modeling_outputs import CausalLMOutput
 
-from . import distillation
+from . import distillation, logprobs
 from .configuration_dispatcher import DispatcherConfig
+
+
+@dataclass
+class ScoredOutput(CausalLMOutput):
+    """Outputs of a preference or policy loss: CausalLMOutput's, and the log-probabilities that the loss is made of."""
+
+    logprobs: Optional[torch.Tensor] = None
 
 
 def active_levels(levels, length):
@@ -482,14 +491,19 @@ class DispatcherHybridForCausalLM(DispatcherPreTrainedModel, GenerationMixin):
     def forward(self, input_ids=None, attention_mask=None, labels=None, inputs_embeds=None,
                 use_cache=None, output_attentions=None, output_hidden_states=None,
                 return_dict=None, teacher_logits=None, teacher_tokens=None, distill_temperature=1.0,
-                distill_weight=1.0, **kwargs):
+                distill_weight=1.0, preference=None, policy=None, **kwargs):
         """labels (B, T): the loss is the mean cross-entropy of the next tokens (-100: ignored).
 
         teacher_logits, teacher_tokens (B, T, k), as teacher_targets gives them for the same tokens: the loss is the
         mean over the positions of distill_weight times the distillation loss at distill_temperature plus
         (1 - distill_weight) times the cross-entropy of the next token (distillation.py). With labels, positions
         without a next token or whose next token is -100 count for nothing; without, every position counts and
-        distill_weight must be 1."""
+        distill_weight must be 1.
+
+        preference, policy: a dict of the arguments of logprobs.preference_loss or policy_loss behind the tokens, which are
+        the next tokens of labels: preference=dict(reference=..., beta=...) on 2 n sequences, the preferred ones first, or
+        policy=dict(old_logprobs=..., advantages=..., ...), its log-probabilities (B, T) placed as token_logprobs gives them.
+        The result has the loss's log-probabilities as `logprobs` (ScoredOutput; without return_dict the last element)."""
         if input_ids is None:
             raise ValueError("DispatcherHybridForCausalLM requires input_ids "
                              "(the tree mask is built from token identities)")
@@ -499,7 +513,33 @@ class DispatcherHybridForCausalLM(DispatcherPreTrainedModel, GenerationMixin):
             raise ValueError(f"sequence length {length} exceeds max_len {self.config.max_len}")
         if (teacher_logits is None) != (teacher_tokens is None):
             raise ValueError("teacher_logits and teacher_tokens come together")
-        mask = self._tree_mask(input_ids, length)
+        if sum(a is not None for a in (teacher_logits, preference, policy)) > 1:
+            raise ValueError("one of teacher_logits, preference and policy: they are losses of their own")
+        if (preference is not None or policy is not None) and labels is None:
+            raise ValueError("preference and policy losses need labels")
+        x, hidden_states = self._trunk(input_ids, output_hidden_states)
+        logits = self.lm_head(x)
+        loss = scores = None
+        if teacher_logits is not None:
+            loss = self._distillation_loss(logits, teacher_logits, teacher_tokens, labels, distill_temperature,
+                                           distill_weight)
+        elif preference is not None:
+            loss, scores = self._scored("preference_loss", logits)(logits, self._next_tokens(labels), **preference)
+        elif policy is not None:
+            loss, scores = self._scored("policy_loss", logits)(logits, self._next_tokens(labels), **policy)
+        elif labels is not None:
+            loss = F.cross_entropy(logits[:, :-1].reshape(-1, logits.size(-1)),
+                                   labels[:, 1:].reshape(-1))
+        if not return_dict:
+            out = (loss, logits) if loss is not None else (logits,)
+            return out if scores is None else (*out, scores)
+        if scores is not None:
+            return ScoredOutput(loss=loss, logits=logits, hidden_states=hidden_states, logprobs=scores)
+        return CausalLMOutput(loss=loss, logits=logits, hidden_states=hidden_states)
+
+    def _trunk(self, input_ids, output_hidden_states=None):
+        """norm_out's output, and the states entering every block and it (None: not wanted)."""
+        mask = self._tree_mask(input_ids, input_ids.size(1))
         hidden_states = () if output_hidden_states else None
         x = self._embed(input_ids)
         if self._fused_norm_ok(x, output_hidden_states):
@@ -515,17 +555,7 @@ class DispatcherHybridForCausalLM(DispatcherPreTrainedModel, GenerationMixin):
             x = self.norm_out(x)
         if output_hidden_states:
             hidden_states = hidden_states + (x,)
-        logits = self.lm_head(x)
-        loss = None
-        if teacher_logits is not None:
-            loss = self._distillation_loss(logits, teacher_logits, teacher_tokens, labels, distill_temperature,
-                                           distill_weight)
-        elif labels is not None:
-            loss = F.cross_entropy(logits[:, :-1].reshape(-1, logits.size(-1)),
-                                   labels[:, 1:].reshape(-1))
-        if not return_dict:
-            return (loss, logits) if loss is not None else (logits,)
-        return CausalLMOutput(loss=loss, logits=logits, hidden_states=hidden_states)
+        return x, hidden_states
 
     def _embed(self, input_ids):
         if getattr(self, "_fused_vocab", False):
@@ -538,14 +568,54 @@ class DispatcherHybridForCausalLM(DispatcherPreTrainedModel, GenerationMixin):
         # the logits stay whole and the labels move instead: a slice of the logits costs a copy of them, and another
         # one of their gradient
         if labels is not None:
-            labels = F.pad(labels[:, 1:], (0, 1), value=-100)
+            labels = self._next_tokens(labels)
         loss = distillation.distillation_loss
-        if getattr(self, "_fused_vocab", False):
-            if not logits.is_cuda:
-                raise RuntimeError("the fused loss is enabled but the logits are on the CPU; move the model to the GPU "
-                                   "or call enable_fused_vocab(False)")
+        if self._vocab_kernels(logits):
             from .fused_vocab import distillation_loss as loss
         return loss(logits, teacher_logits, teacher_tokens, labels, temperature, weight)
+
+    @staticmethod
+    def _next_tokens(labels):
+        return F.pad(labels[:, 1:], (0, 1), value=-100)
+
+    def _vocab_kernels(self, x):
+        """Whether a loss on x runs on the kernels; raises where they are enabled and cannot."""
+        if not getattr(self, "_fused_vocab", False):
+            return False
+        if not x.is_cuda:
+            raise RuntimeError("the fused loss is enabled but the logits are on the CPU; move the model to the GPU "
+                               "or call enable_fused_vocab(False)")
+        return True
+
+    def _scored(self, name, logits):
+        """A function of logprobs.py, on the kernels where they are enabled."""
+        if self._vocab_kernels(logits):
+            from . import fused_logprobs
+            return getattr(fused_logprobs, name)
+        return getattr(logprobs, name)
+
+    @torch.no_grad()
+    def token_logprobs(self, input_ids, labels=None, temperature=1.0, entropy=False):
+        """Log-probabilities of the next tokens, (B, T) fp32: position t has that of labels[:, t + 1] (labels None: of
+        input_ids) given the tokens up to t, 0 where there is none or it is -100; with `entropy` the entropies of those
+        positions too. What a policy loss needs of the policy that sampled and of a reference model, and summed over a
+        sequence what a preference loss needs of the latter.
+
+        Under enable_fused_vocab() the vocabulary head and its softmax are one product that stores no logits and leaves
+        the -100 positions out (dh_head_logprob; the logits rounded as the head rounds them), while nothing stands around
+        the head."""
+        if input_ids.size(1) > self.config.max_len:
+            raise ValueError(f"sequence length {input_ids.size(1)} exceeds max_len {self.config.max_len}")
+        tokens = self._next_tokens(input_ids if labels is None else labels)
+        x, _ = self._trunk(input_ids)
+        if self._vocab_kernels(x) and not torch.is_autocast_enabled("cuda"):
+            from .fused_gates import plain_linear
+            from .fused_logprobs import head_logprobs
+            head = self.lm_head
+            if x.dtype in (torch.float32, torch.bfloat16) and plain_linear(head, x.dtype, x.shape[-1], x.device):
+                return head_logprobs(x, head.weight, tokens, temperature, entropy=entropy, round_logits=True)
+        logits = self.lm_head(x)
+        return self._scored("token_logprobs", logits)(logits, tokens, temperature, entropy=entropy)
 
     @torch.no_grad()
     def teacher_targets(self, input_ids, k):
@@ -560,12 +630,14 @@ class DispatcherHybridForCausalLM(DispatcherPreTrainedModel, GenerationMixin):
     def enable_fused_vocab(self, enabled=True):
         """Run the vocabulary's ends of training on the gfx950 kernels: the embedding rows and their gradient
         (dh_embed_fwd / dh_embed_bwd, while nothing stands around the embedding), the distillation loss and its gradient
-        (dh_distill_fwd / dh_distill_bwd) and teacher_targets (dh_top_logits). Independent of enable_fused_gates.
+        (dh_distill_fwd / dh_distill_bwd), teacher_targets (dh_top_logits), token_logprobs (dh_head_logprob) and the
+        preference and policy losses with their gradient (dh_preference_fwd, dh_policy_fwd, dh_logprob_bwd). Independent of
+        enable_fused_gates.
 
         Loads the kernel library now (raising ImportError if it is missing). fp32 and bf16 on the GPU; returns self.
         """
         if enabled:
-            from . import fused_vocab  # noqa: F401  (fail now, not mid-forward)
+            from . import fused_logprobs, fused_vocab  # noqa: F401  (fail now, not mid-forward)
         self._fused_vocab = bool(enabled)
         return self
 
