@@ -425,13 +425,18 @@ __device__ __forceinline__ void wait_vm() {  // s_waitcnt vmcnt(N), other counte
 }
 
 // Operands through LDS by the DMA path, S stages (S - 1 K tiles on their way while one is multiplied); the fragments of a K tile's
-// two halves in two register sets, one read while the other is multiplied. The K tiles of a workgroup's column tiles follow each
+// two halves in two register sets, one read while the other is multiplied. Reads and loads stand between the products: in a burst
+// behind the barrier they hold both waves of a SIMD up (5631 rows, 256 x 256 tiles: 506 us in bursts, 478 so). The K tiles of a workgroup's column tiles follow each
 // other without a pause: the next column tile's first are on their way while the sums of the last take its accumulators. Slot p of
 // LDS row R holds the row's chunk p ^ (R & 7), which makes the fragment reads free of bank conflicts.
 template <typename T, bool ENT, int TM, int TN, int WGM, int WGN, int S>
 __global__ __launch_bounds__(64 * WGM * WGN) void dma_kernel(Args a) {
   constexpr int NW = WGM * WGN, BM = 16 * TM * WGM, BN = 16 * TN * WGN, GX = BM / 8 / NW, GW = BN / 8 / NW;
   static_assert(GX * 8 * NW == BM && GW * 8 * NW == BN, "tile rows must split into 8-row groups per wave");
+  // fragments read beside the products of one column tile. fp32 fragments are four products in a chain each, which the compiler
+  // has to mix (held apart as bf16's: 329 rows 309 us, 292 free)
+  constexpr bool kSpread = sizeof(T) == 2;
+  constexpr int FJ = kSpread ? (TM + TN + TN - 1) / TN : TM + TN;
   constexpr int PER = GX + GW, E = kE<T>;
   __shared__ __align__(1024) unsigned char sw[S][BN * kRowBytes], sx[S][BM * kRowBytes];
   __shared__ int sy[BM];
@@ -442,19 +447,14 @@ __global__ __launch_bounds__(64 * WGM * WGN) void dma_kernel(Args a) {
   const int nk = a.K / (8 * E);
   const int fw = (wn * 16 * TN + r) * kRowBytes, fx = (wm * 16 * TM + r) * kRowBytes;
   const int c0 = (g ^ (r & 7)) << 4, c1 = ((4 + g) ^ (r & 7)) << 4;
-  auto read = [&](uint4 (&wf)[TN], uint4 (&xf)[TM], int st, int c) {
-#pragma unroll
-    for (int j = 0; j < TN; ++j) wf[j] = *reinterpret_cast<const uint4*>(&sw[st][fw + j * 16 * kRowBytes + c]);
-#pragma unroll
-    for (int i = 0; i < TM; ++i) xf[i] = *reinterpret_cast<const uint4*>(&sx[st][fx + i * 16 * kRowBytes + c]);
+  // the f-th fragment of a K tile's half
+  auto read = [&](uint4 (&wf)[TN], uint4 (&xf)[TM], int f, int st, int c) {
+    if (f < TM)
+      xf[f < TM ? f : 0] = *reinterpret_cast<const uint4*>(&sx[st][fx + f * 16 * kRowBytes + c]);
+    else
+      wf[f < TM ? 0 : f - TM] = *reinterpret_cast<const uint4*>(&sw[st][fw + (f - TM) * 16 * kRowBytes + c]);
   };
   f32x4 acc[TN][TM];
-  auto mma_all = [&](const uint4 (&wf)[TN], const uint4 (&xf)[TM]) {
-#pragma unroll
-    for (int j = 0; j < TN; ++j)
-#pragma unroll
-      for (int i = 0; i < TM; ++i) Frag<T>::mma(acc[j][i], wf[j], xf[i]);
-  };
   for (int item = item_of(blockIdx.x, gridDim.x); item < q.mt * q.parts; item += gridDim.x) {
     int mt, part;
     item_at(q, item, mt, part);
@@ -478,17 +478,24 @@ __global__ __launch_bounds__(64 * WGM * WGN) void dma_kernel(Args a) {
         wo[u] = ((uint32_t)min(R, a.V - 1 - n0) * (uint32_t)a.ldw + (uint32_t)(((lane & 7) ^ (R & 7)) * E)) * (uint32_t)sizeof(T);
       }
     };
-    auto issue = [&](int st) {
+    auto load_one = [&](int u, int st) {   // the u-th of a K tile's PER loads
       const int kb = next_k * kRowBytes;
-#pragma unroll
-      for (int u = 0; u < GW; ++u) dma16(wbase + kb, wo[u], lds_addr(&sw[st][(NW * u + wave) * 1024]));
-#pragma unroll
-      for (int u = 0; u < GX; ++u) dma16((const char*)a.h + kb, xo[u], lds_addr(&sx[st][(NW * u + wave) * 1024]));
+      if (u < GW)
+        dma16(wbase + kb, wo[u < GW ? u : 0], lds_addr(&sw[st][(NW * u + wave) * 1024]));
+      else
+        dma16((const char*)a.h + kb, xo[u < GW ? 0 : u - GW], lds_addr(&sx[st][(NW * (u - GW) + wave) * 1024]));
+    };
+    auto advance = [&] {
       if (++next_k == nk) {                // (behind the last tile its own again: read by nobody)
         next_k = 0;
         next_n = min(next_n + 1, n_end - 1);
         columns();
       }
+    };
+    auto issue = [&](int st) {
+#pragma unroll
+      for (int u = 0; u < PER; ++u) load_one(u, st);
+      advance();
     };
     State sums[TM];
 #pragma unroll
@@ -502,7 +509,8 @@ __global__ __launch_bounds__(64 * WGM * WGN) void dma_kernel(Args a) {
     __syncthreads();
     issue(S - 1);
     uint4 aw[TN], ax[TM], bw[TN], bx[TM];
-    read(aw, ax, 0, c0);
+#pragma unroll
+    for (int f = 0; f < TM + TN; ++f) read(aw, ax, f, 0, c0);
     int st = 0;
     for (int nt = n_first; nt < n_end; ++nt) {
 #pragma unroll
@@ -510,17 +518,33 @@ __global__ __launch_bounds__(64 * WGM * WGN) void dma_kernel(Args a) {
 #pragma unroll
         for (int i = 0; i < TM; ++i) acc[j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
       for (int kt = 0; kt < nk; ++kt) {
-        read(bw, bx, st, c1);              // step 1 of the K tile ...
-        mma_all(aw, ax);                   // ... under step 0's products
+        // step 0's products, with the reads of step 1's fragments between them
+#pragma unroll
+        for (int j = 0; j < TN; ++j) {
+#pragma unroll
+          for (int f = j * FJ; f < (j + 1) * FJ && f < TM + TN; ++f) read(bw, bx, f, st, c1);
+#pragma unroll
+          for (int i = 0; i < TM; ++i) Frag<T>::mma(acc[j][i], aw[j], ax[i]);
+          if (kSpread) __builtin_amdgcn_sched_barrier(0);
+        }
         __builtin_amdgcn_sched_barrier(0);
         wait_vm<(S - 2) * PER>();          // the next K tile is there (nothing else was stored or loaded since)
         __syncthreads();                   // for everyone, and this one has been read
-        issue(st);
-        st = st + 1 == S ? 0 : st + 1;
-        read(aw, ax, st, c0);              // its step 0 ...
+        const int nst = st + 1 == S ? 0 : st + 1;
+        // step 1's products, with the reads of the next K tile's step 0 and the loads into this one's place between them
+#pragma unroll
+        for (int j = 0; j < TN; ++j) {
+#pragma unroll
+          for (int f = j * FJ; f < (j + 1) * FJ && f < TM + TN; ++f) read(aw, ax, f, nst, c0);
+#pragma unroll
+          for (int u = j * PER / TN; u < (j + 1) * PER / TN; ++u) load_one(u, st);
+#pragma unroll
+          for (int i = 0; i < TM; ++i) Frag<T>::mma(acc[j][i], bw[j], bx[i]);
+          if (kSpread) __builtin_amdgcn_sched_barrier(0);
+        }
         __builtin_amdgcn_sched_barrier(0);
-        mma_all(bw, bx);                   // ... under step 1's products
-        __builtin_amdgcn_sched_barrier(0);
+        advance();
+        st = nst;
       }
       take_tile<ENT>(a, acc, sums, sy + wm * 16 * TM, sz + wm * 16 * TM, nt * BN + wn * 16 * TN);
     }
