@@ -10,7 +10,7 @@
 // that meets it. So a row leaves a few numbers for each workgroup instead of V logits.
 //
 // Launches: the rows that count, in their order, and how the tiles are dealt out (compact_kernel; their number is known on the
-// device only); the product; the join. Up to 64 rows: the product (few_kernel, the weight's bytes bound it) and the join.
+// device only); the product; the join. Up to 32 rows: the product (few_kernel, the weight's bytes bound it) and the join.
 
 #include "dh_rows.h"
 
@@ -95,6 +95,7 @@ __global__ __launch_bounds__(kCT) void compact_kernel(Args a, int bm, int groups
   const int lo = blockIdx.x * kChunk, hi = min(lo + kChunk, a.rows);
   auto live = [&](int r) { return whole(a.tokens, a.wide, r) != a.ignore; };
   int before = 0;
+#pragma unroll 8
   for (int r = tid; r < lo; r += kCT) before += live(r);
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) before += __shfl_xor(before, o);
@@ -665,17 +666,17 @@ struct Form {
   int kind, bm, bn, groups, slots, id;
 };
 // The forms of the DMA kernel, and what a tile of each takes at K = 1024, microseconds on a full card: the form whose rounds of tiles
-// take least. bf16, V 50257, d 1024, us of a call by rows, 256 x 256 / 128 x 256 / 64 x 256 / 64 x 64: 64 46 / 34 / 32 / 36; 128 46 / 34
-// / 36 / 41; 256 46 / 47 / 54 / 57; 512 70 / 75 / 81 / 90; 1024 117 / 116 / 136 / 155; 5300 440 / 500 / 607 / 732. (A tile's share of a
-// full card falls with its size; a few large tiles leave most of the card idle: 2000 rows of V 1000 are 32 of 256 x 256.) fp32 is
-// bound by its products whatever the tile, and 32 x 128 tiles have the fewest empty rows: us at 200, 329, 501, 4096 rows 205, 292,
-// 413, 3090; 64 x 64 236, 321, 412, 3055; 128 x 128 255, 372, 491, 2995.
+// take least. bf16, V 50257, d 1024, us of a call by rows, 256 x 256 / 128 x 256 / 64 x 256 / 64 x 64: 64 42 / 32 / 31 / 33; 128 41 / 33
+// / 32 / 39; 256 41 / 42 / 48 / 59; 512 64 / 71 / 82 / 94; 640 88 / 70 / 87 / 111; 1024 112 / 109 / 130 / 163; 5300 441 / 464 / 570 / 766.
+// (A few large tiles leave most of the card idle: 2000 rows of V 1000 are 32 of 256 x 256.) fp32 is bound by its products whatever the
+// tile, and 32 x 128 tiles have the fewest empty rows: us at 200, 329, 501, 4096 rows 205, 292, 413, 3090; 64 x 64 236, 321, 412, 3055;
+// 128 x 128 255, 372, 491, 2995.
 struct Timed {
   Form form;
   float us;
 };
-constexpr Timed kBf16[] = {{{1, 256, 256, 256, 2, 0}, 25.5f}, {{1, 128, 256, 256, 2, 1}, 15.f}, {{1, 64, 256, 256, 2, 2}, 9.4f},
-                           {{1, 64, 64, 512, 2, 3}, 5.7f}};
+constexpr Timed kBf16[] = {{{1, 256, 256, 256, 2, 0}, 25.f}, {{1, 128, 256, 256, 2, 1}, 13.6f}, {{1, 64, 256, 256, 2, 2}, 8.7f},
+                           {{1, 64, 64, 512, 2, 3}, 5.9f}};
 constexpr Form kFp32 = {1, 32, 128, 512, 2, 0};
 // up to 32 rows (as many as LDS holds beside the rings) the form for few: 16 rows 23 us, the 64 x 256 tiles 32; fp32 38 and 51
 Form form_of(int dtype, int64_t rows, int d, int V, bool fast) {

@@ -219,12 +219,10 @@ __global__ __launch_bounds__(kThreads<N>) void forward_kernel(Rows a, int parts,
   if (N != kT && tid == 0) finish_row<ENT>(a, r, v, zy, bad, o);
 }
 
-// rows split over workgroups: their sums joined, a wave a row
+// a row split over workgroups: its sums joined, by a wave
 template <typename T, bool ENT>
-__global__ __launch_bounds__(kT) void join_kernel(Rows a, int parts, const Sums* part, Results o) {
+__device__ __forceinline__ void join_row(const Rows& a, int r, int parts, const Sums* part, const Results& o) {
   const int lane = threadIdx.x & 63;
-  const int r = blockIdx.x * kW + (threadIdx.x >> 6);
-  if (r >= a.rows) return;
   const int64_t y = whole(a.tokens, a.wide, r);
   if (y == a.ignore) return;               // the first launch wrote it
   const bool bad = y < 0 || y >= a.V;
@@ -234,6 +232,11 @@ __global__ __launch_bounds__(kT) void join_kernel(Rows a, int parts, const Sums*
   if (lane < parts) v = part[(int64_t)r * parts + lane];
   v = wave_join<ENT>(v, a.c);
   if (lane == 0) finish_row<ENT>(a, r, v, zy, bad, o);
+}
+template <typename T, bool ENT>
+__global__ __launch_bounds__(kT) void join_kernel(Rows a, int parts, const Sums* part, Results o) {
+  const int r = blockIdx.x * kW + (threadIdx.x >> 6);
+  if (r < a.rows) join_row<T, ENT>(a, r, parts, part, o);
 }
 
 // ---- the losses on the rows' log-probabilities ------------------------------------------------------------------------
@@ -283,36 +286,43 @@ __device__ __forceinline__ double log1p_exp(double x) {        // log(1 + e^x)
   return x > 0.0 ? x + log1p(exp(-x)) : log1p(exp(x));
 }
 
-// a workgroup a pair: half of its waves a sequence
-__global__ __launch_bounds__(kT) void preference_kernel(Preference f, const double* lp, const Kept* kept, float* losses,
-                                                        float* sums, float* coef, Part* part, int mean, float* loss,
-                                                        float* divisor) {
-  __shared__ Part red[kW];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = blockIdx.x, half = wave / (kW / 2);
+// Where the losses' results go: losses null where one is reduced, loss null where not.
+struct LossResults {
+  float *losses, *values, *by_lp, *by_ent; // values: a sequence's S; by_lp, by_ent: the derivatives without the divisor
+  Part* part;
+  int mean;
+  float *loss, *divisor;
+};
+
+// pair i by a workgroup of N threads, half of them a sequence; the result is thread 0's
+template <int N>
+__device__ __forceinline__ Part preference_pair(const Preference& f, int i, const double* lp, const Kept* kept, const LossResults& o,
+                                                Part (&red)[N / 64]) {
+  constexpr int W = N / 64;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = wave / (W / 2);
   const int64_t first = (int64_t)(half ? f.pairs + i : i) * f.T;
   Part p{0.0, 0};
 #pragma unroll 4
-  for (int t = threadIdx.x % (kT / 2); t < f.T; t += kT / 2) {
+  for (int t = threadIdx.x % (N / 2); t < f.T; t += N / 2) {
     p.sum += lp[first + t];
     p.n += kept[first + t].live;
   }
   p = wave_part(p);
   if (lane == 0) red[wave] = p;
   __syncthreads();
-  if (threadIdx.x) return;
+  if (threadIdx.x) return Part{0.0, 0};
   double gain[2], count[2];
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    Part q = red[h * (kW / 2)];
-#pragma unroll
-    for (int w = 1; w < kW / 2; ++w) {
-      q.sum += red[h * (kW / 2) + w].sum;
-      q.n += red[h * (kW / 2) + w].n;
+    Part q = red[h * (W / 2)];
+    for (int w = 1; w < W / 2; ++w) {
+      q.sum += red[h * (W / 2) + w].sum;
+      q.n += red[h * (W / 2) + w].n;
     }
     const int s = h ? f.pairs + i : i;
     count[h] = f.average && q.n > 1 ? (double)q.n : 1.0;
     const double S = q.sum / count[h];
-    sums[s] = (float)S;
+    o.values[s] = (float)S;
     gain[h] = S;
     if (f.reference)
       gain[h] -= f.wide ? reinterpret_cast<const double*>(f.reference)[s] : (double)reinterpret_cast<const float*>(f.reference)[s];
@@ -330,15 +340,34 @@ __global__ __launch_bounds__(kT) void preference_kernel(Preference f, const doub
     slope = 2.0 * l;
     l *= l;
   }
-  if (losses) losses[i] = (float)l;
-  coef[i] = (float)(slope / count[0]);
-  coef[f.pairs + i] = (float)(-slope / count[1]);
-  if (!loss) return;
-  const Part one{l, 1};
+  if (o.losses) o.losses[i] = (float)l;
+  o.by_lp[i] = (float)(slope / count[0]);
+  o.by_lp[f.pairs + i] = (float)(-slope / count[1]);
+  return Part{l, 1};
+}
+__global__ __launch_bounds__(kT) void preference_kernel(Preference f, const double* lp, const Kept* kept, LossResults o) {
+  __shared__ Part red[kW];
+  const Part p = preference_pair<kT>(f, blockIdx.x, lp, kept, o, red);
+  if (threadIdx.x || !o.loss) return;
   if (gridDim.x == 1)
-    write_loss(one, mean, loss, divisor);
+    write_loss(p, o.mean, o.loss, o.divisor);
   else
-    part[i] = one;
+    o.part[blockIdx.x] = p;
+}
+// few rows, split: joined by the workgroup that goes on with the pairs
+constexpr int kJT = 1024;
+template <typename T>
+__global__ __launch_bounds__(kJT) void join_preference_kernel(Rows a, int parts, const Sums* part, Results rows, Preference f, LossResults o) {
+  __shared__ Part red[kJT / 64];
+  for (int r = threadIdx.x >> 6; r < a.rows; r += kJT / 64) join_row<T, false>(a, r, parts, part, rows);
+  Part p{0.0, 0};
+  for (int i = 0; i < f.pairs; ++i) {
+    __syncthreads();                       // the rows, and the pair before
+    const Part q = preference_pair<kJT>(f, i, rows.lp64, rows.kept, o, red);
+    p.sum += q.sum;
+    p.n += q.n;
+  }
+  if (threadIdx.x == 0 && o.loss) write_loss(p, o.mean, o.loss, o.divisor);
 }
 
 struct Policy {
@@ -351,26 +380,24 @@ struct Policy {
   double low, high, kl, ent;               // 1 - clip, 1 + clip_high, the weights
 };
 
-// by_lp, by_ent: the loss's derivatives in lp and H without the divisor
-__global__ __launch_bounds__(kT) void policy_kernel(Policy f, const double* lp, const double* ent, const Kept* kept,
-                                                    float* losses, float* by_lp, float* by_ent, Part* part, int mean,
-                                                    float* loss, float* divisor) {
-  __shared__ Part red[kW];
-  __shared__ int counts[kW];
+// unit u of the rows by a workgroup of N threads; the result is thread 0's
+template <int N>
+__device__ __forceinline__ Part policy_unit(const Policy& f, int64_t u, const double* lp, const double* ent, const Kept* kept,
+                                            const LossResults& o, Part (&red)[N / 64], int (&counts)[N / 64]) {
+  constexpr int W = N / 64;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t lo = (int64_t)blockIdx.x * f.unit, hi = lo + f.unit < f.rows ? lo + f.unit : f.rows;
+  const int64_t lo = u * f.unit, hi = lo + f.unit < f.rows ? lo + f.unit : f.rows;
   double share = 1.0;
-  int length = 0;
   if (f.by_sequence) {
+    int length = 0;
 #pragma unroll 4
-    for (int64_t r = lo + threadIdx.x; r < hi; r += kT) length += kept[r].live;
+    for (int64_t r = lo + threadIdx.x; r < hi; r += N) length += kept[r].live;
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) length += __shfl_xor(length, o);
     if (lane == 0) counts[wave] = length;
     __syncthreads();
     length = 0;
-#pragma unroll
-    for (int w = 0; w < kW; ++w) length += counts[w];
+    for (int w = 0; w < W; ++w) length += counts[w];
     share = 1.0 / (double)(length > 0 ? length : 1);
   }
   Part p{0.0, 0};
@@ -378,7 +405,7 @@ __global__ __launch_bounds__(kT) void policy_kernel(Policy f, const double* lp, 
     // (all asked for at once; what stands where a row is ignored is not looked at)
     const bool live = kept[r].live;
     const float advantage = f.advantage[r / f.adv_div], old = f.old[r], reference = f.reference ? f.reference[r] : 0.f;
-    const double x = lp[r], h = by_ent ? ent[r] : 0.0;
+    const double x = lp[r], h = o.by_ent ? ent[r] : 0.0;
     double l = 0.0, slope = 0.0;
     if (live) {
       const double A = (double)advantage, ratio = exp(x - (double)old);
@@ -391,23 +418,22 @@ __global__ __launch_bounds__(kT) void policy_kernel(Policy f, const double* lp, 
         l += f.kl * (more - d);
         slope -= f.kl * more;
       }
-      if (by_ent) l -= f.ent * h;
+      if (o.by_ent) l -= f.ent * h;
       ++p.n;
     }
     p.sum += l;
-    if (losses) losses[r] = (float)l;
-    by_lp[r] = (float)(slope * share);
-    if (by_ent) by_ent[r] = live ? (float)(-f.ent * share) : 0.f;
+    if (o.losses) o.losses[r] = (float)l;
+    o.by_lp[r] = (float)(slope * share);
+    if (o.by_ent) o.by_ent[r] = live ? (float)(-f.ent * share) : 0.f;
   };
 #pragma unroll 2
-  for (int64_t r = lo + threadIdx.x; r < hi; r += kT) row(r);
-  if (!loss) return;
+  for (int64_t r = lo + threadIdx.x; r < hi; r += N) row(r);
+  if (!o.loss) return p;                   // (not looked at)
   p = wave_part(p);
   if (lane == 0) red[wave] = p;
   __syncthreads();
-  if (threadIdx.x) return;
-#pragma unroll
-  for (int w = 1; w < kW; ++w) {
+  if (threadIdx.x) return Part{0.0, 0};
+  for (int w = 1; w < W; ++w) {
     p.sum += red[w].sum;
     p.n += red[w].n;
   }
@@ -415,10 +441,33 @@ __global__ __launch_bounds__(kT) void policy_kernel(Policy f, const double* lp, 
     p.sum *= share;
     p.n = p.n > 0;
   }
+  return p;
+}
+__global__ __launch_bounds__(kT) void policy_kernel(Policy f, const double* lp, const double* ent, const Kept* kept, LossResults o) {
+  __shared__ Part red[kW];
+  __shared__ int counts[kW];
+  const Part p = policy_unit<kT>(f, blockIdx.x, lp, ent, kept, o, red, counts);
+  if (threadIdx.x || !o.loss) return;
   if (gridDim.x == 1)
-    write_loss(p, mean, loss, divisor);
+    write_loss(p, o.mean, o.loss, o.divisor);
   else
-    part[blockIdx.x] = p;
+    o.part[blockIdx.x] = p;
+}
+// few rows, split: joined by the workgroup that goes on with the units
+template <typename T, bool ENT>
+__global__ __launch_bounds__(kJT) void join_policy_kernel(Rows a, int parts, const Sums* part, Results rows, Policy f, int units,
+                                                          LossResults o) {
+  __shared__ Part red[kJT / 64];
+  __shared__ int counts[kJT / 64];
+  for (int r = threadIdx.x >> 6; r < a.rows; r += kJT / 64) join_row<T, ENT>(a, r, parts, part, rows);
+  Part p{0.0, 0};
+  for (int u = 0; u < units; ++u) {
+    __syncthreads();                       // the rows, and the unit before
+    const Part q = policy_unit<kJT>(f, u, rows.lp64, rows.ent64, rows.kept, o, red, counts);
+    p.sum += q.sum;
+    p.n += q.n;
+  }
+  if (threadIdx.x == 0 && o.loss) write_loss(p, o.mean, o.loss, o.divisor);
 }
 
 // ---- backward ---------------------------------------------------------------------------------------------------------
@@ -549,8 +598,9 @@ Rows rows_of(const void* logits, int64_t sb, int64_t st, int64_t B, int T, int V
   return a;
 }
 
+// joined: whether rows that are split are joined here
 template <typename T, bool ENT>
-int forward(const char* who, int dtype, const Rows& a, const Results& o, void* ws, hipStream_t s) {
+int forward(const char* who, int dtype, const Rows& a, const Results& o, void* ws, bool joined, hipStream_t s) {
   if (by_waves(a.rows, a.V, dtype, kWaveForward)) {
     forward_kernel<T, ENT, 64><<<dim3((unsigned)((a.rows + kW - 1) / kW)), dim3(kT), 0, s>>>(a, 1, nullptr, o);
     return dh_check_launch(who);
@@ -562,13 +612,22 @@ int forward(const char* who, int dtype, const Rows& a, const Results& o, void* w
   }
   forward_kernel<T, ENT, kT><<<dim3((unsigned)a.rows * parts), dim3(kT), 0, s>>>(a, parts, (Sums*)ws, o);
   if (int st = dh_check_launch(who)) return st;
+  if (!joined) return 0;
   join_kernel<T, ENT><<<dim3((unsigned)((a.rows + kW - 1) / kW)), dim3(kT), 0, s>>>(a, parts, (const Sums*)ws, o);
   return dh_check_launch(who);
 }
-int forward(const char* who, int dtype, const Rows& a, bool ent, const Results& o, void* ws, hipStream_t s) {
+int forward(const char* who, int dtype, const Rows& a, bool ent, const Results& o, void* ws, bool joined, hipStream_t s) {
   if (a.rows == 0) return 0;
-  if (dtype == DH_BF16) return ent ? forward<bf16_t, true>(who, dtype, a, o, ws, s) : forward<bf16_t, false>(who, dtype, a, o, ws, s);
-  return ent ? forward<float, true>(who, dtype, a, o, ws, s) : forward<float, false>(who, dtype, a, o, ws, s);
+  if (dtype == DH_BF16)
+    return ent ? forward<bf16_t, true>(who, dtype, a, o, ws, joined, s) : forward<bf16_t, false>(who, dtype, a, o, ws, joined, s);
+  return ent ? forward<float, true>(who, dtype, a, o, ws, joined, s) : forward<float, false>(who, dtype, a, o, ws, joined, s);
+}
+// Rows few enough for one workgroup to join them on its way to the loss, in units of its own or not at all (48 rows of V 50257, policy
+// loss: a launch less, 3 us): 0 or the parts of a row.
+constexpr int kFewRows = 64, kFewUnits = 4;
+int few_parts(const Rows& a, int64_t units, int dtype) {
+  const int parts = a.rows > 0 && a.rows <= kFewRows && units <= kFewUnits ? parts_of(a.rows, a.V, dtype) : 1;
+  return parts > 1 ? parts : 0;
 }
 
 template <typename T, bool ENT>
@@ -622,7 +681,7 @@ extern "C" int dh_logprob_fwd(int dtype, const void* logits, int64_t stride_b, i
   DH_REQUIRE(workspace_bytes >= need && (need == 0 || (workspace && (uintptr_t)workspace % 8 == 0)), DH_ERR_INVALID_ARG,
              "%s: workspace of %lld bytes, %lld needed", who, (long long)workspace_bytes, (long long)need);
   return forward(who, dtype, a, entropy != nullptr, Results{logprob, entropy, nullptr, nullptr, (Kept*)row_kept}, workspace,
-                 (hipStream_t)stream);
+                 true, (hipStream_t)stream);
 }
 
 extern "C" int dh_logprob_bwd(int dtype, const void* logits, int64_t stride_b, int64_t stride_t, int64_t B, int T, int V,
@@ -689,11 +748,20 @@ extern "C" int dh_preference_fwd(int dtype, const void* logits, int64_t stride_b
   double* lp = (double*)(ws + l.lp64);
   Part* part = (Part*)(ws + l.part);
   Kept* kept = (Kept*)row_kept;
-  if (int st = forward(who, dtype, a, false, Results{nullptr, nullptr, lp, nullptr, kept}, ws, s)) return st;
+  const Results rows{nullptr, nullptr, lp, nullptr, kept};
+  const int parts = few_parts(a, pairs, dtype);
+  if (int st = forward(who, dtype, a, false, rows, ws, parts == 0, s)) return st;
+  const LossResults o{reduction ? nullptr : pair_loss, sums, coef, nullptr, part, reduction == 1, reduction ? loss : nullptr, divisor};
+  const Preference f{(int)pairs, T, kind, average, beta, margin, label_smoothing, reference, reference_bits == 64};
+  if (parts) {
+    if (dtype == DH_BF16)
+      join_preference_kernel<bf16_t><<<dim3(1), dim3(kJT), 0, s>>>(a, parts, (const Sums*)ws, rows, f, o);
+    else
+      join_preference_kernel<float><<<dim3(1), dim3(kJT), 0, s>>>(a, parts, (const Sums*)ws, rows, f, o);
+    return dh_check_launch(who);
+  }
   if (pairs) {
-    const Preference f{(int)pairs, T, kind, average, beta, margin, label_smoothing, reference, reference_bits == 64};
-    preference_kernel<<<dim3((unsigned)pairs), dim3(kT), 0, s>>>(f, lp, kept, reduction ? nullptr : pair_loss, sums, coef, part,
-                                                                 reduction == 1, reduction ? loss : nullptr, divisor);
+    preference_kernel<<<dim3((unsigned)pairs), dim3(kT), 0, s>>>(f, lp, kept, o);
     if (int st = dh_check_launch(who)) return st;
   }
   if (!reduction || pairs == 1) return 0;
@@ -744,13 +812,28 @@ extern "C" int dh_policy_fwd(int dtype, const void* logits, int64_t stride_b, in
   double *lp = (double*)(ws + l.lp64), *h = ent ? (double*)(ws + l.ent64) : nullptr;
   Part* part = (Part*)(ws + l.part);
   Kept* kept = (Kept*)row_kept;
-  if (int st = forward(who, dtype, a, ent, Results{logprob, nullptr, lp, h, kept}, ws, s)) return st;
+  const Results rows{logprob, nullptr, lp, h, kept};
+  const int parts = few_parts(a, units, dtype);
+  if (int st = forward(who, dtype, a, ent, rows, ws, parts == 0, s)) return st;
+  const LossResults o{reduction ? nullptr : row_loss, nullptr, by_logprob, by_entropy, part, mean, reduction ? loss : nullptr, divisor};
+  const Policy f{a.rows, T, by_sequence ? T : (int)kUnit, by_sequence, old_logprob, advantage,
+                 kl_weight > 0.0 ? reference_logprob : nullptr, per_sequence ? T : 1, 1.0 - clip, 1.0 + clip_high, kl_weight,
+                 entropy_weight};
+  if (parts) {
+    const Sums* sums = (const Sums*)ws;
+    const dim3 one(1), block(kJT);
+    if (dtype == DH_BF16 && ent)
+      join_policy_kernel<bf16_t, true><<<one, block, 0, s>>>(a, parts, sums, rows, f, (int)units, o);
+    else if (dtype == DH_BF16)
+      join_policy_kernel<bf16_t, false><<<one, block, 0, s>>>(a, parts, sums, rows, f, (int)units, o);
+    else if (ent)
+      join_policy_kernel<float, true><<<one, block, 0, s>>>(a, parts, sums, rows, f, (int)units, o);
+    else
+      join_policy_kernel<float, false><<<one, block, 0, s>>>(a, parts, sums, rows, f, (int)units, o);
+    return dh_check_launch(who);
+  }
   if (units) {
-    const Policy f{a.rows, T, by_sequence ? T : (int)kUnit, by_sequence, old_logprob, advantage,
-                   kl_weight > 0.0 ? reference_logprob : nullptr, per_sequence ? T : 1, 1.0 - clip, 1.0 + clip_high, kl_weight,
-                   entropy_weight};
-    policy_kernel<<<dim3((unsigned)units), dim3(kT), 0, s>>>(f, lp, h, kept, reduction ? nullptr : row_loss, by_logprob, by_entropy,
-                                                             part, mean, reduction ? loss : nullptr, divisor);
+    policy_kernel<<<dim3((unsigned)units), dim3(kT), 0, s>>>(f, lp, h, kept, o);
     if (int st = dh_check_launch(who)) return st;
   }
   if (!reduction || units == 1) return 0;

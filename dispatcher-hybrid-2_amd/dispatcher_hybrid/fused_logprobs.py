@@ -120,7 +120,7 @@ def token_logprobs(logits, tokens, temperature=1.0, ignore_index=-100, entropy=F
 
     logits (..., V) fp32 or bf16, entries of -inf allowed; tokens (...) int32 or int64. A position whose token is ignore_index
     counts for nothing: zeros, a gradient of zeros, whatever its logits hold. Another token outside the vocabulary makes its
-    position's values and all of its gradient NaN."""
+    position's values and all of its gradient NaN. Fewer than 2^22 positions, up to 2^24 logits each (as for the losses)."""
     plain.check_tokens("token_logprobs", logits, tokens, temperature)
     args = (logits, tokens, float(temperature), int(ignore_index), bool(entropy))
     if type(logits) in _PLAIN and logits.is_cuda and plain_eager():
@@ -225,10 +225,9 @@ def preference_loss(logits, tokens, reference=None, beta=0.1, loss="sigmoid", av
     args = (logits, tokens, reference, plain.KINDS.index(loss), bool(average), float(beta), float(margin), float(label_smoothing),
             int(ignore_index), plain.PAIR_REDUCTIONS.index(reduction))
     if type(logits) in _PLAIN and logits.is_cuda and plain_eager():
-        out = _native.preference_loss(*args)
-    else:
-        _hip.require_gpu(logits, "preference_loss")
-        out = torch.ops.dispatcher.preference_loss(*args)
+        return tuple(_native.preference_loss(*args))
+    _hip.require_gpu(logits, "preference_loss")
+    out = torch.ops.dispatcher.preference_loss(*args)
     return out[0], out[1].detach()
 
 
@@ -303,8 +302,7 @@ def policy_loss(logits, tokens, old_logprobs, advantages, reference_logprobs=Non
             float(kl_weight), float(entropy_weight), float(temperature), int(ignore_index),
             plain.TOKEN_REDUCTIONS.index(reduction))
     if type(logits) in _PLAIN and logits.is_cuda and plain_eager():
-        out = _native.policy_loss(*args)
-    else:
-        _hip.require_gpu(logits, "policy_loss")
-        out = torch.ops.dispatcher.policy_loss(*args)
+        return tuple(_native.policy_loss(*args))
+    _hip.require_gpu(logits, "policy_loss")
+    out = torch.ops.dispatcher.policy_loss(*args)
     return out[0], out[1].detach()
