@@ -84,15 +84,17 @@ struct Args {
 __device__ __forceinline__ int row_at(const Args& a, int i) { return a.index ? a.index[i] : i; }
 
 // ---- the rows that count ----------------------------------------------------------------------------------------------
-constexpr int kCT = 1024, kChunk = 4 * kCT;                    // threads, rows a workgroup
+constexpr int kCT = 1024;
+// rows a workgroup: one a thread, more where the workgroups' reads of all rows before their own would add up
+int chunk_of(int64_t rows) { return kCT * (int)(rows <= 32768 ? 1 : rows <= (1 << 20) ? rows / 32768 : 32); }
 
-// A workgroup counts the live rows before its own (all of them read by every one: 8 MB a million rows, beside a product of 70 ms)
-// and places those of its chunk. The last one deals out the tiles: the number of parts whose longest workgroup is shortest.
-__global__ __launch_bounds__(kCT) void compact_kernel(Args a, int bm, int groups, int* index, Plan* plan) {
+// A workgroup counts the live rows before its own and places those of its chunk. The last one deals out the tiles: the number of parts
+// whose longest workgroup is shortest.
+__global__ __launch_bounds__(kCT) void compact_kernel(Args a, int bm, int groups, int chunk, int* index, Plan* plan) {
   __shared__ int red[kCT / 64], base, total;
   __shared__ int64_t best[kCT / 64];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int lo = blockIdx.x * kChunk, hi = min(lo + kChunk, a.rows);
+  const int lo = blockIdx.x * chunk, hi = min(lo + chunk, a.rows);
   auto live = [&](int r) { return whole(a.tokens, a.wide, r) != a.ignore; };
   int before = 0;
 #pragma unroll 8
@@ -746,8 +748,9 @@ int run(Args& a, const Form& t, char* ws, const Layout& l, hipStream_t s, const 
   a.nt = (a.V + t.bn - 1) / t.bn;
   a.plan = (Plan*)ws;
   a.index = (int*)(ws + l.index);
-  compact_kernel<<<dim3((unsigned)((a.rows + kChunk - 1) / kChunk)), dim3(kCT), 0, s>>>(a, t.bm, t.groups, (int*)(ws + l.index),
-                                                                                       (Plan*)ws);
+  const int chunk = chunk_of(a.rows);
+  compact_kernel<<<dim3((unsigned)((a.rows + chunk - 1) / chunk)), dim3(kCT), 0, s>>>(a, t.bm, t.groups, chunk, (int*)(ws + l.index),
+                                                                                     (Plan*)ws);
   if (int st = dh_check_launch(who)) return st;
   const dim3 grid((unsigned)t.groups);
   if (t.kind == 1) {

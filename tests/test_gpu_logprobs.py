@@ -606,3 +606,15 @@ def test_ratio_of_one_and_of_the_clip_itself():
     got, = torch.autograd.grad(rows.sum(), leaf)
     want, = torch.autograd.grad((ops().token_logprobs(leaf, tok) * -adv).sum(), leaf)
     assert (got - want).abs().max() <= 4e-6 * want.abs().max()
+
+
+@pytest.mark.parametrize("rows", [1024, 1025, 33000, 70001])
+def test_head_of_many_rows(rows):
+    """Rows sorted out by several workgroups, one and more a thread: the values of the same rows alone."""
+    h, w, tokens = head_inputs((rows,), 257, 64, torch.bfloat16, 76, ignored=0.5)
+    lp, ent = ops().head_logprobs(h, w, tokens, entropy=True)
+    live = tokens != IGNORE
+    check_head((lp, ent), h, w, tokens, 1.0)
+    a, b = ops().head_logprobs(h[live], w, tokens[live], entropy=True)
+    assert (a - lp[live]).abs().max() < 1e-5 and (b - ent[live]).abs().max() < 1e-5
+    assert not bool(lp[~live].any()) and not bool(ent[~live].any())
