@@ -219,24 +219,24 @@ __global__ __launch_bounds__(kThreads<N>) void forward_kernel(Rows a, int parts,
   if (N != kT && tid == 0) finish_row<ENT>(a, r, v, zy, bad, o);
 }
 
-// a row split over workgroups: its sums joined, by a wave
-template <typename T, bool ENT>
+// a row split over workgroups: its sums joined, by G lanes (r past the last row: nothing)
+template <typename T, bool ENT, int G>
 __device__ __forceinline__ void join_row(const Rows& a, int r, int parts, const Sums* part, const Results& o) {
-  const int lane = threadIdx.x & 63;
-  const int64_t y = whole(a.tokens, a.wide, r);
-  if (y == a.ignore) return;               // the first launch wrote it
-  const bool bad = y < 0 || y >= a.V;
+  const int lane = threadIdx.x % G;
+  const int64_t y = r < a.rows ? whole(a.tokens, a.wide, r) : a.ignore;
+  const bool on = y != a.ignore, bad = y < 0 || y >= a.V;      // (the first launch wrote ignored rows)
   float zy = 0.f;
-  if (lane == 0 && !bad) zy = Elem<T>::load(row_of<T>(a, r) + y);
+  if (lane == 0 && on && !bad) zy = Elem<T>::load(row_of<T>(a, r) + y);
   Sums v{-INFINITY, 0.f, 0.f};
-  if (lane < parts) v = part[(int64_t)r * parts + lane];
-  v = wave_join<ENT>(v, a.c);
-  if (lane == 0) finish_row<ENT>(a, r, v, zy, bad, o);
+  if (on)
+    for (int k = lane; k < parts; k += G) v = join<ENT>(v, part[(int64_t)r * parts + k], a.c);
+#pragma unroll
+  for (int o = G / 2; o > 0; o >>= 1) v = join<ENT>(v, Sums{__shfl_xor(v.m, o), __shfl_xor(v.s, o), ENT ? __shfl_xor(v.t, o) : 0.f}, a.c);
+  if (lane == 0 && on) finish_row<ENT>(a, r, v, zy, bad, o);
 }
 template <typename T, bool ENT>
 __global__ __launch_bounds__(kT) void join_kernel(Rows a, int parts, const Sums* part, Results o) {
-  const int r = blockIdx.x * kW + (threadIdx.x >> 6);
-  if (r < a.rows) join_row<T, ENT>(a, r, parts, part, o);
+  join_row<T, ENT, 16>(a, blockIdx.x * (kT / 16) + (threadIdx.x >> 4), parts, part, o);
 }
 
 // ---- the losses on the rows' log-probabilities ------------------------------------------------------------------------
@@ -359,7 +359,7 @@ constexpr int kJT = 1024;
 template <typename T>
 __global__ __launch_bounds__(kJT) void join_preference_kernel(Rows a, int parts, const Sums* part, Results rows, Preference f, LossResults o) {
   __shared__ Part red[kJT / 64];
-  for (int r = threadIdx.x >> 6; r < a.rows; r += kJT / 64) join_row<T, false>(a, r, parts, part, rows);
+  join_row<T, false, 16>(a, threadIdx.x >> 4, parts, part, rows);
   Part p{0.0, 0};
   for (int i = 0; i < f.pairs; ++i) {
     __syncthreads();                       // the rows, and the pair before
@@ -459,7 +459,7 @@ __global__ __launch_bounds__(kJT) void join_policy_kernel(Rows a, int parts, con
                                                           LossResults o) {
   __shared__ Part red[kJT / 64];
   __shared__ int counts[kJT / 64];
-  for (int r = threadIdx.x >> 6; r < a.rows; r += kJT / 64) join_row<T, ENT>(a, r, parts, part, rows);
+  join_row<T, ENT, 16>(a, threadIdx.x >> 4, parts, part, rows);
   Part p{0.0, 0};
   for (int u = 0; u < units; ++u) {
     __syncthreads();                       // the rows, and the unit before
@@ -613,7 +613,7 @@ int forward(const char* who, int dtype, const Rows& a, const Results& o, void* w
   forward_kernel<T, ENT, kT><<<dim3((unsigned)a.rows * parts), dim3(kT), 0, s>>>(a, parts, (Sums*)ws, o);
   if (int st = dh_check_launch(who)) return st;
   if (!joined) return 0;
-  join_kernel<T, ENT><<<dim3((unsigned)((a.rows + kW - 1) / kW)), dim3(kT), 0, s>>>(a, parts, (const Sums*)ws, o);
+  join_kernel<T, ENT><<<dim3((unsigned)((a.rows + kT / 16 - 1) / (kT / 16))), dim3(kT), 0, s>>>(a, parts, (const Sums*)ws, o);
   return dh_check_launch(who);
 }
 int forward(const char* who, int dtype, const Rows& a, bool ent, const Results& o, void* ws, bool joined, hipStream_t s) {
@@ -624,7 +624,7 @@ int forward(const char* who, int dtype, const Rows& a, bool ent, const Results& 
 }
 // Rows few enough for one workgroup to join them on its way to the loss, in units of its own or not at all (48 rows of V 50257, policy
 // loss: a launch less, 3 us): 0 or the parts of a row.
-constexpr int kFewRows = 64, kFewUnits = 4;
+constexpr int kFewRows = kJT / 16, kFewUnits = 4;
 int few_parts(const Rows& a, int64_t units, int dtype) {
   const int parts = a.rows > 0 && a.rows <= kFewRows && units <= kFewUnits ? parts_of(a.rows, a.V, dtype) : 1;
   return parts > 1 ? parts : 0;
