@@ -173,7 +173,8 @@ def preference_loss(logits, tokens, reference=None, beta=0.1, loss="sigmoid", av
         if label_smoothing:
             pairs = pairs - label_smoothing * torch.nn.functional.logsigmoid(-x)
     elif loss == "hinge":
-        pairs = torch.relu(1.0 - x)
+        # (a factor of NaN: a broken pair's gradient is NaN too)
+        pairs = torch.where(x >= 1.0, torch.zeros_like(x), 1.0 - x) * torch.where(x.isnan(), math.nan, 1.0)
     else:
         pairs = (d - 0.5 / beta) ** 2
     out = pairs if reduction == "none" else pairs.sum() / n if reduction == "mean" and n else \

@@ -92,6 +92,19 @@ def test_preference_against_pairs(kind, beta, average, margin, eps):
         assert torch.autograd.gradcheck(f, z.clone().requires_grad_())
 
 
+@pytest.mark.parametrize("kind,beta,average,margin,eps", KINDS)
+def test_a_broken_pair_is_nan_throughout(kind, beta, average, margin, eps):
+    z, tokens, _ = case((4, 3), 7, 8, ignored=0.0)
+    tokens[2, 1], tokens[0, 2] = 7, IGNORE                     # outside the vocabulary; no part of an answer
+    zz = z.clone().requires_grad_()
+    pairs, sums = plain.preference_loss(zz, tokens, beta=beta, loss=kind, average=average, margin=margin, label_smoothing=eps,
+                                        reduction="none")
+    dz, = torch.autograd.grad(pairs.sum(), zz)
+    assert pairs.isnan().tolist() == [True, False] and sums.isnan().tolist() == [False, False, True, False]
+    live = tokens != IGNORE
+    assert dz[[0, 2]][live[[0, 2]]].isnan().all() and not dz[0, 2].any() and dz[[1, 3]].isfinite().all()
+
+
 @pytest.mark.parametrize("clip,high,kl,w,per_sequence", [(0.2, None, 0.0, 0.0, False), (0.1, 0.4, 0.3, 0.02, True), (1.0, 0.5, 0.0, 0.1, True)])
 def test_policy_against_rows(clip, high, kl, w, per_sequence):
     B, T, V, tau = 3, 6, 13, 0.8
