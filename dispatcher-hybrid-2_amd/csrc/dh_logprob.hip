@@ -17,7 +17,8 @@
 // exponent; the read of z bounds it. Few rows are split over several workgroups, whose sums a second launch joins. The losses
 // add one launch over the rows' lp (and one that adds their parts), which also leaves a and e. Backward: z once more, and dz;
 // m, 1 / sum and the mean exponent are all it needs of a row. A row with a = e = 0 (a clipped ratio, a pair behind the hinge)
-// is not read.
+// is not read. bytes bound both: 5994 of 8192 rows of 50257 bf16 forward 105 us (602 MB, 5.7 TB/s; a bare read reaches 6.1), backward
+// 269 (1426 MB, 5.3 TB/s; a copy 5.2); with H, 5631 rows, 112 (VALU busy for 82% of it) and 262.
 //
 // Sums over V are fp32 (a thread's over 4 pieces at a time), what follows from a row's sums is fp64, lp included until it is
 // returned: sequence sums, ratios and their comparison with the clip are of unrounded lp.
@@ -793,7 +794,7 @@ extern "C" int dh_policy_fwd(int dtype, const void* logits, int64_t stride_b, in
                  entropy_weight > -INFINITY && entropy_weight < INFINITY,
              DH_ERR_INVALID_ARG, "%s: clip %g and %g, weights %g and %g", who, clip, clip_high, kl_weight, entropy_weight);
   DH_REQUIRE(by_entropy || entropy_weight == 0.0, DH_ERR_INVALID_ARG, "%s: an entropy weight of %g, and no by_entropy", who, entropy_weight);
-  DH_REQUIRE(reference_logprob || kl_weight == 0.0, DH_ERR_INVALID_ARG, "%s: a KL weight of %g without a reference", who, kl_weight);
+  DH_REQUIRE(a.rows == 0 || reference_logprob || kl_weight == 0.0, DH_ERR_INVALID_ARG, "%s: a KL weight of %g without a reference", who, kl_weight);
   DH_REQUIRE(a.rows == 0 || (old_logprob && advantage && logprob && by_logprob && row_kept), DH_ERR_INVALID_ARG,
              "%s: null pointer argument", who);
   DH_REQUIRE(reduction ? loss && divisor : a.rows == 0 || row_loss, DH_ERR_INVALID_ARG, "%s: null pointer argument", who);

@@ -264,6 +264,14 @@ def test_tensors_of_inference_mode():
     assert torch.equal(torch.autograd.grad(loss, leaf)[0], want[-1])
 
 
+@pytest.mark.parametrize("shape", [(0, 5), (3, 0)])
+def test_a_policy_step_of_nothing_with_a_reference(shape):
+    z = torch.randn(*shape, 11, device=DEV, requires_grad=True)
+    tok, none = torch.zeros(shape, dtype=torch.long, device=DEV), torch.zeros(shape, device=DEV)
+    loss, lp = ops().policy_loss(z, tok, none, none, none, kl_weight=0.1, entropy_weight=0.1, reduction="sum")
+    assert loss == 0 and lp.shape == shape and torch.autograd.grad(loss, z)[0].shape == z.shape
+
+
 def test_constants_of_other_types():
     z, tokens, old, ref, adv, sums = data(4, 9, 501, torch.float32, 24)
     old, ref, adv, sums = (t.bfloat16().float() for t in (old, ref, adv, sums))
