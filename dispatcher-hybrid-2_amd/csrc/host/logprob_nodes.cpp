@@ -33,6 +33,25 @@ Tensor workspace(int64_t bytes, const Tensor& like) {
   if (bytes > 0) ws = at::empty({bytes}, like.options().dtype(at::kByte).requires_grad(false));
   return ws;
 }
+// What a loss keeps for its backward pass, `numbers` of them, and behind them its workspace: one allocation, as long as the latter
+// is small.
+struct Buffer {
+  Tensor kept, ws;
+  float* at = nullptr;
+  void* scratch = nullptr;
+  Buffer(int64_t numbers, int64_t bytes, const at::TensorOptions& f32) {
+    const int64_t first = (numbers + 3) / 4 * 4, more = bytes > 0 ? (bytes + 3) / 4 : 0;
+    const bool together = more <= 65536;
+    kept = at::empty({together ? first + more : numbers}, f32);
+    at = kept.data_ptr<float>();
+    if (together) {
+      scratch = at + first;
+    } else {
+      ws = at::empty({more}, f32);
+      scratch = ws.data_ptr();
+    }
+  }
+};
 void* at_(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 float* floats(const Tensor& t) { return t.defined() ? t.data_ptr<float>() : nullptr; }
 // fp32 on one stride
@@ -202,15 +221,15 @@ Loss preference(const Tensor& logits, const Tensor& tokens, const Tensor& refere
   Loss o;
   o.loss = f.reduction ? at::empty({}, f32) : at::empty({pairs}, f32);
   o.values = at::empty({2 * pairs}, f32);
-  o.kept = at::empty({preference_kept(a.n, pairs)}, f32);
-  float* kept = floats(o.kept);
   const int64_t bytes = lib.dh_preference_workspace_bytes(a.code, pairs, narrow(a.T), a.V);
-  const Tensor ws = workspace(bytes, logits);
+  const Buffer buffer(preference_kept(a.n, pairs), bytes, f32);
+  o.kept = buffer.kept;
+  float* kept = buffer.at;
   check(lib.dh_preference_fwd(a.code, a.z.data_ptr(), a.sb, a.st, pairs, narrow(a.T), a.V, a.tokens.data_ptr(), a.token_bits,
                               f.ignore_index, at_(reference), reference.defined() && reference.scalar_type() == at::kDouble ? 64 : 32,
                               narrow(f.kind), f.average, f.beta, f.margin, f.smoothing, narrow(f.reduction),
                               f.reduction ? nullptr : floats(o.loss), floats(o.values), kept + 4 * a.n, kept,
-                              f.reduction ? floats(o.loss) : nullptr, kept + 4 * a.n + 2 * pairs, at_(ws), bytes,
+                              f.reduction ? floats(o.loss) : nullptr, kept + 4 * a.n + 2 * pairs, buffer.scratch, bytes,
                               stream_of(logits)),
         what);
   return o;
@@ -247,25 +266,20 @@ struct PreferenceLoss : torch::autograd::Function<PreferenceLoss> {
     ctx->set_materialize_grads(false);
     if (logits.requires_grad()) ctx->save_for_backward({logits, savable(tokens), savable(reference), o.kept});
     ctx->mark_non_differentiable({o.values});
-    ctx->saved_data["kind"] = kind;
-    ctx->saved_data["average"] = average;
-    ctx->saved_data["beta"] = beta;
-    ctx->saved_data["margin"] = margin;
-    ctx->saved_data["smoothing"] = smoothing;
-    ctx->saved_data["ignore"] = ignore_index;
-    ctx->saved_data["reduction"] = reduction;
+    ctx->saved_data["numbers"] = std::vector<double>{beta, margin, smoothing};
+    ctx->saved_data["whole"] = std::vector<int64_t>{kind, average, ignore_index, reduction};
     return {o.loss, o.values};
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
     variable_list out(10);
     if (!grads[0].defined()) return out;
     const auto saved = ctx->get_saved_variables();
-    auto& d = ctx->saved_data;
+    const auto f = ctx->saved_data["numbers"].toDoubleVector();
+    const auto i = ctx->saved_data["whole"].toIntVector();
     out[0] = at::GradMode::is_enabled()
-                 ? by_torch(again_preference, saved[0], saved[1], maybe(saved[2]), d["kind"].toInt(), d["average"].toBool(),
-                            d["beta"].toDouble(), d["margin"].toDouble(), d["smoothing"].toDouble(), d["ignore"].toInt(),
-                            d["reduction"].toInt(), grads[0])
-                 : preference_grad(grads[0], saved[0], saved[1], saved[3], d["ignore"].toInt(), d["reduction"].toInt());
+                 ? by_torch(again_preference, saved[0], saved[1], maybe(saved[2]), i[0], i[1] != 0, f[0], f[1], f[2], i[2], i[3],
+                            grads[0])
+                 : preference_grad(grads[0], saved[0], saved[1], saved[3], i[2], i[3]);
     return out;
   }
 };
@@ -295,15 +309,15 @@ Loss policy(const Tensor& logits, const Tensor& tokens, const Tensor& old_, cons
   Loss o;
   o.loss = f.reduction ? at::empty({}, f32) : at::empty(shape, f32);
   o.values = at::empty(shape, f32);
-  o.kept = at::empty({policy_kept(a.n, f.entropy)}, f32);
-  float* kept = floats(o.kept);
   const int64_t bytes = lib.dh_policy_workspace_bytes(a.code, a.B, narrow(a.T), a.V, ent);
-  const Tensor ws = workspace(bytes, logits);
+  const Buffer buffer(policy_kept(a.n, f.entropy), bytes, f32);
+  o.kept = buffer.kept;
+  float* kept = buffer.at;
   check(lib.dh_policy_fwd(a.code, a.z.data_ptr(), a.sb, a.st, a.B, narrow(a.T), a.V, a.tokens.data_ptr(), a.token_bits,
                           f.ignore_index, f.temperature, floats(old), floats(advantages), per_sequence, floats(reference), f.clip,
                           f.clip_high, f.kl, f.entropy, narrow(f.reduction), f.reduction ? nullptr : floats(o.loss),
                           floats(o.values), kept + 4 * a.n, ent ? kept + 5 * a.n : nullptr, kept,
-                          f.reduction ? floats(o.loss) : nullptr, kept + (ent ? 6 : 5) * a.n, at_(ws), bytes, stream_of(logits)),
+                          f.reduction ? floats(o.loss) : nullptr, kept + (ent ? 6 : 5) * a.n, buffer.scratch, bytes, stream_of(logits)),
         what);
   return o;
 }
@@ -339,26 +353,20 @@ struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
     if (logits.requires_grad())
       ctx->save_for_backward({logits, savable(tokens), savable(old), savable(advantages), savable(reference), o.kept});
     ctx->mark_non_differentiable({o.values});
-    ctx->saved_data["clip"] = clip;
-    ctx->saved_data["clip_high"] = clip_high;
-    ctx->saved_data["kl"] = kl;
-    ctx->saved_data["entropy"] = entropy;
-    ctx->saved_data["temperature"] = temperature;
-    ctx->saved_data["ignore"] = ignore_index;
-    ctx->saved_data["reduction"] = reduction;
+    ctx->saved_data["numbers"] = std::vector<double>{clip, clip_high, kl, entropy, temperature};
+    ctx->saved_data["whole"] = std::vector<int64_t>{ignore_index, reduction};
     return {o.loss, o.values};
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
     variable_list out(12);
     if (!grads[0].defined()) return out;
     const auto saved = ctx->get_saved_variables();
-    auto& d = ctx->saved_data;
-    const double entropy = d["entropy"].toDouble(), temperature = d["temperature"].toDouble();
-    const int64_t ignore = d["ignore"].toInt(), reduction = d["reduction"].toInt();
+    const auto f = ctx->saved_data["numbers"].toDoubleVector();
+    const auto i = ctx->saved_data["whole"].toIntVector();
     out[0] = at::GradMode::is_enabled()
-                 ? by_torch(again_policy, saved[0], saved[1], saved[2], saved[3], maybe(saved[4]), d["clip"].toDouble(),
-                            d["clip_high"].toDouble(), d["kl"].toDouble(), entropy, temperature, ignore, reduction, grads[0])
-                 : policy_grad(grads[0], saved[0], saved[1], saved[5], entropy, temperature, ignore, reduction);
+                 ? by_torch(again_policy, saved[0], saved[1], saved[2], saved[3], maybe(saved[4]), f[0], f[1], f[2], f[3], f[4], i[0],
+                            i[1], grads[0])
+                 : policy_grad(grads[0], saved[0], saved[1], saved[5], f[3], f[4], i[0], i[1]);
     return out;
   }
 };

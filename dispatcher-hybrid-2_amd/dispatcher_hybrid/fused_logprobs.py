@@ -163,7 +163,10 @@ def head_logprobs(hidden, weight, tokens, temperature=1.0, ignore_index=-100, en
 @torch.library.custom_op("dispatcher::preference_loss", mutates_args=(), device_types="cuda")
 def _preference_op(logits: torch.Tensor, tokens: torch.Tensor, reference: Optional[torch.Tensor], kind: int, average: bool,
                    beta: float, margin: float, label_smoothing: float, ignore_index: int, reduction: int) -> List[torch.Tensor]:
-    return list(_native.preference(logits, tokens, reference, kind, average, beta, margin, label_smoothing, ignore_index, reduction))
+    loss, sums, kept = _native.preference(logits, tokens, reference, kind, average, beta, margin, label_smoothing, ignore_index,
+                                          reduction)
+    n, T = logits.shape[0], logits.shape[1]
+    return [loss, sums, kept[:4 * n * T + 2 * (n // 2) + 1].clone()]           # (a size that its fake form can say)
 
 
 @_preference_op.register_fake
@@ -236,8 +239,9 @@ def preference_loss(logits, tokens, reference=None, beta=0.1, loss="sigmoid", av
 def _policy_op(logits: torch.Tensor, tokens: torch.Tensor, old_logprobs: torch.Tensor, advantages: torch.Tensor,
                reference_logprobs: Optional[torch.Tensor], clip: float, clip_high: float, kl_weight: float,
                entropy_weight: float, temperature: float, ignore_index: int, reduction: int) -> List[torch.Tensor]:
-    return list(_native.policy(logits, tokens, old_logprobs, advantages, reference_logprobs, clip, clip_high, kl_weight,
-                               entropy_weight, temperature, ignore_index, reduction))
+    loss, scores, kept = _native.policy(logits, tokens, old_logprobs, advantages, reference_logprobs, clip, clip_high, kl_weight,
+                                        entropy_weight, temperature, ignore_index, reduction)
+    return [loss, scores, kept[:(6 if entropy_weight != 0.0 else 5) * _count(logits.shape[:-1]) + 1].clone()]
 
 
 @_policy_op.register_fake
