@@ -190,13 +190,15 @@ __global__ __launch_bounds__(256) void join_kernel(Args a, int slots_a_part, int
   constexpr int kAhead = 4;
   const int lane = threadIdx.x & 63;
   const int i = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int live = a.plan ? a.plan->live : a.rows;
-  if (i >= live) return;
-  const int slots = a.plan ? a.plan->parts * slots_a_part : slots_if_all;
+  if (i >= a.rows) return;
+  // (asked for at once; behind the last live row there is anything)
+  const int live = a.plan ? a.plan->live : a.rows, slots = a.plan ? a.plan->parts * slots_a_part : slots_if_all;
   const int r = row_at(a, i);
+  const float z = a.zy[i];
+  if (i >= live) return;
   const int64_t y = whole(a.tokens, a.wide, r);
   const bool bad = y < 0 || y >= a.V;
-  const float zy = bad ? 0.f : a.zy[i];
+  const float zy = bad ? 0.f : z;
   const State* part = a.part + (int64_t)i * slots;
   State v{-INFINITY, 0.f, 0.f};
   for (int k = lane; k < slots; k += 64 * kAhead) {
@@ -681,24 +683,32 @@ struct Timed {
 constexpr Timed kBf16[] = {{{1, 256, 256, 256, 2, 0}, 25.f}, {{1, 128, 256, 256, 2, 1}, 13.6f}, {{1, 64, 256, 256, 2, 2}, 8.7f},
                            {{1, 64, 64, 512, 2, 3}, 5.9f}};
 constexpr Form kFp32 = {1, 32, 128, 512, 2, 0};
-// up to 32 rows (as many as LDS holds beside the rings) the form for few: 16 rows 23 us, the 64 x 256 tiles 32; fp32 38 and 51
-Form form_of(int dtype, int64_t rows, int d, int V, bool fast) {
-  if (!fast) return dtype == DH_F32 && rows <= 512 ? Form{0, 64, 64, 1024, 2, 0} : Form{0, 128, 128, 512, 2, 1};
-  if (rows <= 32 && (rows <= 16 ? 16 : 32) * (int64_t)d * (dtype == DH_BF16 ? 2 : 4) <= kFewLds)
-    return Form{2, 0, 0, kFewGroups, 1, 0};
-  if (dtype == DH_F32) return kFp32;
+// Staged through registers, the same rule. V 50257, d 1001, us by rows, 64 x 64 / 128 x 128 tiles: bf16 1 36 / 42; 64 45 / 46; 128 68 /
+// 44; 4096 1105 / 651; fp32 64 102 / 151; 128 179 / 153; 1024 1071 / 980. V 5000, d 777: bf16 512 30 / 34; fp32 512 84 / 123.
+constexpr Timed kStagedBf16[] = {{{0, 64, 64, 1024, 2, 0}, 22.f}, {{0, 128, 128, 512, 2, 1}, 26.f}};
+constexpr Timed kStagedFp32[] = {{{0, 64, 64, 1024, 2, 0}, 82.f}, {{0, 128, 128, 512, 2, 1}, 140.f}};
+
+template <int N>
+Form least(const Timed (&forms)[N], int64_t rows, int V) {
   int best = 0;
-  double least = 1e30;
-  for (int i = 0; i < 4; ++i) {
-    const Form& f = kBf16[i].form;
+  double us = 1e30;
+  for (int i = 0; i < N; ++i) {
+    const Form& f = forms[i].form;
     const int64_t tiles = ((rows + f.bm - 1) / f.bm) * ((V + f.bn - 1) / f.bn);
-    const double us = (double)((tiles + f.groups - 1) / f.groups) * kBf16[i].us;
-    if (us < least) {
-      least = us;
+    const double takes = (double)((tiles + f.groups - 1) / f.groups) * forms[i].us;
+    if (takes < us) {
+      us = takes;
       best = i;
     }
   }
-  return kBf16[best].form;
+  return forms[best].form;
+}
+// up to 32 rows (as many as LDS holds beside the rings) the form for few: 16 rows 22 us, the 64 x 256 tiles 31; fp32 36 and 51
+Form form_of(int dtype, int64_t rows, int d, int V, bool fast) {
+  if (!fast) return dtype == DH_F32 ? least(kStagedFp32, rows, V) : least(kStagedBf16, rows, V);
+  if (rows <= 32 && (rows <= 16 ? 16 : 32) * (int64_t)d * (dtype == DH_BF16 ? 2 : 4) <= kFewLds)
+    return Form{2, 0, 0, kFewGroups, 1, 0};
+  return dtype == DH_F32 ? kFp32 : least(kBf16, rows, V);
 }
 struct Layout {
   int64_t index, part, zy, bytes;

@@ -703,7 +703,7 @@ int dh_policy_fwd(int dtype, const void* logits, int64_t stride_b, int64_t strid
  * the logits in memory: z = hidden . weight^T in fp32 sums (round_logits: rounded to bf16 then, as a bf16 head stores them), and
  * the rest as in dh_logprob_fwd. Rows whose token is ignore_index are not computed, but where there are few rows.
  *   hidden (rows, d) of row stride hidden_stride, weight (V, d) of row stride weight_stride, both of dtype and of unit stride inside
- *   a row; any d, alignment and (not negative) strides, the fast kernels at d a multiple of 64 and 16-byte aligned rows of bf16.
+ *   a row; any d, alignment and (not negative) strides, the fast kernels at d a multiple of 64 (fp32: 32) and 16-byte aligned rows.
  *   workspace: dh_head_logprob_workspace_bytes(dtype, rows, V) bytes, 16-byte aligned, needed during the call only.
  *   rows < 2^22, d <= 2^20, V <= 2^24, 2^-126 <= tau <= 2^126.
  */
