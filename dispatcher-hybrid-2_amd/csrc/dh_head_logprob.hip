@@ -11,7 +11,7 @@
 // TFLOP/s of products, on the matrix cores in 66% of the cycles), 16 rows 22 (the weight at 5.5 TB/s, and the join).
 //
 // Launches: the rows that count, in their order, and how the tiles are dealt out (compact_kernel; their number is known on the
-// device only); the product; the join. Up to 32 rows: the product (few_kernel, the weight's bytes bound it) and the join.
+// device only; up to 1024 rows the product's workgroups do this themselves); the product; the join. Up to 32 rows: the product (few_kernel, the weight's bytes bound it) and the join.
 
 #include "dh_rows.h"
 
@@ -75,8 +75,9 @@ struct Args {
   int round;                               // bf16 logits
   float c;                                 // log2(e) / tau
   double inv_tau;
-  const Plan* plan;
-  const int* index;                        // the live rows; null: all
+  int self;                                // few enough rows for every workgroup of the product to sort them out itself
+  Plan* plan;
+  int* index;                              // the live rows; null: all
   State* part;                             // [compact row][slots]
   float* zy;                               // [compact row]
   float *lp, *ent;
@@ -89,60 +90,16 @@ constexpr int kCT = 1024;
 // rows a workgroup: one a thread, more where the workgroups' reads of all rows before their own would add up
 int chunk_of(int64_t rows) { return kCT * (int)(rows <= 32768 ? 1 : rows <= (1 << 20) ? rows / 32768 : 32); }
 
-// A workgroup counts the live rows before its own and places those of its chunk. The last one deals out the tiles: the number of parts
-// whose longest workgroup is shortest.
-__global__ __launch_bounds__(kCT) void compact_kernel(Args a, int bm, int groups, int chunk, int* index, Plan* plan) {
-  __shared__ int red[kCT / 64], base, total;
-  __shared__ int64_t best[kCT / 64];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int lo = blockIdx.x * chunk, hi = min(lo + chunk, a.rows);
-  auto live = [&](int r) { return whole(a.tokens, a.wide, r) != a.ignore; };
-  int before = 0;
-#pragma unroll 8
-  for (int r = tid; r < lo; r += kCT) before += live(r);
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) before += __shfl_xor(before, o);
-  if (lane == 0) red[wave] = before;
-  __syncthreads();
-  if (tid == 0) {
-    int n = 0;
-    for (int w = 0; w < kCT / 64; ++w) n += red[w];
-    base = n;
-  }
-  __syncthreads();
-  int at = base;
-  for (int r0 = lo; r0 < hi; r0 += kCT) {  // uniform
-    const int r = r0 + tid;
-    const bool in = r < hi, on = in && live(r);
-    const uint64_t mask = __builtin_amdgcn_ballot_w64(on);
-    __syncthreads();
-    if (lane == 0) red[wave] = __popcll(mask);
-    __syncthreads();
-    int place = at + __popcll(mask & ((1ull << lane) - 1)), all = 0;
-    for (int w = 0; w < kCT / 64; ++w) {
-      if (w < wave) place += red[w];
-      all += red[w];
-    }
-    if (on) index[place] = r;
-    if (in && !on) {
-      a.lp[r] = 0.f;
-      if (a.ent) a.ent[r] = 0.f;
-    }
-    at += all;
-  }
-  if ((int)blockIdx.x != (int)gridDim.x - 1) return;
-  if (tid == 0) total = at;
-  __syncthreads();
-  const int n = total, mt = (n + bm - 1) / bm;
-  if (mt == 0) {
-    if (tid == 0) *plan = Plan{0, 0, 1, a.nt};
-    return;
-  }
-  // rounds of the workgroups times the tiles of a part (and half a tile that beginning and ending one takes)
+// How n live rows' tiles are dealt out, by a workgroup of N threads: the number of parts whose longest workgroup is shortest, rounds of
+// the workgroups times the tiles of a part (and half a tile that beginning and ending one takes).
+template <int N>
+__device__ __forceinline__ Plan deal(int n, int nt, int bm, int groups, int64_t (&best)[N / 64]) {
+  const int tid = threadIdx.x, mt = (n + bm - 1) / bm;
+  if (mt == 0) return Plan{0, 0, 1, nt};   // uniform
   int64_t mine = INT64_MAX;
-  const int most = max(1, min(a.nt, 2 * groups / mt));         // (mt p and the cost: at most some 2^27)
-  for (int p = tid + 1; p <= most; p += kCT) {
-    const uint32_t per = (uint32_t)(a.nt + p - 1) / (uint32_t)p, rounds = (uint32_t)(mt * p + groups - 1) / (uint32_t)groups;
+  const int most = max(1, min(nt, 2 * groups / mt));           // (mt p and the cost: at most some 2^27)
+  for (int p = tid + 1; p <= most; p += N) {
+    const uint32_t per = (uint32_t)(nt + p - 1) / (uint32_t)p, rounds = (uint32_t)(mt * p + groups - 1) / (uint32_t)groups;
     mine = min(mine, (int64_t)(rounds * (2 * per + 1)) << 20 | p);
   }
 #pragma unroll
@@ -150,13 +107,79 @@ __global__ __launch_bounds__(kCT) void compact_kernel(Args a, int bm, int groups
     const int64_t other = __shfl_xor(mine, o);
     mine = min(mine, other);
   }
-  if (lane == 0) best[wave] = mine;
+  if ((tid & 63) == 0) best[tid >> 6] = mine;
   __syncthreads();
-  if (tid == 0) {
-    for (int w = 1; w < kCT / 64; ++w) mine = min(mine, best[w]);
-    const int p = (int)(mine & 0xfffff), per = (a.nt + p - 1) / p;
-    *plan = Plan{n, mt, (a.nt + per - 1) / per, per};
+  mine = best[0];
+  for (int w = 1; w < N / 64; ++w) mine = min(mine, best[w]);
+  const int p = __builtin_amdgcn_readfirstlane((int)(mine & 0xfffff)), per = (nt + p - 1) / p;
+  return Plan{n, mt, (nt + per - 1) / per, per};
+}
+__device__ __forceinline__ bool counts(const Args& a, int r) { return whole(a.tokens, a.wide, r) != a.ignore; }
+__device__ __forceinline__ void skip_row(const Args& a, int r) {
+  a.lp[r] = 0.f;
+  if (a.ent) a.ent[r] = 0.f;
+}
+// the live rows of [lo, hi), in their order, to list[at ...]; returns at and their number. write: whether the others' results are
+template <int N, typename I>
+__device__ __forceinline__ int sort_out(const Args& a, int lo, int hi, int at, I* list, bool write, int (&red)[N / 64]) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  for (int r0 = lo; r0 < hi; r0 += N) {    // uniform
+    const int r = r0 + tid;
+    const bool in = r < hi, on = in && counts(a, r);
+    const uint64_t mask = __builtin_amdgcn_ballot_w64(on);
+    __syncthreads();
+    if (lane == 0) red[wave] = __popcll(mask);
+    __syncthreads();
+    int place = at + __popcll(mask & ((1ull << lane) - 1)), all = 0;
+    for (int w = 0; w < N / 64; ++w) {
+      if (w < wave) place += red[w];
+      all += red[w];
+    }
+    if (on) list[place] = (I)r;
+    if (write && in && !on) skip_row(a, r);
+    at += __builtin_amdgcn_readfirstlane(all);
   }
+  return at;
+}
+
+// A workgroup counts the live rows before its own and places those of its chunk. The last one deals out the tiles.
+__global__ __launch_bounds__(kCT) void compact_kernel(Args a, int bm, int groups, int chunk) {
+  __shared__ int red[kCT / 64];
+  __shared__ int64_t best[kCT / 64];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int lo = blockIdx.x * chunk, hi = min(lo + chunk, a.rows);
+  int before = 0;
+#pragma unroll 8
+  for (int r = tid; r < lo; r += kCT) before += counts(a, r);
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) before += __shfl_xor(before, o);
+  if (lane == 0) red[wave] = before;
+  __syncthreads();
+  int base = 0;
+  for (int w = 0; w < kCT / 64; ++w) base += red[w];
+  const int n = sort_out<kCT>(a, lo, hi, __builtin_amdgcn_readfirstlane(base), a.index, true, red);
+  if ((int)blockIdx.x != (int)gridDim.x - 1) return;
+  const Plan q = deal<kCT>(n, a.nt, bm, groups, best);
+  if (tid == 0) *a.plan = q;
+}
+
+// What a workgroup of the product begins with: the plan, and where its rows are listed. Up to kSelf rows every one sorts them out
+// itself, which takes less than the launch before it would (5 us of 33 for 128 rows), and the first leaves plan and list for the join.
+constexpr int kSelf = 1024;
+typedef uint16_t listed;                   // (2 KB of LDS: four 64 x 64 staged workgroups on a CU, three with 4 KB)
+template <int N>
+__device__ __forceinline__ Plan begin(const Args& a, int bm, listed* list, int (&red)[N / 64], int64_t (&best)[N / 64]) {
+  if (!a.self) return *a.plan;
+  const bool first = blockIdx.x == 0;
+  const int n = sort_out<N>(a, 0, a.rows, 0, list, first, red);
+  const Plan q = deal<N>(n, a.nt, bm, gridDim.x, best);
+  __syncthreads();
+  if (first) {
+    for (int i = threadIdx.x; i < n; i += N) a.index[i] = list[i];
+    if (threadIdx.x == 0) *a.plan = q;
+    __builtin_amdgcn_s_waitcnt((7 << 4) | (15 << 8));          // s_waitcnt vmcnt(0): what follows counts its own loads
+  }
+  return q;
 }
 
 // Item i of the tiles dealt out: row tile m, part p. Row tiles in groups of eight, a group's parts one after another, its row tiles
@@ -169,9 +192,9 @@ __device__ __forceinline__ void item_at(const Plan& q, int i, int& m, int& p) {
 // item of a workgroup in a round: XCD id % 8 takes a contiguous eighth
 __device__ __forceinline__ int item_of(int id, int groups) { return (id & 7) * (groups >> 3) + (id >> 3); }
 
-// the token of a compact row as a column, -1: none
-__device__ __forceinline__ int token_at(const Args& a, int row, int live) {
-  const int64_t k = row < live ? whole(a.tokens, a.wide, row_at(a, row)) : -1;
+// the token of a row as a column, -1: none
+__device__ __forceinline__ int column_of(const Args& a, int r) {
+  const int64_t k = whole(a.tokens, a.wide, r);
   return k >= 0 && k < a.V ? (int)k : -1;
 }
 
@@ -340,9 +363,13 @@ __global__ __launch_bounds__(256) void staged_kernel(Args a) {
   __shared__ __align__(16) unsigned char sw[2][BN * kRS], sx[2][BM * kRS];
   __shared__ int sy[BM];
   __shared__ float sz[BM];
+  __shared__ listed list[kSelf];
+  __shared__ int red[4];
+  __shared__ int64_t best[4];
   const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave & 1, wn = wave >> 1;
-  const Plan q = *a.plan;
+  const Plan q = begin<256>(a, BM, list, red, best);
+  auto live_row = [&](int i) { return a.self ? (int)list[i] : a.index[i]; };
   const int nk = (a.K + 8 * E - 1) / (8 * E), kc = (tid & 7) * E;
   for (int item = item_of(blockIdx.x, gridDim.x); item < q.mt * q.parts; item += gridDim.x) {
     int mt, part;
@@ -351,12 +378,12 @@ __global__ __launch_bounds__(256) void staged_kernel(Args a) {
     const T* xp[TM];
 #pragma unroll
     for (int i = 0; i < TM; ++i)
-      xp[i] = (const T*)a.h + (int64_t)row_at(a, min(m0 + (tid >> 3) + 32 * i, q.live - 1)) * a.ldh;
+      xp[i] = (const T*)a.h + (int64_t)live_row(min(m0 + (tid >> 3) + 32 * i, q.live - 1)) * a.ldh;
     State st[TM];
 #pragma unroll
     for (int i = 0; i < TM; ++i) st[i] = State{-INFINITY, 0.f, 0.f};
     __syncthreads();                       // the item before has read its tokens
-    if (tid < BM) sy[tid] = token_at(a, m0 + tid, q.live);
+    if (tid < BM) sy[tid] = m0 + tid < q.live ? column_of(a, live_row(m0 + tid)) : -1;
     const int n_end = min((part + 1) * q.per, a.nt);
     for (int nt = part * q.per; nt < n_end; ++nt) {
       const int n0 = nt * BN;
@@ -447,9 +474,13 @@ __global__ __launch_bounds__(64 * WGM * WGN) void dma_kernel(Args a) {
   __shared__ __align__(1024) unsigned char sw[S][BN * kRowBytes], sx[S][BM * kRowBytes];
   __shared__ int sy[BM];
   __shared__ float sz[BM];
+  __shared__ listed list[kSelf];
+  __shared__ int red[NW];
+  __shared__ int64_t best[NW];
   const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave % WGM, wn = wave / WGM;
-  const Plan q = *a.plan;
+  const Plan q = begin<64 * NW>(a, BM, list, red, best);
+  auto live_row = [&](int i) { return a.self ? (int)list[i] : a.index[i]; };
   const int nk = a.K / (8 * E);
   const int fw = (wn * 16 * TN + r) * kRowBytes, fx = (wm * 16 * TM + r) * kRowBytes;
   const int c0 = (g ^ (r & 7)) << 4, c1 = ((4 + g) ^ (r & 7)) << 4;
@@ -471,7 +502,7 @@ __global__ __launch_bounds__(64 * WGM * WGN) void dma_kernel(Args a) {
 #pragma unroll
     for (int u = 0; u < GX; ++u) {
       const int R = 8 * (NW * u + wave) + (lane >> 3);
-      xo[u] = ((uint32_t)row_at(a, min(m0 + R, q.live - 1)) * (uint32_t)a.ldh + (uint32_t)(((lane & 7) ^ (R & 7)) * E)) * (uint32_t)sizeof(T);
+      xo[u] = ((uint32_t)live_row(min(m0 + R, q.live - 1)) * (uint32_t)a.ldh + (uint32_t)(((lane & 7) ^ (R & 7)) * E)) * (uint32_t)sizeof(T);
     }
     int next_n = n_first, next_k = 0;      // what is loaded next
     const char* wbase = nullptr;
@@ -508,7 +539,7 @@ __global__ __launch_bounds__(64 * WGM * WGN) void dma_kernel(Args a) {
     for (int i = 0; i < TM; ++i) sums[i] = State{-INFINITY, 0.f, 0.f};
     columns();
     __syncthreads();                       // the item before has been read
-    if (tid < BM) sy[tid] = token_at(a, m0 + tid, q.live);
+    if (tid < BM) sy[tid] = m0 + tid < q.live ? column_of(a, live_row(m0 + tid)) : -1;
 #pragma unroll
     for (int u = 0; u < S - 1; ++u) issue(u);
     wait_vm<(S - 2) * PER>();              // loads return in their order
@@ -617,7 +648,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_kernel(Args a) {
   else
     wait_vm<0>();
   __builtin_amdgcn_sched_barrier(0);
-  if (tid < BM) sy[tid] = token_at(a, tid, a.rows);
+  if (tid < BM) sy[tid] = tid < a.rows ? column_of(a, tid) : -1;
   __syncthreads();
   int t = 0, place = 0;
   for (int at = first; at < end; ++at) {
@@ -759,10 +790,12 @@ int run(Args& a, const Form& t, char* ws, const Layout& l, hipStream_t s, const 
   a.nt = (a.V + t.bn - 1) / t.bn;
   a.plan = (Plan*)ws;
   a.index = (int*)(ws + l.index);
-  const int chunk = chunk_of(a.rows);
-  compact_kernel<<<dim3((unsigned)((a.rows + chunk - 1) / chunk)), dim3(kCT), 0, s>>>(a, t.bm, t.groups, chunk, (int*)(ws + l.index),
-                                                                                     (Plan*)ws);
-  if (int st = dh_check_launch(who)) return st;
+  a.self = a.rows <= kSelf;
+  if (!a.self) {
+    const int chunk = chunk_of(a.rows);
+    compact_kernel<<<dim3((unsigned)((a.rows + chunk - 1) / chunk)), dim3(kCT), 0, s>>>(a, t.bm, t.groups, chunk);
+    if (int st = dh_check_launch(who)) return st;
+  }
   const dim3 grid((unsigned)t.groups);
   if (t.kind == 1) {
     if (sizeof(T) == 4) {
