@@ -11,7 +11,8 @@
 // TFLOP/s of products, on the matrix cores in 66% of the cycles), 16 rows 22 (the weight at 5.5 TB/s, and the join).
 //
 // Launches: the rows that count, in their order, and how the tiles are dealt out (compact_kernel; their number is known on the
-// device only; up to 1024 rows the product's workgroups do this themselves); the product; the join. Up to 32 rows: the product (few_kernel, the weight's bytes bound it) and the join.
+// device only; up to 1024 rows the product's workgroups do this themselves); the product; the join. Up to 32 rows: the product
+// (few_kernel, the weight's bytes bound it) and the join.
 
 #include "dh_rows.h"
 
@@ -164,7 +165,7 @@ __global__ __launch_bounds__(kCT) void compact_kernel(Args a, int bm, int groups
 }
 
 // What a workgroup of the product begins with: the plan, and where its rows are listed. Up to kSelf rows every one sorts them out
-// itself, which takes less than the launch before it would (5 us of 33 for 128 rows), and the first leaves plan and list for the join.
+// itself, which takes less than a launch before it (128 rows 31.6 us with that, 29.0 so), and the first leaves plan and list for the join.
 constexpr int kSelf = 1024;
 typedef uint16_t listed;                   // (2 KB of LDS: four 64 x 64 staged workgroups on a CU, three with 4 KB)
 template <int N>
@@ -702,11 +703,11 @@ struct Form {
   int kind, bm, bn, groups, slots, id;
 };
 // The forms of the DMA kernel, and what a tile of each takes at K = 1024, microseconds on a full card: the form whose rounds of tiles
-// take least. bf16, V 50257, d 1024, us of a call by rows, 256 x 256 / 128 x 256 / 64 x 256 / 64 x 64: 64 42 / 32 / 31 / 33; 128 41 / 33
-// / 32 / 39; 256 41 / 42 / 48 / 59; 512 64 / 71 / 82 / 94; 640 88 / 70 / 87 / 111; 1024 112 / 109 / 130 / 163; 5300 441 / 464 / 570 / 766.
+// take least. bf16, V 50257, d 1024, us of a call by rows, 256 x 256 / 128 x 256 / 64 x 256 / 64 x 64: 64 38 / 29 / 28 / 30; 128 38 / 31
+// / 29 / 35; 256 39 / 39 / 46 / 52; 512 63 / 66 / 78 / 93; 640 86 / 67 / 84 / 109; 1024 110 / 111 / 125 / 159; 5300 440 / 460 / 571 / 751.
 // (A few large tiles leave most of the card idle: 2000 rows of V 1000 are 32 of 256 x 256.) fp32 is bound by its products whatever the
 // tile, and 32 x 128 tiles have the fewest empty rows: us at 200, 329, 501, 4096 rows 205, 292, 413, 3090; 64 x 64 236, 321, 412, 3055;
-// 128 x 128 255, 372, 491, 2995.
+// 128 x 128 255, 372, 491, 2995 (all with a launch that sorted the rows out, 5 us).
 struct Timed {
   Form form;
   float us;
@@ -714,8 +715,8 @@ struct Timed {
 constexpr Timed kBf16[] = {{{1, 256, 256, 256, 2, 0}, 25.f}, {{1, 128, 256, 256, 2, 1}, 13.6f}, {{1, 64, 256, 256, 2, 2}, 8.7f},
                            {{1, 64, 64, 512, 2, 3}, 5.9f}};
 constexpr Form kFp32 = {1, 32, 128, 512, 2, 0};
-// Staged through registers, the same rule. V 50257, d 1001, us by rows, 64 x 64 / 128 x 128 tiles: bf16 1 36 / 42; 64 45 / 46; 128 68 /
-// 44; 4096 1105 / 651; fp32 64 102 / 151; 128 179 / 153; 1024 1071 / 980. V 5000, d 777: bf16 512 30 / 34; fp32 512 84 / 123.
+// Staged through registers, the same rule. V 50257, d 1001, us by rows, 64 x 64 / 128 x 128 tiles: bf16 1 33 / 39; 64 41 / 42; 128 62 /
+// 41; 4096 1083 / 648; fp32 64 97 / 150; 128 174 / 149; 1024 1062 / 977. V 5000, d 777: bf16 512 27 / 30; fp32 512 78 / 125.
 constexpr Timed kStagedBf16[] = {{{0, 64, 64, 1024, 2, 0}, 22.f}, {{0, 128, 128, 512, 2, 1}, 26.f}};
 constexpr Timed kStagedFp32[] = {{{0, 64, 64, 1024, 2, 0}, 82.f}, {{0, 128, 128, 512, 2, 1}, 140.f}};
 
@@ -734,7 +735,8 @@ Form least(const Timed (&forms)[N], int64_t rows, int V) {
   }
   return forms[best].form;
 }
-// up to 32 rows (as many as LDS holds beside the rings) the form for few: 16 rows 22 us, the 64 x 256 tiles 31; fp32 36 and 51
+// up to 32 rows (as many as LDS holds beside the rings) the form for few: 16 rows 21 us, the 64 x 256 tiles 27; fp32 36 us,
+// its tiles 51 (5 of these the launch that sorted the rows out)
 Form form_of(int dtype, int64_t rows, int d, int V, bool fast) {
   if (!fast) return dtype == DH_F32 ? least(kStagedFp32, rows, V) : least(kStagedBf16, rows, V);
   if (rows <= 32 && (rows <= 16 ? 16 : 32) * (int64_t)d * (dtype == DH_BF16 ? 2 : 4) <= kFewLds)
