@@ -517,6 +517,8 @@ class DispatcherHybridForCausalLM(DispatcherPreTrainedModel, GenerationMixin):
             raise ValueError("one of teacher_logits, preference and policy: they are losses of their own")
         if (preference is not None or policy is not None) and labels is None:
             raise ValueError("preference and policy losses need labels")
+        if any(args.get("ignore_index", -100) != -100 for args in (preference, policy) if args is not None):
+            raise ValueError("labels are ignored where they are -100; a preference or policy loss takes no other ignore_index")
         x, hidden_states = self._trunk(input_ids, output_hidden_states)
         logits = self.lm_head(x)
         loss = scores = None

@@ -317,3 +317,16 @@ def test_model_scores_and_trains_on_the_cpu():
     for call in (lambda: m(ids, labels=labels, preference={}), lambda: m(ids, labels=labels, policy=policy), lambda: m.token_logprobs(ids)):
         with pytest.raises(RuntimeError, match="CPU"):
             call()
+
+
+@pytest.mark.parametrize("name", ["preference", "policy"])
+def test_model_losses_ignore_what_labels_ignore(name):
+    """(the last position has no next token: with another ignore_index it would count as a token outside the vocabulary)"""
+    cfgd, sd = tiny("tiny_a")
+    m = product_model(cfgd, sd)
+    ids = torch.randint(0, 255, (2, 8), generator=torch.Generator().manual_seed(2))
+    args = dict(old_logprobs=torch.zeros(2, 8), advantages=torch.ones(2)) if name == "policy" else {}
+    with pytest.raises(ValueError, match="-100"):
+        m(ids, labels=ids, **{name: dict(args, ignore_index=0)})
+    out = m(ids, labels=ids, **{name: dict(args, ignore_index=IGNORE)})
+    assert bool(out.loss.isfinite())
