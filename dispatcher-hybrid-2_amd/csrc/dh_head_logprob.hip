@@ -460,9 +460,10 @@ __device__ __forceinline__ void wait_vm() {  // s_waitcnt vmcnt(N), other counte
 
 // Operands through LDS by the DMA path, S stages (S - 1 K tiles on their way while one is multiplied); the fragments of a K tile's
 // two halves in two register sets, one read while the other is multiplied. Reads and loads stand between the products: in a burst
-// behind the barrier they hold both waves of a SIMD up (5631 rows, 256 x 256 tiles: 506 us in bursts, 478 so). The K tiles of a workgroup's column tiles follow each
-// other without a pause: the next column tile's first are on their way while the sums of the last take its accumulators. Slot p of
-// LDS row R holds the row's chunk p ^ (R & 7), which makes the fragment reads free of bank conflicts.
+// behind the barrier they hold both waves of a SIMD up (5631 rows, 256 x 256 tiles: 506 us in bursts, 478 so). The K tiles of a
+// workgroup's column tiles follow each other without a pause: the next column tile's first are on their way while the sums of the
+// last take its accumulators. Slot p of LDS row R holds the row's chunk p ^ (R & 7), which makes the fragment reads free of bank
+// conflicts.
 template <typename T, bool ENT, int TM, int TN, int WGM, int WGN, int S>
 __global__ __launch_bounds__(64 * WGM * WGN) void dma_kernel(Args a) {
   constexpr int NW = WGM * WGN, BM = 16 * TM * WGM, BN = 16 * TN * WGN, GX = BM / 8 / NW, GW = BN / 8 / NW;
