@@ -14,7 +14,7 @@
 //                       over the rows, their number, or each sequence's number and the number of sequences
 //
 // Forward: one pass over the row with the running maximum m and the sums of E = exp((z - m) / tau) and, for H, of E times its
-// exponent; the read of z bounds it. Few rows are split over several workgroups, whose sums a second launch joins. The losses
+// exponent; the read of z bounds it. Few long rows are split over several workgroups, whose sums a second launch joins. The losses
 // add one launch over the rows' lp (and one that adds their parts), which also leaves a and e. Backward: z once more, and dz;
 // m, 1 / sum and the mean exponent are all it needs of a row. A row with a = e = 0 (a clipped ratio, a pair behind the hinge)
 // is not read. bytes bound both: 5994 of 8192 rows of 50257 bf16 forward 105 us (602 MB, 5.7 TB/s; a bare read reaches 6.1), backward
@@ -555,19 +555,27 @@ __global__ __launch_bounds__(kThreads<N>) void backward_kernel(Rows a, int parts
 
 // ---- sizes ------------------------------------------------------------------------------------------------------------
 // workgroups a row: enough for 1024 in all, each with at least two pieces a thread
+int64_t row_bytes(int V, int dtype) { return (int64_t)V * (dtype == DH_BF16 ? 2 : 4); }
 int parts_of(int64_t rows, int V, int dtype) {
-  const int64_t pieces = ((int64_t)V * (dtype == DH_BF16 ? 2 : 4) + 15) / 16;
   int64_t p = 1024 / (rows > 0 ? rows : 1);
-  const int64_t most = pieces / (2 * kT);
+  const int64_t most = (row_bytes(V, dtype) + 15) / 16 / (2 * kT);
   if (p > most) p = most;
   if (p > kMaxParts) p = kMaxParts;
   return p < 1 ? 1 : (int)p;
+}
+// ... of the forward pass, where split rows cost a launch that joins them: few and long ones are split. us, whole / split: bf16 with
+// entropies, V 8192 1 row 4.7 / 6.6, 512 rows 7.2 / 10.3; V 50257 1 row 7.7 / 7.3 (and less of the host's time), 16 8.6 / 8.3, 64 9.4 /
+// 10.0, 256 11.1 / 14.6; V 80000 16 12.2 / 8.9, 128 13.4 / 13.1, 256 15.6 / 17.5; V 151936 64 17.3 / 12.7, 128 18.3 / 17.4, 256 24.1 /
+// 27.8. fp32, V 50257 64 12.8 / 12.1, 128 13.2 / 14.3.
+constexpr int64_t kWhole = 112 << 10;
+int forward_parts(int64_t rows, int V, int dtype) {
+  return rows >= 256 || row_bytes(V, dtype) <= kWhole * (rows < 64 ? 1 : rows / 64) ? 1 : parts_of(rows, V, dtype);
 }
 // A wave a row: rows of up to this many bytes, as many as fill the card so. us with a wave and with a workgroup a row, 16384 rows of
 // bf16: V 6000 forward 42 and 58, backward 82 and 98; 8000 51 and 64, 114 and 110; 12000 74 and 95, 169 and 147; 16000 93 and 105, 224
 // and 206. fp32, V 4000 49 and 63, 112 and 134; 8000 91 and 100, 222 and 212.
 constexpr int kWaveForward = 32768, kWaveBackward = 16384;
-bool by_waves(int64_t rows, int V, int dtype, int bytes) { return (int64_t)V * (dtype == DH_BF16 ? 2 : 4) <= bytes && rows >= 1024; }
+bool by_waves(int64_t rows, int V, int dtype, int bytes) { return row_bytes(V, dtype) <= bytes && rows >= 1024; }
 
 int check(const char* who, int dtype, const Rows& a, int token_bits, double tau) {
   DH_REQUIRE(dtype == DH_F32 || dtype == DH_BF16, DH_ERR_UNSUPPORTED_DTYPE, "%s: dtype %d", who, dtype);
@@ -606,7 +614,7 @@ int forward(const char* who, int dtype, const Rows& a, const Results& o, void* w
     forward_kernel<T, ENT, 64><<<dim3((unsigned)((a.rows + kW - 1) / kW)), dim3(kT), 0, s>>>(a, 1, nullptr, o);
     return dh_check_launch(who);
   }
-  const int parts = parts_of(a.rows, a.V, dtype);
+  const int parts = forward_parts(a.rows, a.V, dtype);
   if (parts == 1) {
     forward_kernel<T, ENT, kWide><<<dim3((unsigned)a.rows), dim3(kWide), 0, s>>>(a, 1, nullptr, o);
     return dh_check_launch(who);
@@ -623,11 +631,11 @@ int forward(const char* who, int dtype, const Rows& a, bool ent, const Results& 
     return ent ? forward<bf16_t, true>(who, dtype, a, o, ws, joined, s) : forward<bf16_t, false>(who, dtype, a, o, ws, joined, s);
   return ent ? forward<float, true>(who, dtype, a, o, ws, joined, s) : forward<float, false>(who, dtype, a, o, ws, joined, s);
 }
-// Rows few enough for one workgroup to join them on its way to the loss, in units of its own or not at all (48 rows of V 50257, policy
-// loss: a launch less, 3 us): 0 or the parts of a row.
-constexpr int kFewRows = kJT / 16, kFewUnits = 4;
+// Split rows few enough for one workgroup to join them on its way to the loss, in units of its own or not at all: a launch less, us so /
+// with a launch that joins them: V 50257 fp32, one pair of 24 12.3 / 13.5 where two pairs of 8 15.1 / 15.7, four 23.4 / 18.1.
+constexpr int kFewRows = kJT / 16, kFewUnits = 2;
 int few_parts(const Rows& a, int64_t units, int dtype) {
-  const int parts = a.rows > 0 && a.rows <= kFewRows && units <= kFewUnits ? parts_of(a.rows, a.V, dtype) : 1;
+  const int parts = a.rows > 0 && a.rows <= kFewRows && units <= kFewUnits ? forward_parts(a.rows, a.V, dtype) : 1;
   return parts > 1 ? parts : 0;
 }
 
@@ -654,7 +662,7 @@ struct Layout {
 constexpr int64_t kUnit = 256;             // rows a workgroup of the policy loss where sequences do not matter
 Layout layout_of(int op, int64_t rows, int64_t units, int V, int dtype, bool ent) {
   Layout l;
-  const int parts = parts_of(rows, V, dtype);
+  const int parts = forward_parts(rows, V, dtype);
   l.lp64 = parts > 1 ? (rows * parts * (int64_t)sizeof(Sums) + 7) / 8 * 8 : 0;
   l.ent64 = l.lp64 + (op ? rows * 8 : 0);
   l.part = l.ent64 + (op && ent ? rows * 8 : 0);

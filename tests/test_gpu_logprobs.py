@@ -105,7 +105,7 @@ def inputs(lead, V, dtype, seed, ignored=0.2, banned=0.0, scale=2.0):
 
 
 SHAPES = [((1,), 1), ((1,), 7), ((1,), 50257), ((3, 5), 257), ((2, 9), 50257), ((70,), 5003), ((2, 1031), 1003), ((1100,), 4097),
-          ((1, 2, 3), 8191), ((515,), 16400), ((1500,), 37)]
+          ((1, 2, 3), 8191), ((515,), 16400), ((1500,), 37), ((2, 3), 80001), ((130,), 140001)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -159,7 +159,7 @@ def test_layouts(dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("rows,V", [(3, 50257), (700, 50257), (1200, 1003), (300, 1003)])
+@pytest.mark.parametrize("rows,V", [(3, 50257), (700, 50257), (1200, 1003), (300, 1003), (12, 80001), (12, 50257)])
 def test_awkward_rows(rows, V, dtype):
     """Rows of -inf, the lowest value, one +inf, one NaN, one value; tokens outside the vocabulary and closed ones; ignored rows
     that hold NaN."""
@@ -415,7 +415,7 @@ KINDS = [("sigmoid", 0.1, False, 0.0, 0.0, True), ("sigmoid", 0.5, False, 0.3, 0
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("n,T,V", [(1, 1, 50257), (1, 24, 50257), (3, 37, 1003), (70, 9, 257), (2, 300, 5003), (5, 700, 130)])
+@pytest.mark.parametrize("n,T,V", [(1, 1, 50257), (1, 24, 50257), (3, 37, 1003), (70, 9, 257), (2, 300, 5003), (5, 700, 130), (2, 5, 80001), (3, 24, 60007)])
 def test_preference_loss(n, T, V, dtype):
     for i, (kind, beta, average, margin, eps, with_ref) in enumerate(KINDS):
         say("preference", n, T, V, dtype, kind)
@@ -517,7 +517,7 @@ POLICY = [(1.0, 0.2, 0.2, 0.0, 0.0, False), (0.8, 0.2, 0.3, 0.1, 0.01, True), (1
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("lead,V", [((1, 1), 50257), ((4, 12), 50257), ((3, 37), 1003), ((7,), 257), ((2, 3, 90), 511), ((300, 5), 131),
-                                    ((2, 700), 2049)])
+                                    ((2, 700), 2049), ((2, 5), 80001), ((1, 64), 60007), ((5, 14), 60007)])
 def test_policy_loss(lead, V, dtype):
     for i, (tau, clip, high, kl, w, by_sequence) in enumerate(POLICY):
         say("policy", lead, V, dtype, tau)
