@@ -517,9 +517,10 @@ __global__ __launch_bounds__(kThreads<N>) void backward_kernel(Rows a, int parts
   const T* z = row_of<T>(a, r);
   const int64_t y = whole(a.tokens, a.wide, r);
   const float ref = finite_ref(k.m), inv_tau = (float)a.inv_tau;
-  const float gy = ga * inv_tau;
-  // dz of a logit that is not the token's: E (f0 + f1 times its exponent in base 2)
-  const float f0 = -(ga - ge * k.lean) * k.inv * inv_tau, f1 = -ge * (float)kLn2 * k.inv * inv_tau;
+  // tau dz of a logit that is not the token's: E (f0 + f1 times its exponent in base 2); the token's has ga besides. 1 / tau, up to
+  // 2^126, comes last: inside f0 and f1 it would overflow where E is 0 or the two cancel. (us inside / last: 2048 rows of 50257 bf16
+  // with entropies 85.0 / 85.1, 16384 of 4000 47.9 / 48.6.)
+  const float f0 = -(ga - ge * k.lean) * k.inv, f1 = -ge * (float)kLn2 * k.inv;
   auto value = [&](float x) {
     const Exponent h = exponent_of<kFull<T>>(x - ref, a.c);
     const float e = exp_of<kFull<T>>(h);
@@ -534,8 +535,10 @@ __global__ __launch_bounds__(kThreads<N>) void backward_kernel(Rows a, int parts
     for (int j = 0; j < E; ++j) x[j] = value(x[j]);
     if (p == yp) {
 #pragma unroll
-      for (int j = 0; j < E; ++j) x[j] += j == yj ? gy : 0.f;
+      for (int j = 0; j < E; ++j) x[j] += j == yj ? ga : 0.f;
     }
+#pragma unroll
+    for (int j = 0; j < E; ++j) x[j] *= inv_tau;
     store(p, pack<T>(x));
   };
   int p = c.p0 + tid;
@@ -549,7 +552,7 @@ __global__ __launch_bounds__(kThreads<N>) void backward_kernel(Rows a, int parts
   for (; p < c.p1; p += N) put(p, load16(from + (int64_t)p * E));
   if (tid < c.singles) {
     const int i = c.single(tid, a.V);
-    Elem<T>::store(out + i, value(Elem<T>::load(z + i)) + (i == y ? gy : 0.f));
+    Elem<T>::store(out + i, (value(Elem<T>::load(z + i)) + (i == y ? ga : 0.f)) * inv_tau);
   }
 }
 
