@@ -106,6 +106,9 @@ def _values(logits, tokens, temperature, ignore_index, entropy):
     z = torch.where(live.unsqueeze(-1), logits.to(wide), zero)
     # (a factor of NaN: the row's gradient is NaN too)
     factor = torch.where(bad, nan, torch.ones_like(zero))
+    if temperature < 1.0:                  # (of differences: a logit over the temperature may be past the type where they are not)
+        most = z.detach().amax(-1, keepdim=True)
+        z = z - torch.where(most.isfinite(), most, zero)
     log_p = torch.log_softmax(z / temperature, -1)
     lp = log_p.gather(-1, torch.where(live & ~bad, tokens, torch.zeros_like(tokens)).long().unsqueeze(-1)).squeeze(-1)
     lp = torch.where(live, lp * factor, zero)

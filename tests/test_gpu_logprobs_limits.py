@@ -37,3 +37,16 @@ def test_gradients_at_extreme_temperatures(rows, V, dtype):
         ref = Rows(z, tokens, tau)
         lp, ent = ops().token_logprobs(leaf, tokens, temperature=tau, entropy=True)
         ref.check_grad(torch.autograd.grad((lp, ent), leaf, (a * tau, e.clamp(-1, 1) * tau))[0], a * tau, e.clamp(-1, 1) * tau)
+
+
+def test_create_graph_at_the_least_temperature():
+    """With create_graph a gradient is the torch formula's: the same numbers."""
+    z, tokens = inputs((5,), 1003, torch.float32, 33, ignored=0.0)
+    z[:, 7] = 16.0
+    tokens[1] = 7
+    leaf = z.clone().requires_grad_()
+    out = ops().token_logprobs(leaf, tokens, temperature=2.0 ** -126, entropy=True)
+    by = (torch.ones(5, device=DEV), torch.ones(5, device=DEV))
+    first, = torch.autograd.grad(out, leaf, by, retain_graph=True)
+    again, = torch.autograd.grad(out, leaf, by, create_graph=True)
+    assert bool(first.isfinite().all()) and torch.equal(first, again.detach())
