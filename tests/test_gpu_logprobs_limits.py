@@ -1,4 +1,4 @@
-"""The post-training operators where numbers end: temperatures at the ends of their range with gradients. Bounds: test_gpu_logprobs."""
+"""The post-training operators where numbers end, and rows laid out as they seldom are. Bounds: test_gpu_logprobs."""
 
 import pytest
 import torch
@@ -50,3 +50,36 @@ def test_create_graph_at_the_least_temperature():
     first, = torch.autograd.grad(out, leaf, by, retain_graph=True)
     again, = torch.autograd.grad(out, leaf, by, create_graph=True)
     assert bool(first.isfinite().all()) and torch.equal(first, again.detach())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,V", [(40, 50257), (1500, 1003), (1030, 9001)])
+def test_gradients_of_broadcast_rows(rows, V, dtype):
+    """One row of logits for many positions (stride 0): every position's gradient against float64, and all of them equal. (A gradient
+    row's pieces begin at its own 16-byte boundary, but its elements depend on the row's kept numbers alone; the token's own is a sum
+    that may be rounded once or twice.)"""
+    say("broadcast", rows, V, dtype)
+    z = (2 * torch.randn(1, V, device=DEV, generator=gen(34))).to(dtype).expand(rows, V)
+    for entropy in (True, False):
+        for token in (5, V - 1):
+            tokens = torch.full((rows,), token, device=DEV)
+            leaf = z.detach().requires_grad_()
+            assert leaf.stride(0) == 0
+            out = ops().token_logprobs(leaf, tokens, temperature=0.8, entropy=entropy)
+            by = (torch.full((rows,), 0.75, device=DEV), torch.full((rows,), -1.5, device=DEV))
+            dz, = torch.autograd.grad(out, leaf, by if entropy else by[0])
+            Rows(z, tokens, 0.8).check_grad(dz, by[0], by[1] if entropy else None)
+            others = torch.arange(V, device=DEV) != token
+            assert bool((dz[:, others] == dz[:1, others]).all())
+    # gradients that differ from position to position, summed over them
+    a = torch.randn(rows, device=DEV, generator=gen(35))
+    one = z[0].detach().clone().requires_grad_()
+    lp = ops().token_logprobs(one.expand(rows, V), tokens, temperature=0.8)
+    got, = torch.autograd.grad(lp, one, a)
+    p = torch.softmax(one.detach().double() / 0.8, 0)
+    want = -a.double().sum() * p / 0.8
+    want[V - 1] += a.double().sum() / 0.8
+    # each position's value off by 20 u or a half step of its type, their sum in fp32 by as many u as positions, rounded to the type
+    size = a.double().abs().sum() * (p + (torch.arange(V, device=DEV) == V - 1)) / 0.8
+    step = torch.finfo(dtype).eps / 2
+    assert bool(((got.double() - want).abs() <= size * ((20 + 40 + rows) * 2.0 ** -24 + step) + step * want.abs() + 1e-12).all())
