@@ -3,7 +3,7 @@
 import pytest
 import torch
 
-from test_gpu_logprobs import DEV, TYPES, Rows, gen, inputs, ops, say
+from test_gpu_logprobs import DEV, TYPES, U, Rows, gen, inputs, ops, say
 
 pytestmark = pytest.mark.gpu
 
@@ -83,3 +83,49 @@ def test_gradients_of_broadcast_rows(rows, V, dtype):
     size = a.double().abs().sum() * (p + (torch.arange(V, device=DEV) == V - 1)) / 0.8
     step = torch.finfo(dtype).eps / 2
     assert bool(((got.double() - want).abs() <= size * ((20 + 40 + rows) * 2.0 ** -24 + step) + step * want.abs() + 1e-12).all())
+
+
+# (the form: few rows; by DMA 64 x 64, 64 x 256, 128 x 256, 256 x 256 tiles, rows sorted out by a launch; staged 64 x 64 and 128 x 128
+# tiles, rows that are not aligned)
+ROUNDED = [(1, 50257, 1024, 0), (9, 50257, 1024, 0), (32, 1003, 512, 0), (64, 1003, 512, 0), (64, 50257, 1024, 0), (90, 50257, 1024, 0),
+           (512, 50257, 1024, 0), (1100, 5003, 320, 0), (5, 5003, 77, 0), (700, 5003, 77, 0), (1100, 5003, 203, 0), (20, 1003, 512, 1)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,V,d,shift", ROUNDED)
+def test_head_rounds_its_logits(rows, V, d, shift, dtype):
+    """Eighths and whole numbers, whose fp32 sums are exact in any order: with round_logits the logits are those sums rounded to bf16,
+    no other numbers. Sums of some tens, so that most change by it; fp32 logits do not."""
+    say("rounded", rows, V, d, shift, dtype)
+    g = gen(36)
+    most = int((3 * 1600 / 0.03125 / d) ** 0.5)                  # sums of d products: a standard deviation of 40
+    assert most <= 256 and 3 * most * d < 2 ** 21                # whole numbers of bf16, eighths of fp32
+    h = torch.randint(-most, most + 1, (rows, d + shift), device=DEV, generator=g).to(dtype)[:, shift:]
+    w = (torch.randint(-2, 3, (V, d + shift), device=DEV, generator=g) / 8).to(dtype)[:, shift:]
+    tokens = torch.randint(0, V, (rows,), device=DEV, generator=g)
+    tokens[3::7] = -100
+    tau = 16.0
+    rounded = ops().head_logprobs(h, w, tokens, temperature=tau, entropy=True, round_logits=True)
+    whole = ops().head_logprobs(h, w, tokens, temperature=tau, entropy=True)
+    if dtype == torch.float32:
+        assert all(torch.equal(x, y) for x, y in zip(rounded, whole))
+    apart = 0
+    for r in range(0, rows, 256):
+        part, z = slice(r, r + 256), h[r:r + 256].double() @ w.double().t()
+        near = z.to(torch.bfloat16).double() if dtype == torch.bfloat16 else z
+        found = []
+        for got, logits in ((rounded, near), (whole, z)):
+            ref = Rows(logits, tokens[part], tau)
+            # fp32 logits with exponents rounded once; 200 additions that a term passes through (lanes, tiles, slots)
+            rel = U * (4 * ref.near.abs() + 3)
+            rel_s = (ref.p * rel).sum(1) + 200 * U
+            err_lp = rel_s + U * (ref.lp.abs() + 30)
+            lean = ref.lean.abs()
+            err_ent = rel_s * (1 + lean) + (ref.p * ref.near.abs() * (rel + 4 * U)).sum(1) + U * (ref.ent + 30) + 200 * U * lean
+            for x, want, err in ((got[0], ref.lp, err_lp), (got[1], ref.ent, err_ent)):
+                off = (x[part].double() - want).abs() - torch.where(ref.live, err, 0.0)
+                assert bool((off <= 0).all()), off.max()
+            found.append((ref.lp, err_lp))
+        apart += int(((found[0][0] - found[1][0]).abs() > 10 * (found[0][1] + found[1][1])).sum())
+    live = int((tokens != -100).sum())
+    assert apart > live // 2 if dtype == torch.bfloat16 else apart == 0                         # (the bounds tell the two apart)
