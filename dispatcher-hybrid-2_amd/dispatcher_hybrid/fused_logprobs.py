@@ -223,7 +223,9 @@ def preference_loss(logits, tokens, reference=None, beta=0.1, loss="sigmoid", av
         "squared"   (D - 1 / (2 beta))^2             (no margin)
 
     reduction: "mean" over the pairs (NaN when there is none), "sum" or "none" (n losses). A token outside the vocabulary makes
-    its sequence's logprob, its pair's loss and the gradient of the pair's answers NaN."""
+    its sequence's logprob, its pair's loss and the gradient of the pair's answers NaN. A token of probability 0 (its logit -inf)
+    makes its sequence's logprob -inf: the squared loss is inf and its pair's gradients infinite or NaN, those of the others are
+    numbers."""
     plain.check_preference(logits, tokens, reference, beta, loss, margin, label_smoothing, reduction)
     args = (logits, tokens, reference, plain.KINDS.index(loss), bool(average), float(beta), float(margin), float(label_smoothing),
             int(ignore_index), plain.PAIR_REDUCTIONS.index(reduction))
@@ -298,7 +300,9 @@ def policy_loss(logits, tokens, old_logprobs, advantages, reference_logprobs=Non
 
     clip_high: clip when None. reduction: "mean" over the positions (NaN when there is none), "sequence": the mean over the
     sequences that have a position of each one's mean, "sum" or "none". A token outside the vocabulary makes its position's loss
-    and all of its gradient NaN."""
+    and all of its gradient NaN. A token of probability 0 (its logit -inf) has a ratio of 0; with a KL term its position's loss is
+    NaN and its gradient infinite or NaN. So is the gradient, and inf the loss, of a ratio times its advantage that is past fp32 and
+    not clipped."""
     clip_high = clip if clip_high is None else clip_high
     plain.check_policy(logits, tokens, old_logprobs, advantages, reference_logprobs, clip, clip_high, kl_weight, entropy_weight,
                        temperature, reduction)

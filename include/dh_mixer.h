@@ -667,7 +667,8 @@ int dh_logprob_bwd(int dtype, const void* logits, int64_t stride_b, int64_t stri
  *   reduction 0: pair_loss (pairs) alone; 1: loss = their mean (NaN of none), divisor = pairs; 2: loss = their sum, divisor = 1.
  *   reference (2 pairs) fp32 or fp64 (reference_bits); sums (2 pairs): S; coef (2 pairs): the derivative of a pair's loss in a
  *   log-probability of the sequence, the by_logprob of dh_logprob_bwd (logprob_div T, stride 1; dloss_div T and dloss_mod pairs
- *   for reduction 0). All fp32 but the reference. S and all that follows are fp64 inside.
+ *   for reduction 0). All fp32 but the reference. S and all that follows are fp64 inside; a token of probability 0 (S = -inf) has
+ *   an infinite slope under kind 2 alone.
  *   workspace: dh_preference_workspace_bytes(dtype, pairs, T, V) bytes, 8-byte aligned.
  *   0 < beta < inf, finite margin, 0 <= label_smoothing <= 1/2; 2 pairs T < 2^22, fewer than 2^21 pairs.
  */
@@ -686,7 +687,8 @@ int dh_preference_fwd(int dtype, const void* logits, int64_t stride_b, int64_t s
  *   reduction 0: rows only; 1: loss = the mean over the rows that are not ignored (NaN of none), divisor = their number; 2: the
  *   sum, divisor = 1; 3: the mean over the sequences that have such a row of each one's mean, divisor = their number.
  *   logprob (B * T): x; by_logprob, by_entropy (B * T): the derivatives of the loss times the divisor, for dh_logprob_bwd.
- *   old_logprob, reference_logprob (B * T), advantage (B * T or B), fp32. The ratio and what follows are fp64 inside.
+ *   old_logprob, reference_logprob (B * T), advantage (B * T or B), fp32. The ratio and what follows are fp64 inside; by_logprob is
+ *   infinite where ratio A, not clipped, is past fp32, and for a token of probability 0 under a KL term (row_loss NaN).
  *   workspace: dh_policy_workspace_bytes(dtype, B, T, V, by_entropy given) bytes, 8-byte aligned.
  *   0 <= clip <= 1, 0 <= clip_high < inf, 0 <= kl_weight < inf, finite entropy_weight.
  */

@@ -3,6 +3,7 @@
 import pytest
 import torch
 
+from dispatcher_hybrid import logprobs as plain
 from test_gpu_logprobs import DEV, TYPES, U, Rows, gen, inputs, ops, say
 
 pytestmark = pytest.mark.gpu
@@ -129,3 +130,40 @@ def test_head_rounds_its_logits(rows, V, d, shift, dtype):
         apart += int(((found[0][0] - found[1][0]).abs() > 10 * (found[0][1] + found[1][1])).sum())
     live = int((tokens != -100).sum())
     assert apart > live // 2 if dtype == torch.bfloat16 else apart == 0                         # (the bounds tell the two apart)
+
+
+def kinds_of(x):
+    """-inf, a number, inf or NaN."""
+    return torch.where(x.isnan(), 2, torch.where(x.isinf(), x.sign(), 0))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("V", [3, 1003, 50257])
+def test_infinite_slopes_as_in_the_formulas(V, dtype):
+    """Tokens of probability 0 and ratios past fp32: the losses and gradients that are no numbers are those of the torch formulas."""
+    z = (2 * torch.randn(4, 3, V, device=DEV, generator=gen(37))).to(dtype)
+    tokens = torch.randint(0, V - 1, (4, 3), device=DEV, generator=gen(38))
+    tokens[:, 2] = -100
+    tokens[0, 1], z[0, 1, V - 1] = V - 1, -float("inf")
+    z[2, 0, V // 2] = -float("inf")                              # (closed, not the token)
+    tokens[2, 0] = 0 if V // 2 else 1
+    lp = plain.token_logprobs(z.double(), tokens)
+    near = torch.where(lp.isfinite(), lp, -5.0).float()
+    far = near - 95.0
+    signs = torch.tensor([[1.0], [-1.0], [1.0], [-1.0]], device=DEV).expand(4, 3)
+    calls = [lambda f, x, kind=kind, red=red, roll=roll: f.preference_loss(x.roll(roll, 0), tokens.roll(roll, 0), loss=kind, reduction=red)
+             for kind in ("sigmoid", "hinge", "squared") for red in ("none", "mean") for roll in (0, 2)]
+    calls += [lambda f, x, old=old, kl=kl, red=red: f.policy_loss(x, tokens, old, signs, near, kl_weight=kl, reduction=red)
+              for old in (near, far) for kl in (0.0, 0.1) for red in ("none", "sequence")]
+    for i, call in enumerate(calls):
+        found = []
+        for f in (ops(), plain):
+            leaf = z.clone().requires_grad_()
+            loss, values = call(f, leaf)
+            found.append([loss.detach(), values, torch.autograd.grad(loss.sum(), leaf)[0]])
+        for j, (x, y) in enumerate(zip(*found)):
+            say("call", i, "output", j)
+            assert torch.equal(kinds_of(x.float()), kinds_of(y.float()))
+            ok = kinds_of(y.float()) == 0
+            # (that numbers are right is other tests' matter: here to 1e-4 and a step of the type)
+            assert torch.allclose(x.float()[ok], y.float()[ok], rtol=1e-4 + torch.finfo(x.dtype).eps, atol=1e-4)

@@ -45,3 +45,44 @@ def test_small_temperatures_against_float64():
         assert ((lp.double() - want).abs() <= slack + 2.0 ** -24 * 5 * want.abs()).all()
         h = -(p * ref.clamp(min=-800)).sum(1)
         assert ((ent.double() - h).abs() <= 4 * (slack * (1 + h) + 2.0 ** -24 * (p * d * d).sum(1))).all()
+
+
+def closed_pairs():
+    """Two pairs of one token each, the answer of the first pair's preferred sequence of probability 0."""
+    z = torch.tensor([[[1.0, -math.inf, 0.0]], [[0.5, 1.0, 2.0]], [[0.0, 1.0, 2.0]], [[2.0, 0.0, 1.0]]])
+    return z.requires_grad_(), torch.tensor([[1], [0], [0], [1]])
+
+
+def test_preference_of_a_closed_token():
+    """An answer of probability 0 has a log-probability of -inf. The slopes of the sigmoid and the hinge are bounded, so its pair's
+    gradients are numbers; that of the squared loss is infinite, and a probability of 0 times it NaN. The other pair has its own."""
+    for first in (True, False):
+        for kind in ("sigmoid", "hinge", "squared"):
+            z, tokens = closed_pairs()
+            if not first:                                        # the closed answer is the one that is not preferred
+                z, tokens = z.detach().roll(2, 0).requires_grad_(), tokens.roll(2, 0)
+            loss, sums = plain.preference_loss(z, tokens, loss=kind, reduction="none")
+            assert sums.isinf().tolist() == [first, False, not first, False]
+            dz, = torch.autograd.grad(loss.sum(), z)
+            assert loss[1].isfinite() and dz[[1, 3]].isfinite().all()
+            if kind == "squared":
+                assert loss[0] == math.inf and not dz[[0, 2]].isfinite().any() and dz[[0, 2]].isnan().any()
+            else:
+                assert loss[0] == (math.inf if first else 0.0) and dz[[0, 2]].isfinite().all()
+
+
+def test_policy_of_a_closed_token_and_of_a_ratio_past_fp32():
+    """A closed token has a ratio of 0, and with a KL term a slope of -inf; a ratio of e^95 that its advantage does not clip is inf."""
+    z, tokens = closed_pairs()
+    ones, low = torch.ones(4, 1), torch.full((4, 1), -2.0)
+    loss, _ = plain.policy_loss(z, tokens, low, ones, reduction="none")
+    dz, = torch.autograd.grad(loss.sum(), z)
+    assert loss[0] == 0 and loss.isfinite().all() and dz.isfinite().all()
+    loss, _ = plain.policy_loss(z, tokens, low, ones, low, kl_weight=0.1, reduction="none")
+    dz, = torch.autograd.grad(loss.sum(), z)
+    assert loss[0].isnan() and not dz[0].isfinite().any() and loss[1:].isfinite().all() and dz[1:].isfinite().all()
+    old = torch.tensor([[-2.0], [-97.0], [-2.0], [-97.0]])
+    loss, _ = plain.policy_loss(z, tokens, old, torch.tensor([[1.0], [-1.0], [1.0], [1.0]]), reduction="none")
+    dz, = torch.autograd.grad(loss.sum(), z)
+    assert loss[1] == math.inf and not dz[1].isfinite().any() and dz[1].isnan().any()
+    assert loss[3] == -torch.tensor(1.2) and not dz[3].any()     # clipped
