@@ -2,17 +2,18 @@
 // for gfx950 (inference). For a row h (d wide), the weight W (V, d), a temperature tau and the row's token y:
 //   z_v = h . W_v (fp32 sums; round_logits: rounded to the operands' type),  p = softmax(z / tau)
 //   lp = log p_y,  H = - sum_v p_v log p_v
-// A row whose token is ignore_index is not computed: lp = H = 0.
+// A row whose token is ignore_index has lp = H = 0. It is not computed, but by few_kernel, whose join puts the zeros in its place.
 //
 // The product's tiles stay in the accumulators. A lane of a tile holds some columns of its rows and keeps, over all the tiles that
 // its workgroup takes of a row, the running maximum m of z and the sums of e = exp((z - m) / tau) and of e times its exponent;
 // lanes are joined when the workgroup ends with the row, workgroups by a last launch. A token's own logit is written by the lane
-// that meets it. So a row leaves a few numbers for each workgroup instead of V logits. V 50257, d 1024, bf16: 5300 rows 405 us (1348
-// TFLOP/s of products, on the matrix cores in 66% of the cycles), 16 rows 22 (the weight at 5.5 TB/s, and the join).
+// that meets it. So a row leaves a few numbers for each workgroup instead of V logits. V 50257, d 1024, bf16: 5300 rows 427 us (1277
+// TFLOP/s of products, on the matrix cores in 66% of the cycles), 16 rows 23 (the weight at 5.6 TB/s, and the join).
 //
 // Launches: the rows that count, in their order, and how the tiles are dealt out (compact_kernel; their number is known on the
-// device only; up to 1024 rows the product's workgroups do this themselves); the product; the join. Up to 32 rows: the product
-// (few_kernel, the weight's bytes bound it) and the join.
+// device only; up to 1024 rows the product's workgroups do this themselves); the product; the join. Up to 32 rows that are aligned, of
+// whole 128-byte lines and beside the rings in LDS (64 KB of them, padded to 16 or 32 rows): the product (few_kernel, the weight's bytes
+// bound it) and the join.
 
 #include "dh_rows.h"
 
@@ -704,11 +705,13 @@ struct Form {
   int kind, bm, bn, groups, slots, id;
 };
 // The forms of the DMA kernel, and what a tile of each takes at K = 1024, microseconds on a full card: the form whose rounds of tiles
-// take least. bf16, V 50257, d 1024, us of a call by rows, 256 x 256 / 128 x 256 / 64 x 256 / 64 x 64: 64 38 / 29 / 28 / 30; 128 38 / 31
-// / 29 / 35; 256 39 / 39 / 46 / 52; 512 63 / 66 / 78 / 93; 640 86 / 67 / 84 / 109; 1024 110 / 111 / 125 / 159; 5300 440 / 460 / 571 / 751.
-// (A few large tiles leave most of the card idle: 2000 rows of V 1000 are 32 of 256 x 256.) fp32 is bound by its products whatever the
-// tile, and 32 x 128 tiles have the fewest empty rows: us at 200, 329, 501, 4096 rows 205, 292, 413, 3090; 64 x 64 236, 321, 412, 3055;
-// 128 x 128 255, 372, 491, 2995 (all with a launch that sorted the rows out, 5 us).
+// take least, of all rows (how many count is known on the device only). us of a call without entropies, weights that no cache holds (three
+// in turn, a graph), V 50257, d 1024. bf16 by rows, 256 x 256 / 128 x 256 / 64 x 256 / 64 x 64: 64 41 / 33 / 31 / 32; 128 39 / 32 / 36 / 44;
+// 256 41 / 42 / 56 / 63; 512 64 / 68 / 84 / 100; 640 86 / 69 / 103 / 127; 1024 112 / 107 / 145 / 178; 4096 329 / 349 / 517 / 658; 5300
+// 426 / 449 / 673 / 850. (A few large tiles leave most of the card idle: 2000 rows of V 1000 are 32 of 256 x 256.) fp32 is bound by its
+// products whatever the tile, and 32 x 128 tiles have the fewest empty rows: 200, 329, 501, 4096 rows 200, 289, 413, 3055. (Chosen on an
+// earlier version, whose rows were sorted out by a launch of 5 us: 205, 292, 413, 3090; 64 x 64 236, 321, 412, 3055; 128 x 128 255, 372,
+// 491, 2995.)
 struct Timed {
   Form form;
   float us;
@@ -716,8 +719,8 @@ struct Timed {
 constexpr Timed kBf16[] = {{{1, 256, 256, 256, 2, 0}, 25.f}, {{1, 128, 256, 256, 2, 1}, 13.6f}, {{1, 64, 256, 256, 2, 2}, 8.7f},
                            {{1, 64, 64, 512, 2, 3}, 5.9f}};
 constexpr Form kFp32 = {1, 32, 128, 512, 2, 0};
-// Staged through registers, the same rule. V 50257, d 1001, us by rows, 64 x 64 / 128 x 128 tiles: bf16 1 33 / 39; 64 41 / 42; 128 62 /
-// 41; 4096 1083 / 648; fp32 64 97 / 150; 128 174 / 149; 1024 1062 / 977. V 5000, d 777: bf16 512 27 / 30; fp32 512 78 / 125.
+// Staged through registers, the same rule. V 50257, d 1001, us by rows, 64 x 64 / 128 x 128 tiles: bf16 1 39 / 42; 64 50 / 51; 128 75 /
+// 51; 512 187 / 142; 4096 1164 / 775; fp32 64 100 / 156; 128 183 / 157; 1024 1073 / 1011. V 5000, d 777: bf16 512 29 / 31; fp32 512 79 / 123.
 constexpr Timed kStagedBf16[] = {{{0, 64, 64, 1024, 2, 0}, 22.f}, {{0, 128, 128, 512, 2, 1}, 26.f}};
 constexpr Timed kStagedFp32[] = {{{0, 64, 64, 1024, 2, 0}, 82.f}, {{0, 128, 128, 512, 2, 1}, 140.f}};
 
@@ -736,8 +739,7 @@ Form least(const Timed (&forms)[N], int64_t rows, int V) {
   }
   return forms[best].form;
 }
-// up to 32 rows (as many as LDS holds beside the rings) the form for few: 16 rows 21 us, the 64 x 256 tiles 27; fp32 36 us,
-// its tiles 51 (5 of these the launch that sorted the rows out)
+// up to 32 rows (as many as LDS holds beside the rings) the form for few: 16 rows 23 us, the 64 x 256 tiles 31; fp32 51 us, its tiles 54
 Form form_of(int dtype, int64_t rows, int d, int V, bool fast) {
   if (!fast) return dtype == DH_F32 ? least(kStagedFp32, rows, V) : least(kStagedBf16, rows, V);
   if (rows <= 32 && (rows <= 16 ? 16 : 32) * (int64_t)d * (dtype == DH_BF16 ? 2 : 4) <= kFewLds)

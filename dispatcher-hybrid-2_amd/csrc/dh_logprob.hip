@@ -17,8 +17,8 @@
 // exponent; the read of z bounds it. Few long rows are split over several workgroups, whose sums a second launch joins. The losses
 // add one launch over the rows' lp (and one that adds their parts), which also leaves a and e. Backward: z once more, and dz;
 // m, 1 / sum and the mean exponent are all it needs of a row. A row with a = e = 0 (a clipped ratio, a pair behind the hinge)
-// is not read. bytes bound both: 5994 of 8192 rows of 50257 bf16 forward 105 us (602 MB, 5.7 TB/s; a bare read reaches 6.1), backward
-// 269 (1426 MB, 5.3 TB/s; a copy 5.2); with H, 5631 rows, 112 (VALU busy for 82% of it) and 262.
+// is not read. bytes bound both: 5994 of 8192 rows of 50257 bf16 forward 107 us (602 MB, 5.6 TB/s; a bare read reaches 6.1), backward
+// 269 (1426 MB, 5.3 TB/s; a copy of 734 MB 5.2, of 2 GiB 4.9); with H, 5631 rows, 115 (VALU busy for 82% of it) and 261.
 //
 // Sums over V are fp32 (a thread's over 4 pieces at a time), what follows from a row's sums is fp64, lp included until it is
 // returned: sequence sums, ratios and their comparison with the clip are of unrounded lp.
